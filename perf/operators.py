@@ -294,14 +294,14 @@ def _plan(s):
     have = live & (at // page < held_out[:, None])
     slots = torch.gather(entries, 1, (at // page).clamp(max=width - 1)) * page + at % page
     slots = torch.where(have, slots, -1).to(torch.int32)
-    status = ((~fits) & (need <= width)).any().int() + 2 * ((~fits) & (need > width)).any().int()
+    status = torch.where(fits, 0, torch.where(need <= width, 1, 2)).to(torch.int32)
     depth, ancestors = node, slots
     if s["parents"] is not None:
         seen = _ancestor_matrix(s["parents"]) & live[:, :, None] & live[:, None, :]
         depth = seen.sum(-1) - 1
         ancestors = _bits(seen)
     positions = torch.where(live, lengths[:, None] + depth, 0).to(torch.int32)
-    return [slots, positions, held_out, span_out, status.to(torch.int32).view(1), table, ring, ancestors]
+    return [slots, positions, held_out, span_out, status, table, ring, ancestors]
 
 
 def _values(cache, name, dtype=torch.float32):
@@ -408,9 +408,9 @@ def work(case):
     if op == "plan":
         batch, nodes, page = case["batch"], case["nodes"], case["page"]
         # in: length, count, held pages, parents, a table entry per page of the new tokens; out:
-        # slot, position (and a 64-bit ancestor word) of each, held pages
+        # slot, position (and a 64-bit ancestor word) of each, held pages, status
         each = 2 * 4 + (12 if case["tree"] else 0)
-        return {"bytes": batch * (16 + nodes * each + 4 * ((nodes + page - 1) // page)), "flops": 0}
+        return {"bytes": batch * (20 + nodes * each + 4 * ((nodes + page - 1) // page)), "flops": 0}
     if op == "write":
         width = case["kv"] * case["hd"]
         size = 2 if case["dtype"] == "bf16" else 4
