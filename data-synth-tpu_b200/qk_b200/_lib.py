@@ -52,6 +52,27 @@ class MoeDesc(ctypes.Structure):
 QK_COMPUTE_BF16, QK_COMPUTE_INT8_Q8 = 0, 1
 
 
+class LogitsDesc(ctypes.Structure):
+    """``qk_logits_desc`` of include/qk_b200.h."""
+
+    _fields_ = [
+        ("history", _p),
+        ("history_lengths", _p),
+        ("prompt_lengths", _p),
+        ("history_capacity", _i),
+        ("bias_count", _i),
+        ("bias_ids", _p),
+        ("bias", _p),
+        ("repetition", _p),
+        ("frequency", _p),
+        ("presence", _p),
+        ("temperature", _p),
+        ("drafts", _p),
+        ("ancestors", _p),
+        ("mask", _p),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "qk_version": (ctypes.c_char_p, []),
@@ -105,6 +126,18 @@ SIGNATURES = {
         [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _sz, _p],
     ),
     "qk_kv_q8_attention_combine": (_i, [_p, _i, _i, _i, _i, _p, _p, _p]),
+    "qk_paged_plan": (_i, [_p] * 7 + [_i] * 5 + [_p] * 7),
+    "qk_kv_q8_write_slots": (
+        _i,
+        [_p, _p, _i, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i, _i64, _i, _i, _p],
+    ),
+    "qk_tree_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "qk_tree_attention": (
+        _i,
+        [_p, _i64] + [_p] * 9 + [ctypes.c_float] + [_i] * 6 + [_i64, _i, _i, _p, _p, _sz, _p],
+    ),
+    "qk_tree_attention_check": (_i, [_p, _p]),
+    "qk_process_logits": (_i, [ctypes.POINTER(LogitsDesc), _p, _i, _i, _i, _i, _p, _p]),
     "qk_qsa_block_scores": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _p, _p]),
     "qk_qsa_select": (_i, [_p, _p, _i, _i, _i, _i, _p, _p, _p]),
     "qk_qsa_update_keys": (

@@ -370,6 +370,88 @@ int qk_kv_q8_decode_attention_partial(const uint16_t* q, const int8_t* k_codes,
 int qk_kv_q8_attention_combine(const float* parts, int R, int B, int hq, int head_dim,
                                const uint16_t* gate, uint16_t* out, qk_stream_t stream);
 
+/* ---- paged Q8 cache and draft trees ---------------------------------------------
+ * No counterpart in the reference (its cache is a static [B, T] array and it decodes one
+ * token per step). A pool of pages is a Q8 cache of `rows` rows (one, for a pool shared by all
+ * requests) whose rows * T slots are cut into pages of page_size (a power of two in
+ * [16, 1024], dividing T): token t of request b lies in slot
+ * table[b, t / page_size] * page_size + t % page_size, table int32 [B, width]. */
+
+/* Plan of one step that appends count_b tokens to each request, N at most. Page takes and
+ * returns bring request b from held[b] pages to ceil((lengths[b] + counts[b]) / page_size):
+ * takes come from the head of `ring` (int32 [pages], `span` = {head, number of free pages}) in
+ * request order, returns go behind its tail and can be taken from the next step on. A request
+ * whose takes do not all fit takes none and keeps its pages. Out: slots int32 [B, N] (-1 past
+ * counts[b] and where no page is held), positions int32 [B, N] (lengths[b] + depth; 0 past
+ * counts[b]), held_out [B] and span_out [2] (other arrays than held and span; table and ring
+ * change in place), status int32 [B]: 0, or the sum of 1 (no free pages), 2 (the table is too
+ * narrow), 4 (length, count or held out of range, brought into it), 8 (a parent that is not an
+ * earlier node; taken as -1). With ancestors (uint64 [B, N], N <= 64; 0 past counts[b]) bit j of
+ * word i says that node j is node i or above it: parents int32 [B, N] holds each node's parent
+ * (an earlier node, -1: the prefix), or is NULL for a chain. */
+int qk_paged_plan(int32_t* table, const int32_t* held, int32_t* ring, const int32_t* span,
+                  const int32_t* lengths, const int32_t* counts, const int32_t* parents, int B, int width,
+                  int pages, int page_size, int N, int32_t* slots, int32_t* positions,
+                  uint64_t* ancestors, int32_t* held_out, int32_t* span_out, int32_t* status,
+                  qk_stream_t stream);
+
+/* The append of attention_cache.py:26-43 by slot: token i's keys and values (kv_heads * head_dim
+ * values, tokens key_stride / value_stride values apart, 16-byte aligned) are quantised into slot
+ * slots[i] of [0, rows * T); other slots (-1: padding) are dropped. The same codec and the same
+ * bytes as qk_kv_q8_append. Two tokens must not name one slot. head_dim a multiple of 32, or 8 or
+ * 16. */
+int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64_t key_stride,
+                         int64_t value_stride, const int32_t* slots, int8_t* k_codes, int8_t* v_codes,
+                         uint16_t* k_scale, uint16_t* v_scale, int64_t tokens, int rows, int64_t T,
+                         int kv_heads, int head_dim, qk_stream_t stream);
+
+/* Attention of up to N <= 64 drafted tokens per request (N = 1: plain decoding). Node i < counts[b]
+ * (counts NULL: N) of request b, whose key and value are already in the cache as token
+ * lengths[b] + i, sees the prefix t < lengths[b] and the nodes j < counts[b] of its ancestor word
+ * ancestors[b, i] (uint64 [B, N]); out = softmax(q . k * scale) v over them with k, v = code *
+ * scale, times sigmoid(gate) when gate != NULL, rounded once to BF16. Nothing else in the cache has
+ * a say, whatever it holds; a node that sees nothing and nodes i >= counts[b] are zero. q BF16
+ * [B, N, hq, head_dim] with tokens q_stride values apart (a multiple of 8), gate and out contiguous;
+ * hq a multiple of kv_heads, head_dim 64, 128 or 256. The workspace (256-byte aligned) must be
+ * zeroed before its first call; calls that share one must not overlap. qk_tree_attention_check
+ * synchronises `stream`, reports an earlier call's table entry outside the cache
+ * (QK_ERR_INVALID_ARGUMENT; its tokens were left out) or a bounded wait that gave up
+ * (QK_ERR_TIMEOUT), and clears the report. */
+size_t qk_tree_attention_workspace_bytes(int B, int N, int hq, int kv_heads, int head_dim);
+int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes, const int8_t* v_codes,
+                      const uint16_t* k_scale, const uint16_t* v_scale, const int32_t* table,
+                      const int32_t* lengths, const int32_t* counts, const uint64_t* ancestors,
+                      const uint16_t* gate, float scale, int B, int N, int hq, int kv_heads,
+                      int head_dim, int rows, int64_t T, int width, int page_size, uint16_t* out,
+                      void* workspace, size_t workspace_bytes, qk_stream_t stream);
+int qk_tree_attention_check(const void* workspace, qk_stream_t stream);
+
+/* ---- logits before the choice ---------------------------------------------------
+ * No counterpart in the reference (its decoding is greedy, run.py:46-55). Per request b and row i
+ * (a node of its draft tree), for every token v:
+ *   x = logit; if v is in the context: x = x > 0 ? x / repetition : x * repetition;
+ *   x -= frequency * n + presence * [n > 0]; x += bias(v); x *= 1 / temperature;
+ *   x = -inf where bit v of the row's mask is 0.
+ * n counts v in the history from prompt_length on and in the drafts of the row's ancestor word; the
+ * context is these and the prompt. Every array may be NULL (no such rule). */
+typedef struct qk_logits_desc {
+  const int32_t* history;         /* [B, history_capacity]; ids outside the vocabulary are ignored */
+  const int32_t* history_lengths; /* [B]                                                         */
+  const int32_t* prompt_lengths;  /* [B]; NULL: 0                                                */
+  int history_capacity;           /* below 2^20                                                  */
+  int bias_count;                 /* at most 1024                                                */
+  const int32_t* bias_ids;        /* [B, bias_count]; ids outside the vocabulary are ignored, of
+                                     several biases of one token the last holds                  */
+  const float* bias;              /* [B, bias_count]                                             */
+  const float *repetition, *frequency, *presence, *temperature; /* [B]; temperature above 0      */
+  const int32_t* drafts;          /* [B, N], N <= 64                                             */
+  const uint64_t* ancestors;      /* [B, N]                                                      */
+  const int32_t* mask;            /* [B, N, ceil(V / 32)], bit v % 32 of word v / 32: allowed    */
+} qk_logits_desc;
+/* logits [B, N, V] (BF16 or FP32 by in_dtype) -> out FP32 [B, N, V] (may be the FP32 input). */
+int qk_process_logits(const qk_logits_desc* desc, const void* logits, int in_dtype, int B, int N, int V,
+                      float* out, qk_stream_t stream);
+
 /* ---- sparse token selection (QSA indexer) -------------------------------------
  * Replaces the selection half of attention_cache.py:84-125 select_tokens, once the block
  * keys are current. qk_qsa_block_scores: query BF16 [B, heads, dim] (normed, rotated),
