@@ -54,6 +54,19 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "memory");
 }
 
+// Each thread of the warp reads 32 consecutive 32-bit columns of its own lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -64,6 +77,17 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 // Instruction descriptor of kind::f16: BF16 A and B, FP32 D, both K-major, M = 128, N.
 __device__ __forceinline__ uint32_t idesc_bf16_m128(uint32_t n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// The same with an MN-major B (the transposed operand: N contiguous in shared memory).
+__device__ __forceinline__ uint32_t idesc_bf16_m128_bmn(uint32_t n) { return idesc_bf16_m128(n) | (1u << 16); }
+
+// Shared-memory matrix descriptor of an MN-major operand, 128-byte swizzle: atoms of 8 K rows x
+// 64 values of the M or N dimension (128 B per K row), blocks of 64 values `mn_stride` bytes
+// apart, groups of 8 K rows `k_stride` bytes apart.
+__device__ __forceinline__ uint64_t sdesc_sw128_mn(uint32_t saddr, uint32_t mn_stride, uint32_t k_stride) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>((mn_stride >> 4) & 0x3fffu) << 16) |
+         (static_cast<uint64_t>((k_stride >> 4) & 0x3fffu) << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // Shared-memory matrix descriptor, K-major, 128-byte swizzle: 8-row x 128-byte atoms,
