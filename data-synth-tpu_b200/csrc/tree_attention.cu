@@ -36,6 +36,7 @@ constexpr uint32_t kColO = 0, kColQ = 256, kColS = 384;  // TMEM columns
 constexpr float kLazyGrowth = 8.f;                       // in powers of two
 constexpr uint32_t kHugeScale = 0x7c00;                  // BF16 bits of 2^121: times 127 leaves FP32's range
 constexpr int kBadRing = 4;
+constexpr int kUnitCost = 4;  // what a unit costs besides its tiles (Q, the output), in tiles
 
 struct TreeArgs {
   const uint16_t* q;
@@ -53,12 +54,21 @@ struct TreeArgs {
   int* status;
   float* part;   // [2 * CTAs][HD][part_rows] unnormalised O
   float* stats;  // [2 * CTAs][2][part_rows] maximum (log2) and sum
+  struct Cut* cuts;  // [CTAs]
+};
+
+// What a range's CTA knows of the unit that its range begins inside of, where it is the first
+// to do so: the unit, its parts (consecutive ranges) and which record of the first range is its.
+struct Cut {
+  int b, head, row_tile, count, parts, record;
 };
 
 struct Request {
   int length, count, tiles, row_tiles;
   bool cut;
-  __device__ int64_t work(int kv) const { return static_cast<int64_t>(kv) * row_tiles * tiles; }
+  // A unit's share of the ranges: its tiles and kUnitCost steps that stand for Q and the output.
+  __device__ int steps() const { return tiles + kUnitCost; }
+  __device__ int64_t work(int kv) const { return tiles ? static_cast<int64_t>(kv) * row_tiles * steps() : 0; }
 };
 
 __device__ __forceinline__ Request load_request(const TreeArgs& a, int b) {
@@ -73,23 +83,24 @@ __device__ __forceinline__ Request load_request(const TreeArgs& a, int b) {
   return r;
 }
 
-// The CTAs' ranges of a total of `total` tiles, at least one tile each.
+// The CTAs' ranges of a total of `total` steps, at least one step each.
 __device__ __forceinline__ int ranges(int64_t total, int ctas) {
   return static_cast<int>(total < ctas ? total : ctas);
 }
 __device__ __forceinline__ int64_t range_start(int64_t total, int n, int c) { return c * total / n; }
-__device__ __forceinline__ int range_owner(int64_t total, int n, int64_t tile) {
-  return static_cast<int>(((tile + 1) * n - 1) / total);
+__device__ __forceinline__ int range_owner(int64_t total, int n, int64_t step) {
+  return static_cast<int>(((step + 1) * n - 1) / total);
 }
 
-// Total work of all requests, and the request that holds tile `want` of it with the tile's
+// Total work of all requests, and the request that holds step `want` of it with the step's
 // offset in it: threads sum consecutive requests, a block scan, one thread walks its few.
 struct Located {
   int64_t total, offset;
   int b;
 };
-template <int THREADS, class Want>
+template <class Want>
 __device__ __forceinline__ Located locate(const TreeArgs& a, Located* shared, int64_t* warps, Want want, bool report) {
+  constexpr int THREADS = kThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + THREADS - 1) / THREADS;
   const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
@@ -114,9 +125,9 @@ __device__ __forceinline__ Located locate(const TreeArgs& a, Located* shared, in
   }
   if (tid == 0) *shared = Located{total, 0, a.B};
   __syncthreads();
-  const int64_t tile = want(total);
-  if (tile >= before && tile < before + sum) {
-    int64_t off = tile - before;
+  const int64_t step = want(total);
+  if (step >= before && step < before + sum) {
+    int64_t off = step - before;
     for (int b = b0; b < b1; ++b) {
       const int64_t w = load_request(a, b).work(a.kv);
       if (off < w) {
@@ -131,33 +142,43 @@ __device__ __forceinline__ Located locate(const TreeArgs& a, Located* shared, in
   return *shared;
 }
 
-// The pieces of a CTA's range: tiles [t0, t1) of one unit each.
+// The pieces of a CTA's range: tiles [t0, t1) of one unit each. A unit's last steps are not tiles:
+// a range that holds nothing else of the unit has no piece of it.
 struct Segment {
   Request r;
   int b, head, row_tile, t0, t1, index;
+  bool first;  // the range begins with it
   __device__ bool whole() const { return t0 == 0 && t1 == r.tiles; }
 };
 struct Walk {
   int b, index;
   int64_t offset, left;
+  bool first;
   __device__ bool next(const TreeArgs& a, Segment& s) {
-    if (left <= 0) return false;
-    for (;; ++b) {
-      s.r = load_request(a, b);
-      const int64_t w = s.r.work(a.kv);
-      if (offset < w) break;
-      offset -= w;
+    while (left > 0) {
+      for (;; ++b) {
+        s.r = load_request(a, b);
+        const int64_t w = s.r.work(a.kv);
+        if (offset < w) break;
+        offset -= w;
+      }
+      const int steps = s.r.steps();
+      const int unit = static_cast<int>(offset / steps);
+      s.b = b;
+      s.head = unit / s.r.row_tiles;
+      s.row_tile = unit % s.r.row_tiles;
+      s.t0 = static_cast<int>(offset % steps);
+      const int end = static_cast<int>(min(static_cast<int64_t>(steps), s.t0 + left));
+      left -= end - s.t0;
+      offset += end - s.t0;
+      s.t1 = min(end, s.r.tiles);
+      s.first = first;
+      first = false;
+      if (s.t0 >= s.t1) continue;
+      s.index = index++;
+      return true;
     }
-    const int unit = static_cast<int>(offset / s.r.tiles);
-    s.b = b;
-    s.head = unit / s.r.row_tiles;
-    s.row_tile = unit % s.r.row_tiles;
-    s.t0 = static_cast<int>(offset % s.r.tiles);
-    s.t1 = static_cast<int>(min(static_cast<int64_t>(s.r.tiles), s.t0 + left));
-    s.index = index++;
-    left -= s.t1 - s.t0;
-    offset += s.t1 - s.t0;
-    return true;
+    return false;
   }
 };
 
@@ -180,12 +201,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// The gate, rounded to BF16 with its product right after: the approximate exponential and
+// reciprocal (2^-22 each) do, at an eighth of the instructions of the exact ones.
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + exp2_fast(x * -1.44269504088896341f)));
+  return y;
+}
+
 __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   uint4 r;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                : "l"(p));
   return r;
+}
+
+__device__ __forceinline__ void sts_v4(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 // Four int8 codes times a BF16 scale (in both halves of `scale2`) -> two BF16 pairs. A byte c
@@ -213,59 +246,65 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 
 // ---- decode warps -------------------------------------------------------------------------
 
-// A thread's share of a tile: 16 channels of SPT consecutive tokens (all in one page).
+// A thread's share of a tile: 16 channels of SPT consecutive tokens (all in one page; codes[i] of
+// token i ^ swap), and their group's scales (token i in half i % 2 of word i / 2).
 template <int HD>
 struct Share {
   static constexpr int SPT = HD / 32;
   uint4 codes[SPT];
-  uint16_t scales[8];  // SPT used
+  uint32_t scales[SPT / 2];
 };
 
 template <int HD>
 __device__ __forceinline__ void load_share(const TreeArgs& a, const int8_t* codes, const uint16_t* scale, int head,
-                                           int page, int token, int total, int chunk, Share<HD>& s) {
+                                           int page, int token, int total, int chunk, int swap, Share<HD>& s) {
   constexpr int SPT = HD / 32;
+  if (token >= total) {
 #pragma unroll
-  for (int i = 0; i < SPT; ++i) s.codes[i] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < SPT; ++i) s.codes[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-  for (int i = 0; i < SPT; ++i) s.scales[i] = 0;
-  if (token >= total) return;
+    for (int i = 0; i < SPT / 2; ++i) s.scales[i] = 0;
+    return;
+  }
   const int row = page / a.pages_per_row;
   const int64_t in_row = (static_cast<int64_t>(page - row * a.pages_per_row) << a.shift) + (token & ((1 << a.shift) - 1));
   const int D = a.kv * HD, G = D / 32;
   const int8_t* c = codes + (row * a.T + in_row) * D + head * HD + chunk * 16;
   const uint16_t* p = scale + (static_cast<int64_t>(row) * G + head * (HD / 32) + chunk / 2) * a.T + in_row;
+  const int8_t *even = c + swap * D, *odd = c - swap * D;
 #pragma unroll
-  for (int i = 0; i < SPT; ++i) s.codes[i] = ld_stream_v4(c + static_cast<int64_t>(i) * D);
+  for (int i = 0; i < SPT; ++i) s.codes[i] = ld_stream_v4((i & 1 ? odd : even) + i * D);
   if (SPT == 8) {
     const uint4 v = ld_nc_v4(p);
 #pragma unroll
-    for (int i = 0; i < SPT; ++i) s.scales[i] = static_cast<uint16_t>(word(v, i / 2) >> (16 * (i & 1)));
+    for (int i = 0; i < SPT / 2; ++i) s.scales[i] = word(v, i);
   } else {
 #pragma unroll
-    for (int i = 0; i < SPT / 2; ++i) {
-      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-      s.scales[2 * i] = static_cast<uint16_t>(v);
-      s.scales[2 * i + 1] = static_cast<uint16_t>(v >> 16);
-    }
+    for (int i = 0; i < SPT / 2; ++i) s.scales[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
   }
 }
 
-template <int HD, bool VALUES>
+// Both kinds of decode warps run one copy of this code (K or V by run-time values), and the
+// buffered tile moves to the front instead of the loop being unrolled over buffers: with a copy per
+// kind and buffer the CTA's hot code left the instruction cache and ran at a tenth of its speed.
+template <int HD>
 __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint8_t* tiles, Walk walk) {
   constexpr int SPT = HD / 32, CHUNKS = HD / 16;
   constexpr uint32_t kStageBytes = kTile * HD * 2;
+  const bool values = threadIdx.x >= (kSoftmaxWarps + 4) * 32;
   const int t = (threadIdx.x - kSoftmaxWarps * 32) & 127;
   const int chunk = t % CHUNKS, sub = (t / CHUNKS) * SPT;  // tokens sub .. sub + SPT - 1 of a tile
-  // 16-byte pieces 2 chunk and 2 chunk + 1 of a token's row, in atoms of 64 channels; half of the
-  // lanes store the odd piece first so that 8 lanes fill 8 different 16-byte banks
+  // A token's 16 channels are the 16-byte pieces 2 chunk and 2 chunk + 1 of its row, in atoms of 64
+  // channels, piece j at j ^ (token % 8). Half of the lanes take their tokens in the order 1, 0, 3,
+  // 2, ..: then 8 lanes' stores fill the 8 different 16-byte banks.
   const int swap = HD == 64 ? (t / CHUNKS) & 1 : (chunk >> 2) & 1;
-  const int8_t* codes = VALUES ? a.v_codes : a.k_codes;
-  const uint16_t* scale = VALUES ? a.v_scale : a.k_scale;
-  uint64_t* full = VALUES ? ctl.bar.v_full : ctl.bar.k_full;
-  uint64_t* empty = VALUES ? ctl.bar.v_empty : ctl.bar.k_empty;
-  uint32_t it = 0;
-  Segment seg;
+  const int8_t* codes = values ? a.v_codes : a.k_codes;
+  const uint16_t* scale = values ? a.v_scale : a.k_scale;
+  uint64_t* full = values ? ctl.bar.v_full : ctl.bar.k_full;
+  uint64_t* empty = values ? ctl.bar.v_empty : ctl.bar.k_empty;
+  const uint32_t mine = smem_addr(tiles) + (values ? kStages * kStageBytes : 0) + (chunk >> 2) * (kTile * 128) +
+                        ((sub ^ swap) << 7 | (((chunk & 3) * 2) ^ ((sub ^ swap) & 7)) << 4);
+  const uint32_t select[2] = {swap ? 0x3232u : 0x1010u, swap ? 0x1010u : 0x3232u};
   // the loads run two tiles ahead of the stores, page numbers one further, across units
   Walk ahead = walk;
   Segment aseg;
@@ -275,80 +314,84 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
     atile = aseg.t0;
     atotal = aseg.r.length + aseg.r.count;
   }
-  auto page_of = [&](const Segment& s, int tile, int total) {
-    const int token = tile * kTile + sub;
-    if (token >= total) return 0;
-    const int page = __ldg(a.table + static_cast<int64_t>(s.b) * a.width + (token >> a.shift));
+  auto page_of = [&]() {
+    const int token = atile * kTile + sub;
+    if (!amore || token >= atotal) return 0;
+    const int page = __ldg(a.table + static_cast<int64_t>(aseg.b) * a.width + (token >> a.shift));
     if (page < 0 || page >= a.pages) {
       *a.status = QK_ERR_INVALID_ARGUMENT;
       return 0;
     }
     return page;
   };
-  int page = amore ? page_of(aseg, atile, atotal) : 0;
-  Share<HD> buf[2];
-  auto fetch = [&](Share<HD>& s) {
-    if (!amore) return;
-    load_share<HD>(a, codes, scale, aseg.head, page, atile * kTile + sub, atotal, chunk, s);
-    if (++atile == aseg.t1) {
-      amore = ahead.next(a, aseg);
-      if (amore) {
-        atile = aseg.t0;
-        atotal = aseg.r.length + aseg.r.count;
+  int page = page_of();
+  Share<HD> cur, next;
+  Segment seg;
+  int tile = 0;
+  seg.t1 = 0;
+  uint32_t it = 0;
+  bool primed = false;
+  for (;;) {
+    cur = next;
+    if (amore) {
+      load_share<HD>(a, codes, scale, aseg.head, page, atile * kTile + sub, atotal, chunk, swap, next);
+      if (++atile == aseg.t1) {
+        amore = ahead.next(a, aseg);
+        if (amore) {
+          atile = aseg.t0;
+          atotal = aseg.r.length + aseg.r.count;
+        }
+      }
+      page = page_of();
+    }
+    if (!primed) {
+      primed = true;
+      continue;
+    }
+    if (tile == seg.t1) {
+      if (!walk.next(a, seg)) return true;
+      tile = seg.t0;
+    }
+    const int token0 = tile * kTile + sub;
+    if (tile * kTile + kTile > seg.r.length) {  // drafts, or past the end
+      const int total = seg.r.length + seg.r.count;
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) {
+        const int token = token0 + i;
+        const uint32_t mask = i & 1 ? 0xffff0000u : 0xffffu;
+        const uint32_t bits = cur.scales[i / 2] >> (16 * (i & 1)) & 0x7fffu;
+        if (token >= total) {
+          cur.scales[i / 2] &= ~mask;
+        } else if (values && token >= seg.r.length && bits >= kHugeScale) {
+          // a draft's value that is not finite must not reach the rows that do not see it (0 * inf):
+          // zero here, NaN at the end for those that do
+          atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][chunk / 2]),
+                   1ull << (token - seg.r.length));
+          cur.scales[i / 2] &= ~mask;
+        }
       }
     }
-    if (amore) page = page_of(aseg, atile, atotal);
-  };
-  fetch(buf[0]);
-  fetch(buf[1]);
-  auto store = [&](const Share<HD>& s, const Segment& seg, int tile) {
     const uint32_t stage = it % kStages;
     if (!warp_wait(&empty[stage], ((it / kStages) & 1) ^ 1)) return false;
-    uint8_t* base = tiles + stage * kStageBytes + (chunk >> 2) * (kTile * 128);
-    const int total = seg.r.length + seg.r.count;
+    const uint32_t base = mine + stage * kStageBytes;
 #pragma unroll
     for (int i = 0; i < SPT; ++i) {
-      const int token = tile * kTile + sub + i;
-      uint32_t bits = token < total ? s.scales[i] : 0;
-      if (VALUES && token >= seg.r.length && (bits & 0x7fffu) >= kHugeScale) {
-        // a draft's value that is not finite must not reach the rows that do not see it (0 * inf):
-        // zero here, NaN at the end for those that do
-        atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][chunk / 2]),
-                 1ull << (token - seg.r.length));
-        bits = 0;
-      }
-      const uint32_t two = bits | (bits << 16);
+      const uint32_t two = __byte_perm(cur.scales[i / 2], 0, select[i & 1]);
       const __nv_bfloat162 scale2 = *reinterpret_cast<const __nv_bfloat162*>(&two);
       uint4 piece[2];
-      decode4(s.codes[i].x, scale2, piece[0].x, piece[0].y);
-      decode4(s.codes[i].y, scale2, piece[0].z, piece[0].w);
-      decode4(s.codes[i].z, scale2, piece[1].x, piece[1].y);
-      decode4(s.codes[i].w, scale2, piece[1].z, piece[1].w);
-      const int row = sub + i;
-      const int first = ((chunk & 3) * 2 + swap) ^ (row & 7);
-      uint8_t* to = base + row * 128;
-      *reinterpret_cast<uint4*>(to + first * 16) = swap ? piece[1] : piece[0];
-      *reinterpret_cast<uint4*>(to + (first ^ 1) * 16) = swap ? piece[0] : piece[1];
+      decode4(cur.codes[i].x, scale2, piece[0].x, piece[0].y);
+      decode4(cur.codes[i].y, scale2, piece[0].z, piece[0].w);
+      decode4(cur.codes[i].z, scale2, piece[1].x, piece[1].y);
+      decode4(cur.codes[i].w, scale2, piece[1].z, piece[1].w);
+      const uint32_t to = base ^ (i << 7 | i << 4);
+      sts_v4(to, piece[0]);
+      sts_v4(to ^ 16, piece[1]);
     }
     fence_proxy_async_smem();
     mbar_arrive(&full[stage]);
     ++it;
-    return true;
-  };
-  int which = 0;
-  while (walk.next(a, seg)) {
-    for (int tile = seg.t0; tile < seg.t1; ++tile) {
-      if (which == 0) {
-        if (!store(buf[0], seg, tile)) return false;
-        fetch(buf[0]);
-      } else {
-        if (!store(buf[1], seg, tile)) return false;
-        fetch(buf[1]);
-      }
-      which ^= 1;
-    }
+    ++tile;
   }
-  return true;
 }
 
 // ---- MMA warp -----------------------------------------------------------------------------
@@ -517,6 +560,12 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, Wa
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];
+        uint4 gate[4];
+        if (a.gate && live) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) gate[j] = ld_nc_v4(a.gate + at + c * 32 + j * 8);
+        }
+        __syncwarp();
         tmem_ld32(tm + kColO + c * 32, o);
         tmem_wait_ld();
         const bool poisoned = bad[c] & path;
@@ -528,9 +577,9 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, Wa
           for (int k = 0; k < 8; ++k) f[k] = poisoned ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[j * 8 + k]) * inv;
           if (a.gate) {
             float z[8];
-            unpack8(ld_nc_v4(a.gate + at + c * 32 + j * 8), z);
+            unpack8(gate[j], z);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] *= sigmoid_ref(z[k]);
+            for (int k = 0; k < 8; ++k) f[k] *= sigmoid_fast(z[k]);
           }
           uint32_t w[4];
 #pragma unroll
@@ -540,7 +589,7 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, Wa
         __syncwarp();
       }
     } else {
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg.index ? 1 : 0);
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg.first ? 0 : 1);
       float* part = a.part + slot * HD * a.part_rows + warp * 32 + lane;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
@@ -594,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
   pdl_wait();
   pdl_trigger();
   const int me = blockIdx.x;
-  const Located at = locate<kThreads>(
+  const Located at = locate(
       a, &ctl.located, ctl.warps,
       [&](int64_t total) {
         const int n = ranges(total, gridDim.x);
@@ -603,8 +652,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
       me == 0);
   tc_fence_after();
   const int n = ranges(at.total, gridDim.x);
-  Walk walk{at.b, 0, at.offset, 0};
+  Walk walk{at.b, 0, at.offset, 0, true};
   if (me < n) walk.left = range_start(at.total, n, me + 1) - range_start(at.total, n, me);
+
+  if (threadIdx.x == 0) {
+    Cut cut{0, 0, 0, 0, 0, 0};
+    if (me > 0 && me < n) {
+      const Request r = load_request(a, at.b);
+      const int unit = static_cast<int>(at.offset / r.steps()), t = static_cast<int>(at.offset % r.steps());
+      const int64_t unit0 = range_start(at.total, n, me) - t;
+      const int c0 = range_owner(at.total, n, unit0), c1 = range_owner(at.total, n, unit0 + r.tiles - 1);
+      if (t > 0 && t < r.tiles && c0 == me - 1)
+        cut = Cut{at.b, unit / r.row_tiles, unit % r.row_tiles, r.count, c1 - c0 + 1,
+                  2 * c0 + (range_start(at.total, n, c0) == unit0 ? 0 : 1)};
+    }
+    a.cuts[me] = cut;
+  }
 
   // rows of nodes that are not there
   if (a.counts) {
@@ -618,8 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
 
   bool ok = true;
   if (warp < kSoftmaxWarps) ok = softmax_role<HD>(a, ctl, walk);
-  else if (warp < kSoftmaxWarps + 4) ok = decode_role<HD, false>(a, ctl, tiles, walk);
-  else if (warp < kMmaWarp) ok = decode_role<HD, true>(a, ctl, tiles + kStages * kStageBytes, walk);
+  else if (warp < kMmaWarp) ok = decode_role<HD>(a, ctl, tiles, walk);
   else if (lane == 0) ok = mma_role<HD>(a, ctl, tiles, tiles + kStages * kStageBytes, walk);
   if (!ok) *a.status = QK_ERR_TIMEOUT;
   tc_fence_before();
@@ -632,84 +694,110 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
 
 // ---- joining the partials of a cut unit ------------------------------------------------------
 
-// Block (c, piece): if range c begins inside a unit and is the first to do so, the unit's rows
-// 32 r .. and channels 16 g .. of that piece: the parts' maxima give their weights, 4 groups of
-// warps add every fourth part (8 channels per thread in flight), shared memory adds the groups
-// in order.
-constexpr int kJoinThreads = 256, kJoinCols = 16;
+// Pieces of the cut units (32 rows x 16 channels each) in turn over the blocks. A unit can have as
+// many parts as there are ranges, so nothing walks them one by one: 8 warps each take every eighth
+// part's statistics (a lane per row) for the common maximum and the weights, then 4 pairs of warps
+// add every fourth part's channels (8 per thread) and shared memory adds the groups in a fixed order.
+constexpr int kJoinThreads = 256, kJoinCols = 16, kMaxRanges = 256;
 
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(TreeArgs a, int ctas) {
-  __shared__ Located located;
-  __shared__ int64_t warps[kJoinThreads / 32];
+  __shared__ int used[kMaxRanges], warps[kJoinThreads / 32];
+  __shared__ float weight[kMaxRanges][32];
+  __shared__ float red[2][8][32];
   __shared__ float acc[4][kJoinCols][33];
+  static_assert(kMaxRanges == kJoinThreads, "a thread per range");
   pdl_wait();
   pdl_trigger();
-  const int me = blockIdx.x + 1;
-  const Located at = locate<kJoinThreads>(
-      a, &located, warps,
-      [&](int64_t total) {
-        const int n = ranges(total, ctas);
-        return me < n ? range_start(total, n, me) : total;
-      },
-      false);
-  const int n = ranges(at.total, ctas);
-  if (me >= n) return;
-  const Request r = load_request(a, at.b);
-  const int unit = static_cast<int>(at.offset / r.tiles), t = static_cast<int>(at.offset % r.tiles);
-  if (t == 0) return;
-  const int64_t start = range_start(at.total, n, me), unit0 = start - t;
-  const int c0 = range_owner(at.total, n, unit0);
-  if (c0 != me - 1) return;
-  const int c1 = range_owner(at.total, n, unit0 + r.tiles - 1);
-  const int head = unit / r.row_tiles, row0 = (unit % r.row_tiles) * kRows;
-  const int group = blockIdx.y % (a.part_rows / 32), col0 = blockIdx.y / (a.part_rows / 32) * kJoinCols;
-  if (row0 + group * 32 >= r.count * a.rep) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = warp & 1, quarter = warp >> 1;
-  const int pr = a.part_rows, in_tile = group * 32 + lane;
-  // the first part is the second record of its CTA unless the CTA's range begins with the unit
-  const bool begins = range_start(at.total, n, c0) == unit0;
-  auto slot = [&](int c) { return 2 * static_cast<int64_t>(c) + (c == c0 && !begins ? 1 : 0); };
-  float m = -INFINITY;
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, a.stats[slot(c) * 2 * pr + in_tile]);
-  const float shift = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int c = c0; c <= c1; ++c) {
-    const float* st = a.stats + slot(c) * 2 * pr + in_tile;
-    const float w = exp2_fast(st[0] - shift);
-    l = fmaf(st[pr], w, l);
-    if ((c - c0) % 4 != quarter) continue;
-    const float* part = a.part + (slot(c) * HD + col0 + half * 8) * pr + in_tile;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = fmaf(part[j * pr], w, o[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc[quarter][half * 8 + j][lane] = o[j];
+  Cut mine{0, 0, 0, 0, 0, 0};
+  if (threadIdx.x < ctas) mine = a.cuts[threadIdx.x];
+  // the cut units in the order of their ranges, the same in every block
+  const uint32_t ballot = __ballot_sync(0xffffffffu, mine.parts > 0);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = __popc(ballot);
   __syncthreads();
-  if (quarter) return;
-  const int row = row0 + in_tile, node = row / a.rep;
-  if (node >= r.count) return;
-  const int64_t to = ((static_cast<int64_t>(at.b) * a.N + node) * a.hq + head * a.rep + row % a.rep) * HD + col0 + half * 8;
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  float f[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = half * 8 + j;
-    f[j] = ((acc[0][c][lane] + acc[1][c][lane]) + (acc[2][c][lane] + acc[3][c][lane])) * inv;
+  int found = 0, at = __popc(ballot & ((1u << (threadIdx.x & 31)) - 1));
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    if (w < threadIdx.x >> 5) at += warps[w];
+    found += warps[w];
   }
-  if (a.gate) {
-    float z[8];
-    unpack8(ld_nc_v4(a.gate + to), z);
+  if (mine.parts) used[at] = threadIdx.x;
+  __syncthreads();
+  const int groups = a.part_rows / 32, pieces = groups * (HD / kJoinCols);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = warp & 1, quarter = warp >> 1;
+  const int pr = a.part_rows;
+  for (int p = blockIdx.x; p < found * pieces; p += gridDim.x) {
+    const Cut cut = a.cuts[used[p / pieces]];
+    const int group = p % pieces % groups, col0 = p % pieces / groups * kJoinCols;
+    const int in_tile = group * 32 + lane, row = cut.row_tile * kRows + in_tile;
+    if (row - lane >= cut.count * a.rep) continue;
+    // the first part may be the second record of its range, the others are the first of theirs
+    auto slot = [&](int i) { return static_cast<int64_t>(i ? (cut.record & ~1) + 2 * i : cut.record); };
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int i = warp; i < cut.parts; i += 8) {
+      const float x = a.stats[slot(i) * 2 * pr + in_tile];
+      weight[i][lane] = x;
+      m = fmaxf(m, x);
+    }
+    red[0][warp][lane] = m;
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= sigmoid_ref(z[j]);
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, red[0][w][lane]);
+    const float shift = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < cut.parts; i += 8) {
+      const float w = exp2_fast(weight[i][lane] - shift);
+      weight[i][lane] = w;
+      l = fmaf(a.stats[slot(i) * 2 * pr + pr + in_tile], w, l);
+    }
+    red[1][warp][lane] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) l += red[1][w][lane];
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = quarter; i < cut.parts; i += 4) {
+      const float w = weight[i][lane];
+      const float* part = a.part + (slot(i) * HD + col0 + half * 8) * pr + in_tile;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = fmaf(part[j * pr], w, o[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[quarter][half * 8 + j][lane] = o[j];
+    __syncthreads();
+    const int node = row / a.rep;
+    if (quarter == 0 && node < cut.count) {
+      const int64_t to =
+          ((static_cast<int64_t>(cut.b) * a.N + node) * a.hq + cut.head * a.rep + row % a.rep) * HD + col0 + half * 8;
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = half * 8 + j;
+        f[j] = ((acc[0][k][lane] + acc[1][k][lane]) + (acc[2][k][lane] + acc[3][k][lane])) * inv;
+      }
+      if (a.gate) {
+        float z[8];
+        unpack8(ld_nc_v4(a.gate + to), z);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= sigmoid_fast(z[j]);
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+      *reinterpret_cast<uint4*>(a.out + to) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncthreads();  // weight, red and acc are free again
   }
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
-  *reinterpret_cast<uint4*>(a.out + to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-constexpr size_t kHeader = 256;
+constexpr size_t kHeader = 256 + kMaxRanges * sizeof(Cut);
+static_assert(kHeader % 256 == 0, "the partials begin aligned");
+
+// One CTA per SM: each holds all of its SM's tensor memory.
+int tree_ctas() { return sm_count() < kMaxRanges ? sm_count() : kMaxRanges; }
 
 int part_rows(int N, int rep) {
   const int rows = (N * rep + 31) / 32 * 32;
@@ -721,12 +809,11 @@ int launch(const TreeArgs& a, cudaStream_t st) {
   const size_t smem = 1024 + 2 * kStages * static_cast<size_t>(kTile) * HD * 2;
   const int rc = allow_smem(reinterpret_cast<const void*>(tree_attention_kernel<HD>), smem);
   if (rc) return rc;
-  const int ctas = sm_count();
+  const int ctas = tree_ctas();
   cudaError_t e = launch_dependent(tree_attention_kernel<HD>, dim3(ctas), dim3(kThreads), smem, st, a);
   if (e != cudaSuccess) return cuda_error(e, "tree_attention_kernel");
   if (ctas > 1) {
-    e = launch_dependent(tree_join_kernel<HD>, dim3(ctas - 1, a.part_rows / 32 * (HD / kJoinCols)), dim3(kJoinThreads), 0,
-                         st, a, ctas);
+    e = launch_dependent(tree_join_kernel<HD>, dim3(4 * ctas), dim3(kJoinThreads), 0, st, a, ctas);
     if (e != cudaSuccess) return cuda_error(e, "tree_join_kernel");
   }
   count_launch(2);
@@ -742,7 +829,7 @@ extern "C" {
 
 size_t qk_tree_attention_workspace_bytes(int B, int N, int hq, int kv_heads, int head_dim) {
   if (B <= 0 || N <= 0 || N > 64 || kv_heads <= 0 || hq <= 0 || hq % kv_heads || head_dim <= 0) return kHeader;
-  return kHeader + 2 * static_cast<size_t>(sm_count()) * part_rows(N, hq / kv_heads) * (head_dim + 2) * sizeof(float);
+  return kHeader + 2 * static_cast<size_t>(tree_ctas()) * part_rows(N, hq / kv_heads) * (head_dim + 2) * sizeof(float);
 }
 
 int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes, const int8_t* v_codes,
@@ -798,8 +885,9 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   a.T = T;
   a.out = out;
   a.status = static_cast<int*>(workspace);
+  a.cuts = reinterpret_cast<Cut*>(static_cast<uint8_t*>(workspace) + 256);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeader);
-  a.stats = a.part + 2 * static_cast<size_t>(sm_count()) * a.part_rows * head_dim;
+  a.stats = a.part + 2 * static_cast<size_t>(tree_ctas()) * a.part_rows * head_dim;
   return head_dim == 256   ? launch<256>(a, as_stream(stream))
          : head_dim == 128 ? launch<128>(a, as_stream(stream))
                            : launch<64>(a, as_stream(stream));
