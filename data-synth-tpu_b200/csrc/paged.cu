@@ -84,7 +84,6 @@ __device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* warps, int64
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a) {
   __shared__ int64_t warps[kPlanThreads / 32];
-  __shared__ int64_t sums[2];
   __shared__ uint64_t word[kTreeNodes];
   __shared__ int up[kTreeNodes];
   const int b = blockIdx.y, tid = threadIdx.x;

@@ -10,14 +10,15 @@
 // in tiles of 128: S = Q K^T and O += P V are M = 128 products over tiles of 64 tokens, so the
 // cache is read and decoded once for up to 128 rows. Work: (request, KV head, row tile) units
 // times their token tiles, laid end to end and cut into one equal range per SM; a unit cut by a
-// range's end leaves FP32 partials (O, maximum, sum) that a second kernel joins.
+// range's end has several parts. Each part leaves O, maximum and sum in FP32, and a second kernel
+// joins them, divides, gates and rounds.
 //
 // One CTA per SM, three kinds of warps joined by mbarriers (every wait bounded):
 //  * 4 softmax warps, a thread per row: Q to TMEM once per unit; then per tile S from TMEM, mask,
 //    running maximum and sum in FP32, P as BF16 back over S's columns. O (FP32, in TMEM) is rescaled
 //    only when a row's maximum grows by more than 2^8: P stays below 2^8, exact enough in FP32.
-//  * 8 decode warps (4 for K, 4 for V): 16-byte loads of codes straight to registers two tiles
-//    ahead, int8 -> BF16 with the group's scale (one rounding, as the cache's BF16 read has it),
+//  * 8 decode warps (4 for K, 4 for V): asynchronous copies of codes and scales two tiles ahead,
+//    int8 -> BF16 with the group's scale (one rounding, as the cache's BF16 read has it),
 //    stored as 128-byte swizzled tiles: K-major for K, and the same bytes read as an MN-major
 //    operand for V (no transposition).
 //  * 1 warp issues the MMAs: Q and P from TMEM, K and V from shared memory.
@@ -48,19 +49,19 @@ struct TreeArgs {
   const uint16_t* gate;
   float scale_log2;         // |scale| * log2(e), above zero
   uint32_t q_keep, q_flip;  // Q's bits & keep ^ flip: nothing for a scale of zero, the sign for a negative one
-  int B, N, hq, kv, rep, pages, pages_per_row, width, shift, part_rows;
+  int B, N, hq, kv, rep, pages, pages_per_row, width, shift, row_tiles, part_rows;
   int64_t T;
   uint16_t* out;
   int* status;
-  float* part;   // [2 * CTAs][HD][part_rows] unnormalised O
-  float* stats;  // [2 * CTAs][2][part_rows] maximum (log2) and sum
-  struct Cut* cuts;  // [CTAs]
+  float* part;          // [units + CTAs][HD][part_rows] unnormalised O
+  float* stats;         // [units + CTAs][2][part_rows] maximum (log2) and sum
+  struct Parts* parts;  // [units]
 };
 
-// What a range's CTA knows of the unit that its range begins inside of, where it is the first
-// to do so: the unit, its parts (consecutive ranges) and which record of the first range is its.
-struct Cut {
-  int b, head, row_tile, count, parts, record;
+// A unit's parts: the ranges first .. first + count - 1. The part of unit u in range c is record
+// u + c, which no two parts share: units and ranges both go up along the work.
+struct Parts {
+  int first, count;
 };
 
 struct Request {
@@ -147,13 +148,11 @@ __device__ __forceinline__ Located locate(const TreeArgs& a, Located* shared, in
 struct Segment {
   Request r;
   int b, head, row_tile, t0, t1, index;
-  bool first;  // the range begins with it
-  __device__ bool whole() const { return t0 == 0 && t1 == r.tiles; }
+  int64_t start;  // the unit's first step in the whole work
 };
 struct Walk {
   int b, index;
-  int64_t offset, left;
-  bool first;
+  int64_t offset, left, at;  // at: the next step in the whole work
   __device__ bool next(const TreeArgs& a, Segment& s) {
     while (left > 0) {
       for (;; ++b) {
@@ -169,11 +168,11 @@ struct Walk {
       s.row_tile = unit % s.r.row_tiles;
       s.t0 = static_cast<int>(offset % steps);
       const int end = static_cast<int>(min(static_cast<int64_t>(steps), s.t0 + left));
+      s.start = at - s.t0;
       left -= end - s.t0;
       offset += end - s.t0;
+      at += end - s.t0;
       s.t1 = min(end, s.r.tiles);
-      s.first = first;
-      first = false;
       if (s.t0 >= s.t1) continue;
       s.index = index++;
       return true;
@@ -209,16 +208,44 @@ __device__ __forceinline__ float sigmoid_fast(float x) {
   return y;
 }
 
-__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
+// Pairs of FP32 in one instruction, and a three-way maximum.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
 __device__ __forceinline__ void sts_v4(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds_v4_at(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_at(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 // Four int8 codes times a BF16 scale (in both halves of `scale2`) -> two BF16 pairs. A byte c
@@ -246,51 +273,30 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 
 // ---- decode warps -------------------------------------------------------------------------
 
-// A thread's share of a tile: 16 channels of SPT consecutive tokens (all in one page; codes[i] of
-// token i ^ swap), and their group's scales (token i in half i % 2 of word i / 2).
+// Raw codes and scales wait in shared memory, kRaw tiles ahead, each thread's own: 16-byte
+// asynchronous copies of its 16 channels of SPT consecutive tokens (all in one page; row i of token
+// i ^ swap), then its group's scales (token i in half i % 2 of word i / 2). Nobody else reads them,
+// so the thread's own copy groups are all the synchronisation they need.
+constexpr int kRaw = 2;
 template <int HD>
-struct Share {
-  static constexpr int SPT = HD / 32;
-  uint4 codes[SPT];
-  uint32_t scales[SPT / 2];
+struct Raw {
+  uint4 row[kRaw][HD / 32 + 1][kDecodeWarps * 32];
 };
 
-template <int HD>
-__device__ __forceinline__ void load_share(const TreeArgs& a, const int8_t* codes, const uint16_t* scale, int head,
-                                           int page, int token, int total, int chunk, int swap, Share<HD>& s) {
-  constexpr int SPT = HD / 32;
-  if (token >= total) {
-#pragma unroll
-    for (int i = 0; i < SPT; ++i) s.codes[i] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < SPT / 2; ++i) s.scales[i] = 0;
-    return;
-  }
-  const int row = page / a.pages_per_row;
-  const int64_t in_row = (static_cast<int64_t>(page - row * a.pages_per_row) << a.shift) + (token & ((1 << a.shift) - 1));
-  const int D = a.kv * HD, G = D / 32;
-  const int8_t* c = codes + (row * a.T + in_row) * D + head * HD + chunk * 16;
-  const uint16_t* p = scale + (static_cast<int64_t>(row) * G + head * (HD / 32) + chunk / 2) * a.T + in_row;
-  const int8_t *even = c + swap * D, *odd = c - swap * D;
-#pragma unroll
-  for (int i = 0; i < SPT; ++i) s.codes[i] = ld_stream_v4((i & 1 ? odd : even) + i * D);
-  if (SPT == 8) {
-    const uint4 v = ld_nc_v4(p);
-#pragma unroll
-    for (int i = 0; i < SPT / 2; ++i) s.scales[i] = word(v, i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < SPT / 2; ++i) s.scales[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-  }
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int SIZE>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(SIZE), "r"(bytes) : "memory");
 }
 
-// Both kinds of decode warps run one copy of this code (K or V by run-time values), and the
-// buffered tile moves to the front instead of the loop being unrolled over buffers: with a copy per
-// kind and buffer the CTA's hot code left the instruction cache and ran at a tenth of its speed.
+// Both kinds of decode warps run one copy of this code (K or V by run-time values): with a copy
+// each the CTA's hot code left the instruction cache.
 template <int HD>
-__device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint8_t* tiles, Walk walk) {
+__device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint8_t* tiles, Raw<HD>& raw, Walk walk) {
   constexpr int SPT = HD / 32, CHUNKS = HD / 16;
-  constexpr uint32_t kStageBytes = kTile * HD * 2;
+  constexpr uint32_t kStageBytes = kTile * HD * 2, kRawRow = kDecodeWarps * 32 * 16, kRawTile = (SPT + 1) * kRawRow;
   const bool values = threadIdx.x >= (kSoftmaxWarps + 4) * 32;
   const int t = (threadIdx.x - kSoftmaxWarps * 32) & 127;
   const int chunk = t % CHUNKS, sub = (t / CHUNKS) * SPT;  // tokens sub .. sub + SPT - 1 of a tile
@@ -305,7 +311,9 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
   const uint32_t mine = smem_addr(tiles) + (values ? kStages * kStageBytes : 0) + (chunk >> 2) * (kTile * 128) +
                         ((sub ^ swap) << 7 | (((chunk & 3) * 2) ^ ((sub ^ swap) & 7)) << 4);
   const uint32_t select[2] = {swap ? 0x3232u : 0x1010u, swap ? 0x1010u : 0x3232u};
-  // the loads run two tiles ahead of the stores, page numbers one further, across units
+  const uint32_t my_raw = smem_addr(&raw) + (threadIdx.x - kSoftmaxWarps * 32) * 16;
+  const int D = a.kv * HD, G = D / 32;
+  // the copies run kRaw tiles ahead of the stores, page numbers one further, across units
   Walk ahead = walk;
   Segment aseg;
   int atile = 0, atotal = 0;
@@ -316,25 +324,28 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
   }
   auto page_of = [&]() {
     const int token = atile * kTile + sub;
-    if (!amore || token >= atotal) return 0;
-    const int page = __ldg(a.table + static_cast<int64_t>(aseg.b) * a.width + (token >> a.shift));
-    if (page < 0 || page >= a.pages) {
-      *a.status = QK_ERR_INVALID_ARGUMENT;
-      return 0;
-    }
-    return page;
+    return amore && token < atotal ? __ldg(a.table + static_cast<int64_t>(aseg.b) * a.width + (token >> a.shift)) : 0;
   };
   int page = page_of();
-  Share<HD> cur, next;
-  Segment seg;
-  int tile = 0;
-  seg.t1 = 0;
-  uint32_t it = 0;
-  bool primed = false;
-  for (;;) {
-    cur = next;
+  auto copy = [&](uint32_t slot) {
     if (amore) {
-      load_share<HD>(a, codes, scale, aseg.head, page, atile * kTile + sub, atotal, chunk, swap, next);
+      const uint32_t to = my_raw + slot * kRawTile;
+      const int token = atile * kTile + sub;
+      const uint32_t live = token < atotal;
+      if (page < 0 || page >= a.pages) {  // reported, and read as page 0
+        *a.status = QK_ERR_INVALID_ARGUMENT;
+        page = 0;
+      }
+      const int row = a.pages == a.pages_per_row ? 0 : page / a.pages_per_row;
+      const int64_t in_row =
+          (static_cast<int64_t>(page - row * a.pages_per_row) << a.shift) + (live ? token & ((1 << a.shift) - 1) : 0);
+      const int8_t* c = codes + (row * a.T + in_row) * D + aseg.head * HD + chunk * 16;
+      const int8_t *even = c + swap * D, *odd = c - swap * D;
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) cp_async16_or_zero(to + i * kRawRow, (i & 1 ? odd : even) + i * D, live * 16);
+      const uint16_t* p = scale + (static_cast<int64_t>(row) * G + aseg.head * (HD / 32) + chunk / 2) * a.T + in_row;
+      if (SPT == 8) cp_async16_or_zero(to + SPT * kRawRow, p, live * 16);
+      else cp_async_small<SPT == 8 ? 4 : SPT * 2>(to + SPT * kRawRow, p, live * SPT * 2);
       if (++atile == aseg.t1) {
         amore = ahead.next(a, aseg);
         if (amore) {
@@ -344,54 +355,67 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
       }
       page = page_of();
     }
-    if (!primed) {
-      primed = true;
-      continue;
-    }
-    if (tile == seg.t1) {
-      if (!walk.next(a, seg)) return true;
-      tile = seg.t0;
-    }
-    const int token0 = tile * kTile + sub;
-    if (tile * kTile + kTile > seg.r.length) {  // drafts, or past the end
-      const int total = seg.r.length + seg.r.count;
+    cp_async_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < kRaw; ++i) copy(i);
+  Segment seg;
+  uint32_t it = 0;
+  while (walk.next(a, seg)) {
+#pragma unroll 1
+    for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
+      const uint32_t from = my_raw + (it % kRaw) * kRawTile;
+      cp_async_wait<kRaw - 1>();
+      uint32_t scales[4];
+      if (SPT == 8) {
+        const uint4 v = lds_v4_at(from + SPT * kRawRow);
 #pragma unroll
-      for (int i = 0; i < SPT; ++i) {
-        const int token = token0 + i;
-        const uint32_t mask = i & 1 ? 0xffff0000u : 0xffffu;
-        const uint32_t bits = cur.scales[i / 2] >> (16 * (i & 1)) & 0x7fffu;
-        if (token >= total) {
-          cur.scales[i / 2] &= ~mask;
-        } else if (values && token >= seg.r.length && bits >= kHugeScale) {
-          // a draft's value that is not finite must not reach the rows that do not see it (0 * inf):
-          // zero here, NaN at the end for those that do
-          atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][chunk / 2]),
-                   1ull << (token - seg.r.length));
-          cur.scales[i / 2] &= ~mask;
+        for (int i = 0; i < SPT / 2; ++i) scales[i] = word(v, i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < SPT / 2; ++i) scales[i] = lds_at(from + SPT * kRawRow + 4 * i);
+      }
+      if (tile * kTile + kTile > seg.r.length) {  // drafts, or past the end
+        const int total = seg.r.length + seg.r.count;
+#pragma unroll
+        for (int i = 0; i < SPT; ++i) {
+          const int token = tile * kTile + sub + i;
+          const uint32_t mask = i & 1 ? 0xffff0000u : 0xffffu;
+          const uint32_t bits = scales[i / 2] >> (16 * (i & 1)) & 0x7fffu;
+          if (token >= total) {
+            scales[i / 2] &= ~mask;
+          } else if (values && token >= seg.r.length && bits >= kHugeScale) {
+            // a draft's value that is not finite must not reach the rows that do not see it (0 * inf):
+            // zero here, NaN at the end for those that do
+            atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][chunk / 2]),
+                     1ull << (token - seg.r.length));
+            scales[i / 2] &= ~mask;
+          }
         }
       }
-    }
-    const uint32_t stage = it % kStages;
-    if (!warp_wait(&empty[stage], ((it / kStages) & 1) ^ 1)) return false;
-    const uint32_t base = mine + stage * kStageBytes;
+      const uint32_t stage = it % kStages;
+      if (!warp_wait(&empty[stage], ((it / kStages) & 1) ^ 1)) return false;
+      const uint32_t base = mine + stage * kStageBytes;
 #pragma unroll
-    for (int i = 0; i < SPT; ++i) {
-      const uint32_t two = __byte_perm(cur.scales[i / 2], 0, select[i & 1]);
-      const __nv_bfloat162 scale2 = *reinterpret_cast<const __nv_bfloat162*>(&two);
-      uint4 piece[2];
-      decode4(cur.codes[i].x, scale2, piece[0].x, piece[0].y);
-      decode4(cur.codes[i].y, scale2, piece[0].z, piece[0].w);
-      decode4(cur.codes[i].z, scale2, piece[1].x, piece[1].y);
-      decode4(cur.codes[i].w, scale2, piece[1].z, piece[1].w);
-      const uint32_t to = base ^ (i << 7 | i << 4);
-      sts_v4(to, piece[0]);
-      sts_v4(to ^ 16, piece[1]);
+      for (int i = 0; i < SPT; ++i) {
+        const uint4 code = lds_v4_at(from + i * kRawRow);
+        const uint32_t two = __byte_perm(scales[i / 2], 0, select[i & 1]);
+        const __nv_bfloat162 scale2 = *reinterpret_cast<const __nv_bfloat162*>(&two);
+        uint4 piece[2];
+        decode4(code.x, scale2, piece[0].x, piece[0].y);
+        decode4(code.y, scale2, piece[0].z, piece[0].w);
+        decode4(code.z, scale2, piece[1].x, piece[1].y);
+        decode4(code.w, scale2, piece[1].z, piece[1].w);
+        const uint32_t to = base ^ (i << 7 | i << 4);
+        sts_v4(to, piece[0]);
+        sts_v4(to ^ 16, piece[1]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&full[stage]);
+      copy(it % kRaw);
     }
-    fence_proxy_async_smem();
-    mbar_arrive(&full[stage]);
-    ++it;
-    ++tile;
   }
+  return true;
 }
 
 // ---- MMA warp -----------------------------------------------------------------------------
@@ -447,42 +471,70 @@ __device__ __forceinline__ bool mma_role(const TreeArgs& a, Control& ctl, uint8_
 
 // ---- softmax warps ------------------------------------------------------------------------
 
+// Q of a unit to TMEM. Rows pass through 4 KB of shared memory per warp (32 rows x 128 B, row r's
+// 16-byte piece j at j ^ (r % 8)): a thread owns a row in TMEM, but 8 threads read 128 B of a row from
+// global memory, which takes a quarter of the cache-line lookups of a thread per row.
 template <int HD>
-__device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, Walk walk) {
+__device__ __forceinline__ void load_q(const TreeArgs& a, const Segment& seg, uint32_t tm, uint32_t stage) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = seg.row_tile * kRows + warp * 32 + lane, node = row / a.rep;
+  const uint16_t* q = a.q + static_cast<int64_t>(seg.b) * a.N * a.q_stride + static_cast<int64_t>(seg.head) * a.rep * HD;
+  const int mine = node < seg.r.count ? node * static_cast<int>(a.q_stride) + (row - node * a.rep) * HD : -1;
+  int at[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) at[i] = __shfl_sync(0xffffffffu, mine, 4 * i + lane / 8);
+#pragma unroll 1
+  for (int c = 0; c < HD / 64; ++c) {
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = at[i] >= 0 ? ld_nc_v4(q + at[i] + c * 64 + lane % 8 * 8) : make_uint4(0, 0, 0, 0);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + lane / 8;
+      sts_v4(stage + r * 128 + ((lane ^ r) & 7) * 16, v[i]);
+    }
+    __syncwarp();
+    uint32_t u[32];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 x = lds_v4_at(stage + lane * 128 + ((i ^ lane) & 7) * 16);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) u[i * 4 + w] = (word(x, w) & a.q_keep) ^ a.q_flip;
+    }
+    tmem_st32(tm + kColQ + c * 32, u);
+  }
+  tmem_wait_st();
+}
+
+template <int HD>
+__device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, uint32_t stage, Walk walk, int64_t total,
+                                             int ctas) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(warp * 32) << 16);
-  Segment seg;
+  Segment seg, next;
   uint32_t it = 0;
-  while (walk.next(a, seg)) {
-    const int row = seg.row_tile * kRows + warp * 32 + lane;
-    const int node = row / a.rep, h = seg.head * a.rep + row % a.rep;
-    const bool live = node < seg.r.count;
-    const bool busy = seg.row_tile * kRows + warp * 32 < seg.r.count * a.rep;  // the same for the warp
-    const int64_t bn = static_cast<int64_t>(seg.b) * a.N + node;
-    uint64_t path = 0;
-    if (live) {
-      path = a.ancestors[bn];
-      if (seg.r.count < 64) path &= (1ull << seg.r.count) - 1;
-    }
-    if (busy) {
-      const uint4* q = reinterpret_cast<const uint4*>(a.q + bn * a.q_stride + static_cast<int64_t>(h) * HD);
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        uint32_t r[32];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint4 v = live ? ld_nc_v4(q + c * 8 + j) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) r[j * 4 + w] = (word(v, w) & a.q_keep) ^ a.q_flip;
-        }
-        tmem_st32(tm + kColQ + c * 32, r);
-      }
-      tmem_wait_st();
-    }
+  bool more = walk.next(a, next);
+  auto busy_of = [&](const Segment& s) { return s.row_tile * kRows + warp * 32 < s.r.count * a.rep; };
+  auto give_q = [&](const Segment& s) {
+    if (busy_of(s)) load_q<HD>(a, s, tm, stage);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl.bar.q_full);
-
+  };
+  if (more) give_q(next);
+  while (more) {
+    seg = next;
+    const int row = seg.row_tile * kRows + warp * 32 + lane;
+    const int node = row / a.rep;
+    const bool live = node < seg.r.count;
+    const bool busy = busy_of(seg);  // the same for the warp
+    uint64_t path = 0;
+    if (live) {
+      path = a.ancestors[static_cast<int64_t>(seg.b) * a.N + node];
+      if (seg.r.count < 64) path &= (1ull << seg.r.count) - 1;
+    }
     float m = -INFINITY, l = 0.f;
     for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
       if (!warp_wait(&ctl.bar.s_full[it & 1], (it / 2) & 1)) return false;
@@ -504,9 +556,13 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, Wa
           for (int j = 0; j < 64; ++j)
             if (!(see >> j & 1)) s[j / 32][j % 32] = 0xff800000u;
         }
-        float top = __uint_as_float(s[0][0]);
+        float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
-        for (int j = 1; j < 64; ++j) top = fmaxf(top, __uint_as_float(s[j / 32][j % 32]));
+        for (int j = 0; j < 64; j += 4) {
+          top = max3(top, __uint_as_float(s[j / 32][j % 32]), __uint_as_float(s[j / 32][j % 32 + 1]));
+          top2 = max3(top2, __uint_as_float(s[j / 32][j % 32 + 2]), __uint_as_float(s[j / 32][j % 32 + 3]));
+        }
+        top = fmaxf(top, top2);
         top *= a.scale_log2;
         const bool grow = top > m + kLazyGrowth;
         if (__any_sync(0xffffffffu, grow)) {
@@ -531,17 +587,22 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, Wa
           }
         }
         const float shift = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), shift2 = pair(-shift, -shift);
+        uint64_t sum[2] = {0, 0};
         uint32_t p[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          const float x = exp2_fast(fmaf(__uint_as_float(s[j / 16][(2 * j) % 32]), a.scale_log2, -shift));
-          const float y = exp2_fast(fmaf(__uint_as_float(s[j / 16][(2 * j + 1) % 32]), a.scale_log2, -shift));
-          sum[j & 1] += x;
-          sum[2 + (j & 1)] += y;
+          float x, y;
+          unpair(fma2(pair(__uint_as_float(s[j / 16][(2 * j) % 32]), __uint_as_float(s[j / 16][(2 * j + 1) % 32])), scale2,
+                      shift2), x, y);
+          x = exp2_fast(x);
+          y = exp2_fast(y);
+          sum[j & 1] = add2(sum[j & 1], pair(x, y));
           p[j] = pack_bf16x2(x, y);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float even, odd;
+        unpair(add2(sum[0], sum[1]), even, odd);
+        l += even + odd;
         tmem_st32(cols, p);
         tmem_wait_st();
         tc_fence_before();
@@ -550,61 +611,38 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, Wa
       if (lane == 0) mbar_arrive(&ctl.bar.p_full[it & 1]);
     }
 
+    // every product with this Q is done: the next unit's Q goes in and its first scores are on their
+    // way while this unit's O leaves
+    more = walk.next(a, next);
+    if (more) give_q(next);
     if (!warp_wait(&ctl.bar.o_full, seg.index & 1)) return false;
     if (!busy) continue;
     tc_fence_after();
+    // The unit's part of O as it is, FP32, channel by channel (32 rows are 128 B): the join divides,
+    // gates and rounds. A quarter of the instructions of doing that here, where nothing hides them.
     const uint64_t* bad = ctl.bad[seg.index % kBadRing];
-    if (seg.whole()) {
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      const int64_t at = (bn * a.hq + h) * HD;
+    const int unit = (seg.b * a.kv + seg.head) * a.row_tiles + seg.row_tile;
+    const int64_t record = static_cast<int64_t>(unit) + blockIdx.x;
+    float* part = a.part + record * HD * a.part_rows + warp * 32 + lane;
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        uint4 gate[4];
-        if (a.gate && live) {
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld32(tm + kColO + c * 32, o);
+      tmem_wait_ld();
+      if (bad[c] & path) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) gate[j] = ld_nc_v4(a.gate + at + c * 32 + j * 8);
-        }
-        __syncwarp();
-        tmem_ld32(tm + kColO + c * 32, o);
-        tmem_wait_ld();
-        const bool poisoned = bad[c] & path;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (!live) break;
-          float f[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) f[k] = poisoned ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[j * 8 + k]) * inv;
-          if (a.gate) {
-            float z[8];
-            unpack8(gate[j], z);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] *= sigmoid_fast(z[k]);
-          }
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2(f[2 * k], f[2 * k + 1]);
-          *reinterpret_cast<uint4*>(a.out + at + c * 32 + j * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        __syncwarp();
+        for (int j = 0; j < 32; ++j) o[j] = 0x7fc00000u;
       }
-    } else {
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg.first ? 0 : 1);
-      float* part = a.part + slot * HD * a.part_rows + warp * 32 + lane;
-#pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tm + kColO + c * 32, o);
-        tmem_wait_ld();
-        const bool poisoned = bad[c] & path;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          part[(c * 32 + j) * a.part_rows] = poisoned ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[j]);
-      }
-      float* stats = a.stats + slot * 2 * a.part_rows + warp * 32 + lane;
-      stats[0] = m;
-      stats[a.part_rows] = l;
+      for (int j = 0; j < 32; ++j) part[(c * 32 + j) * a.part_rows] = __uint_as_float(o[j]);
+      __syncwarp();
     }
+    float* stats = a.stats + record * 2 * a.part_rows + warp * 32 + lane;
+    stats[0] = m;
+    stats[a.part_rows] = l;
+    if (seg.t0 == 0 && threadIdx.x == 0)
+      a.parts[unit] = Parts{static_cast<int>(blockIdx.x), range_owner(total, ctas, seg.start + seg.r.tiles - 1) -
+                                                              static_cast<int>(blockIdx.x) + 1};
     tc_fence_before();
     if (seg.r.length < seg.t1 * kTile) {  // the unit saw drafts: its record of bad values is read, clear it
       asm volatile("bar.sync 1, %0;" ::"r"(32 * min(kSoftmaxWarps, (seg.r.count * a.rep - seg.row_tile * kRows + 31) / 32)) : "memory");
@@ -652,36 +690,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
       me == 0);
   tc_fence_after();
   const int n = ranges(at.total, gridDim.x);
-  Walk walk{at.b, 0, at.offset, 0, true};
-  if (me < n) walk.left = range_start(at.total, n, me + 1) - range_start(at.total, n, me);
-
-  if (threadIdx.x == 0) {
-    Cut cut{0, 0, 0, 0, 0, 0};
-    if (me > 0 && me < n) {
-      const Request r = load_request(a, at.b);
-      const int unit = static_cast<int>(at.offset / r.steps()), t = static_cast<int>(at.offset % r.steps());
-      const int64_t unit0 = range_start(at.total, n, me) - t;
-      const int c0 = range_owner(at.total, n, unit0), c1 = range_owner(at.total, n, unit0 + r.tiles - 1);
-      if (t > 0 && t < r.tiles && c0 == me - 1)
-        cut = Cut{at.b, unit / r.row_tiles, unit % r.row_tiles, r.count, c1 - c0 + 1,
-                  2 * c0 + (range_start(at.total, n, c0) == unit0 ? 0 : 1)};
-    }
-    a.cuts[me] = cut;
-  }
-
-  // rows of nodes that are not there
-  if (a.counts) {
-    const int64_t row16 = static_cast<int64_t>(a.hq) * HD / 8;
-    for (int64_t i = me; i < static_cast<int64_t>(a.B) * a.N; i += gridDim.x) {
-      if (static_cast<int>(i % a.N) < load_request(a, static_cast<int>(i / a.N)).count) continue;
-      for (int64_t j = threadIdx.x; j < row16; j += kThreads)
-        reinterpret_cast<uint4*>(a.out)[i * row16 + j] = make_uint4(0, 0, 0, 0);
-    }
+  Walk walk{at.b, 0, at.offset, 0, 0};
+  if (me < n) {
+    walk.at = range_start(at.total, n, me);
+    walk.left = range_start(at.total, n, me + 1) - walk.at;
   }
 
   bool ok = true;
-  if (warp < kSoftmaxWarps) ok = softmax_role<HD>(a, ctl, walk);
-  else if (warp < kMmaWarp) ok = decode_role<HD>(a, ctl, tiles, walk);
+  if (warp < kSoftmaxWarps) ok = softmax_role<HD>(a, ctl, smem_addr(tiles) + 2 * kStages * kStageBytes + sizeof(Raw<HD>) + warp * 4096, walk, at.total, n);
+  else if (warp < kMmaWarp) ok = decode_role<HD>(a, ctl, tiles, *reinterpret_cast<Raw<HD>*>(tiles + 2 * kStages * kStageBytes), walk);
   else if (lane == 0) ok = mma_role<HD>(a, ctl, tiles, tiles + kStages * kStageBytes, walk);
   if (!ok) *a.status = QK_ERR_TIMEOUT;
   tc_fence_before();
@@ -692,130 +709,146 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
   }
 }
 
-// ---- joining the partials of a cut unit ------------------------------------------------------
+// ---- joining a unit's parts ------------------------------------------------------------------
 
-// Pieces of the cut units (32 rows x 16 channels each) in turn over the blocks. A unit can have as
-// many parts as there are ranges, so nothing walks them one by one: 8 warps each take every eighth
-// part's statistics (a lane per row) for the common maximum and the weights, then 4 pairs of warps
-// add every fourth part's channels (8 per thread) and shared memory adds the groups in a fixed order.
-constexpr int kJoinThreads = 256, kJoinCols = 16, kMaxRanges = 256;
+// Every row of the output, also those of nodes that are not there, in pieces of 32 rows (a lane
+// each) x 16 channels. WARPS warps share a piece: 1 where there are enough pieces to fill the GPU, 8
+// where few units have many parts (a unit can have as many as there are ranges): each takes every
+// WARPS-th part, and shared memory adds them in a fixed order.
+constexpr int kJoinWarps = 8, kJoinCols = 16;
 
-template <int HD>
-__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(TreeArgs a, int ctas) {
-  __shared__ int used[kMaxRanges], warps[kJoinThreads / 32];
-  __shared__ float weight[kMaxRanges][32];
-  __shared__ float red[2][8][32];
-  __shared__ float acc[4][kJoinCols][33];
-  static_assert(kMaxRanges == kJoinThreads, "a thread per range");
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs a, int pieces) {
+  __shared__ float red[WARPS > 1 ? WARPS : 1][2][32];
+  __shared__ float acc[WARPS > 1 ? WARPS : 1][kJoinCols][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
   pdl_trigger();
-  Cut mine{0, 0, 0, 0, 0, 0};
-  if (threadIdx.x < ctas) mine = a.cuts[threadIdx.x];
-  // the cut units in the order of their ranges, the same in every block
-  const uint32_t ballot = __ballot_sync(0xffffffffu, mine.parts > 0);
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = __popc(ballot);
-  __syncthreads();
-  int found = 0, at = __popc(ballot & ((1u << (threadIdx.x & 31)) - 1));
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    if (w < threadIdx.x >> 5) at += warps[w];
-    found += warps[w];
+  const int p = WARPS > 1 ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
+  if (p >= pieces) return;
+  const int groups = a.part_rows / 32, pr = a.part_rows;
+  const int group = p % groups, col0 = p / groups % (HD / kJoinCols) * kJoinCols;
+  const int unit = p / groups / (HD / kJoinCols);
+  const int b = unit / (a.kv * a.row_tiles), head = unit / a.row_tiles % a.kv, row_tile = unit % a.row_tiles;
+  const int in_tile = group * 32 + lane, row = row_tile * kRows + in_tile, node = row / a.rep;
+  const int count = load_request(a, b).count;
+  const int64_t to =
+      ((static_cast<int64_t>(b) * a.N + node) * a.hq + head * a.rep + (row - node * a.rep)) * HD + col0;
+  uint4* out = reinterpret_cast<uint4*>(a.out + to);
+  if (row - lane >= count * a.rep) {  // nobody in these rows
+    if (warp % WARPS == 0 && node < a.N) out[0] = out[1] = make_uint4(0, 0, 0, 0);
+    return;
   }
-  if (mine.parts) used[at] = threadIdx.x;
-  __syncthreads();
-  const int groups = a.part_rows / 32, pieces = groups * (HD / kJoinCols);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = warp & 1, quarter = warp >> 1;
-  const int pr = a.part_rows;
-  for (int p = blockIdx.x; p < found * pieces; p += gridDim.x) {
-    const Cut cut = a.cuts[used[p / pieces]];
-    const int group = p % pieces % groups, col0 = p % pieces / groups * kJoinCols;
-    const int in_tile = group * 32 + lane, row = cut.row_tile * kRows + in_tile;
-    if (row - lane >= cut.count * a.rep) continue;
-    // the first part may be the second record of its range, the others are the first of theirs
-    auto slot = [&](int i) { return static_cast<int64_t>(i ? (cut.record & ~1) + 2 * i : cut.record); };
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int i = warp; i < cut.parts; i += 8) {
-      const float x = a.stats[slot(i) * 2 * pr + in_tile];
-      weight[i][lane] = x;
-      m = fmaxf(m, x);
-    }
-    red[0][warp][lane] = m;
-    __syncthreads();
+  uint4 gate[2];
+  if (a.gate && node < count) {
+    gate[0] = ld_nc_v4(a.gate + to);
+    gate[1] = ld_nc_v4(a.gate + to + 8);
+  }
+  const Parts parts = a.parts[unit];
+  const int64_t record = static_cast<int64_t>(unit) + parts.first;
+  const int first = WARPS > 1 ? warp : 0;
+  // one pass with a running maximum, as over tiles
+  float m = -INFINITY, l = 0.f, o[kJoinCols];
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, red[0][w][lane]);
-    const float shift = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < cut.parts; i += 8) {
-      const float w = exp2_fast(weight[i][lane] - shift);
-      weight[i][lane] = w;
-      l = fmaf(a.stats[slot(i) * 2 * pr + pr + in_tile], w, l);
-    }
-    red[1][warp][lane] = l;
+  for (int j = 0; j < kJoinCols; ++j) o[j] = 0.f;
+#pragma unroll 2
+  for (int i = first; i < parts.count; i += WARPS) {
+    const float* st = a.stats + (record + i) * 2 * pr + in_tile;
+    const float* part = a.part + ((record + i) * HD + col0) * pr + in_tile;
+    const float x = st[0], y = st[pr];
+    float v[kJoinCols];
+#pragma unroll
+    for (int j = 0; j < kJoinCols; ++j) v[j] = part[j * pr];
+    const float top = fmaxf(m, x), shift = top == -INFINITY ? 0.f : top;
+    const float keep = exp2_fast(m - shift), w = exp2_fast(x - shift);
+    m = top;
+    l = fmaf(l, keep, y * w);
+#pragma unroll
+    for (int j = 0; j < kJoinCols; ++j) o[j] = fmaf(o[j], keep, v[j] * w);
+  }
+  if (WARPS > 1) {
+    red[warp][0][lane] = m;
+    red[warp][1][lane] = l;
+#pragma unroll
+    for (int j = 0; j < kJoinCols; ++j) acc[warp][j][lane] = o[j];
     __syncthreads();
+    if (warp) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red[w][0][lane]);
+    const float shift = top == -INFINITY ? 0.f : top;
     l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) l += red[1][w][lane];
-    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = quarter; i < cut.parts; i += 4) {
-      const float w = weight[i][lane];
-      const float* part = a.part + (slot(i) * HD + col0 + half * 8) * pr + in_tile;
+    for (int j = 0; j < kJoinCols; ++j) o[j] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = fmaf(part[j * pr], w, o[j]);
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = exp2_fast(red[w][0][lane] - shift);
+      l = fmaf(red[w][1][lane], f, l);
+#pragma unroll
+      for (int j = 0; j < kJoinCols; ++j) o[j] = fmaf(acc[w][j][lane], f, o[j]);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[quarter][half * 8 + j][lane] = o[j];
-    __syncthreads();
-    const int node = row / a.rep;
-    if (quarter == 0 && node < cut.count) {
-      const int64_t to =
-          ((static_cast<int64_t>(cut.b) * a.N + node) * a.hq + cut.head * a.rep + row % a.rep) * HD + col0 + half * 8;
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int k = half * 8 + j;
-        f[j] = ((acc[0][k][lane] + acc[1][k][lane]) + (acc[2][k][lane] + acc[3][k][lane])) * inv;
-      }
-      if (a.gate) {
-        float z[8];
-        unpack8(ld_nc_v4(a.gate + to), z);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= sigmoid_fast(z[j]);
-      }
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
-      *reinterpret_cast<uint4*>(a.out + to) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __syncthreads();  // weight, red and acc are free again
   }
+  if (node >= a.N) return;
+  const float inv = node < count && (l > 0.f || l != l) ? 1.f / l : 0.f;
+  uint32_t w[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float f[8], z[8];
+    unpack8(gate[h], z);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] = inv == 0.f ? 0.f : o[h * 8 + j] * inv;
+      if (a.gate) f[j] *= node < count ? sigmoid_fast(z[j]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[h * 4 + j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+  }
+  out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  out[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-constexpr size_t kHeader = 256 + kMaxRanges * sizeof(Cut);
-static_assert(kHeader % 256 == 0, "the partials begin aligned");
-
-// One CTA per SM: each holds all of its SM's tensor memory.
-int tree_ctas() { return sm_count() < kMaxRanges ? sm_count() : kMaxRanges; }
+constexpr size_t kHeader = 256;
 
 int part_rows(int N, int rep) {
   const int rows = (N * rep + 31) / 32 * 32;
   return rows < kRows ? rows : kRows;
 }
 
+struct Layout {
+  int row_tiles, part_rows;
+  int64_t units, records;
+  size_t parts, part, stats, bytes;
+};
+Layout layout_of(int B, int N, int hq, int kv, int hd) {
+  Layout w;
+  const int rep = hq / kv;
+  w.row_tiles = (N * rep + kRows - 1) / kRows;
+  w.part_rows = part_rows(N, rep);
+  w.units = static_cast<int64_t>(B) * kv * w.row_tiles;
+  w.records = w.units + sm_count();
+  w.parts = kHeader;
+  w.stats = w.parts + (w.units * sizeof(Parts) + 255) / 256 * 256;
+  w.part = w.stats + static_cast<size_t>(w.records) * 2 * w.part_rows * sizeof(float);
+  w.bytes = w.part + static_cast<size_t>(w.records) * hd * w.part_rows * sizeof(float);
+  return w;
+}
+
 template <int HD>
-int launch(const TreeArgs& a, cudaStream_t st) {
-  const size_t smem = 1024 + 2 * kStages * static_cast<size_t>(kTile) * HD * 2;
+int launch(const TreeArgs& a, const Layout& w, cudaStream_t st) {
+  const size_t smem = 1024 + 2 * kStages * static_cast<size_t>(kTile) * HD * 2 + sizeof(Raw<HD>) + kSoftmaxWarps * 4096;
   const int rc = allow_smem(reinterpret_cast<const void*>(tree_attention_kernel<HD>), smem);
   if (rc) return rc;
-  const int ctas = tree_ctas();
-  cudaError_t e = launch_dependent(tree_attention_kernel<HD>, dim3(ctas), dim3(kThreads), smem, st, a);
+  // one CTA per SM: each holds all of its SM's tensor memory
+  cudaError_t e = launch_dependent(tree_attention_kernel<HD>, dim3(sm_count()), dim3(kThreads), smem, st, a);
   if (e != cudaSuccess) return cuda_error(e, "tree_attention_kernel");
-  if (ctas > 1) {
-    e = launch_dependent(tree_join_kernel<HD>, dim3(4 * ctas), dim3(kJoinThreads), 0, st, a, ctas);
-    if (e != cudaSuccess) return cuda_error(e, "tree_join_kernel");
+  const int pieces = static_cast<int>(w.units * (w.part_rows / 32) * (HD / kJoinCols));
+  if (pieces >= 16 * sm_count()) {
+    e = launch_dependent(tree_join_kernel<HD, 1>, dim3((pieces + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, st,
+                         a, pieces);
+  } else {
+    e = launch_dependent(tree_join_kernel<HD, kJoinWarps>, dim3(pieces), dim3(kJoinWarps * 32), 0, st, a, pieces);
   }
+  if (e != cudaSuccess) return cuda_error(e, "tree_join_kernel");
   count_launch(2);
   return QK_OK;
 }
@@ -829,7 +862,7 @@ extern "C" {
 
 size_t qk_tree_attention_workspace_bytes(int B, int N, int hq, int kv_heads, int head_dim) {
   if (B <= 0 || N <= 0 || N > 64 || kv_heads <= 0 || hq <= 0 || hq % kv_heads || head_dim <= 0) return kHeader;
-  return kHeader + 2 * static_cast<size_t>(tree_ctas()) * part_rows(N, hq / kv_heads) * (head_dim + 2) * sizeof(float);
+  return layout_of(B, N, hq, kv_heads, head_dim).bytes;
 }
 
 int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes, const int8_t* v_codes,
@@ -853,7 +886,10 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
              "q, gate, out and the cache must be 16-byte aligned");
   QK_REQUIRE(q_stride >= static_cast<int64_t>(hq) * head_dim && q_stride % 8 == 0,
              "tokens of q must be a multiple of 8 values apart and not overlap");
-  const size_t need = qk_tree_attention_workspace_bytes(B, N, hq, kv_heads, head_dim);
+  QK_REQUIRE(static_cast<int64_t>(N) * q_stride < (1ll << 31), "a request's queries must span fewer than 2^31 values");
+  const Layout w = layout_of(B, N, hq, kv_heads, head_dim);
+  QK_REQUIRE(w.units * (w.part_rows / 32) * (head_dim / kJoinCols) < (1ll << 31), "too many rows in one call");
+  const size_t need = w.bytes;
   if (!workspace || workspace_bytes < need)
     return set_error(QK_ERR_WORKSPACE, "tree attention workspace needs %zu bytes, got %zu", need, workspace_bytes);
   QK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "workspace must be 256-byte aligned");
@@ -881,16 +917,18 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   a.pages_per_row = static_cast<int>(T / page_size);
   a.width = width;
   while ((1 << a.shift) < page_size) ++a.shift;
-  a.part_rows = part_rows(N, a.rep);
+  a.row_tiles = w.row_tiles;
+  a.part_rows = w.part_rows;
   a.T = T;
   a.out = out;
-  a.status = static_cast<int*>(workspace);
-  a.cuts = reinterpret_cast<Cut*>(static_cast<uint8_t*>(workspace) + 256);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeader);
-  a.stats = a.part + 2 * static_cast<size_t>(tree_ctas()) * a.part_rows * head_dim;
-  return head_dim == 256   ? launch<256>(a, as_stream(stream))
-         : head_dim == 128 ? launch<128>(a, as_stream(stream))
-                           : launch<64>(a, as_stream(stream));
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.status = reinterpret_cast<int*>(ws);
+  a.parts = reinterpret_cast<Parts*>(ws + w.parts);
+  a.part = reinterpret_cast<float*>(ws + w.part);
+  a.stats = reinterpret_cast<float*>(ws + w.stats);
+  return head_dim == 256   ? launch<256>(a, w, as_stream(stream))
+         : head_dim == 128 ? launch<128>(a, w, as_stream(stream))
+                           : launch<64>(a, w, as_stream(stream));
 }
 
 int qk_tree_attention_check(const void* workspace, qk_stream_t stream) {
