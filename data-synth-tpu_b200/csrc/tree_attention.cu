@@ -17,12 +17,14 @@
 //  * 4 softmax warps, a thread per row: Q to TMEM once per unit; then per tile S from TMEM, mask,
 //    running maximum and sum in FP32, P as BF16 back over S's columns. O (FP32, in TMEM) is rescaled
 //    only when a row's maximum grows by more than 2^8: P stays below 2^8, exact enough in FP32.
-//  * 8 decode warps (4 for K, 4 for V): asynchronous copies of codes and scales two tiles ahead,
-//    int8 -> BF16 with the group's scale (one rounding, as the cache's BF16 read has it),
-//    stored as 128-byte swizzled tiles: K-major for K, and the same bytes read as an MN-major
-//    operand for V (no transposition).
+//  * 16 decode warps (8 for K, 8 for V): codes and scales from shared memory, where a copy warp's
+//    tensor copies bring them two tiles ahead; int8 -> BF16 with the group's scale (one rounding, as
+//    the cache's BF16 read has it), stored as 128-byte swizzled tiles: K-major for K, and the same
+//    bytes read as an MN-major operand for V (no transposition).
 //  * 1 warp issues the MMAs: Q and P from TMEM, K and V from shared memory.
 // TMEM: O 256 columns, Q 128, two S/P buffers of 64.
+#include <cuda.h>  // CUtensorMap and its enums; the encoder is looked up at run time
+
 #include "umma.cuh"
 
 namespace qk {
@@ -31,8 +33,14 @@ namespace {
 constexpr int kTile = 64;   // tokens per tile
 constexpr int kRows = 128;  // query rows per tile
 constexpr int kStages = 2;
-constexpr int kSoftmaxWarps = 4, kDecodeWarps = 8;
-constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 1) * 32;
+constexpr int kRaw = 2;     // raw tiles (codes and scales) in flight
+constexpr int kSoftmaxWarps = 4, kDecodeWarps = 16, kSide = kDecodeWarps / 2;  // half decode K, half V
+constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kCopyWarp = kMmaWarp + 1;
+constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 4) * 32;  // whole warpgroups
+// Registers per thread: 80 at launch for 6 warpgroups (480 in all); softmax 152, four decode groups
+// 64 each, the last group 64.
+constexpr int kSoftmaxRegs = 152, kOtherRegs = 64;
+static_assert(kSoftmaxRegs + 5 * kOtherRegs <= 6 * 80, "the shares fit the launch's registers");
 constexpr uint32_t kColO = 0, kColQ = 256, kColS = 384;  // TMEM columns
 constexpr float kLazyGrowth = 8.f;                       // in powers of two
 constexpr uint32_t kHugeScale = 0x7c00;                  // BF16 bits of 2^121: times 127 leaves FP32's range
@@ -184,6 +192,7 @@ struct Walk {
 struct Barriers {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[2], p_full[2], q_full, o_full;
+  uint64_t raw_full[2][kRaw], raw_empty[2][kRaw];  // K, V
 };
 
 struct Control {
@@ -273,108 +282,118 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 
 // ---- decode warps -------------------------------------------------------------------------
 
-// Raw codes and scales wait in shared memory, kRaw tiles ahead, each thread's own: 16-byte
-// asynchronous copies of its 16 channels of SPT consecutive tokens (all in one page; row i of token
-// i ^ swap), then its group's scales (token i in half i % 2 of word i / 2). Nobody else reads them,
-// so the thread's own copy groups are all the synchronisation they need.
-constexpr int kRaw = 2;
+// A raw tile as the copies leave it: K codes, V codes [token][HD], then per box of a page's tokens
+// the K scales and the V scales [group][token].
 template <int HD>
 struct Raw {
-  uint4 row[kRaw][HD / 32 + 1][kDecodeWarps * 32];
+  static constexpr uint32_t kCodes = kTile * HD, kGroups = HD / 32;
+  static constexpr uint32_t kScales = kTile / 16 * 128 > kTile * kGroups * 2 ? kTile / 16 * 128 : kTile * kGroups * 2;
+  static constexpr uint32_t kBytes = 2 * (kCodes + kScales);
+  // bytes from one box's scales to the next's: copies land on 128-byte boundaries
+  static __device__ uint32_t box_stride(uint32_t box) { return box * kGroups * 2 < 128 ? 128 : box * kGroups * 2; }
 };
 
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-template <int SIZE>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(SIZE), "r"(bytes) : "memory");
+struct Maps {
+  CUtensorMap k_codes, v_codes, k_scale, v_scale;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
 }
 
-// Both kinds of decode warps run one copy of this code (K or V by run-time values): with a copy
-// each the CTA's hot code left the instruction cache.
+// The copy warp: per tile a box of min(page, 64) tokens per lane, four tensor copies each (codes and
+// scales of K and V), kRaw tiles ahead; page numbers one tile further.
 template <int HD>
-__device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint8_t* tiles, Raw<HD>& raw, Walk walk) {
-  constexpr int SPT = HD / 32, CHUNKS = HD / 16;
-  constexpr uint32_t kStageBytes = kTile * HD * 2, kRawRow = kDecodeWarps * 32 * 16, kRawTile = (SPT + 1) * kRawRow;
-  const bool values = threadIdx.x >= (kSoftmaxWarps + 4) * 32;
-  const int t = (threadIdx.x - kSoftmaxWarps * 32) & 127;
-  const int chunk = t % CHUNKS, sub = (t / CHUNKS) * SPT;  // tokens sub .. sub + SPT - 1 of a tile
-  // A token's 16 channels are the 16-byte pieces 2 chunk and 2 chunk + 1 of its row, in atoms of 64
-  // channels, piece j at j ^ (token % 8). Half of the lanes take their tokens in the order 1, 0, 3,
-  // 2, ..: then 8 lanes' stores fill the 8 different 16-byte banks.
-  const int swap = HD == 64 ? (t / CHUNKS) & 1 : (chunk >> 2) & 1;
-  const int8_t* codes = values ? a.v_codes : a.k_codes;
-  const uint16_t* scale = values ? a.v_scale : a.k_scale;
-  uint64_t* full = values ? ctl.bar.v_full : ctl.bar.k_full;
-  uint64_t* empty = values ? ctl.bar.v_empty : ctl.bar.k_empty;
-  const uint32_t mine = smem_addr(tiles) + (values ? kStages * kStageBytes : 0) + (chunk >> 2) * (kTile * 128) +
-                        ((sub ^ swap) << 7 | (((chunk & 3) * 2) ^ ((sub ^ swap) & 7)) << 4);
-  const uint32_t select[2] = {swap ? 0x3232u : 0x1010u, swap ? 0x1010u : 0x3232u};
-  const uint32_t my_raw = smem_addr(&raw) + (threadIdx.x - kSoftmaxWarps * 32) * 16;
-  const int D = a.kv * HD, G = D / 32;
-  // the copies run kRaw tiles ahead of the stores, page numbers one further, across units
-  Walk ahead = walk;
-  Segment aseg;
-  int atile = 0, atotal = 0;
-  bool amore = ahead.next(a, aseg);
-  if (amore) {
-    atile = aseg.t0;
-    atotal = aseg.r.length + aseg.r.count;
-  }
-  auto page_of = [&]() {
-    const int token = atile * kTile + sub;
-    return amore && token < atotal ? __ldg(a.table + static_cast<int64_t>(aseg.b) * a.width + (token >> a.shift)) : 0;
-  };
-  int page = page_of();
-  auto copy = [&](uint32_t slot) {
-    if (amore) {
-      const uint32_t to = my_raw + slot * kRawTile;
-      const int token = atile * kTile + sub;
-      const uint32_t live = token < atotal;
+__device__ __forceinline__ bool copy_role(const TreeArgs& a, Control& ctl, const Maps& maps, uint32_t raw, Walk walk) {
+  const int lane = threadIdx.x & 31;
+  const int box = min(1 << a.shift, kTile), boxes = kTile / box;
+  Segment seg;
+  uint32_t it = 0;
+  uint32_t issued[2] = {0, 0};
+  bool ok = true;
+  while (ok && walk.next(a, seg)) {
+    const int total = seg.r.length + seg.r.count;
+    const int32_t* table = a.table + static_cast<int64_t>(seg.b) * a.width;
+    auto page_of = [&](int tile) {
+      const int token = tile * kTile + lane * box;
+      return tile < seg.t1 && lane < boxes && token < total ? __ldg(table + (token >> a.shift)) : 0;
+    };
+    int page = page_of(seg.t0);
+    for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
+      const uint32_t slot = it % kRaw;
+      const int token = tile * kTile + lane * box;
+      const int live = min((total - tile * kTile + box - 1) / box, boxes);
       if (page < 0 || page >= a.pages) {  // reported, and read as page 0
         *a.status = QK_ERR_INVALID_ARGUMENT;
         page = 0;
       }
       const int row = a.pages == a.pages_per_row ? 0 : page / a.pages_per_row;
-      const int64_t in_row =
-          (static_cast<int64_t>(page - row * a.pages_per_row) << a.shift) + (live ? token & ((1 << a.shift) - 1) : 0);
-      const int8_t* c = codes + (row * a.T + in_row) * D + aseg.head * HD + chunk * 16;
-      const int8_t *even = c + swap * D, *odd = c - swap * D;
+      const int in_page = token & ((1 << a.shift) - 1);
+      const int in_row = ((page - row * a.pages_per_row) << a.shift) + in_page, y = (page << a.shift) + in_page;
+      const int plane = (row * a.kv + seg.head) * (HD / 32);
+      const uint32_t to = raw + slot * Raw<HD>::kBytes + lane * box * HD;
+      const uint32_t scales = raw + slot * Raw<HD>::kBytes + 2 * Raw<HD>::kCodes + lane * Raw<HD>::box_stride(box);
 #pragma unroll
-      for (int i = 0; i < SPT; ++i) cp_async16_or_zero(to + i * kRawRow, (i & 1 ? odd : even) + i * D, live * 16);
-      const uint16_t* p = scale + (static_cast<int64_t>(row) * G + aseg.head * (HD / 32) + chunk / 2) * a.T + in_row;
-      if (SPT == 8) cp_async16_or_zero(to + SPT * kRawRow, p, live * 16);
-      else cp_async_small<SPT == 8 ? 4 : SPT * 2>(to + SPT * kRawRow, p, live * SPT * 2);
-      if (++atile == aseg.t1) {
-        amore = ahead.next(a, aseg);
-        if (amore) {
-          atile = aseg.t0;
-          atotal = aseg.r.length + aseg.r.count;
+      for (int v = 0; v < 2; ++v) {
+        uint64_t* full = &ctl.bar.raw_full[v][slot];
+        ok = ok && warp_wait(&ctl.bar.raw_empty[v][slot], ((it / kRaw) & 1) ^ 1);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(full, live * box * (HD + 2 * (HD / 32)));
+        __syncwarp();
+        if (lane < live) {
+          tma_load_2d(to + v * Raw<HD>::kCodes, v ? &maps.v_codes : &maps.k_codes, seg.head * HD, y, full);
+          tma_load_2d(scales + v * Raw<HD>::kScales, v ? &maps.v_scale : &maps.k_scale, in_row, plane, full);
         }
+        ++issued[v];
       }
-      page = page_of();
+      if (!ok) break;
+      page = page_of(tile + 1);
     }
-    cp_async_commit();
-  };
-#pragma unroll 1
-  for (int i = 0; i < kRaw; ++i) copy(i);
+  }
+  // every copy issued must have landed before the CTA leaves (bounded, should a reader have given up)
+  for (int v = 0; v < 2; ++v)
+    for (uint32_t i = issued[v] > kRaw ? issued[v] - kRaw : 0; i < issued[v]; ++i)
+      warp_wait(&ctl.bar.raw_full[v][i % kRaw], (i / kRaw) & 1);
+  return ok;
+}
+
+// 16 decode warps, the first 8 for K, the others for V, all in one copy of this code: with a copy
+// each the CTA's hot code left the instruction cache.
+template <int HD>
+__device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint32_t tiles, uint32_t raw, Walk walk) {
+  constexpr int SPT = HD / 64, CHUNKS = HD / 16;  // a thread's share of a tile: 16 channels of SPT tokens
+  constexpr uint32_t kStageBytes = kTile * HD * 2;
+  const bool values = threadIdx.x >= (kSoftmaxWarps + kSide) * 32;
+  const int t = (threadIdx.x - kSoftmaxWarps * 32) & (kSide * 32 - 1), lane = threadIdx.x & 31;
+  const int chunk = t % CHUNKS, sub = (t / CHUNKS) * SPT;
+  // A token's 16 channels are the 16-byte pieces 2 chunk and 2 chunk + 1 of its row, in atoms of 64
+  // channels, piece j at j ^ (token % 8). Half of the lanes take their tokens in the order 1, 0, 3,
+  // 2, ..: then 8 lanes' stores fill the 8 different 16-byte banks (at 64 channels they do anyway).
+  const int swap = HD == 64 ? 0 : (chunk >> 2) & 1;
+  uint64_t* full = values ? ctl.bar.v_full : ctl.bar.k_full;
+  uint64_t* empty = values ? ctl.bar.v_empty : ctl.bar.k_empty;
+  const uint32_t mine = tiles + (values ? kStages * kStageBytes : 0) + (chunk >> 2) * (kTile * 128) +
+                        ((sub ^ swap) << 7 | (((chunk & 3) * 2) ^ ((sub ^ swap) & 7)) << 4);
+  const uint32_t select[2] = {swap ? 0x3232u : 0x1010u, swap ? 0x1010u : 0x3232u};
+  const uint32_t from0 = raw + (values ? Raw<HD>::kCodes : 0) + sub * HD + chunk * 16;
+  const int box = min(1 << a.shift, kTile);
+  const uint32_t scales0 = raw + 2 * Raw<HD>::kCodes + (values ? Raw<HD>::kScales : 0) +
+                           sub / box * Raw<HD>::box_stride(box) + (chunk / 2 * box + (sub & (box - 1) & ~1)) * 2;
   Segment seg;
   uint32_t it = 0;
   while (walk.next(a, seg)) {
 #pragma unroll 1
     for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
-      const uint32_t from = my_raw + (it % kRaw) * kRawTile;
-      cp_async_wait<kRaw - 1>();
-      uint32_t scales[4];
-      if (SPT == 8) {
-        const uint4 v = lds_v4_at(from + SPT * kRawRow);
-#pragma unroll
-        for (int i = 0; i < SPT / 2; ++i) scales[i] = word(v, i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < SPT / 2; ++i) scales[i] = lds_at(from + SPT * kRawRow + 4 * i);
-      }
+      const uint32_t slot = it % kRaw, stage = it % kStages;
+      if (!warp_wait(&ctl.bar.raw_full[values][slot], (it / kRaw) & 1)) return false;
+      const uint32_t from = from0 + slot * Raw<HD>::kBytes;
+      uint32_t scales[2];
+      scales[0] = lds_at(scales0 + slot * Raw<HD>::kBytes);
+      if (SPT == 4) scales[1] = lds_at(scales0 + slot * Raw<HD>::kBytes + 4);
+      if (SPT == 1) scales[0] >>= 16 * (sub & 1);
       if (tile * kTile + kTile > seg.r.length) {  // drafts, or past the end
         const int total = seg.r.length + seg.r.count;
 #pragma unroll
@@ -393,26 +412,30 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
           }
         }
       }
-      const uint32_t stage = it % kStages;
       if (!warp_wait(&empty[stage], ((it / kStages) & 1) ^ 1)) return false;
       const uint32_t base = mine + stage * kStageBytes;
+      uint4 code[SPT];
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) code[i] = lds_v4_at(from + (i ^ swap) * HD);
 #pragma unroll
       for (int i = 0; i < SPT; ++i) {
-        const uint4 code = lds_v4_at(from + i * kRawRow);
         const uint32_t two = __byte_perm(scales[i / 2], 0, select[i & 1]);
         const __nv_bfloat162 scale2 = *reinterpret_cast<const __nv_bfloat162*>(&two);
         uint4 piece[2];
-        decode4(code.x, scale2, piece[0].x, piece[0].y);
-        decode4(code.y, scale2, piece[0].z, piece[0].w);
-        decode4(code.z, scale2, piece[1].x, piece[1].y);
-        decode4(code.w, scale2, piece[1].z, piece[1].w);
+        decode4(code[i].x, scale2, piece[0].x, piece[0].y);
+        decode4(code[i].y, scale2, piece[0].z, piece[0].w);
+        decode4(code[i].z, scale2, piece[1].x, piece[1].y);
+        decode4(code[i].w, scale2, piece[1].z, piece[1].w);
         const uint32_t to = base ^ (i << 7 | i << 4);
         sts_v4(to, piece[0]);
         sts_v4(to ^ 16, piece[1]);
       }
       fence_proxy_async_smem();
-      mbar_arrive(&full[stage]);
-      copy(it % kRaw);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&full[stage]);
+        mbar_arrive(&ctl.bar.raw_empty[values][slot]);
+      }
     }
   }
   return true;
@@ -420,50 +443,64 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
 
 // ---- MMA warp -----------------------------------------------------------------------------
 
+// One lane of the (converged) warp, the same each time. The whole warp runs the role and only the
+// instructions themselves are one lane's: their operands are then known to be uniform; issued from
+// a lane's own branch each took about 80 cycles.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
+}
+
 template <int HD>
-__device__ __forceinline__ bool mma_role(const TreeArgs& a, Control& ctl, uint8_t* ktiles, uint8_t* vtiles, Walk walk) {
+__device__ __forceinline__ bool mma_role(const TreeArgs& a, Control& ctl, uint32_t ktiles, uint32_t vtiles, Walk walk) {
   constexpr uint32_t kStageBytes = kTile * HD * 2;
-  const uint32_t tm = ctl.tmem;
+  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
   const uint32_t idesc_s = idesc_bf16_m128(kTile), idesc_o = idesc_bf16_m128_bmn(HD);
+  const uint64_t kdesc = sdesc_sw128(ktiles, 1024u), vdesc = sdesc_sw128_mn(vtiles, kTile * 128, 1024u);
   Segment seg;
   uint32_t it = 0;
   auto scores = [&](uint32_t i) {
     const uint32_t stage = i % kStages;
-    if (!mbar_wait_bounded(&ctl.bar.k_full[stage], (i / kStages) & 1)) return false;
+    if (!warp_wait(&ctl.bar.k_full[stage], (i / kStages) & 1)) return false;
     tc_fence_after();
-    const uint32_t base = smem_addr(ktiles + stage * kStageBytes);
+    const uint64_t desc = kdesc + stage * (kStageBytes >> 4);
+    const uint32_t d = tm + kColS + (i & 1) * kTile;
+    if (elect_one()) {
 #pragma unroll
-    for (int k = 0; k < HD / 16; ++k) {
-      const uint64_t desc = sdesc_sw128(base + (k / 4) * (kTile * 128) + (k % 4) * 32, 1024u);
-      umma_ts(tm + kColS + (i & 1) * kTile, tm + kColQ + k * 8, desc, idesc_s, k != 0);
+      for (int k = 0; k < HD / 16; ++k)
+        umma_ts(d, tm + kColQ + k * 8, desc + ((k / 4) * (kTile * 128) + (k % 4) * 32 >> 4), idesc_s, k != 0);
+      umma_commit(&ctl.bar.k_empty[stage]);
+      umma_commit(&ctl.bar.s_full[i & 1]);
     }
-    umma_commit(&ctl.bar.k_empty[stage]);
-    umma_commit(&ctl.bar.s_full[i & 1]);
+    __syncwarp();
     return true;
   };
   auto values = [&](uint32_t i, bool first) {
     const uint32_t stage = i % kStages;
-    if (!mbar_wait_bounded(&ctl.bar.v_full[stage], (i / kStages) & 1)) return false;
-    if (!mbar_wait_bounded(&ctl.bar.p_full[i & 1], (i / 2) & 1)) return false;
+    if (!warp_wait(&ctl.bar.v_full[stage], (i / kStages) & 1)) return false;
+    if (!warp_wait(&ctl.bar.p_full[i & 1], (i / 2) & 1)) return false;
     tc_fence_after();
-    const uint32_t base = smem_addr(vtiles + stage * kStageBytes);
+    const uint64_t desc = vdesc + stage * (kStageBytes >> 4);
+    const uint32_t p = tm + kColS + (i & 1) * kTile;
+    if (elect_one()) {
 #pragma unroll
-    for (int k = 0; k < kTile / 16; ++k) {
-      const uint64_t desc = sdesc_sw128_mn(base + k * 2048, kTile * 128, 1024u);
-      umma_ts(tm + kColO, tm + kColS + (i & 1) * kTile + k * 8, desc, idesc_o, !first || k != 0);
+      for (int k = 0; k < kTile / 16; ++k) umma_ts(tm + kColO, p + k * 8, desc + k * (2048 >> 4), idesc_o, !first || k != 0);
+      umma_commit(&ctl.bar.v_empty[stage]);
     }
-    umma_commit(&ctl.bar.v_empty[stage]);
+    __syncwarp();
     return true;
   };
   while (walk.next(a, seg)) {
-    if (!mbar_wait_bounded(&ctl.bar.q_full, seg.index & 1)) return false;
+    if (!warp_wait(&ctl.bar.q_full, seg.index & 1)) return false;
     tc_fence_after();
     const int n = seg.t1 - seg.t0;
     for (int j = 0; j <= n; ++j) {
       if (j < n && !scores(it + j)) return false;
       if (j > 0 && !values(it + j - 1, j == 1)) return false;
     }
-    umma_commit(&ctl.bar.o_full);
+    if (elect_one()) umma_commit(&ctl.bar.o_full);
+    __syncwarp();
     it += n;
   }
   return true;
@@ -653,7 +690,7 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __grid_constant__ Maps maps, TreeArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Control ctl;
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -661,10 +698,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&ctl.bar.k_full[i], 128);
+      mbar_init(&ctl.bar.k_full[i], kSide);
       mbar_init(&ctl.bar.k_empty[i], 1);
-      mbar_init(&ctl.bar.v_full[i], 128);
+      mbar_init(&ctl.bar.v_full[i], kSide);
       mbar_init(&ctl.bar.v_empty[i], 1);
+    }
+    for (int i = 0; i < kRaw; ++i) {
+      for (int v = 0; v < 2; ++v) {
+        mbar_init(&ctl.bar.raw_full[v][i], 1);
+        mbar_init(&ctl.bar.raw_empty[v][i], kSide);
+      }
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.bar.s_full[i], 1);
@@ -675,7 +718,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
     fence_mbar_init();
   }
   if (threadIdx.x < kBadRing * 8) ctl.bad[threadIdx.x / 8][threadIdx.x % 8] = 0;
-  constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps;
   if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, 512);
   tc_fence_before();
   pdl_wait();
@@ -696,10 +738,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(TreeArgs a)
     walk.left = range_start(at.total, n, me + 1) - walk.at;
   }
 
+  const uint32_t ktiles = smem_addr(tiles), vtiles = ktiles + kStages * kStageBytes, raw = vtiles + kStages * kStageBytes;
+  const uint32_t rows = raw + kRaw * Raw<HD>::kBytes;
   bool ok = true;
-  if (warp < kSoftmaxWarps) ok = softmax_role<HD>(a, ctl, smem_addr(tiles) + 2 * kStages * kStageBytes + sizeof(Raw<HD>) + warp * 4096, walk, at.total, n);
-  else if (warp < kMmaWarp) ok = decode_role<HD>(a, ctl, tiles, *reinterpret_cast<Raw<HD>*>(tiles + 2 * kStages * kStageBytes), walk);
-  else if (lane == 0) ok = mma_role<HD>(a, ctl, tiles, tiles + kStages * kStageBytes, walk);
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    ok = softmax_role<HD>(a, ctl, rows + warp * 4096, walk, at.total, n);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp < kMmaWarp) ok = decode_role<HD>(a, ctl, ktiles, raw, walk);
+    else if (warp == kCopyWarp) ok = copy_role<HD>(a, ctl, maps, raw, walk);
+    else if (warp == kMmaWarp) ok = mma_role<HD>(a, ctl, ktiles, vtiles, walk);
+  }
   if (!ok) *a.status = QK_ERR_TIMEOUT;
   tc_fence_before();
   __syncthreads();
@@ -814,6 +864,23 @@ int part_rows(int N, int rep) {
   return rows < kRows ? rows : kRows;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A row-major matrix [rows, width] with rows `pitch` bytes apart, in boxes of box_rows x box_width.
+bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64_t width, uint64_t rows, uint64_t pitch,
+            uint32_t box_width, uint32_t box_rows) {
+  EncodeTiledFn fn = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {width, rows};
+  const cuuint64_t strides[1] = {pitch};
+  const cuuint32_t box[2] = {box_width, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct Layout {
   int row_tiles, part_rows;
   int64_t units, records;
@@ -834,12 +901,12 @@ Layout layout_of(int B, int N, int hq, int kv, int hd) {
 }
 
 template <int HD>
-int launch(const TreeArgs& a, const Layout& w, cudaStream_t st) {
-  const size_t smem = 1024 + 2 * kStages * static_cast<size_t>(kTile) * HD * 2 + sizeof(Raw<HD>) + kSoftmaxWarps * 4096;
+int launch(const Maps& maps, const TreeArgs& a, const Layout& w, cudaStream_t st) {
+  const size_t smem = 1024 + 2 * kStages * static_cast<size_t>(kTile) * HD * 2 + kRaw * Raw<HD>::kBytes + kSoftmaxWarps * 4096;
   const int rc = allow_smem(reinterpret_cast<const void*>(tree_attention_kernel<HD>), smem);
   if (rc) return rc;
   // one CTA per SM: each holds all of its SM's tensor memory
-  cudaError_t e = launch_dependent(tree_attention_kernel<HD>, dim3(sm_count()), dim3(kThreads), smem, st, a);
+  cudaError_t e = launch_dependent(tree_attention_kernel<HD>, dim3(sm_count()), dim3(kThreads), smem, st, maps, a);
   if (e != cudaSuccess) return cuda_error(e, "tree_attention_kernel");
   const int pieces = static_cast<int>(w.units * (w.part_rows / 32) * (HD / kJoinCols));
   if (pieces >= 16 * sm_count()) {
@@ -926,9 +993,17 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   a.parts = reinterpret_cast<Parts*>(ws + w.parts);
   a.part = reinterpret_cast<float*>(ws + w.part);
   a.stats = reinterpret_cast<float*>(ws + w.stats);
-  return head_dim == 256   ? launch<256>(a, w, as_stream(stream))
-         : head_dim == 128 ? launch<128>(a, w, as_stream(stream))
-                           : launch<64>(a, w, as_stream(stream));
+  Maps maps;
+  const uint64_t D = static_cast<uint64_t>(kv_heads) * head_dim, slots = static_cast<uint64_t>(rows) * T;
+  const uint32_t box = page_size < kTile ? page_size : kTile;
+  if (!encode(&maps.k_codes, k_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, D, slots, D, head_dim, box) ||
+      !encode(&maps.v_codes, v_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, D, slots, D, head_dim, box) ||
+      !encode(&maps.k_scale, k_scale, CU_TENSOR_MAP_DATA_TYPE_UINT16, T, rows * (D / 32), 2 * T, box, head_dim / 32) ||
+      !encode(&maps.v_scale, v_scale, CU_TENSOR_MAP_DATA_TYPE_UINT16, T, rows * (D / 32), 2 * T, box, head_dim / 32))
+    return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the cache");
+  return head_dim == 256   ? launch<256>(maps, a, w, as_stream(stream))
+         : head_dim == 128 ? launch<128>(maps, a, w, as_stream(stream))
+                           : launch<64>(maps, a, w, as_stream(stream));
 }
 
 int qk_tree_attention_check(const void* workspace, qk_stream_t stream) {
