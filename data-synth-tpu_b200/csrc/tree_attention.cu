@@ -35,7 +35,7 @@ constexpr int kRows = 128;  // query rows per tile
 constexpr int kStages = 2;
 constexpr int kRaw = 2;     // raw tiles (codes and scales) in flight
 constexpr int kSoftmaxWarps = 4, kDecodeWarps = 16, kSide = kDecodeWarps / 2;  // half decode K, half V
-constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kCopyWarp = kMmaWarp + 1;
+constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kCopyWarp = kMmaWarp + 1;  // and one more
 constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 4) * 32;  // whole warpgroups
 // Registers per thread: 80 at launch for 6 warpgroups (480 in all); softmax 152, four decode groups
 // 64 each, the last group 64.
@@ -57,7 +57,7 @@ struct TreeArgs {
   const uint16_t* gate;
   float scale_log2;         // |scale| * log2(e), above zero
   uint32_t q_keep, q_flip;  // Q's bits & keep ^ flip: nothing for a scale of zero, the sign for a negative one
-  int B, N, hq, kv, rep, pages, pages_per_row, width, shift, row_tiles, part_rows;
+  int B, N, hq, kv, rep, pages, pages_per_row, width, room, shift, row_tiles, part_rows;  // room: tokens of a table row
   int64_t T;
   uint16_t* out;
   int* status;
@@ -77,110 +77,62 @@ struct Request {
   bool cut;
   // A unit's share of the ranges: its tiles and kUnitCost steps that stand for Q and the output.
   __device__ int steps() const { return tiles + kUnitCost; }
-  __device__ int64_t work(int kv) const { return tiles ? static_cast<int64_t>(kv) * row_tiles * steps() : 0; }
+  __device__ int work(int kv) const { return tiles ? kv * row_tiles * steps() : 0; }
 };
 
 __device__ __forceinline__ Request load_request(const TreeArgs& a, int b) {
-  const int64_t room = min(static_cast<int64_t>(a.width) << a.shift, int64_t(0x7fffffc0));
   const int n = a.lengths[b], c = a.counts ? a.counts[b] : a.N;
   Request r;
-  r.length = static_cast<int>(min(static_cast<int64_t>(max(n, 0)), room));
-  r.count = static_cast<int>(min(static_cast<int64_t>(min(max(c, 0), a.N)), room - r.length));
+  r.length = min(max(n, 0), a.room);
+  r.count = min(min(max(c, 0), a.N), a.room - r.length);
   r.cut = r.length != n || r.count != c;
   r.row_tiles = (r.count * a.rep + kRows - 1) / kRows;
   r.tiles = r.count ? (r.length + r.count + kTile - 1) / kTile : 0;
   return r;
 }
 
-// The CTAs' ranges of a total of `total` steps, at least one step each.
-__device__ __forceinline__ int ranges(int64_t total, int ctas) {
-  return static_cast<int>(total < ctas ? total : ctas);
-}
-__device__ __forceinline__ int64_t range_start(int64_t total, int n, int c) { return c * total / n; }
-__device__ __forceinline__ int range_owner(int64_t total, int n, int64_t step) {
-  return static_cast<int>(((step + 1) * n - 1) / total);
-}
-
-// Total work of all requests, and the request that holds step `want` of it with the step's
-// offset in it: threads sum consecutive requests, a block scan, one thread walks its few.
-struct Located {
-  int64_t total, offset;
-  int b;
+// The CTAs' ranges of a total of `total` steps: n of them, the first total % n one step longer. All
+// counts of steps fit 31 bits (the host checks): 64-bit divisions alone cost as much as two tiles.
+struct Ranges {
+  int n, each, longer;
+  __device__ Ranges(int total, int ctas)
+      : n(min(total, ctas)), each(n ? total / n : 0), longer(n ? total - each * n : 0) {}
+  __device__ int start(int c) const { return c * each + min(c, longer); }
+  __device__ int owner(int step) const {
+    const int head = longer * (each + 1);
+    return step < head ? step / (each + 1) : longer + (step - head) / each;
+  }
 };
-template <class Want>
-__device__ __forceinline__ Located locate(const TreeArgs& a, Located* shared, int64_t* warps, Want want, bool report) {
-  constexpr int THREADS = kThreads;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (a.B + THREADS - 1) / THREADS;
-  const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-  int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Request r = load_request(a, b);
-    if (r.cut && report) *a.status = QK_ERR_INVALID_ARGUMENT;
-    sum += r.work(a.kv);
-  }
-  int64_t s = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
-  }
-  if (lane == 31) warps[warp] = s;
-  __syncthreads();
-  int64_t before = s - sum, total = 0;
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += warps[w];
-    total += warps[w];
-  }
-  if (tid == 0) *shared = Located{total, 0, a.B};
-  __syncthreads();
-  const int64_t step = want(total);
-  if (step >= before && step < before + sum) {
-    int64_t off = step - before;
-    for (int b = b0; b < b1; ++b) {
-      const int64_t w = load_request(a, b).work(a.kv);
-      if (off < w) {
-        shared->offset = off;
-        shared->b = b;
-        break;
-      }
-      off -= w;
-    }
-  }
-  __syncthreads();
-  return *shared;
-}
 
 // The pieces of a CTA's range: tiles [t0, t1) of one unit each. A unit's last steps are not tiles:
 // a range that holds nothing else of the unit has no piece of it.
 struct Segment {
   Request r;
   int b, head, row_tile, t0, t1, index;
-  int64_t start;  // the unit's first step in the whole work
+  int start;  // the unit's first step in the whole work
 };
 struct Walk {
+  Request r;
   int b, index;
-  int64_t offset, left, at;  // at: the next step in the whole work
+  int offset, left, at;  // in request b's work; of the range; the next step in the whole work
   __device__ bool next(const TreeArgs& a, Segment& s) {
     while (left > 0) {
-      for (;; ++b) {
-        s.r = load_request(a, b);
-        const int64_t w = s.r.work(a.kv);
-        if (offset < w) break;
+      for (int w = r.work(a.kv); offset >= w; w = r.work(a.kv)) {
         offset -= w;
+        r = load_request(a, ++b);
       }
-      const int steps = s.r.steps();
-      const int unit = static_cast<int>(offset / steps);
+      const int steps = r.steps(), unit = offset / steps;
+      s.r = r;
       s.b = b;
-      s.head = unit / s.r.row_tiles;
-      s.row_tile = unit % s.r.row_tiles;
-      s.t0 = static_cast<int>(offset % steps);
-      const int end = static_cast<int>(min(static_cast<int64_t>(steps), s.t0 + left));
+      s.head = unit / r.row_tiles;
+      s.row_tile = unit - s.head * r.row_tiles;
+      s.t0 = offset - unit * steps;
+      const int end = min(steps, s.t0 + left), did = end - s.t0;
       s.start = at - s.t0;
-      left -= end - s.t0;
-      offset += end - s.t0;
-      at += end - s.t0;
-      s.t1 = min(end, s.r.tiles);
+      left -= did;
+      offset += did;
+      at += did;
+      s.t1 = min(end, r.tiles);
       if (s.t0 >= s.t1) continue;
       s.index = index++;
       return true;
@@ -188,6 +140,47 @@ struct Walk {
     return false;
   }
 };
+
+// The whole work and where range `me` of it begins; every warp finds out for itself (a lane per
+// request, no barrier).
+__device__ __forceinline__ Walk locate(const TreeArgs& a, int me, int& total, bool report) {
+  const int lane = threadIdx.x & 31;
+  total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    int w = 0;
+    if (b0 + lane < a.B) {
+      const Request r = load_request(a, b0 + lane);
+      w = r.work(a.kv);
+      if (r.cut && report) *a.status = QK_ERR_INVALID_ARGUMENT;
+    }
+    total += __reduce_add_sync(0xffffffffu, w);
+  }
+  const Ranges ranges(total, gridDim.x);
+  Walk walk{};
+  if (me >= ranges.n) return walk;
+  walk.at = ranges.start(me);
+  walk.left = ranges.start(me + 1) - walk.at;
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int w = b0 + lane < a.B ? load_request(a, b0 + lane).work(a.kv) : 0;
+    int upto = before + w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto - before, o);
+      if (lane >= o) upto += u;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, upto > walk.at);
+    if (past) {
+      const int which = __ffs(past) - 1;
+      walk.b = b0 + which;
+      walk.offset = walk.at - __shfl_sync(0xffffffffu, upto - w, which);
+      break;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  walk.r = load_request(a, walk.b);
+  return walk;
+}
 
 struct Barriers {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
@@ -198,8 +191,6 @@ struct Barriers {
 struct Control {
   Barriers bar;
   uint64_t bad[kBadRing][8];  // per unit and channel group: drafts whose value scale is not finite
-  Located located;
-  int64_t warps[kThreads / 32];
   uint32_t tmem;
 };
 
@@ -304,59 +295,57 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// The copy warp: per tile a box of min(page, 64) tokens per lane, four tensor copies each (codes and
-// scales of K and V), kRaw tiles ahead; page numbers one tile further.
+// A copy warp for K and one for V: per tile a box of min(page, 64) tokens per lane, two tensor copies
+// each (codes and scales), kRaw tiles ahead; page numbers one tile further. One warp for both was the
+// slowest of all: a tile's worth of its instructions took as long as two tiles of the others'.
 template <int HD>
-__device__ __forceinline__ bool copy_role(const TreeArgs& a, Control& ctl, const Maps& maps, uint32_t raw, Walk walk) {
+__device__ __forceinline__ bool copy_role(const TreeArgs& a, Control& ctl, const Maps& maps, uint32_t raw, int v,
+                                          Walk walk) {
   const int lane = threadIdx.x & 31;
-  const int box = min(1 << a.shift, kTile), boxes = kTile / box;
+  const int box = min(1 << a.shift, kTile), boxes = kTile / box, mine = lane * box;
+  const uint32_t codes = raw + v * Raw<HD>::kCodes + mine * HD;
+  const uint32_t scales = raw + 2 * Raw<HD>::kCodes + v * Raw<HD>::kScales + lane * Raw<HD>::box_stride(box);
+  const CUtensorMap* code_map = v ? &maps.v_codes : &maps.k_codes;
+  const CUtensorMap* scale_map = v ? &maps.v_scale : &maps.k_scale;
+  uint64_t *full = ctl.bar.raw_full[v], *empty = ctl.bar.raw_empty[v];
   Segment seg;
   uint32_t it = 0;
-  uint32_t issued[2] = {0, 0};
   bool ok = true;
   while (ok && walk.next(a, seg)) {
     const int total = seg.r.length + seg.r.count;
     const int32_t* table = a.table + static_cast<int64_t>(seg.b) * a.width;
     auto page_of = [&](int tile) {
-      const int token = tile * kTile + lane * box;
+      const int token = tile * kTile + mine;
       return tile < seg.t1 && lane < boxes && token < total ? __ldg(table + (token >> a.shift)) : 0;
     };
     int page = page_of(seg.t0);
     for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
       const uint32_t slot = it % kRaw;
-      const int token = tile * kTile + lane * box;
-      const int live = min((total - tile * kTile + box - 1) / box, boxes);
-      if (page < 0 || page >= a.pages) {  // reported, and read as page 0
+      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) {  // reported, and read as page 0
         *a.status = QK_ERR_INVALID_ARGUMENT;
         page = 0;
       }
-      const int row = a.pages == a.pages_per_row ? 0 : page / a.pages_per_row;
-      const int in_page = token & ((1 << a.shift) - 1);
-      const int in_row = ((page - row * a.pages_per_row) << a.shift) + in_page, y = (page << a.shift) + in_page;
-      const int plane = (row * a.kv + seg.head) * (HD / 32);
-      const uint32_t to = raw + slot * Raw<HD>::kBytes + lane * box * HD;
-      const uint32_t scales = raw + slot * Raw<HD>::kBytes + 2 * Raw<HD>::kCodes + lane * Raw<HD>::box_stride(box);
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        uint64_t* full = &ctl.bar.raw_full[v][slot];
-        ok = ok && warp_wait(&ctl.bar.raw_empty[v][slot], ((it / kRaw) & 1) ^ 1);
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(full, live * box * (HD + 2 * (HD / 32)));
-        __syncwarp();
-        if (lane < live) {
-          tma_load_2d(to + v * Raw<HD>::kCodes, v ? &maps.v_codes : &maps.k_codes, seg.head * HD, y, full);
-          tma_load_2d(scales + v * Raw<HD>::kScales, v ? &maps.v_scale : &maps.k_scale, in_row, plane, full);
-        }
-        ++issued[v];
+      const int y = (page << a.shift) + ((tile * kTile + mine) & ((1 << a.shift) - 1));  // the slot
+      int x = y, plane = seg.head * (HD / 32);
+      if (a.pages != a.pages_per_row) {  // a cache of several rows: the slot's row and time
+        const int row = page / a.pages_per_row;
+        x -= (row * a.pages_per_row) << a.shift;
+        plane += row * a.kv * (HD / 32);
       }
+      const int live = min((total - tile * kTile + box - 1) / box, boxes);
+      ok = warp_wait(&empty[slot], ((it / kRaw) & 1) ^ 1);
       if (!ok) break;
+      if (lane == 0) mbar_expect_tx(&full[slot], live * box * (HD + 2 * (HD / 32)));
+      __syncwarp();
+      if (lane < live) {
+        tma_load_2d(codes + slot * Raw<HD>::kBytes, code_map, seg.head * HD, y, &full[slot]);
+        tma_load_2d(scales + slot * Raw<HD>::kBytes, scale_map, x, plane, &full[slot]);
+      }
       page = page_of(tile + 1);
     }
   }
   // every copy issued must have landed before the CTA leaves (bounded, should a reader have given up)
-  for (int v = 0; v < 2; ++v)
-    for (uint32_t i = issued[v] > kRaw ? issued[v] - kRaw : 0; i < issued[v]; ++i)
-      warp_wait(&ctl.bar.raw_full[v][i % kRaw], (i / kRaw) & 1);
+  for (uint32_t i = it > kRaw ? it - kRaw : 0; i < it; ++i) warp_wait(&full[i % kRaw], (i / kRaw) & 1);
   return ok;
 }
 
@@ -520,34 +509,39 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const Segment& seg, ui
   int at[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) at[i] = __shfl_sync(0xffffffffu, mine, 4 * i + lane / 8);
+  constexpr int kAtOnce = HD >= 128 ? 2 : 1;  // pieces of 64 channels in flight
 #pragma unroll 1
-  for (int c = 0; c < HD / 64; ++c) {
-    uint4 v[8];
+  for (int c0 = 0; c0 < HD / 64; c0 += kAtOnce) {
+    uint4 v[kAtOnce][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = at[i] >= 0 ? ld_nc_v4(q + at[i] + c * 64 + lane % 8 * 8) : make_uint4(0, 0, 0, 0);
-    __syncwarp();
+    for (int c = 0; c < kAtOnce; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + lane / 8;
-      sts_v4(stage + r * 128 + ((lane ^ r) & 7) * 16, v[i]);
+      for (int i = 0; i < 8; ++i)
+        v[c][i] = at[i] >= 0 ? ld_nc_v4(q + at[i] + (c0 + c) * 64 + lane % 8 * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < kAtOnce; ++c) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + lane / 8;
+        sts_v4(stage + r * 128 + ((lane ^ r) & 7) * 16, v[c][i]);
+      }
+      __syncwarp();
+      uint32_t u[32];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 x = lds_v4_at(stage + lane * 128 + ((i ^ lane) & 7) * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) u[i * 4 + w] = (word(x, w) & a.q_keep) ^ a.q_flip;
+      }
+      tmem_st32(tm + kColQ + (c0 + c) * 32, u);
     }
-    __syncwarp();
-    uint32_t u[32];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint4 x = lds_v4_at(stage + lane * 128 + ((i ^ lane) & 7) * 16);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) u[i * 4 + w] = (word(x, w) & a.q_keep) ^ a.q_flip;
-    }
-    tmem_st32(tm + kColQ + c * 32, u);
   }
   tmem_wait_st();
 }
 
 template <int HD>
-__device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, uint32_t stage, Walk walk, int64_t total,
-                                             int ctas) {
+__device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, uint32_t stage, Walk walk, int total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(warp * 32) << 16);
   Segment seg, next;
@@ -678,8 +672,8 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
     stats[0] = m;
     stats[a.part_rows] = l;
     if (seg.t0 == 0 && threadIdx.x == 0)
-      a.parts[unit] = Parts{static_cast<int>(blockIdx.x), range_owner(total, ctas, seg.start + seg.r.tiles - 1) -
-                                                              static_cast<int>(blockIdx.x) + 1};
+      a.parts[unit] = Parts{static_cast<int>(blockIdx.x),
+                            Ranges(total, gridDim.x).owner(seg.start + seg.r.tiles - 1) - static_cast<int>(blockIdx.x) + 1};
     tc_fence_before();
     if (seg.r.length < seg.t1 * kTile) {  // the unit saw drafts: its record of bad values is read, clear it
       asm volatile("bar.sync 1, %0;" ::"r"(32 * min(kSoftmaxWarps, (seg.r.count * a.rep - seg.row_tile * kRows + 31) / 32)) : "memory");
@@ -695,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   __shared__ Control ctl;
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr uint32_t kStageBytes = kTile * HD * 2;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&ctl.bar.k_full[i], kSide);
@@ -720,34 +714,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   if (threadIdx.x < kBadRing * 8) ctl.bad[threadIdx.x / 8][threadIdx.x % 8] = 0;
   if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, 512);
   tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   pdl_wait();
   pdl_trigger();
-  const int me = blockIdx.x;
-  const Located at = locate(
-      a, &ctl.located, ctl.warps,
-      [&](int64_t total) {
-        const int n = ranges(total, gridDim.x);
-        return me < n ? range_start(total, n, me) : total;
-      },
-      me == 0);
-  tc_fence_after();
-  const int n = ranges(at.total, gridDim.x);
-  Walk walk{at.b, 0, at.offset, 0, 0};
-  if (me < n) {
-    walk.at = range_start(at.total, n, me);
-    walk.left = range_start(at.total, n, me + 1) - walk.at;
-  }
+  int total;
+  const Walk walk = locate(a, blockIdx.x, total, threadIdx.x < 32 && blockIdx.x == 0);
 
   const uint32_t ktiles = smem_addr(tiles), vtiles = ktiles + kStages * kStageBytes, raw = vtiles + kStages * kStageBytes;
   const uint32_t rows = raw + kRaw * Raw<HD>::kBytes;
   bool ok = true;
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    ok = softmax_role<HD>(a, ctl, rows + warp * 4096, walk, at.total, n);
+    ok = softmax_role<HD>(a, ctl, rows + warp * 4096, walk, total);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp < kMmaWarp) ok = decode_role<HD>(a, ctl, ktiles, raw, walk);
-    else if (warp == kCopyWarp) ok = copy_role<HD>(a, ctl, maps, raw, walk);
+    else if (warp == kCopyWarp || warp == kCopyWarp + 1) ok = copy_role<HD>(a, ctl, maps, raw, warp - kCopyWarp, walk);
     else if (warp == kMmaWarp) ok = mma_role<HD>(a, ctl, ktiles, vtiles, walk);
   }
   if (!ok) *a.status = QK_ERR_TIMEOUT;
@@ -956,6 +939,9 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   QK_REQUIRE(static_cast<int64_t>(N) * q_stride < (1ll << 31), "a request's queries must span fewer than 2^31 values");
   const Layout w = layout_of(B, N, hq, kv_heads, head_dim);
   QK_REQUIRE(w.units * (w.part_rows / 32) * (head_dim / kJoinCols) < (1ll << 31), "too many rows in one call");
+  QK_REQUIRE(static_cast<int64_t>(width) * page_size < (1ll << 31) - kTile, "a table row must span fewer than 2^31 - 64 tokens");
+  QK_REQUIRE(w.units * (static_cast<int64_t>(width) * page_size / kTile + kUnitCost + 1) < (1ll << 31),
+             "too many requests of such a length in one call");
   const size_t need = w.bytes;
   if (!workspace || workspace_bytes < need)
     return set_error(QK_ERR_WORKSPACE, "tree attention workspace needs %zu bytes, got %zu", need, workspace_bytes);
@@ -983,6 +969,7 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   a.pages = static_cast<int>(rows * T / page_size);
   a.pages_per_row = static_cast<int>(T / page_size);
   a.width = width;
+  a.room = static_cast<int>(static_cast<int64_t>(width) * page_size);
   while ((1 << a.shift) < page_size) ++a.shift;
   a.row_tiles = w.row_tiles;
   a.part_rows = w.part_rows;
