@@ -14,14 +14,14 @@
 // joins them, divides, gates and rounds.
 //
 // One CTA per SM, three kinds of warps joined by mbarriers (every wait bounded):
-//  * 4 softmax warps, a thread per row: Q to TMEM once per unit; then per tile S from TMEM, mask,
+//  * 8 softmax warps, two threads per row: Q to TMEM once per unit; then per tile S from TMEM, mask,
 //    running maximum and sum in FP32, P as BF16 back over S's columns. O (FP32, in TMEM) is rescaled
 //    only when a row's maximum grows by more than 2^8: P stays below 2^8, exact enough in FP32.
-//  * 16 decode warps (8 for K, 8 for V): codes and scales from shared memory, where a copy warp's
-//    tensor copies bring them two tiles ahead; int8 -> BF16 with the group's scale (one rounding, as
+//  * 8 decode warps (4 for K, 4 for V): codes and scales from shared memory, where a copy warp each
+//    brings them by tensor copies two tiles ahead; int8 -> BF16 with the group's scale (one rounding, as
 //    the cache's BF16 read has it), stored as 128-byte swizzled tiles: K-major for K, and the same
 //    bytes read as an MN-major operand for V (no transposition).
-//  * 1 warp issues the MMAs: Q and P from TMEM, K and V from shared memory.
+//  * 2 warps issue the MMAs, Q K^T and P V: Q and P from TMEM, K and V from shared memory.
 // TMEM: O 256 columns, Q 128, two S/P buffers of 64.
 #include <cuda.h>  // CUtensorMap and its enums; the encoder is looked up at run time
 
@@ -34,17 +34,17 @@ constexpr int kTile = 64;   // tokens per tile
 constexpr int kRows = 128;  // query rows per tile
 constexpr int kStages = 2;
 constexpr int kRaw = 2;     // raw tiles (codes and scales) in flight
-constexpr int kSoftmaxWarps = 4, kDecodeWarps = 16, kSide = kDecodeWarps / 2;  // half decode K, half V
-constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kCopyWarp = kMmaWarp + 1;  // and one more
-constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 4) * 32;  // whole warpgroups
-// Registers per thread: 80 at launch for 6 warpgroups (480 in all); softmax 152, four decode groups
-// 64 each, the last group 64.
-constexpr int kSoftmaxRegs = 152, kOtherRegs = 64;
-static_assert(kSoftmaxRegs + 5 * kOtherRegs <= 6 * 80, "the shares fit the launch's registers");
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 8, kSide = kDecodeWarps / 2;  // half decode K, half V
+constexpr int kScoreWarp = kSoftmaxWarps + kDecodeWarps, kCopyWarp = kScoreWarp + 1;  // K, then V; then the values' warp
+constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 4) * 32;                 // whole warpgroups
+// Registers per thread: 96 at launch for 5 warpgroups (480 in all).
+constexpr int kSoftmaxRegs = 128, kOtherRegs = 72;
+static_assert(2 * kSoftmaxRegs + 3 * kOtherRegs <= 5 * 96, "the shares fit the launch's registers");
 constexpr uint32_t kColO = 0, kColQ = 256, kColS = 384;  // TMEM columns
 constexpr float kLazyGrowth = 8.f;                       // in powers of two
 constexpr uint32_t kHugeScale = 0x7c00;                  // BF16 bits of 2^121: times 127 leaves FP32's range
 constexpr int kBadRing = 4;
+constexpr uint32_t kQStage = 2048;  // bytes per softmax warp
 constexpr int kUnitCost = 4;  // what a unit costs besides its tiles (Q, the output), in tiles
 
 struct TreeArgs {
@@ -62,7 +62,7 @@ struct TreeArgs {
   uint16_t* out;
   int* status;
   float* part;          // [units + CTAs][HD][part_rows] unnormalised O
-  float* stats;         // [units + CTAs][2][part_rows] maximum (log2) and sum
+  float* stats;         // [units + CTAs][3][part_rows] maximum (log2) and two sums
   struct Parts* parts;  // [units]
 };
 
@@ -184,12 +184,13 @@ __device__ __forceinline__ Walk locate(const TreeArgs& a, int me, int& total, bo
 
 struct Barriers {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], p_full[2], q_full, o_full;
+  uint64_t s_full[kStages], p_full[kStages], q_full, o_full;
   uint64_t raw_full[2][kRaw], raw_empty[2][kRaw];  // K, V
 };
 
 struct Control {
   Barriers bar;
+  float top[2][kRows];        // the row maxima that a row's two warps swap
   uint64_t bad[kBadRing][8];  // per unit and channel group: drafts whose value scale is not finite
   uint32_t tmem;
 };
@@ -248,23 +249,29 @@ __device__ __forceinline__ uint32_t lds_at(uint32_t addr) {
   return v;
 }
 
-// Four int8 codes times a BF16 scale (in both halves of `scale2`) -> two BF16 pairs. A byte c
-// under the exponent of 128 is 128 + (c & 127), exact in BF16; minus 128, or 256 where the sign
-// bit was set, it is the code; the product rounds once.
-__device__ __forceinline__ void decode4(uint32_t codes, __nv_bfloat162 scale2, uint32_t& lo, uint32_t& hi) {
-  const uint32_t t[2] = {__byte_perm(codes, 0x43434343u, 0x4140), __byte_perm(codes, 0x43434343u, 0x4342)};
+// Four int8 codes times a BF16 scale s >= 0 -> two BF16 pairs, each code * s rounded once. With the
+// sign bit flipped a code c is the byte u = c + 128; under the exponent of 128 it reads f = 128 + u
+// below 128 and f = 2 u from there, so s (f / 2 - 128) is A = s c / 2 for negative codes and s c for
+// others: one fused multiply-add with h = s / 2, k = -128 s (both exact), and A - max(-A, 0) doubles
+// the negative ones, which is exact. Half of this runs on the FMA pipe; masking the sign bit off and
+// adding it back took twice the integer instructions, whose pipe is half as wide.
+__device__ __forceinline__ void decode4(uint32_t codes, __nv_bfloat162 h, __nv_bfloat162 k, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = codes ^ 0x80808080u;
+  const uint32_t t[2] = {__byte_perm(u, 0x43434343u, 0x4140), __byte_perm(u, 0x43434343u, 0x4342)};
   uint32_t r[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t mag = t[i] & 0xff7fff7fu, off = t[i] & 0xff80ff80u;
-    const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&mag),
-                                             *reinterpret_cast<const __nv_bfloat162*>(&off)),
-                                     scale2);
+    const __nv_bfloat162 half = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&t[i]), h, k);
+    const __nv_bfloat162 neg = __hfma2_relu(half, __nv_bfloat162{-1.f, -1.f}, __nv_bfloat162{-0.f, -0.f});
+    const __nv_bfloat162 v = __hfma2(neg, __nv_bfloat162{-1.f, -1.f}, half);
     r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
   lo = r[0];
   hi = r[1];
 }
+
+// The two softmax warps of 32 rows.
+__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
 
 // A bounded wait of a whole warp, converged behind it: false for all lanes if one gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
@@ -349,40 +356,47 @@ __device__ __forceinline__ bool copy_role(const TreeArgs& a, Control& ctl, const
   return ok;
 }
 
-// 16 decode warps, the first 8 for K, the others for V, all in one copy of this code: with a copy
-// each the CTA's hot code left the instruction cache.
+// 16 decode warps: 4 for each of K and V and the even and odd tiles (raw slot and stage are the
+// tile's parity), all in one copy of this code: with a copy each the CTA's hot code left the
+// instruction cache. Four warps per tile instead of eight halve what a tile costs besides its values;
+// the other four are at work on the next one meanwhile.
 template <int HD>
 __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint32_t tiles, uint32_t raw, Walk walk) {
-  constexpr int SPT = HD / 64, CHUNKS = HD / 16;  // a thread's share of a tile: 16 channels of SPT tokens
+  constexpr int SPT = HD / 32, CHUNKS = HD / 16;  // a thread's share of a tile: 16 channels of SPT tokens
   constexpr uint32_t kStageBytes = kTile * HD * 2;
   const bool values = threadIdx.x >= (kSoftmaxWarps + kSide) * 32;
-  const int t = (threadIdx.x - kSoftmaxWarps * 32) & (kSide * 32 - 1), lane = threadIdx.x & 31;
+  const int t = threadIdx.x & (kSide * 32 - 1), lane = threadIdx.x & 31;
   const int chunk = t % CHUNKS, sub = (t / CHUNKS) * SPT;
   // A token's 16 channels are the 16-byte pieces 2 chunk and 2 chunk + 1 of its row, in atoms of 64
   // channels, piece j at j ^ (token % 8). Half of the lanes take their tokens in the order 1, 0, 3,
-  // 2, ..: then 8 lanes' stores fill the 8 different 16-byte banks (at 64 channels they do anyway).
-  const int swap = HD == 64 ? 0 : (chunk >> 2) & 1;
-  uint64_t* full = values ? ctl.bar.v_full : ctl.bar.k_full;
-  uint64_t* empty = values ? ctl.bar.v_empty : ctl.bar.k_empty;
-  const uint32_t mine = tiles + (values ? kStages * kStageBytes : 0) + (chunk >> 2) * (kTile * 128) +
-                        ((sub ^ swap) << 7 | (((chunk & 3) * 2) ^ ((sub ^ swap) & 7)) << 4);
+  // 2, ..: then 8 lanes' stores fill the 8 different 16-byte banks.
+  const int swap = HD == 64 ? (t / CHUNKS) & 1 : (chunk >> 2) & 1;
+  uint64_t* full = (values ? ctl.bar.v_full : ctl.bar.k_full);
+  uint64_t* empty = (values ? ctl.bar.v_empty : ctl.bar.k_empty);
+  uint64_t *raw_full = ctl.bar.raw_full[values], *raw_empty = ctl.bar.raw_empty[values];
+  const uint32_t to0 = tiles + (values ? kStages : 0) * kStageBytes + (chunk >> 2) * (kTile * 128) +
+                       ((sub ^ swap) << 7 | (((chunk & 3) * 2) ^ ((sub ^ swap) & 7)) << 4);
   const uint32_t select[2] = {swap ? 0x3232u : 0x1010u, swap ? 0x1010u : 0x3232u};
-  const uint32_t from0 = raw + (values ? Raw<HD>::kCodes : 0) + sub * HD + chunk * 16;
+  const uint32_t from = raw + (values ? Raw<HD>::kCodes : 0) + sub * HD + chunk * 16;
+  const uint32_t from_even = from + swap * HD, from_odd = from - swap * HD;
   const int box = min(1 << a.shift, kTile);
-  const uint32_t scales0 = raw + 2 * Raw<HD>::kCodes + (values ? Raw<HD>::kScales : 0) +
-                           sub / box * Raw<HD>::box_stride(box) + (chunk / 2 * box + (sub & (box - 1) & ~1)) * 2;
+  const uint32_t scales_at = raw + 2 * Raw<HD>::kCodes + (values ? Raw<HD>::kScales : 0) +
+                             sub / box * Raw<HD>::box_stride(box) + (chunk / 2 * box + (sub & (box - 1))) * 2;
   Segment seg;
   uint32_t it = 0;
   while (walk.next(a, seg)) {
 #pragma unroll 1
     for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
-      const uint32_t slot = it % kRaw, stage = it % kStages;
-      if (!warp_wait(&ctl.bar.raw_full[values][slot], (it / kRaw) & 1)) return false;
-      const uint32_t from = from0 + slot * Raw<HD>::kBytes;
-      uint32_t scales[2];
-      scales[0] = lds_at(scales0 + slot * Raw<HD>::kBytes);
-      if (SPT == 4) scales[1] = lds_at(scales0 + slot * Raw<HD>::kBytes + 4);
-      if (SPT == 1) scales[0] >>= 16 * (sub & 1);
+      const uint32_t stage = it & 1, phase = it >> 1 & 1, slot = stage * Raw<HD>::kBytes;
+      if (!warp_wait(&raw_full[stage], phase)) return false;
+      uint32_t scales[SPT / 2];
+#pragma unroll
+      for (int i = 0; i < SPT / 2; ++i) scales[i] = lds_at(scales_at + slot + 4 * i);
+      uint4 code[SPT];
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) code[i] = lds_v4_at((i & 1 ? from_odd : from_even) + slot + i * HD);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[stage]);
       if (tile * kTile + kTile > seg.r.length) {  // drafts, or past the end
         const int total = seg.r.length + seg.r.count;
 #pragma unroll
@@ -401,21 +415,19 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
           }
         }
       }
-      if (!warp_wait(&empty[stage], ((it / kStages) & 1) ^ 1)) return false;
-      const uint32_t base = mine + stage * kStageBytes;
-      uint4 code[SPT];
-#pragma unroll
-      for (int i = 0; i < SPT; ++i) code[i] = lds_v4_at(from + (i ^ swap) * HD);
+      if (!warp_wait(&empty[stage], phase ^ 1)) return false;
 #pragma unroll
       for (int i = 0; i < SPT; ++i) {
         const uint32_t two = __byte_perm(scales[i / 2], 0, select[i & 1]);
         const __nv_bfloat162 scale2 = *reinterpret_cast<const __nv_bfloat162*>(&two);
+        const __nv_bfloat162 h = __hmul2(scale2, __nv_bfloat162{0.5f, 0.5f});
+        const __nv_bfloat162 k = __hmul2(scale2, __nv_bfloat162{-128.f, -128.f});
         uint4 piece[2];
-        decode4(code[i].x, scale2, piece[0].x, piece[0].y);
-        decode4(code[i].y, scale2, piece[0].z, piece[0].w);
-        decode4(code[i].z, scale2, piece[1].x, piece[1].y);
-        decode4(code[i].w, scale2, piece[1].z, piece[1].w);
-        const uint32_t to = base ^ (i << 7 | i << 4);
+        decode4(code[i].x, h, k, piece[0].x, piece[0].y);
+        decode4(code[i].y, h, k, piece[0].z, piece[0].w);
+        decode4(code[i].z, h, k, piece[1].x, piece[1].y);
+        decode4(code[i].w, h, k, piece[1].z, piece[1].w);
+        const uint32_t to = (to0 + stage * kStageBytes) ^ (i << 7 | i << 4);
         sts_v4(to, piece[0]);
         sts_v4(to ^ 16, piece[1]);
       }
@@ -423,7 +435,6 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&full[stage]);
-        mbar_arrive(&ctl.bar.raw_empty[values][slot]);
       }
     }
   }
@@ -441,113 +452,130 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
+// One warp issues the score products, another the value products: the tensor core takes an
+// instruction only shortly before it can run it, so a single issuer stands idle in all its waits.
 template <int HD>
-__device__ __forceinline__ bool mma_role(const TreeArgs& a, Control& ctl, uint32_t ktiles, uint32_t vtiles, Walk walk) {
+__device__ __forceinline__ bool score_role(const TreeArgs& a, Control& ctl, uint32_t ktiles, Walk walk) {
   constexpr uint32_t kStageBytes = kTile * HD * 2;
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
-  const uint32_t idesc_s = idesc_bf16_m128(kTile), idesc_o = idesc_bf16_m128_bmn(HD);
-  const uint64_t kdesc = sdesc_sw128(ktiles, 1024u), vdesc = sdesc_sw128_mn(vtiles, kTile * 128, 1024u);
+  const uint32_t idesc = idesc_bf16_m128(kTile);
+  const uint64_t kdesc = sdesc_sw128(ktiles, 1024u);
   Segment seg;
   uint32_t it = 0;
-  auto scores = [&](uint32_t i) {
-    const uint32_t stage = i % kStages;
-    if (!warp_wait(&ctl.bar.k_full[stage], (i / kStages) & 1)) return false;
-    tc_fence_after();
-    const uint64_t desc = kdesc + stage * (kStageBytes >> 4);
-    const uint32_t d = tm + kColS + (i & 1) * kTile;
-    if (elect_one()) {
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k)
-        umma_ts(d, tm + kColQ + k * 8, desc + ((k / 4) * (kTile * 128) + (k % 4) * 32 >> 4), idesc_s, k != 0);
-      umma_commit(&ctl.bar.k_empty[stage]);
-      umma_commit(&ctl.bar.s_full[i & 1]);
-    }
-    __syncwarp();
-    return true;
-  };
-  auto values = [&](uint32_t i, bool first) {
-    const uint32_t stage = i % kStages;
-    if (!warp_wait(&ctl.bar.v_full[stage], (i / kStages) & 1)) return false;
-    if (!warp_wait(&ctl.bar.p_full[i & 1], (i / 2) & 1)) return false;
-    tc_fence_after();
-    const uint64_t desc = vdesc + stage * (kStageBytes >> 4);
-    const uint32_t p = tm + kColS + (i & 1) * kTile;
-    if (elect_one()) {
-#pragma unroll
-      for (int k = 0; k < kTile / 16; ++k) umma_ts(tm + kColO, p + k * 8, desc + k * (2048 >> 4), idesc_o, !first || k != 0);
-      umma_commit(&ctl.bar.v_empty[stage]);
-    }
-    __syncwarp();
-    return true;
-  };
   while (walk.next(a, seg)) {
     if (!warp_wait(&ctl.bar.q_full, seg.index & 1)) return false;
-    tc_fence_after();
-    const int n = seg.t1 - seg.t0;
-    for (int j = 0; j <= n; ++j) {
-      if (j < n && !scores(it + j)) return false;
-      if (j > 0 && !values(it + j - 1, j == 1)) return false;
+    for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
+      const uint32_t stage = it % kStages, phase = (it / kStages) & 1;
+      if (!warp_wait(&ctl.bar.k_full[stage], phase)) return false;
+      // the weights of the tile before last lie where these scores go: until its product is done
+      if (!warp_wait(&ctl.bar.v_empty[stage], phase ^ 1)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t desc = kdesc + stage * (kStageBytes >> 4);
+        const uint32_t d = tm + kColS + stage * kTile;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          umma_ts(d, tm + kColQ + k * 8, desc + ((k / 4) * (kTile * 128) + (k % 4) * 32 >> 4), idesc, k != 0);
+        umma_commit(&ctl.bar.k_empty[stage]);
+        umma_commit(&ctl.bar.s_full[stage]);
+      }
+      __syncwarp();
     }
-    if (elect_one()) umma_commit(&ctl.bar.o_full);
-    __syncwarp();
-    it += n;
+  }
+  return true;
+}
+
+template <int HD>
+__device__ __forceinline__ bool value_role(const TreeArgs& a, Control& ctl, uint32_t vtiles, Walk walk) {
+  constexpr uint32_t kStageBytes = kTile * HD * 2;
+  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
+  const uint32_t idesc = idesc_bf16_m128_bmn(HD);
+  const uint64_t vdesc = sdesc_sw128_mn(vtiles, kTile * 128, 1024u);
+  Segment seg;
+  uint32_t it = 0;
+  while (walk.next(a, seg)) {
+    for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
+      const uint32_t stage = it % kStages, phase = (it / kStages) & 1;
+      if (!warp_wait(&ctl.bar.v_full[stage], phase)) return false;
+      if (!warp_wait(&ctl.bar.p_full[stage], phase)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t desc = vdesc + stage * (kStageBytes >> 4);
+        const uint32_t p = tm + kColS + stage * kTile;
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_ts(tm + kColO, p + k * 8, desc + k * (2048 >> 4), idesc, tile != seg.t0 || k != 0);
+        umma_commit(&ctl.bar.v_empty[stage]);
+        if (tile + 1 == seg.t1) umma_commit(&ctl.bar.o_full);
+      }
+      __syncwarp();
+    }
   }
   return true;
 }
 
 // ---- softmax warps ------------------------------------------------------------------------
 
-// Q of a unit to TMEM. Rows pass through 4 KB of shared memory per warp (32 rows x 128 B, row r's
-// 16-byte piece j at j ^ (r % 8)): a thread owns a row in TMEM, but 8 threads read 128 B of a row from
-// global memory, which takes a quarter of the cache-line lookups of a thread per row.
+// Q of a unit to TMEM. Rows pass through 2 KB of shared memory per warp (32 rows x 64 B, row r's
+// 16-byte piece j at j ^ (r / 2 % 4)): a thread owns a row in TMEM, but 4 threads read 64 B of a row
+// from global memory, which takes a quarter of the cache-line lookups of a thread per row.
+// The two warps of a row take half of the channels each.
 template <int HD>
 __device__ __forceinline__ void load_q(const TreeArgs& a, const Segment& seg, uint32_t tm, uint32_t stage) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = seg.row_tile * kRows + warp * 32 + lane, node = row / a.rep;
-  const uint16_t* q = a.q + static_cast<int64_t>(seg.b) * a.N * a.q_stride + static_cast<int64_t>(seg.head) * a.rep * HD;
+  const int quarter = threadIdx.x >> 5 & 3, half = threadIdx.x >> 7, lane = threadIdx.x & 31;
+  const int row = seg.row_tile * kRows + quarter * 32 + lane, node = row / a.rep;
+  const uint16_t* q = a.q + static_cast<int64_t>(seg.b) * a.N * a.q_stride + static_cast<int64_t>(seg.head) * a.rep * HD +
+                      half * (HD / 2);
   const int mine = node < seg.r.count ? node * static_cast<int>(a.q_stride) + (row - node * a.rep) * HD : -1;
-  int at[8];
+  int at[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) at[i] = __shfl_sync(0xffffffffu, mine, 4 * i + lane / 8);
-  constexpr int kAtOnce = HD >= 128 ? 2 : 1;  // pieces of 64 channels in flight
-#pragma unroll 1
+  for (int i = 0; i < 4; ++i) at[i] = __shfl_sync(0xffffffffu, mine, 8 * i + lane / 4);
+  constexpr int kAtOnce = HD >= 128 ? 2 : 1;  // pieces of 32 channels in flight
+#pragma unroll
   for (int c0 = 0; c0 < HD / 64; c0 += kAtOnce) {
-    uint4 v[kAtOnce][8];
+    uint4 v[kAtOnce][4];
 #pragma unroll
     for (int c = 0; c < kAtOnce; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[c][i] = at[i] >= 0 ? ld_nc_v4(q + at[i] + (c0 + c) * 64 + lane % 8 * 8) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 4; ++i)
+        v[c][i] = at[i] >= 0 ? ld_nc_v4(q + at[i] + (c0 + c) * 32 + lane % 4 * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int c = 0; c < kAtOnce; ++c) {
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + lane / 8;
-        sts_v4(stage + r * 128 + ((lane ^ r) & 7) * 16, v[c][i]);
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + lane / 4;
+        sts_v4(stage + r * 64 + ((lane ^ r / 2) & 3) * 16, v[c][i]);
       }
       __syncwarp();
-      uint32_t u[32];
+      uint32_t u[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 x = lds_v4_at(stage + lane * 128 + ((i ^ lane) & 7) * 16);
+      for (int i = 0; i < 4; ++i) {
+        const uint4 x = lds_v4_at(stage + lane * 64 + ((i ^ lane / 2) & 3) * 16);
 #pragma unroll
         for (int w = 0; w < 4; ++w) u[i * 4 + w] = (word(x, w) & a.q_keep) ^ a.q_flip;
       }
-      tmem_st32(tm + kColQ + (c0 + c) * 32, u);
+      tmem_st16(tm + kColQ + half * (HD / 4) + (c0 + c) * 16, u);
     }
   }
   tmem_wait_st();
 }
 
+// Two warps per 32 rows, each with half of a tile's tokens: with one, its scores-to-weights chain was
+// the longest of all. They swap their rows' maxima through shared memory, decide alike, and keep a
+// sum each; O's rescaling and Q and O themselves are shared by channels.
 template <int HD>
 __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, uint32_t stage, Walk walk, int total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  constexpr int kHalf = kTile / 2;
+  const int warp = threadIdx.x >> 5, quarter = warp & 3, half = warp >> 2, lane = threadIdx.x & 31;
+  const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t o_cols = tm + kColO + half * (HD / 2);
+  float* my_top = &ctl.top[half][quarter * 32 + lane];
+  const float* other_top = &ctl.top[half ^ 1][quarter * 32 + lane];
   Segment seg, next;
   uint32_t it = 0;
   bool more = walk.next(a, next);
-  auto busy_of = [&](const Segment& s) { return s.row_tile * kRows + warp * 32 < s.r.count * a.rep; };
+  auto busy_of = [&](const Segment& s) { return s.row_tile * kRows + quarter * 32 < s.r.count * a.rep; };
   auto give_q = [&](const Segment& s) {
     if (busy_of(s)) load_q<HD>(a, s, tm, stage);
     tc_fence_before();
@@ -557,8 +585,7 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
   if (more) give_q(next);
   while (more) {
     seg = next;
-    const int row = seg.row_tile * kRows + warp * 32 + lane;
-    const int node = row / a.rep;
+    const int node = (seg.row_tile * kRows + quarter * 32 + lane) / a.rep;
     const bool live = node < seg.r.count;
     const bool busy = busy_of(seg);  // the same for the warp
     uint64_t path = 0;
@@ -571,35 +598,36 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
       if (!warp_wait(&ctl.bar.s_full[it & 1], (it / 2) & 1)) return false;
       if (busy) {
         tc_fence_after();
-        uint32_t s[2][32];
+        uint32_t s[kHalf];
         const uint32_t cols = tm + kColS + (it & 1) * kTile;
-        tmem_ld32(cols, s[0]);
-        tmem_ld32(cols + 32, s[1]);
+        tmem_ld32(cols + half * kHalf, s);
         tmem_wait_ld();
-        const int first = tile * kTile;
-        if (first + kTile > seg.r.length) {  // drafts, or past the end: the row's 64 bits
+        const int first = tile * kTile + half * kHalf;
+        if (first + kHalf > seg.r.length) {  // drafts, or past the end: the row's 32 bits
           const int cut = seg.r.length - first;
-          uint64_t see = 0;
-          if (cut > 0) see = cut < 64 ? (path << cut) | ((1ull << cut) - 1) : ~0ull;
-          else if (cut > -64) see = path >> -cut;
+          uint32_t see = 0;
+          if (cut > 0) see = static_cast<uint32_t>(path << cut) | ((1u << cut) - 1);
+          else if (cut > -64) see = static_cast<uint32_t>(path >> -cut);
           if (!live) see = 0;
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (!(see >> j & 1)) s[j / 32][j % 32] = 0xff800000u;
+          for (int j = 0; j < kHalf; ++j)
+            if (!(see >> j & 1)) s[j] = 0xff800000u;
         }
         float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) {
-          top = max3(top, __uint_as_float(s[j / 32][j % 32]), __uint_as_float(s[j / 32][j % 32 + 1]));
-          top2 = max3(top2, __uint_as_float(s[j / 32][j % 32 + 2]), __uint_as_float(s[j / 32][j % 32 + 3]));
+        for (int j = 0; j < kHalf; j += 4) {
+          top = max3(top, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+          top2 = max3(top2, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
         }
-        top = fmaxf(top, top2);
-        top *= a.scale_log2;
+        *my_top = fmaxf(top, top2);
+        // the pair's scores are both read by then: P may go over either's columns
+        pair_sync(quarter);
+        top = fmaxf(fmaxf(top, top2), *other_top) * a.scale_log2;
         const bool grow = top > m + kLazyGrowth;
         if (__any_sync(0xffffffffu, grow)) {
-          const float next = fmaxf(m, top);
-          const float keep = m == -INFINITY ? 0.f : exp2_fast(m - next);
-          m = next;
+          const float now = fmaxf(m, top);
+          const float keep = m == -INFINITY ? 0.f : exp2_fast(m - now);
+          m = now;
           l *= keep;
           if (tile > seg.t0) {
             // every product so far has left O: the commit of the tile before
@@ -607,25 +635,24 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
             if (!warp_wait(&ctl.bar.v_empty[last % kStages], (last / kStages) & 1)) return false;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
+            for (int c = 0; c < HD / 64; ++c) {
               uint32_t o[32];
-              tmem_ld32(tm + kColO + c * 32, o);
+              tmem_ld32(o_cols + c * 32, o);
               tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-              tmem_st32(tm + kColO + c * 32, o);
+              tmem_st32(o_cols + c * 32, o);
             }
           }
         }
         const float shift = m == -INFINITY ? 0.f : m;
         const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), shift2 = pair(-shift, -shift);
         uint64_t sum[2] = {0, 0};
-        uint32_t p[32];
+        uint32_t p[kHalf / 2];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < kHalf / 2; ++j) {
           float x, y;
-          unpair(fma2(pair(__uint_as_float(s[j / 16][(2 * j) % 32]), __uint_as_float(s[j / 16][(2 * j + 1) % 32])), scale2,
-                      shift2), x, y);
+          unpair(fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, shift2), x, y);
           x = exp2_fast(x);
           y = exp2_fast(y);
           sum[j & 1] = add2(sum[j & 1], pair(x, y));
@@ -634,14 +661,13 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
         float even, odd;
         unpair(add2(sum[0], sum[1]), even, odd);
         l += even + odd;
-        tmem_st32(cols, p);
+        tmem_st16(cols + half * (kHalf / 2), p);
         tmem_wait_st();
         tc_fence_before();
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.bar.p_full[it & 1]);
     }
-
     // every product with this Q is done: the next unit's Q goes in and its first scores are on their
     // way while this unit's O leaves
     more = walk.next(a, next);
@@ -651,14 +677,14 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
     tc_fence_after();
     // The unit's part of O as it is, FP32, channel by channel (32 rows are 128 B): the join divides,
     // gates and rounds. A quarter of the instructions of doing that here, where nothing hides them.
-    const uint64_t* bad = ctl.bad[seg.index % kBadRing];
+    const uint64_t* bad = ctl.bad[seg.index % kBadRing] + half * (HD / 64);
     const int unit = (seg.b * a.kv + seg.head) * a.row_tiles + seg.row_tile;
     const int64_t record = static_cast<int64_t>(unit) + blockIdx.x;
-    float* part = a.part + record * HD * a.part_rows + warp * 32 + lane;
+    float* part = a.part + (record * HD + half * (HD / 2)) * a.part_rows + quarter * 32 + lane;
 #pragma unroll 1
-    for (int c = 0; c < HD / 32; ++c) {
+    for (int c = 0; c < HD / 64; ++c) {
       uint32_t o[32];
-      tmem_ld32(tm + kColO + c * 32, o);
+      tmem_ld32(o_cols + c * 32, o);
       tmem_wait_ld();
       if (bad[c] & path) {
 #pragma unroll
@@ -668,15 +694,16 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
       for (int j = 0; j < 32; ++j) part[(c * 32 + j) * a.part_rows] = __uint_as_float(o[j]);
       __syncwarp();
     }
-    float* stats = a.stats + record * 2 * a.part_rows + warp * 32 + lane;
-    stats[0] = m;
-    stats[a.part_rows] = l;
+    float* stats = a.stats + record * 3 * a.part_rows + quarter * 32 + lane;
+    if (half == 0) stats[0] = m;
+    stats[(1 + half) * a.part_rows] = l;
     if (seg.t0 == 0 && threadIdx.x == 0)
       a.parts[unit] = Parts{static_cast<int>(blockIdx.x),
                             Ranges(total, gridDim.x).owner(seg.start + seg.r.tiles - 1) - static_cast<int>(blockIdx.x) + 1};
     tc_fence_before();
     if (seg.r.length < seg.t1 * kTile) {  // the unit saw drafts: its record of bad values is read, clear it
-      asm volatile("bar.sync 1, %0;" ::"r"(32 * min(kSoftmaxWarps, (seg.r.count * a.rep - seg.row_tile * kRows + 31) / 32)) : "memory");
+      const int pairs = min(kSoftmaxWarps / 2, (seg.r.count * a.rep - seg.row_tile * kRows + 31) / 32);
+      asm volatile("bar.sync 5, %0;" ::"r"(64 * pairs) : "memory");
       if (warp == 0 && lane < 8) ctl.bad[seg.index % kBadRing][lane] = 0;
     }
   }
@@ -712,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     fence_mbar_init();
   }
   if (threadIdx.x < kBadRing * 8) ctl.bad[threadIdx.x / 8][threadIdx.x % 8] = 0;
-  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, 512);
+  if (warp == kScoreWarp) tmem_alloc(&ctl.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -726,17 +753,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
   bool ok = true;
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    ok = softmax_role<HD>(a, ctl, rows + warp * 4096, walk, total);
+    ok = softmax_role<HD>(a, ctl, rows + warp * kQStage, walk, total);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp < kMmaWarp) ok = decode_role<HD>(a, ctl, ktiles, raw, walk);
+    if (warp < kScoreWarp) ok = decode_role<HD>(a, ctl, ktiles, raw, walk);
     else if (warp == kCopyWarp || warp == kCopyWarp + 1) ok = copy_role<HD>(a, ctl, maps, raw, warp - kCopyWarp, walk);
-    else if (warp == kMmaWarp) ok = mma_role<HD>(a, ctl, ktiles, vtiles, walk);
+    else if (warp == kScoreWarp) ok = score_role<HD>(a, ctl, ktiles, walk);
+    else ok = value_role<HD>(a, ctl, vtiles, walk);
   }
   if (!ok) *a.status = QK_ERR_TIMEOUT;
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     tc_fence_after();
     tmem_dealloc(ctl.tmem, 512);
   }
@@ -747,7 +775,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 // Every row of the output, also those of nodes that are not there, in pieces of 32 rows (a lane
 // each) x 16 channels. WARPS warps share a piece: 1 where there are enough pieces to fill the GPU, 8
 // where few units have many parts (a unit can have as many as there are ranges): each takes every
-// WARPS-th part, and shared memory adds them in a fixed order.
+// WARPS-th part, and shared memory adds them in a fixed order. Bound by latency: two rounds of loads,
+// what the piece is and then its parts, so everything that can is asked for in the first.
 constexpr int kJoinWarps = 8, kJoinCols = 16;
 
 template <int HD, int WARPS>
@@ -755,8 +784,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
   __shared__ float red[WARPS > 1 ? WARPS : 1][2][32];
   __shared__ float acc[WARPS > 1 ? WARPS : 1][kJoinCols][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_wait();
-  pdl_trigger();
   const int p = WARPS > 1 ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
   if (p >= pieces) return;
   const int groups = a.part_rows / 32, pr = a.part_rows;
@@ -764,31 +791,33 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
   const int unit = p / groups / (HD / kJoinCols);
   const int b = unit / (a.kv * a.row_tiles), head = unit / a.row_tiles % a.kv, row_tile = unit % a.row_tiles;
   const int in_tile = group * 32 + lane, row = row_tile * kRows + in_tile, node = row / a.rep;
-  const int count = load_request(a, b).count;
   const int64_t to =
       ((static_cast<int64_t>(b) * a.N + node) * a.hq + head * a.rep + (row - node * a.rep)) * HD + col0;
-  uint4* out = reinterpret_cast<uint4*>(a.out + to);
-  if (row - lane >= count * a.rep) {  // nobody in these rows
-    if (warp % WARPS == 0 && node < a.N) out[0] = out[1] = make_uint4(0, 0, 0, 0);
-    return;
-  }
+  const int first = WARPS > 1 ? warp : 0;
+  pdl_wait();
+  pdl_trigger();
   uint4 gate[2];
-  if (a.gate && node < count) {
+  if (a.gate && first == 0 && node < a.N) {
     gate[0] = ld_nc_v4(a.gate + to);
     gate[1] = ld_nc_v4(a.gate + to + 8);
   }
   const Parts parts = a.parts[unit];
+  const int count = load_request(a, b).count;
+  uint4* out = reinterpret_cast<uint4*>(a.out + to);
+  if (row - lane >= count * a.rep) {  // nobody in these rows
+    if (first == 0 && node < a.N) out[0] = out[1] = make_uint4(0, 0, 0, 0);
+    return;
+  }
   const int64_t record = static_cast<int64_t>(unit) + parts.first;
-  const int first = WARPS > 1 ? warp : 0;
   // one pass with a running maximum, as over tiles
   float m = -INFINITY, l = 0.f, o[kJoinCols];
 #pragma unroll
   for (int j = 0; j < kJoinCols; ++j) o[j] = 0.f;
 #pragma unroll 2
   for (int i = first; i < parts.count; i += WARPS) {
-    const float* st = a.stats + (record + i) * 2 * pr + in_tile;
+    const float* st = a.stats + (record + i) * 3 * pr + in_tile;
     const float* part = a.part + ((record + i) * HD + col0) * pr + in_tile;
-    const float x = st[0], y = st[pr];
+    const float x = st[0], y = st[pr] + st[2 * pr];
     float v[kJoinCols];
 #pragma unroll
     for (int j = 0; j < kJoinCols; ++j) v[j] = part[j * pr];
@@ -823,21 +852,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
   }
   if (node >= a.N) return;
   const float inv = node < count && (l > 0.f || l != l) ? 1.f / l : 0.f;
-  uint32_t w[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float f[8], z[8];
-    unpack8(gate[h], z);
+    if (a.gate) unpack8(gate[h], z);
+    uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       f[j] = inv == 0.f ? 0.f : o[h * 8 + j] * inv;
-      if (a.gate) f[j] *= node < count ? sigmoid_fast(z[j]) : 0.f;
+      if (a.gate && inv != 0.f) f[j] *= sigmoid_fast(z[j]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[h * 4 + j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+    out[h] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  out[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  out[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 constexpr size_t kHeader = 256;
@@ -878,21 +906,21 @@ Layout layout_of(int B, int N, int hq, int kv, int hd) {
   w.records = w.units + sm_count();
   w.parts = kHeader;
   w.stats = w.parts + (w.units * sizeof(Parts) + 255) / 256 * 256;
-  w.part = w.stats + static_cast<size_t>(w.records) * 2 * w.part_rows * sizeof(float);
+  w.part = w.stats + static_cast<size_t>(w.records) * 3 * w.part_rows * sizeof(float);
   w.bytes = w.part + static_cast<size_t>(w.records) * hd * w.part_rows * sizeof(float);
   return w;
 }
 
 template <int HD>
 int launch(const Maps& maps, const TreeArgs& a, const Layout& w, cudaStream_t st) {
-  const size_t smem = 1024 + 2 * kStages * static_cast<size_t>(kTile) * HD * 2 + kRaw * Raw<HD>::kBytes + kSoftmaxWarps * 4096;
+  const size_t smem = 1024 + 2 * kStages * static_cast<size_t>(kTile) * HD * 2 + kRaw * Raw<HD>::kBytes + kSoftmaxWarps * kQStage;
   const int rc = allow_smem(reinterpret_cast<const void*>(tree_attention_kernel<HD>), smem);
   if (rc) return rc;
   // one CTA per SM: each holds all of its SM's tensor memory
   cudaError_t e = launch_dependent(tree_attention_kernel<HD>, dim3(sm_count()), dim3(kThreads), smem, st, maps, a);
   if (e != cudaSuccess) return cuda_error(e, "tree_attention_kernel");
   const int pieces = static_cast<int>(w.units * (w.part_rows / 32) * (HD / kJoinCols));
-  if (pieces >= 16 * sm_count()) {
+  if (pieces >= 4 * sm_count()) {
     e = launch_dependent(tree_join_kernel<HD, 1>, dim3((pieces + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, st,
                          a, pieces);
   } else {
