@@ -234,5 +234,24 @@ def stream_handle(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def call_on(device, name, *args):
+    """``name(*args, stream)`` with ``device`` current, on its current stream: for entry points that
+    take plain addresses (``Tensor.data_ptr()`` or None) and the stream last. Leaner than a device
+    guard and stream object of its own: a decode step makes many calls of a few microseconds."""
+    import torch
+
+    if device.type != "cuda":
+        raise ValueError("expected CUDA tensors")
+    index = torch.cuda.current_device() if device.index is None else device.index
+    fn = getattr(_lib or load(), name)
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != QK_OK:
+        check(status)
+
+
 def launch_count():
     return int(load().qk_launch_count())

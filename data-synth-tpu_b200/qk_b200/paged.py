@@ -64,7 +64,7 @@ NO_PAGES, TABLE_FULL, BAD_LENGTH, BAD_PARENT = 1, 2, 4, 8
 
 def _array(t, name, dtype, shape, device):
     """``t`` on ``device``, contiguous and of the dtype; a ValueError for another shape."""
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype != dtype or t.device != device:
         t = t.to(device=device, dtype=dtype)
@@ -102,41 +102,42 @@ def plan_step(table, held, ring, span, lengths, counts, *, nodes, page_size, par
             raise ValueError("a draft tree has at most 64 nodes")
         parents = _array(parents, "parents", i32, (batch, nodes), device)
     if out is None:
-        words = torch.empty((batch, nodes), dtype=torch.int64, device=device) if nodes <= 64 else None
-        new = torch.empty(2 * batch * (nodes + 1) + 2, dtype=i32, device=device)
-        slots, positions, rest = new.split((batch * nodes, batch * nodes, 2 * batch + 2))
-        out = StepPlan(slots.view(batch, nodes), positions.view(batch, nodes), words, rest[:batch], rest[2 * batch:],
-                       rest[batch:2 * batch])
+        slots = torch.empty((batch, nodes), dtype=i32, device=device) if parents is None else torch.empty_like(parents)
+        out = StepPlan(slots, torch.empty_like(slots),
+                       torch.empty((batch, nodes), dtype=torch.int64, device=device) if nodes <= 64 else None,
+                       torch.empty_like(held), torch.empty_like(span), torch.empty_like(held))
     elif out.slots.shape != (batch, nodes) or out.slots.device != device:
         raise ValueError("out must be the plan of as many requests and nodes on the same device")
-    with torch.cuda.device(device):
-        ptr = _lib.ptr
-        _lib.call("qk_paged_plan", ptr(table), ptr(held), ptr(ring), ptr(span), ptr(lengths), ptr(counts), ptr(parents),
-                  batch, width, ring.shape[0], page_size, nodes, ptr(out.slots), ptr(out.positions),
-                  ptr(out.ancestors), ptr(out.held), ptr(out.span), ptr(out.status), _lib.stream_handle(device))
+    _lib.call_on(device, "qk_paged_plan", table.data_ptr(), held.data_ptr(), ring.data_ptr(), span.data_ptr(),
+                 lengths.data_ptr(), counts.data_ptr(), None if parents is None else parents.data_ptr(), batch, width,
+                 ring.shape[0], page_size, nodes, out.slots.data_ptr(), out.positions.data_ptr(),
+                 None if out.ancestors is None else out.ancestors.data_ptr(), out.held.data_ptr(), out.span.data_ptr(),
+                 out.status.data_ptr())
     return out
 
 
 def _cache_geometry(cache, kv, hd, device):
-    """``(rows, T)`` of a Q8 cache on ``device``, whose arrays must be of the framework's layout."""
-    codes, plane = cache["k"], cache["k_scale"]
-    groups = kv * (hd // min(32, hd))
-    if codes.dim() != 3 or codes.shape[2] != kv * hd or tuple(plane.shape) != (codes.shape[0] * groups, codes.shape[1]):
+    """``(k, v, k_scale, v_scale, rows, T)`` of a Q8 cache on ``device``, whose arrays must be of the
+    framework's layout."""
+    k, v, ks, vs = cache["k"], cache["v"], cache["k_scale"], cache["v_scale"]
+    shape, plane = k.shape, ks.shape
+    if len(shape) != 3 or shape[2] != kv * hd or plane != (shape[0] * (kv * hd // min(32, hd)), shape[1]):
         raise ValueError("cache must hold codes [R, T, kv * hd] and scale planes [R * G, T] of these heads")
-    for name in ("k", "v"):
-        c, s = cache[name], cache[name + "_scale"]
-        if c.dtype != torch.int8 or s.dtype != torch.bfloat16:
-            raise TypeError("cache codes must be int8 and scales BF16")
-        if c.device != device or s.device != device:
-            raise ValueError("the cache must be on the device of the tokens")
-        if c.shape != codes.shape or s.shape != plane.shape or not (c.is_contiguous() and s.is_contiguous()):
-            raise ValueError("cache keys and values must be contiguous and of the same shape")
-    return codes.shape[0], codes.shape[1]
+    if k.dtype != torch.int8 or v.dtype != torch.int8 or ks.dtype != torch.bfloat16 or vs.dtype != torch.bfloat16:
+        raise TypeError("cache codes must be int8 and scales BF16")
+    if not (k.device == v.device == ks.device == vs.device == device):
+        raise ValueError("the cache must be on the device of the tokens")
+    if v.shape != shape or vs.shape != plane or not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
+                                                     and vs.is_contiguous()):
+        raise ValueError("cache keys and values must be contiguous and of the same shape")
+    return k, v, ks, vs, shape[0], shape[1]
 
 
 def _tokens(x, width):
     """``x`` ``[..., kv, hd]`` as rows of ``width`` values: ``(x, stride)``; copied only where its
     tokens are not evenly spaced 16-byte aligned rows."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, width
     per = 16 // x.element_size()
     lead = x.shape[:-2]
     dense = x.stride(-1) == 1 and (x.shape[-2] == 1 or x.stride(-2) == x.shape[-1])
@@ -163,18 +164,16 @@ def write_slots(cache, key, value, slots):
         raise ValueError("key and value must be [..., kv, hd] with one slot for every token")
     kv, hd = key.shape[-2:]
     device = key.device
-    rows, time = _cache_geometry(cache, kv, hd, device)
+    k, v, ks, vs, rows, time = _cache_geometry(cache, kv, hd, device)
     code = _dtype_code(key)
     if value.dtype != key.dtype or value.device != device:
         value = value.to(device=device, dtype=key.dtype)
     key, key_stride = _tokens(key, kv * hd)
     value, value_stride = _tokens(value, kv * hd)
-    slots = _array(slots, "slots", torch.int32, tuple(slots.shape), device)
-    with torch.cuda.device(device):
-        ptr = _lib.ptr
-        _lib.call("qk_kv_q8_write_slots", ptr(key), ptr(value), code, key_stride, value_stride, ptr(slots),
-                  ptr(cache["k"]), ptr(cache["v"]), ptr(cache["k_scale"]), ptr(cache["v_scale"]), slots.numel(), rows,
-                  time, kv, hd, _lib.stream_handle(device))
+    slots = _array(slots, "slots", torch.int32, slots.shape, device)
+    _lib.call_on(device, "qk_kv_q8_write_slots", key.data_ptr(), value.data_ptr(), code, key_stride, value_stride,
+                 slots.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), slots.numel(), rows, time, kv,
+                 hd)
     return cache
 
 
@@ -183,13 +182,18 @@ class TreeAttention:
 
     def __init__(self):
         self._ws = {}
+        self._need = {}
 
-    def _workspace(self, device, stream, need):
-        key = (device.index, stream.value)
+    def _workspace(self, device, geometry):
+        """The zeroed workspace of the device's current stream, of the size for ``(B, N, hq, kv, hd)``."""
+        need = self._need.get(geometry)
+        if need is None:
+            with torch.cuda.device(device):
+                need = self._need[geometry] = int(_lib.load().qk_tree_attention_workspace_bytes(*geometry))
+        key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
         ws = self._ws.get(key)
         if ws is None or ws.numel() < need:
-            ws = torch.zeros(need, dtype=torch.uint8, device=device)
-            self._ws[key] = ws
+            ws = self._ws[key] = torch.zeros(need, dtype=torch.uint8, device=device)
         return ws
 
     def __call__(self, q, cache, table, lengths, ancestors, *, page_size, counts=None, gate=None, scale=None, out=None):
@@ -200,50 +204,49 @@ class TreeAttention:
         times ``sigmoid(gate)`` where a gate is given; nodes past ``counts[b]`` are zero."""
         if q.dtype != torch.bfloat16 or q.dim() != 4:
             raise TypeError("q must be BF16 [B, N, query_heads, head_dim]")
-        batch, nodes, hq, hd = q.shape
+        shape, device = q.shape, q.device
+        batch, nodes, hq, hd = shape
         if hd not in (64, 128, 256):
             raise ValueError("head_dim must be 64, 128 or 256")
+        if not 1 <= nodes <= 64:
+            raise ValueError("a request has 1 to 64 nodes")
+        if not q.is_cuda:
+            raise ValueError("expected CUDA tensors")
         kv = cache["k"].shape[-1] // hd
         if kv < 1 or hq % kv:
             raise ValueError("Head counts must have integer repetition factors")
-        device = q.device
-        rows, time = _cache_geometry(cache, kv, hd, device)
+        k, v, ks, vs, rows, time = _cache_geometry(cache, kv, hd, device)
         if table.dim() != 2 or table.shape[0] != batch:
             raise ValueError("table must be [B, width]")
         q, stride = _tokens(q, hq * hd)
-        table = _array(table, "table", torch.int32, tuple(table.shape), device)
+        table = _array(table, "table", torch.int32, table.shape, device)
         lengths = _array(lengths, "lengths", torch.int32, (batch,), device)
         ancestors = _array(ancestors, "ancestors", torch.int64, (batch, nodes), device)
         if counts is not None:
             counts = _array(counts, "counts", torch.int32, (batch,), device)
         if gate is not None:
-            gate = _array(gate, "gate", torch.bfloat16, (batch, nodes, hq, hd), device)
+            gate = _array(gate, "gate", torch.bfloat16, shape, device)
         if out is None:
-            out = torch.empty((batch, nodes, hq, hd), dtype=torch.bfloat16, device=device)
-        elif (out.dtype != torch.bfloat16 or out.shape != (batch, nodes, hq, hd) or out.device != device
-              or not out.is_contiguous()):
+            out = torch.empty(shape, dtype=torch.bfloat16, device=device) if stride != hq * hd else torch.empty_like(q)
+        elif out.dtype != torch.bfloat16 or out.shape != shape or out.device != device or not out.is_contiguous():
             raise ValueError("out must be contiguous BF16 of q's shape")
-        with torch.cuda.device(device):
-            ptr, lib = _lib.ptr, _lib.load()
-            stream = _lib.stream_handle(device)
-            need = lib.qk_tree_attention_workspace_bytes(batch, nodes, hq, kv, hd)
-            ws = self._workspace(device, stream, need)
-            _lib.check(lib.qk_tree_attention(
-                ptr(q), stride, ptr(cache["k"]), ptr(cache["v"]), ptr(cache["k_scale"]), ptr(cache["v_scale"]),
-                ptr(table), ptr(lengths), ptr(counts), ptr(ancestors), ptr(gate),
-                hd ** -0.5 if scale is None else scale, batch, nodes, hq, kv, hd, rows, time, table.shape[1], page_size,
-                ptr(out), ptr(ws), ws.numel(), stream))
+        ws = self._workspace(device, (batch, nodes, hq, kv, hd))
+        _lib.call_on(device, "qk_tree_attention", q.data_ptr(), stride, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+                     vs.data_ptr(), table.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
+                     ancestors.data_ptr(), None if gate is None else gate.data_ptr(), hd ** -0.5 if scale is None else scale,
+                     batch, nodes, hq, kv, hd, rows, time, table.shape[1], page_size, out.data_ptr(), ws.data_ptr(),
+                     ws.numel())
         return out
 
     def check_status(self, device=None):
         """Raise what earlier calls on the current stream reported (a table entry outside the
-        cache, a bounded wait that gave up); synchronises the stream."""
+        cache, a length outside the table, a bounded wait that gave up); synchronises the stream."""
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         with torch.cuda.device(device):
-            stream = _lib.stream_handle(device)
-            ws = self._ws.get((torch.cuda.current_device(), stream.value))
+            index = torch.cuda.current_device()
+            ws = self._ws.get((index, torch._C._cuda_getCurrentRawStream(index)))
             if ws is not None:
-                _lib.call("qk_tree_attention_check", _lib.ptr(ws), stream)
+                _lib.call_on(torch.device("cuda", index), "qk_tree_attention_check", ws.data_ptr())
 
 
 tree_attention = TreeAttention()

@@ -34,7 +34,7 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
     if logits.dim() not in (2, 3):
         raise ValueError("logits must be [B, V] or [B, N, V]")
     code = _dtype_code(logits)
-    device, shape = logits.device, tuple(logits.shape)
+    device, shape = logits.device, logits.shape
     batch, nodes, vocab = shape if len(shape) == 3 else (shape[0], 1, shape[1])
     logits = logits if logits.is_contiguous() else logits.contiguous()
     keep = []  # arrays that the call reads
@@ -76,12 +76,10 @@ def process_logits(logits, *, history=None, history_lengths=None, prompt_lengths
         d.drafts = array(drafts, "drafts", i32, (batch, nodes))
         d.ancestors = array(ancestors, "ancestors", torch.int64, (batch, nodes))
     if out is None:
-        out = torch.empty(shape, dtype=f32, device=device)
-    elif out.dtype != f32 or tuple(out.shape) != shape or out.device != device or not out.is_contiguous():
+        out = torch.empty_like(logits, dtype=f32)
+    elif out.dtype != f32 or out.shape != shape or out.device != device or not out.is_contiguous():
         raise ValueError("out must be contiguous FP32 of the logits' shape")
-    with torch.cuda.device(device):
-        _lib.call("qk_process_logits", ctypes.byref(d), _lib.ptr(logits), code, batch, nodes, vocab, _lib.ptr(out),
-                  _lib.stream_handle(device))
+    _lib.call_on(device, "qk_process_logits", ctypes.byref(d), logits.data_ptr(), code, batch, nodes, vocab, out.data_ptr())
     return out
 
 
