@@ -115,6 +115,39 @@ __global__ void read_kernel(const int8_t* __restrict__ codes, const uint16_t* __
   }
 }
 
+// read_kernel for 8 channels per thread (one 8-byte load of codes, one scale; groups of 8 channels or
+// more): the same values, at an eighth of the index arithmetic, which bounded it (8448 slots of 1024
+// channels to BF16: 51 -> 6 us). I: an index type that holds `total`.
+template <typename I>
+__global__ void __launch_bounds__(256) read8_kernel(const int8_t* __restrict__ codes, const uint16_t* __restrict__ plane,
+                                                    const int32_t* __restrict__ idx, I total, I S, int T, int D8, int G,
+                                                    int group8, int out_bf16, void* __restrict__ out) {
+  const I stride = static_cast<I>(gridDim.x) * blockDim.x;
+  for (I i = static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const I bs = i / D8;
+    const int col = static_cast<int>(i - bs * D8);
+    const int64_t b = bs / S;
+    const int t = wrap_clamp(idx[bs], T);
+    const uint2 c = *reinterpret_cast<const uint2*>(codes + ((b * T + t) * D8 + col) * 8);
+    const float scale = bf16_to_f32(plane[(b * G + col / group8) * T + t]);
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      f[k] = __fmul_rn(static_cast<float>(static_cast<int8_t>((k < 4 ? c.x : c.y) >> (8 * (k & 3)))), scale);
+    if (out_bf16) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = bf16_bits_rne(f[2 * k]) | static_cast<uint32_t>(bf16_bits_rne(f[2 * k + 1])) << 16;
+      reinterpret_cast<uint4*>(out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      float4* o = reinterpret_cast<float4*>(out) + 2 * static_cast<int64_t>(i);
+      o[0] = make_float4(f[0], f[1], f[2], f[3]);
+      o[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  }
+}
+
 int grid_for(int64_t total, int block) {
   int64_t g = (total + block - 1) / block;
   const int64_t cap = static_cast<int64_t>(sm_count()) * 16;
@@ -197,6 +230,19 @@ int qk_kv_q8_read(const int8_t* codes, const uint16_t* plane, const int32_t* ind
   if (B == 0 || S == 0) return QK_OK;
   QK_REQUIRE(codes && plane && indices && out, "null pointer");
   const int D = kv_heads * head_dim;
+  if (group % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+    const int64_t total = static_cast<int64_t>(B) * S * (D / 8);
+    const int grid = grid_for(total, 256);
+    // the stride past the end of a 32-bit index must not wrap
+    if (total < (1ll << 31))
+      read8_kernel<uint32_t><<<grid, 256, 0, as_stream(stream)>>>(codes, plane, indices, static_cast<uint32_t>(total), S, T, D / 8,
+                                                                 D / group, group / 8, out_dtype == QK_OUT_BF16, out);
+    else
+      read8_kernel<uint64_t><<<grid, 256, 0, as_stream(stream)>>>(codes, plane, indices, static_cast<uint64_t>(total), S, T, D / 8,
+                                                                 D / group, group / 8, out_dtype == QK_OUT_BF16, out);
+    QK_LAUNCHED("read8_kernel");
+    return QK_OK;
+  }
   read_kernel<<<grid_for(static_cast<int64_t>(B) * S * D, 256), 256, 0, as_stream(stream)>>>(
       codes, plane, indices, B, S, T, D, group, out_dtype == QK_OUT_BF16, out);
   QK_LAUNCHED("read_kernel");

@@ -191,29 +191,39 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a) {
   }
 }
 
+// rint(x / scale) of the codec. The product with the reciprocal is within 2^-22 of the quotient, of
+// at most 127, so it rounds to the same integer unless it lies that close to a half (or is not
+// finite, or the reciprocal overflowed): then, once in some thousand values, the division decides.
+__device__ __forceinline__ float code_of(float x, float scale, float inverse) {
+  const float q = x * inverse;
+  float n = rintf(q);
+  if (!(fabsf(fabsf(q - n) - 0.5f) >= 1.f / 8192)) n = rintf(__fdiv_rn(x, scale));
+  return fminf(fmaxf(n, -127.f), 127.f);
+}
+
 // Codec and scatter: a thread per 8 channels (one 16-byte load of BF16, two of FP32), the
 // group's maximum over its 4 lanes, 8 bytes of codes per thread and one BF16 scale per group.
-// The arithmetic is the append's: scale = bf16(max|x| / 127), code = rint(x / scale) with IEEE
-// divisions, so a token's codes do not depend on the entry point that wrote it.
+// The codes and scales are the append's (scale = bf16(max|x| / 127), code = rint(x / scale) of IEEE
+// quotients), so a token's bytes do not depend on the entry point that wrote it.
 template <bool BF16>
 __global__ void __launch_bounds__(256) write_slots_kernel(const void* __restrict__ key, const void* __restrict__ value,
                                                           int64_t key_stride, int64_t value_stride,
                                                           const int32_t* __restrict__ slots, int8_t* k_codes,
                                                           int8_t* v_codes, uint16_t* k_scale, uint16_t* v_scale,
-                                                          int64_t total, int D8, int G, int group8, int64_t T,
+                                                          uint32_t total, int D8, int G, int group8, int64_t T,
                                                           int64_t room) {
   pdl_wait();  // launched as a programmatic dependent: the keys' and values' producer first
   pdl_trigger();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;  // below 2^32: checked by the host
   const bool in = i < total;
-  const int col = in ? static_cast<int>(i % D8) : 0;
-  const int64_t item = in ? i / D8 : 0;
+  const uint32_t item = in ? i / D8 : 0;
+  const int col = in ? static_cast<int>(i - item * D8) : 0;
   const bool is_value = item & 1;
   const int64_t token = item >> 1;
   const int64_t slot = in ? slots[token] : -1;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const bool live = in && slot >= 0 && slot < room;
-  if (live) {
+  if (in) {  // also where the slot says padding: the values need not wait for it
     const int64_t at = token * (is_value ? value_stride : key_stride) + col * 8;
     if (BF16) {
       unpack8(ld_nc_v4(static_cast<const uint16_t*>(is_value ? value : key) + at), x);
@@ -233,11 +243,11 @@ __global__ void __launch_bounds__(256) write_slots_kernel(const void* __restrict
   for (int o = group8 >> 1; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!live) return;
   const float scale = bf16_round(__fdiv_rn(amax, 127.f));
-  const float divisor = scale == 0.f ? 1.f : scale;
+  const float divisor = scale == 0.f ? 1.f : scale, inverse = __frcp_rn(divisor);
   uint32_t code[2] = {0, 0};
 #pragma unroll
   for (int t = 0; t < 8; ++t) {
-    const int q = static_cast<int8_t>(fminf(fmaxf(rintf(__fdiv_rn(x[t], divisor)), -127.f), 127.f));
+    const int q = static_cast<int8_t>(code_of(x[t], divisor, inverse));
     code[t >> 2] |= static_cast<uint32_t>(q & 255) << (8 * (t & 3));
   }
   int8_t* codes = is_value ? v_codes : k_codes;
@@ -295,11 +305,11 @@ int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64
              "codes must be 8-byte aligned");
   const int64_t total = tokens * 2 * (D / 8);
   const int64_t grid = (total + 255) / 256;
-  QK_REQUIRE(grid < (1ll << 31), "too many tokens in one call");
+  QK_REQUIRE(grid * 256 < (1ll << 32), "too many tokens in one call");
   const auto kernel = in_dtype == QK_OUT_BF16 ? write_slots_kernel<true> : write_slots_kernel<false>;
   const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, as_stream(stream),
                                          key, value, key_stride, value_stride, slots, k_codes, v_codes, k_scale, v_scale,
-                                         total, D / 8, D / group, group / 8, T, static_cast<int64_t>(rows) * T);
+                                         static_cast<uint32_t>(total), D / 8, D / group, group / 8, T, static_cast<int64_t>(rows) * T);
   if (e != cudaSuccess) return cuda_error(e, "write_slots_kernel");
   count_launch();
   return QK_OK;

@@ -1,24 +1,23 @@
 // Logits before the choice: penalties for repeated tokens, sparse biases, temperature and a
 // grammar's bit mask, in one pass over the vocabulary.
 //
-//   x = logit;  in the context (history or drafted path):  x = x > 0 ? x / r : x * r
+//   x = logit;  in the context (history or drafted path):  x = x > 0 ? x * (1 / r) : x * r
 //   x -= f * count + p * [count > 0];  x += bias;  x /= temperature;  mask bit 0: x = -inf
 //
 // Bound by HBM: a logit in, an FP32 value out, one mask bit per entry. A block owns a tile of
 // the vocabulary of one request and counts the request's history into one 32-bit word per
 // entry in shared memory (the history is re-read by every tile, from L2); the words then serve
-// all rows of the request, one per node of a draft tree. Entries of the word: bits 0-19 the
-// count of generated tokens, then flags: in the prompt, drafted, biased. Most words are zero
-// and take the short path (one multiply); drafted and biased entries, at most a few hundred per
-// request, look their nodes or their bias up in short lists. Counts are integers and the last of
-// several biases of one token wins by its index, so nothing depends on the order of atomics.
+// all rows of the request, one per node of a draft tree. Word: bits 0-19 the count of generated
+// tokens, then flags: in the prompt, drafted, biased. Entries without a word, nearly all, are one
+// multiply; the others look up what they need. Counts are integers and the last of several
+// biases of one token wins by its index, so nothing depends on the order of atomics.
 #include "common.cuh"
 
 namespace qk {
 namespace {
 
 constexpr int kLogitThreads = 256;
-constexpr int kMaxBias = 1024, kMaxNodes = 64;
+constexpr int kMaxBias = 1024, kMaxNodes = 64, kMaxTile = 4096;
 constexpr int kMaxHistory = (1 << 20) - 1;
 constexpr uint32_t kCountMask = (1u << 20) - 1, kPrompt = 1u << 20, kDraft = 1u << 21, kBias = 1u << 22;
 
@@ -27,44 +26,83 @@ struct LogitArgs {
   const void* logits;
   float* out;
   int B, N, V, tile, rows_per_block;
+  bool vector;  // logits and out start on a whole access
 };
 
-struct TileLists {
-  int bias_n;
-  int bias_id[kMaxBias];
-  int bias_at[kMaxBias];
-  int draft[kMaxNodes];
-};
-
-// The rare entries: in the context, drafted or biased.
-__device__ __noinline__ float adjust(float x, uint32_t w, int v, const TileLists& s, const float* bias, int nodes,
-                                     uint64_t path, float rep, float freq, float pres) {
-  int count = w & kCountMask;
-  if (w & kDraft) {
-    for (int j = 0; j < nodes; ++j) count += s.draft[j] == v && (path >> j & 1);
+// Penalties of an entry of word w whose context also has `drafted` occurrences on the row's path.
+struct Penalties {
+  float rep, inv_rep, freq, pres;
+  __device__ float operator()(float x, uint32_t w, int drafted) const {
+    const int count = static_cast<int>(w & kCountMask) + drafted;
+    const float scaled = x * (x > 0.f ? inv_rep : rep);
+    x = count > 0 || (w & kPrompt) ? scaled : x;
+    return count > 0 ? x - fmaf(freq, static_cast<float>(count), pres) : x;
   }
-  if (count > 0 || (w & kPrompt)) x = x > 0.f ? __fdiv_rn(x, rep) : x * rep;
-  if (count > 0) x -= freq * static_cast<float>(count) + pres;
+};
+
+struct Tile {
+  alignas(16) uint32_t words[kMaxTile];
+  uint32_t flags[kMaxTile / 32 + 1];  // a bit per entry that has a word
+  uint64_t draft_path[kMaxNodes];     // per drafted token of the tile: the nodes that carry it
+  int draft_id[kMaxNodes], draft[kMaxNodes], draft_n;
+  int bias_id[kMaxBias];
+  uint16_t bias_at[kMaxBias];
+  int bias_n;
+};
+
+// The rare entries: drafted or biased.
+__device__ __noinline__ float adjust(float x, uint32_t w, int i, int64_t row, const Tile& s, const qk_logits_desc& d,
+                                     const float* bias, const Penalties& penalties) {
+  int drafted = 0;
+  if (w & kDraft) {
+    const uint64_t path = d.ancestors[row];
+    for (int j = 0; j < s.draft_n; ++j)
+      if (s.draft_id[j] == i) drafted = __popcll(s.draft_path[j] & path);
+  }
+  x = penalties(x, w, drafted);
   if (w & kBias) {
     int best = -1;
     for (int j = 0; j < s.bias_n; ++j)
-      if (s.bias_id[j] == v && s.bias_at[j] > best) best = s.bias_at[j];
+      if (s.bias_id[j] == i && s.bias_at[j] > best) best = s.bias_at[j];
     x += bias[best];
   }
   return x;
 }
 
-// VEC entries per thread and step: 4 when every row of logits and out is 16-byte (BF16: 8-byte)
-// aligned, which takes a vocabulary that is a multiple of 4, else 1.
-template <bool BF16, int VEC>
-__global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(LogitArgs a) {
-  extern __shared__ uint32_t words[];
-  __shared__ TileLists s;
-  const int b = blockIdx.z, tid = threadIdx.x;
-  const int v0 = blockIdx.x * a.tile, n = min(a.tile, a.V - v0);
+// 32 bits from bit `at` of a bit array.
+__device__ __forceinline__ uint32_t bits_at(const uint32_t* words, int at, bool next) {
+  return __funnelshift_r(words[at >> 5], next ? words[(at >> 5) + 1] : 0, at & 31);
+}
+
+__device__ __forceinline__ void load8(const float* p, uint32_t (&x)[8]) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+               "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
+}
+
+// Eight entries per thread and access, on multiples of eight of the flat index row * V + v (32 bytes
+// of the output, 16 or 32 of the logits) whatever the vocabulary is: addresses, mask and flags are
+// looked up once for all eight (four per access took 2.5 times the instructions, more than the SMs
+// issue in the time that the bytes take). The ends of a row's tile that are not whole take one entry
+// at a time. kBatch accesses are in flight per thread.
+constexpr int kVec = 8;
+
+template <bool BF16>
+__global__ void __launch_bounds__(kLogitThreads, 4) process_logits_kernel(LogitArgs a) {
+  __shared__ Tile s;
+  constexpr int kBatch = 2, kStep = kLogitThreads * kVec;
+  // the tiles of the first tokens, usually the most frequent and so the slowest, start first
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int v0 = blockIdx.z * a.tile, n = min(a.tile, a.V - v0);
   const qk_logits_desc& d = a.d;
-  for (int i = tid; i < n; i += kLogitThreads) words[i] = 0;
-  if (tid == 0) s.bias_n = 0;
+  for (int i = tid * 4; i < kMaxTile; i += kLogitThreads * 4) *reinterpret_cast<uint4*>(s.words + i) = make_uint4(0, 0, 0, 0);
+  if (tid == 0) s.bias_n = s.draft_n = 0;
   __syncthreads();
   pdl_wait();
   pdl_trigger();
@@ -72,79 +110,143 @@ __global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(LogitArgs
   const int length = room ? min(max(d.history_lengths[b], 0), room) : 0;
   const int prompt = room && d.prompt_lengths ? d.prompt_lengths[b] : 0;
   const int32_t* history = d.history + static_cast<int64_t>(b) * room;
-  for (int i = tid; i < length; i += kLogitThreads) {
-    const uint32_t v = static_cast<uint32_t>(history[i] - v0);
-    if (v < static_cast<uint32_t>(n)) {
-      if (i < prompt) atomicOr(&words[v], kPrompt);
-      else atomicAdd(&words[v], 1u);
+  constexpr int kAhead = 16;  // tokens in flight per thread
+  for (int i0 = tid; i0 < length; i0 += kAhead * kLogitThreads) {
+    uint32_t v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kLogitThreads;
+      v[k] = ~0u;
+      if (i0 - tid + k * kLogitThreads >= length) break;
+      v[k] = i < length ? static_cast<uint32_t>(__ldg(history + i)) - static_cast<uint32_t>(v0) : ~0u;
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (i0 - tid + k * kLogitThreads >= length) break;
+      if (v[k] >= static_cast<uint32_t>(n)) continue;
+      if (i0 + k * kLogitThreads >= prompt) atomicAdd(&s.words[v[k]], 1u);
+      else atomicOr(&s.words[v[k]], kPrompt);
     }
   }
-  if (d.drafts && tid < a.N) {
-    const int id = d.drafts[static_cast<int64_t>(b) * a.N + tid];
-    s.draft[tid] = id;
-    const uint32_t v = static_cast<uint32_t>(id - v0);
-    if (v < static_cast<uint32_t>(n)) atomicOr(&words[v], kDraft);
-  }
+  if (d.drafts && tid < a.N) s.draft[tid] = d.drafts[static_cast<int64_t>(b) * a.N + tid];
   if (d.bias_ids) {
     for (int k = tid; k < d.bias_count; k += kLogitThreads) {
       const int id = d.bias_ids[static_cast<int64_t>(b) * d.bias_count + k];
-      const uint32_t v = static_cast<uint32_t>(id - v0);
+      const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(v0);
       if (v < static_cast<uint32_t>(n)) {
         const int at = atomicAdd(&s.bias_n, 1);
-        s.bias_id[at] = id;
-        s.bias_at[at] = k;
-        atomicOr(&words[v], kBias);
+        s.bias_id[at] = static_cast<int>(v);
+        s.bias_at[at] = static_cast<uint16_t>(k);
+        atomicOr(&s.words[v], kBias);
       }
     }
   }
-  const float rep = d.repetition ? d.repetition[b] : 1.f, freq = d.frequency ? d.frequency[b] : 0.f;
-  const float pres = d.presence ? d.presence[b] : 0.f, inv = d.temperature ? __frcp_rn(d.temperature[b]) : 1.f;
+  Penalties penalties;
+  penalties.rep = d.repetition ? d.repetition[b] : 1.f;
+  penalties.inv_rep = __frcp_rn(penalties.rep);
+  penalties.freq = d.frequency ? d.frequency[b] : 0.f;
+  penalties.pres = d.presence ? d.presence[b] : 0.f;
+  const float inv = d.temperature ? __frcp_rn(d.temperature[b]) : 1.f;
   const float* bias = d.bias + static_cast<int64_t>(b) * d.bias_count;
+  __syncthreads();
+  if (d.drafts && tid < a.N) {  // each token that is drafted once, with the nodes that carry it
+    const int id = s.draft[tid];
+    const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(v0);
+    if (v < static_cast<uint32_t>(n)) {
+      uint64_t path = 0;
+      for (int j = 0; j < a.N; ++j) path |= static_cast<uint64_t>(s.draft[j] == id) << j;
+      if (__ffsll(path) - 1 == tid) {
+        const int at = atomicAdd(&s.draft_n, 1);
+        s.draft_id[at] = static_cast<int>(v);
+        s.draft_path[at] = path;
+        atomicOr(&s.words[v], kDraft);
+      }
+    }
+  }
+  __syncthreads();
+  // flags and list: a thread per 16 entries
+  static_assert(kMaxTile == 16 * kLogitThreads, "16 entries per thread");
+  uint32_t mine = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint4 u = lds_v4(s.words + tid * 16 + q * 4);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) mine |= (word(u, t) != 0 ? 1u : 0u) << (q * 4 + t);
+  }
+  const uint32_t right = __shfl_down_sync(0xffffffffu, mine, 1);
+  if ((tid & 1) == 0) s.flags[tid / 2] = mine | right << 16;
+  if (tid == 0) s.flags[kMaxTile / 32] = 0;
   __syncthreads();
 
   const int mask_words = (a.V + 31) / 32;
   const int r0 = blockIdx.y * a.rows_per_block, r1 = min(r0 + a.rows_per_block, a.N);
   for (int r = r0; r < r1; ++r) {
     const int64_t row = static_cast<int64_t>(b) * a.N + r;
-    const uint64_t path = d.drafts ? d.ancestors[row] : 0;
     const int64_t base = row * a.V + v0;
+    const int lead = a.vector ? static_cast<int>(base & (kVec - 1)) : 0;  // entries before the first whole access
     const uint32_t* mask = d.mask ? reinterpret_cast<const uint32_t*>(d.mask) + row * mask_words : nullptr;
-#pragma unroll 4
-    for (int i = tid * VEC; i < n; i += kLogitThreads * VEC) {
-      float x[VEC];
-      uint32_t w[VEC];
-      if (VEC == 4) {
-        if (BF16) {
-          const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.logits) + base + i);
-          x[0] = __uint_as_float(u.x << 16);
-          x[VEC > 1] = __uint_as_float(u.x & 0xffff0000u);
-          x[VEC > 1 ? 2 : 0] = __uint_as_float(u.y << 16);
-          x[VEC > 1 ? 3 : 0] = __uint_as_float(u.y & 0xffff0000u);
-        } else {
-          const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + base + i);
-          x[0] = u.x;
-          x[VEC > 1] = u.y;
-          x[VEC > 1 ? 2 : 0] = u.z;
-          x[VEC > 1 ? 3 : 0] = u.w;
-        }
-        const uint4 u = lds_v4(words + i);
-        w[0] = u.x;
-        w[VEC > 1] = u.y;
-        w[VEC > 1 ? 2 : 0] = u.z;
-        w[VEC > 1 ? 3 : 0] = u.w;
-      } else {
-        x[0] = BF16 ? bf16_to_f32(static_cast<const uint16_t*>(a.logits)[base + i])
-                    : static_cast<const float*>(a.logits)[base + i];
-        w[0] = words[i];
-      }
-      const uint32_t allowed = mask ? mask[(v0 + i) >> 5] >> ((v0 + i) & 31) : 0xfu;
+    const uint16_t* in16 = static_cast<const uint16_t*>(a.logits) + base;
+    const float* in32 = static_cast<const float*>(a.logits) + base;
+    float* out = a.out + base;
+    for (int i0 = tid * kVec - lead; i0 < n; i0 += kBatch * kStep) {
+      uint32_t x[kBatch][kVec], allowed[kBatch];
 #pragma unroll
-      for (int t = 0; t < VEC; ++t) {
-        if (w[t]) x[t] = adjust(x[t], w[t], v0 + i + t, s, bias, a.N, path, rep, freq, pres);
-        x[t] = allowed >> t & 1 ? x[t] * inv : -INFINITY;
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + k * kStep;
+        allowed[k] = ~0u;
+        if (i >= n) break;
+        if (a.vector && i >= 0 && i + kVec <= n) {
+          if (BF16) {
+            const uint4 u = *reinterpret_cast<const uint4*>(in16 + i);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              x[k][2 * t] = word(u, t) << 16;
+              x[k][2 * t + 1] = word(u, t) & 0xffff0000u;
+            }
+          } else {
+            load8(in32 + i, x[k]);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < kVec; ++t) {
+            x[k][t] = 0;
+            if (i + t >= 0 && i + t < n)
+              x[k][t] = BF16 ? static_cast<uint32_t>(in16[i + t]) << 16 : __float_as_uint(in32[i + t]);
+          }
+        }
+        if (mask) {
+          const int v = v0 + max(i, 0);
+          allowed[k] = bits_at(mask, v, (v & 31) > 32 - kVec && (v >> 5) + 1 < mask_words) << (max(i, 0) - i);
+        }
       }
-      if (VEC == 4) *reinterpret_cast<float4*>(a.out + base + i) = make_float4(x[0], x[VEC > 1], x[VEC > 1 ? 2 : 0], x[VEC > 1 ? 3 : 0]);
-      else a.out[base + i] = x[0];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + k * kStep;
+        if (i >= n) break;
+        const int at = max(i, 0);
+        const uint32_t marked = bits_at(s.flags, at, true) << (at - i) & ((1u << kVec) - 1);
+        float f[kVec];
+#pragma unroll
+        for (int t = 0; t < kVec; ++t) f[t] = __uint_as_float(x[k][t]);
+        if (marked) {
+#pragma unroll
+          for (int t = 0; t < kVec; ++t) {
+            if (marked >> t & 1) {
+              const uint32_t w = s.words[i + t];
+              f[t] = w & (kDraft | kBias) ? adjust(f[t], w, i + t, row, s, d, bias, penalties) : penalties(f[t], w, 0);
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kVec; ++t) f[t] = allowed[k] >> t & 1 ? f[t] * inv : -INFINITY;
+        if (a.vector && i >= 0 && i + kVec <= n) {
+          store8(out + i, f);
+        } else {
+#pragma unroll
+          for (int t = 0; t < kVec; ++t)
+            if (i + t >= 0 && i + t < n) out[i + t] = f[t];
+        }
+      }
     }
   }
 }
@@ -161,7 +263,7 @@ int qk_process_logits(const qk_logits_desc* desc, const void* logits, int in_dty
   QK_REQUIRE(desc, "null pointer");
   const qk_logits_desc& d = *desc;
   QK_REQUIRE(in_dtype == QK_OUT_F32 || in_dtype == QK_OUT_BF16, "logits must be F32 or BF16");
-  QK_REQUIRE(B >= 0 && B <= 65535 && N >= 0 && V > 0, "invalid batch, rows or vocabulary");
+  QK_REQUIRE(B >= 0 && N >= 0 && N <= 65535 && V > 0 && V <= 65535 * 1024, "invalid batch, rows or vocabulary");
   QK_REQUIRE(d.history_capacity >= 0 && d.history_capacity <= kMaxHistory, "a history holds at most %d tokens", kMaxHistory);
   QK_REQUIRE(!d.history || d.history_lengths, "a history needs its lengths");
   QK_REQUIRE(d.bias_count >= 0 && d.bias_count <= kMaxBias, "a request has at most %d biases", kMaxBias);
@@ -170,24 +272,23 @@ int qk_process_logits(const qk_logits_desc* desc, const void* logits, int in_dty
   QK_REQUIRE(!d.drafts || N <= kMaxNodes, "a draft tree has at most %d nodes", kMaxNodes);
   if (B == 0 || N == 0) return QK_OK;
   QK_REQUIRE(logits && out, "null pointer");
-  LogitArgs a{d, logits, out, B, N, V, 0, 0};
+  LogitArgs a{d, logits, out, B, N, V, 0, 0, false};
   if (!a.d.bias_ids) a.d.bias_count = 0;
   // Tiles small enough that the blocks fill the SMs twice over, large enough that the history's
-  // re-reads (one per tile) stay small: at most 4096 words, at least 1024.
-  a.tile = 4096;
+  // re-reads (one per tile) stay small: at most 4096 entries, at least 1024.
+  a.tile = kMaxTile;
   while (a.tile > 1024 && static_cast<int64_t>(B) * N * ((V + a.tile - 1) / a.tile) < 2 * sm_count()) a.tile /= 2;
   const int tiles = (V + a.tile - 1) / a.tile;
-  // a block takes all rows of its request unless that leaves SMs idle
+  // A block takes several rows of its request (each repeats the counting), but leaves 8 blocks per SM
+  // where there are as many: tiles of frequent tokens take longer than others.
   int parts = 1;
-  while (parts < N && static_cast<int64_t>(B) * tiles * parts < 2 * sm_count()) parts *= 2;
+  while (parts < N && static_cast<int64_t>(B) * tiles * parts < 8 * sm_count()) parts *= 2;
   a.rows_per_block = (N + parts - 1) / parts;
   parts = (N + a.rows_per_block - 1) / a.rows_per_block;
   const bool bf16 = in_dtype == QK_OUT_BF16;
-  const bool vec = V % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & (bf16 ? 7 : 15)) == 0 &&
-                   (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const auto kernel = bf16 ? (vec ? process_logits_kernel<true, 4> : process_logits_kernel<true, 1>)
-                           : (vec ? process_logits_kernel<false, 4> : process_logits_kernel<false, 1>);
-  const cudaError_t e = launch_dependent(kernel, dim3(tiles, parts, B), dim3(kLogitThreads), a.tile * 4, as_stream(stream), a);
+  const auto kernel = bf16 ? process_logits_kernel<true> : process_logits_kernel<false>;
+  a.vector = (reinterpret_cast<uintptr_t>(logits) & (bf16 ? 15 : 31)) == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0;
+  const cudaError_t e = launch_dependent(kernel, dim3(B, parts, tiles), dim3(kLogitThreads), 0, as_stream(stream), a);
   if (e != cudaSuccess) return cuda_error(e, "process_logits_kernel");
   count_launch();
   return QK_OK;

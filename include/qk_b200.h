@@ -430,7 +430,7 @@ int qk_tree_attention_check(const void* workspace, qk_stream_t stream);
 /* ---- logits before the choice ---------------------------------------------------
  * No counterpart in the reference (its decoding is greedy, run.py:46-55). Per request b and row i
  * (a node of its draft tree), for every token v:
- *   x = logit; if v is in the context: x = x > 0 ? x / repetition : x * repetition;
+ *   x = logit; if v is in the context: x *= x > 0 ? 1 / repetition : repetition;
  *   x -= frequency * n + presence * [n > 0]; x += bias(v); x *= 1 / temperature;
  *   x = -inf where bit v of the row's mask is 0.
  * n counts v in the history from prompt_length on and in the drafts of the row's ancestor word; the
