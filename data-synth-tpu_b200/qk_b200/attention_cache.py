@@ -112,13 +112,13 @@ def read_quantized(cache, name, indices, c, dtype, *, scale_gather=None):
     codes = cache[name]
     plane = cache[name + "_scale"]
     batch, selected = indices.shape
-    idx = indices.to(device=codes.device, dtype=torch.int32).contiguous()
+    idx = indices if indices.dtype == torch.int32 and indices.device == codes.device else indices.to(
+        device=codes.device, dtype=torch.int32)
+    idx = idx.contiguous()
     out = torch.empty((batch, selected, c.kv_heads, c.head_dim), dtype=dtype, device=codes.device)
-    with torch.cuda.device(codes.device):
-        _lib.call("qk_kv_q8_read", _lib.ptr(codes), _lib.ptr(plane), _lib.ptr(idx), batch,
-                  selected, codes.shape[1], c.kv_heads, c.head_dim,
-                  _lib.QK_OUT_BF16 if dtype == torch.bfloat16 else _lib.QK_OUT_F32,
-                  _lib.ptr(out), _lib.stream_handle(codes.device))
+    _lib.call_on(codes.device, "qk_kv_q8_read", codes.data_ptr(), plane.data_ptr(), idx.data_ptr(), batch, selected,
+                 codes.shape[1], c.kv_heads, c.head_dim, _lib.QK_OUT_BF16 if dtype == torch.bfloat16 else _lib.QK_OUT_F32,
+                 out.data_ptr())
     return out
 
 
