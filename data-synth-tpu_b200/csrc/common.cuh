@@ -360,6 +360,16 @@ __device__ __forceinline__ uint4 ld_nc_v4(const void* p) {
   return r;
 }
 
+// ld_nc_v4 for addresses that are only valid under a condition: it stays where it is written. Without
+// `volatile` the compiler may move the load, as one that has no effects, out of a loop and its condition.
+__device__ __forceinline__ uint4 ld_guarded_v4(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
 __device__ __forceinline__ uint4 lds_v4(const void* p) {
   return *reinterpret_cast<const uint4*>(p);
 }

@@ -226,10 +226,10 @@ __global__ void __launch_bounds__(256) write_slots_kernel(const void* __restrict
   if (in) {  // also where the slot says padding: the values need not wait for it
     const int64_t at = token * (is_value ? value_stride : key_stride) + col * 8;
     if (BF16) {
-      unpack8(ld_nc_v4(static_cast<const uint16_t*>(is_value ? value : key) + at), x);
+      unpack8(ld_guarded_v4(static_cast<const uint16_t*>(is_value ? value : key) + at), x);
     } else {
       const float* p = static_cast<const float*>(is_value ? value : key) + at;
-      const uint4 u = ld_nc_v4(p), v = ld_nc_v4(p + 4);
+      const uint4 u = ld_guarded_v4(p), v = ld_guarded_v4(p + 4);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         x[t] = __uint_as_float(word(u, t));

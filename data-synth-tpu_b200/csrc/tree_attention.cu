@@ -15,12 +15,12 @@
 //
 // One CTA per SM, three kinds of warps joined by mbarriers (every wait bounded):
 //  * 8 softmax warps, two threads per row: Q to TMEM once per unit; then per tile S from TMEM, mask,
-//    running maximum and sum in FP32, P as BF16 back over S's columns. O (FP32, in TMEM) is rescaled
-//    only when a row's maximum grows by more than 2^8: P stays below 2^8, exact enough in FP32.
+//    running maximum and sum in FP32, P as FP16 back over S's columns. O (FP32, in TMEM) is rescaled
+//    only when a row's maximum grows by more than 2^8: P stays below 2^8, far inside FP16's range.
 //  * 8 decode warps (4 for K, 4 for V): codes and scales from shared memory, where a copy warp each
-//    brings them by tensor copies two tiles ahead; int8 -> BF16 with the group's scale (one rounding, as
-//    the cache's BF16 read has it), stored as 128-byte swizzled tiles: K-major for K, and the same
-//    bytes read as an MN-major operand for V (no transposition).
+//    brings them by tensor copies two tiles ahead; int8 -> FP16 with the group's scale (rounded once, to
+//    11 bits where BF16 has 8), stored as 128-byte swizzled tiles: K-major for K, and the same bytes
+//    read as an MN-major operand for V (no transposition).
 //  * 2 warps issue the MMAs, Q K^T and P V: Q and P from TMEM, K and V from shared memory.
 // TMEM: O 256 columns, Q 128, two S/P buffers of 64.
 #include <cuda.h>  // CUtensorMap and its enums; the encoder is looked up at run time
@@ -42,8 +42,11 @@ constexpr int kSoftmaxRegs = 128, kOtherRegs = 72;
 static_assert(2 * kSoftmaxRegs + 3 * kOtherRegs <= 5 * 96, "the shares fit the launch's registers");
 constexpr uint32_t kColO = 0, kColQ = 256, kColS = 384;  // TMEM columns
 constexpr float kLazyGrowth = 8.f;                       // in powers of two
-constexpr uint32_t kHugeScale = 0x7c00;                  // BF16 bits of 2^121: times 127 leaves FP32's range
-constexpr int kBadRing = 4;
+constexpr uint32_t kHugeScale = 0x7c00;                  // BF16 bits of 2^121: times 127 it leaves FP32's range
+constexpr int kBadRing = 4, kFactors = 4;
+// Queries and keys are multiplied by these for FP16: up to 2^22 and 2^20 fit it, and it leaves errors of
+// 2^-19 and 2^-21 to small ones, a few 2^-16 of a score.
+constexpr float kQueryPower = 1.f / 64, kKeyPower = 1.f / 16;
 constexpr uint32_t kQStage = 2048;  // bytes per softmax warp
 constexpr int kUnitCost = 4;  // what a unit costs besides its tiles (Q, the output), in tiles
 
@@ -55,7 +58,7 @@ struct TreeArgs {
   const int32_t *table, *lengths, *counts;
   const uint64_t* ancestors;
   const uint16_t* gate;
-  float scale_log2;         // |scale| * log2(e), above zero
+  float scale_log2;         // |scale| * log2(e) / (kQueryPower * kKeyPower), above zero
   uint32_t q_keep, q_flip;  // Q's bits & keep ^ flip: nothing for a scale of zero, the sign for a negative one
   int B, N, hq, kv, rep, pages, pages_per_row, width, room, shift, row_tiles, part_rows;  // room: tokens of a table row
   int64_t T;
@@ -190,8 +193,9 @@ struct Barriers {
 
 struct Control {
   Barriers bar;
-  float top[2][kRows];        // the row maxima that a row's two warps swap
-  uint64_t bad[kBadRing][8];  // per unit and channel group: drafts whose value scale is not finite
+  float top[2][2][kRows];     // by tile parity: the row maxima that a row's two warps swap
+  float power[kFactors][kSide];  // of V per tile and 16 tokens: the power of two that was divided out
+  uint64_t bad[kBadRing][8];  // per unit and channel group: drafts that are not finite there
   uint32_t tmem;
 };
 
@@ -249,25 +253,36 @@ __device__ __forceinline__ uint32_t lds_at(uint32_t addr) {
   return v;
 }
 
-// Four int8 codes times a BF16 scale s >= 0 -> two BF16 pairs, each code * s rounded once. With the
-// sign bit flipped a code c is the byte u = c + 128; under the exponent of 128 it reads f = 128 + u
-// below 128 and f = 2 u from there, so s (f / 2 - 128) is A = s c / 2 for negative codes and s c for
-// others: one fused multiply-add with h = s / 2, k = -128 s (both exact), and A - max(-A, 0) doubles
-// the negative ones, which is exact. Half of this runs on the FMA pipe; masking the sign bit off and
-// adding it back took twice the integer instructions, whose pipe is half as wide.
-__device__ __forceinline__ void decode4(uint32_t codes, __nv_bfloat162 h, __nv_bfloat162 k, uint32_t& lo, uint32_t& hi) {
+// Four int8 codes times an FP16 scale -> two FP16 pairs, each code * scale rounded once. With the sign
+// bit flipped a code c is the byte c + 128, under the exponent of 1024 it reads 1152 + c; minus 1152 it
+// is the code, exactly. Three and a half instructions per pair, of which one and a half on the integer
+// pipe, which is half as wide: with a sign extension there (and one fused multiply-add) it was slower.
+__device__ __forceinline__ void decode4(uint32_t codes, __half2 scale, uint32_t& lo, uint32_t& hi) {
   const uint32_t u = codes ^ 0x80808080u;
-  const uint32_t t[2] = {__byte_perm(u, 0x43434343u, 0x4140), __byte_perm(u, 0x43434343u, 0x4342)};
+  const uint32_t t[2] = {__byte_perm(u, 0x64646464u, 0x4140), __byte_perm(u, 0x64646464u, 0x4342)};
   uint32_t r[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const __nv_bfloat162 half = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&t[i]), h, k);
-    const __nv_bfloat162 neg = __hfma2_relu(half, __nv_bfloat162{-1.f, -1.f}, __nv_bfloat162{-0.f, -0.f});
-    const __nv_bfloat162 v = __hfma2(neg, __nv_bfloat162{-1.f, -1.f}, half);
+    const __half2 v = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&t[i]), __half2{-1152.f, -1152.f}), scale);
     r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
   lo = r[0];
   hi = r[1];
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
+// The power of two 2^e with the BF16 exponent of `bits` (no sign), e in [-40, 126]: what is divided by
+// it lies below 2 (4 at the top), and FP16 takes it with all its bits down to 2^-14.
+__device__ __forceinline__ float power_of(uint32_t bits) {
+  return __uint_as_float(min(max(bits & 0x7f80u, (127u - 40u) << 7), (127u + 126u) << 7) << 16);
+}
+__device__ __forceinline__ float inverse_power(float power) {
+  return __uint_as_float((254u - (__float_as_uint(power) >> 23)) << 23);
 }
 
 // The two softmax warps of 32 rows.
@@ -356,10 +371,11 @@ __device__ __forceinline__ bool copy_role(const TreeArgs& a, Control& ctl, const
   return ok;
 }
 
-// 16 decode warps: 4 for each of K and V and the even and odd tiles (raw slot and stage are the
-// tile's parity), all in one copy of this code: with a copy each the CTA's hot code left the
-// instruction cache. Four warps per tile instead of eight halve what a tile costs besides its values;
-// the other four are at work on the next one meanwhile.
+// 4 decode warps for K and 4 for V, all in one copy of this code: with a copy each the CTA's hot code
+// left the instruction cache. FP16 has the bits but not the range of the cache's BF16 scales. Keys (and
+// queries) go in with a fixed power of two: what matters of them is a score's absolute error. Values
+// count relatively, so a warp divides the power of two of its 16 tokens' largest scale out of them; it
+// comes back through the weights' exponent.
 template <int HD>
 __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint32_t tiles, uint32_t raw, Walk walk) {
   constexpr int SPT = HD / 32, CHUNKS = HD / 16;  // a thread's share of a tile: 16 channels of SPT tokens
@@ -406,27 +422,39 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
           const uint32_t bits = scales[i / 2] >> (16 * (i & 1)) & 0x7fffu;
           if (token >= total) {
             scales[i / 2] &= ~mask;
-          } else if (values && token >= seg.r.length && bits >= kHugeScale) {
-            // a draft's value that is not finite must not reach the rows that do not see it (0 * inf):
-            // zero here, NaN at the end for those that do
-            atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][chunk / 2]),
-                     1ull << (token - seg.r.length));
+          } else if (token >= seg.r.length && bits >= kHugeScale) {
+            // a draft that is not finite must not reach the rows that do not see it, neither as 0 * inf
+            // nor through its neighbours' power of two: zero here, NaN at the end for those that do (in
+            // a value's group of channels, or for a key in all)
+            for (int g = values ? chunk / 2 : 0; g < (values ? chunk / 2 + 1 : HD / 32); ++g)
+              atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][g]),
+                       1ull << (token - seg.r.length));
             scales[i / 2] &= ~mask;
           }
         }
       }
+      float inverse = kKeyPower;
+      if (values) {
+        uint32_t top = scales[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 1; i < SPT / 2; ++i) top = __vmaxu2(top, scales[i] & 0x7fff7fffu);
+        const float power = power_of(__reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16)));
+        inverse = inverse_power(power);
+        if (lane == 0) ctl.power[it % kFactors][t / 32] = power;
+      }
+#pragma unroll
+      for (int i = 0; i < SPT / 2; ++i)
+        scales[i] = pack_f16x2(__uint_as_float(scales[i] << 16) * inverse, __uint_as_float(scales[i] & 0xffff0000u) * inverse);
       if (!warp_wait(&empty[stage], phase ^ 1)) return false;
 #pragma unroll
       for (int i = 0; i < SPT; ++i) {
         const uint32_t two = __byte_perm(scales[i / 2], 0, select[i & 1]);
-        const __nv_bfloat162 scale2 = *reinterpret_cast<const __nv_bfloat162*>(&two);
-        const __nv_bfloat162 h = __hmul2(scale2, __nv_bfloat162{0.5f, 0.5f});
-        const __nv_bfloat162 k = __hmul2(scale2, __nv_bfloat162{-128.f, -128.f});
+        const __half2 h = *reinterpret_cast<const __half2*>(&two);
         uint4 piece[2];
-        decode4(code[i].x, h, k, piece[0].x, piece[0].y);
-        decode4(code[i].y, h, k, piece[0].z, piece[0].w);
-        decode4(code[i].z, h, k, piece[1].x, piece[1].y);
-        decode4(code[i].w, h, k, piece[1].z, piece[1].w);
+        decode4(code[i].x, h, piece[0].x, piece[0].y);
+        decode4(code[i].y, h, piece[0].z, piece[0].w);
+        decode4(code[i].z, h, piece[1].x, piece[1].y);
+        decode4(code[i].w, h, piece[1].z, piece[1].w);
         const uint32_t to = (to0 + stage * kStageBytes) ^ (i << 7 | i << 4);
         sts_v4(to, piece[0]);
         sts_v4(to ^ 16, piece[1]);
@@ -458,7 +486,7 @@ template <int HD>
 __device__ __forceinline__ bool score_role(const TreeArgs& a, Control& ctl, uint32_t ktiles, Walk walk) {
   constexpr uint32_t kStageBytes = kTile * HD * 2;
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
-  const uint32_t idesc = idesc_bf16_m128(kTile);
+  const uint32_t idesc = idesc_f16_m128(kTile);
   const uint64_t kdesc = sdesc_sw128(ktiles, 1024u);
   Segment seg;
   uint32_t it = 0;
@@ -489,7 +517,7 @@ template <int HD>
 __device__ __forceinline__ bool value_role(const TreeArgs& a, Control& ctl, uint32_t vtiles, Walk walk) {
   constexpr uint32_t kStageBytes = kTile * HD * 2;
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
-  const uint32_t idesc = idesc_bf16_m128_bmn(HD);
+  const uint32_t idesc = idesc_f16_m128_bmn(HD);
   const uint64_t vdesc = sdesc_sw128_mn(vtiles, kTile * 128, 1024u);
   Segment seg;
   uint32_t it = 0;
@@ -538,7 +566,7 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const Segment& seg, ui
     for (int c = 0; c < kAtOnce; ++c)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        v[c][i] = at[i] >= 0 ? ld_nc_v4(q + at[i] + (c0 + c) * 32 + lane % 4 * 8) : make_uint4(0, 0, 0, 0);
+        v[c][i] = at[i] >= 0 ? ld_guarded_v4(q + at[i] + (c0 + c) * 32 + lane % 4 * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int c = 0; c < kAtOnce; ++c) {
       __syncwarp();
@@ -553,7 +581,10 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const Segment& seg, ui
       for (int i = 0; i < 4; ++i) {
         const uint4 x = lds_v4_at(stage + lane * 64 + ((i ^ lane / 2) & 3) * 16);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) u[i * 4 + w] = (word(x, w) & a.q_keep) ^ a.q_flip;
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t y = (word(x, w) & a.q_keep) ^ a.q_flip;
+          u[i * 4 + w] = pack_f16x2(__uint_as_float(y << 16) * kQueryPower, __uint_as_float(y & 0xffff0000u) * kQueryPower);
+        }
       }
       tmem_st16(tm + kColQ + half * (HD / 4) + (c0 + c) * 16, u);
     }
@@ -570,8 +601,6 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
   const int warp = threadIdx.x >> 5, quarter = warp & 3, half = warp >> 2, lane = threadIdx.x & 31;
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t o_cols = tm + kColO + half * (HD / 2);
-  float* my_top = &ctl.top[half][quarter * 32 + lane];
-  const float* other_top = &ctl.top[half ^ 1][quarter * 32 + lane];
   Segment seg, next;
   uint32_t it = 0;
   bool more = walk.next(a, next);
@@ -613,16 +642,29 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
           for (int j = 0; j < kHalf; ++j)
             if (!(see >> j & 1)) s[j] = 0xff800000u;
         }
-        float top = -INFINITY, top2 = -INFINITY;
+        // The weights go out as 2^(score + e - m), e the exponent that V's 16 tokens had divided out:
+        // times V's FP16 values that is the product with V itself, and m bounds them as stored. Sums
+        // take e off again.
+        float add[2], undo[2], top = -INFINITY;
+        if (!warp_wait(&ctl.bar.v_full[it % kStages], (it / kStages) & 1)) return false;
 #pragma unroll
-        for (int j = 0; j < kHalf; j += 4) {
-          top = max3(top, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-          top2 = max3(top2, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
+        for (int g = 0; g < 2; ++g) {
+          const float v = ctl.power[it % kFactors][half * 2 + g];
+          add[g] = static_cast<float>(static_cast<int>(__float_as_uint(v) >> 23) - 127);
+          undo[g] = inverse_power(v);
+          float most = -INFINITY, most2 = -INFINITY;
+#pragma unroll
+          for (int j = 16 * g; j < 16 * g + 16; j += 4) {
+            most = max3(most, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+            most2 = max3(most2, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
+          }
+          top = fmaxf(top, fmaf(fmaxf(most, most2), a.scale_log2, add[g]));
         }
-        *my_top = fmaxf(top, top2);
+        float(*tops)[kRows] = ctl.top[it & 1];
+        tops[half][quarter * 32 + lane] = top;
         // the pair's scores are both read by then: P may go over either's columns
         pair_sync(quarter);
-        top = fmaxf(fmaxf(top, top2), *other_top) * a.scale_log2;
+        top = fmaxf(top, tops[half ^ 1][quarter * 32 + lane]);
         const bool grow = top > m + kLazyGrowth;
         if (__any_sync(0xffffffffu, grow)) {
           const float now = fmaxf(m, top);
@@ -646,21 +688,24 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
           }
         }
         const float shift = m == -INFINITY ? 0.f : m;
-        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), shift2 = pair(-shift, -shift);
-        uint64_t sum[2] = {0, 0};
         uint32_t p[kHalf / 2];
 #pragma unroll
-        for (int j = 0; j < kHalf / 2; ++j) {
-          float x, y;
-          unpair(fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, shift2), x, y);
-          x = exp2_fast(x);
-          y = exp2_fast(y);
-          sum[j & 1] = add2(sum[j & 1], pair(x, y));
-          p[j] = pack_bf16x2(x, y);
+        for (int g = 0; g < 2; ++g) {
+          const uint64_t mul2 = pair(a.scale_log2, a.scale_log2), add2g = pair(add[g] - shift, add[g] - shift);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll
+          for (int j = 8 * g; j < 8 * g + 8; ++j) {
+            float x, y;
+            unpair(fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), mul2, add2g), x, y);
+            x = exp2_fast(x);
+            y = exp2_fast(y);
+            sum[j & 1] = add2(sum[j & 1], pair(x, y));
+            p[j] = pack_f16x2(x, y);
+          }
+          float even, odd;
+          unpair(add2(sum[0], sum[1]), even, odd);
+          l = fmaf(even + odd, undo[g], l);
         }
-        float even, odd;
-        unpair(add2(sum[0], sum[1]), even, odd);
-        l += even + odd;
         tmem_st16(cols + half * (kHalf / 2), p);
         tmem_wait_st();
         tc_fence_before();
@@ -798,8 +843,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
   pdl_trigger();
   uint4 gate[2];
   if (a.gate && first == 0 && node < a.N) {
-    gate[0] = ld_nc_v4(a.gate + to);
-    gate[1] = ld_nc_v4(a.gate + to + 8);
+    gate[0] = ld_guarded_v4(a.gate + to);
+    gate[1] = ld_guarded_v4(a.gate + to + 8);
   }
   const Parts parts = a.parts[unit];
   const int count = load_request(a, b).count;
@@ -986,7 +1031,7 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   a.counts = counts;
   a.ancestors = ancestors;
   a.gate = gate;
-  a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896341f;
+  a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * (1.44269504088896341f / (kQueryPower * kKeyPower));
   a.q_keep = scale == 0.f ? 0u : ~0u;
   a.q_flip = scale < 0.f ? 0x80008000u : 0u;
   a.B = B;

@@ -89,8 +89,11 @@ __device__ __forceinline__ uint32_t idesc_bf16_m128(uint32_t n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// The same with an MN-major B (the transposed operand: N contiguous in shared memory).
-__device__ __forceinline__ uint32_t idesc_bf16_m128_bmn(uint32_t n) { return idesc_bf16_m128(n) | (1u << 16); }
+// FP16 A and B, and the same with an MN-major B (the transposed operand: N contiguous in shared memory).
+__device__ __forceinline__ uint32_t idesc_f16_m128(uint32_t n) {
+  return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t idesc_f16_m128_bmn(uint32_t n) { return idesc_f16_m128(n) | (1u << 16); }
 
 // Shared-memory matrix descriptor of an MN-major operand, 128-byte swizzle: atoms of 8 K rows x
 // 64 values of the M or N dimension (128 B per K row), blocks of 64 values `mn_stride` bytes

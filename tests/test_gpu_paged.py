@@ -391,6 +391,83 @@ def test_tree_attention_steep_and_flat_scores(cuda_device):
     assert (np.abs(out - want) <= bound).all()
 
 
+@pytest.mark.parametrize("hq,kv,hd", [(8, 1, 256), (6, 2, 128), (3, 3, 64)])
+def test_tree_attention_rounds_operands_to_eleven_bits(cuda_device, hq, kv, hd):
+    """The output's own rounding to BF16 (uniform within 2^-9, 1.1e-3 on average, for mantissas spread
+    over [1, 2) at most 1.7e-3 in all) and little else: keys, values and weights carry 11 bits, so each
+    adds an eighth of what BF16 operands would, under 1e-3 together."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    g = torch.Generator(device=cuda_device).manual_seed(hd)
+    cache = random_pool(g, 1, 2048, kv, hd)
+    q = (torch.randn((1, 4, hq, hd), device=cuda_device, generator=g) * 1.5).to(torch.bfloat16)
+    table = torch.arange(8, dtype=torch.int32, device=cuda_device)[None]
+    words = torch.tensor([[1, 3, 5, 15]])
+    out = to_f32(tree_attention(q, cache, table, torch.tensor([2000]), words, page_size=256)).astype(np.float64)
+    want, _ = attention_oracle(q, cache, table.cpu().numpy(), np.array([2000]), np.array([4]),
+                               words.numpy().view(np.uint64), 256, None, hd ** -0.5)
+    assert np.linalg.norm(out - want) <= 2.0e-3 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("size", [2.0 ** -100, 1e-30, 1e-6, 3e4, 1e20, 2.0 ** 100])
+def test_tree_attention_values_of_any_size(cuda_device, hd, size):
+    """Values far outside FP16's range, also next to tiles of ordinary ones, scale the output alone."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    g = torch.Generator(device=cuda_device).manual_seed(7)
+    cache = random_pool(g, 1, 256, 2, hd)
+    q = torch.randn((1, 1, 4, hd), device=cuda_device, generator=g).to(torch.bfloat16)
+    table = torch.arange(4, dtype=torch.int32, device=cuda_device)[None]
+    scale = torch.full((256,), size, device=cuda_device)
+    scale[64:128] = 1.0  # a tile of ordinary values
+    cache["v_scale"].copy_((cache["v_scale"].float() * scale).to(torch.bfloat16))
+    args = (table, torch.tensor([255]), torch.tensor([[1]]))
+    out = to_f32(tree_attention(q, cache, *args, page_size=64)).astype(np.float64)
+    want, bound = attention_oracle(q, cache, table.cpu().numpy(), np.array([255]), np.array([1]),
+                                   np.array([[1]], np.uint64), 64, None, hd ** -0.5)
+    assert np.isfinite(out).all()
+    slack = bound - 1e-6 + 2.0 ** -120  # the absolute part of the bound is for values near one
+    assert (np.abs(out - want) <= slack).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 2.0 ** 125])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_tree_attention_drafts_that_are_not_finite(cuda_device, hd, bad, which):
+    """A draft whose key or value is not finite makes the nodes that see it NaN (in its group of
+    channels for a value), and changes no bit of the others."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    g = torch.Generator(device=cuda_device).manual_seed(6)
+    cache = random_pool(g, 1, 512, 2, hd)
+    q = torch.randn((1, 6, 4, hd), device=cuda_device, generator=g).to(torch.bfloat16)
+    table = torch.tensor([[3, 0, 2, 1]], dtype=torch.int32, device=cuda_device)
+    words = torch.tensor([[1, 3, 5, 11, 21, 37]])  # nodes 1 and 3 see node 1
+    args = (table, torch.tensor([300]), words)
+    good = tree_attention(q, cache, *args, page_size=128)
+    groups = hd // 32
+    slot = int(table[0, 301 // 128]) * 128 + 301 % 128
+    plane = cache[which].view(2, groups, 512)
+    plane[1, groups - 1, slot] = bad  # KV head 1, the last group of its channels
+    out = tree_attention(q, cache, *args, page_size=128)
+    for node in range(6):
+        for head in range(4):
+            row, was = out[0, node, head], good[0, node, head]
+            if node in (1, 3) and head >= 2:
+                nan = torch.isnan(row)
+                assert nan[-32:].all() and (which == "k_scale" or torch.equal(row[:-32], was[:-32]))
+                assert which == "v_scale" or nan.all()
+            else:
+                assert torch.equal(row, was)
+
+
 def test_tree_attention_strided_queries_and_streams(cuda_device):
     """Queries as a slice of the projection's output, and calls on two streams at once: each has a
     workspace of its own."""

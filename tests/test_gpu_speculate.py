@@ -14,7 +14,9 @@ VOCAB = 600
 def model_of(device):
     from qk_b200.decoder import StackConfig, SyntheticDecoder
 
-    return SyntheticDecoder(StackConfig(layers=2, experts=16, top_k=2, qtype="Q4_K", context=96), device, seed=5)
+    # every expert takes every token: with a selection, a near tie in the router may go one way in a pass
+    # of one token and another in a pass of several, and no bound on rounding holds across it
+    return SyntheticDecoder(StackConfig(layers=2, experts=4, top_k=4, qtype="Q4_K", context=96), device, seed=5)
 
 
 def prompts_of(rng, batch):
