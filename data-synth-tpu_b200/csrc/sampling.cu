@@ -4,13 +4,20 @@
 //   x = logit;  in the context (history or drafted path):  x = x > 0 ? x * (1 / r) : x * r
 //   x -= f * count + p * [count > 0];  x += bias;  x /= temperature;  mask bit 0: x = -inf
 //
-// Bound by HBM: a logit in, an FP32 value out, one mask bit per entry. A block owns a tile of
-// the vocabulary of one request and counts the request's history into one 32-bit word per
-// entry in shared memory (the history is re-read by every tile, from L2); the words then serve
-// all rows of the request, one per node of a draft tree. Word: bits 0-19 the count of generated
-// tokens, then flags: in the prompt, drafted, biased. Entries without a word, nearly all, are one
-// multiply; the others look up what they need. Counts are integers and the last of several
-// biases of one token wins by its index, so nothing depends on the order of atomics.
+// A logit in, an FP32 value out and one mask bit per entry: 16 requests of 24 rows of 151937 FP32 logits
+// have to move 475 MB, 72 us, and take 89 us (5.4 TB/s); in BF16 80 us. A single row of 151936 takes 6 us,
+// the latency of its four dependent reads. What made the difference (from 160 us):
+//  * A block owns a tile of the vocabulary of one request and counts the request's history into a 32-bit
+//    word per entry in shared memory; the words then serve all rows of the request, one per node of a draft
+//    tree (each tile re-reads the history, from L2). Word: bits 0-19 the count of generated tokens, then
+//    flags: in the prompt, drafted, biased.
+//  * Few entries have a word. Each warp lists those of its part once, and per row treats them 32 at a time
+//    in shared memory before all entries are scaled, masked and stored: a test per entry and row took
+//    200 instructions per eight entries, more than the SMs issue in the time that the bytes take.
+//  * Rows come by asynchronous copies a row ahead, the first ones before the history is counted.
+//  * Drafted and biased entries have a record, so that no row searches lists or waits for a global read.
+// Counts are integers and the last of several biases of one token holds by its index, so nothing depends on
+// the order of atomics.
 #include <algorithm>
 
 #include "common.cuh"
@@ -21,7 +28,7 @@ namespace {
 constexpr int kLogitThreads = 256, kLogitWarps = kLogitThreads / 32;
 constexpr int kLogitBlocks = 3;  // per SM: shared memory
 constexpr int kVec = 8;  // entries per access
-constexpr int kMaxBias = 1024, kMaxNodes = 64, kMaxTile = 4096;
+constexpr int kMaxBias = 1024, kMaxNodes = 64, kMaxTile = 4096;  // tiles of 2048: 97 us for 89
 constexpr int kMaxHistory = (1 << 20) - 1;
 constexpr uint32_t kCountMask = (1u << 20) - 1, kPrompt = 1u << 20, kDraft = 1u << 21, kBias = 1u << 22;
 
@@ -33,36 +40,30 @@ struct LogitArgs {
   bool vector;  // logits and out start on a whole access
 };
 
-// Penalties of an entry of word w whose context also has `drafted` occurrences on the row's path. In two
-// steps, the first once per entry, the second per row of it: the amount to take off, FP32, where the
-// factor applies (-0 for none), +0 where nothing does.
+// Penalties of an entry of word w whose context also has `drafted` occurrences on the row's path.
 struct Penalties {
   float rep, inv_rep, freq, pres;
-  __device__ uint32_t amount(uint32_t w, int drafted) const {
+  __device__ float operator()(float x, uint32_t w, int drafted) const {
     const int count = static_cast<int>(w & kCountMask) + drafted;
-    const float off = count > 0 ? fmaf(freq, static_cast<float>(count), pres) : 0.f;
-    return count > 0 || (w & kPrompt) ? __float_as_uint(off == 0.f ? -0.f : off) : 0;
-  }
-  __device__ float apply(float x, uint32_t amount) const {
-    const float factor = x > 0.f ? inv_rep : rep;
-    return fmaf(x, amount != 0 ? factor : 1.f, -__uint_as_float(amount));
+    const float scaled = x * (x > 0.f ? inv_rep : rep);
+    x = count > 0 || (w & kPrompt) ? scaled : x;
+    return count > 0 ? x - fmaf(freq, static_cast<float>(count), pres) : x;
   }
 };
 
 // A block's entries: the tile's and the kVec before it, for the rows whose accesses begin there.
-constexpr int kEntries = kMaxTile + kVec, kFlagWords = (kEntries + 31) / 32;
+constexpr int kEntries = kMaxTile + kVec;
 constexpr int kSegment = kMaxTile / kLogitWarps;  // entries per warp and row, at most
 constexpr int kList = kSegment + kVec, kMaskWords = kSegment / 32 + 2;
 // Rows on their way to a warp, and for BF16 the row at hand in FP32.
-constexpr int kStages16 = 2, kStages32 = 2;
+constexpr int kStages16 = 2, kStages32 = 2;  // a third of BF16 costs a block per SM: 80 -> 96 us
 constexpr int kRowBytes = std::max(kStages16 * 2 + 4, kStages32 * 4) * kSegment;
 
 struct Tile {
   alignas(16) uint8_t rows[kLogitWarps][kRowBytes];
   uint32_t masks[kLogitWarps][kStages16][kMaskWords];
-  uint32_t words[kFlagWords * 32];      // per entry; then the amounts
-  uint32_t flags[kFlagWords];           // a bit per drafted or biased entry
-  uint16_t list[kLogitWarps][kList];    // the entries that have a word; the top bit repeats the flag
+  alignas(16) uint32_t words[kEntries];
+  uint16_t list[kLogitWarps][kList];  // the entries that have a word
   // Drafted or biased entries have a record: of a drafted token the number of its first node, of others
   // kMaxNodes + the place of the bias that holds.
   uint32_t record_word[kMaxNodes + kMaxBias];
@@ -72,13 +73,14 @@ struct Tile {
   uint16_t bias_id[kMaxBias], bias_at[kMaxBias];
   int bias_n;
 };
-static_assert(kEntries < 0x8000, "an entry fits 15 bits");
 
-// The rare entries: drafted or biased, `number` that of the record plus one; r the row of the request.
-__device__ __forceinline__ float adjust(float x, uint32_t number, int r, const Tile& s, const Penalties& penalties) {
-  const uint32_t i = number - 1, w = s.record_word[i];
-  x = penalties.apply(x, penalties.amount(w, i < kMaxNodes ? __popcll(s.path[i] & s.ancestors[r]) : 0));
-  return w & kBias ? x + s.record_bias[i] : x;
+// An entry of word w in row r of the request. The word of a drafted or biased one has its record's number
+// in place of the count.
+__device__ __forceinline__ float processed(float x, uint32_t w, int r, const Tile& s, const Penalties& penalties) {
+  if (!(w & (kDraft | kBias))) return penalties(x, w, 0);
+  const uint32_t i = w & kCountMask, whole = s.record_word[i];
+  x = penalties(x, whole, i < kMaxNodes ? __popcll(s.path[i] & s.ancestors[r]) : 0);
+  return whole & kBias ? x + s.record_bias[i] : x;
 }
 
 // The bias of an entry: the last of the request's list that names it, by its place in the tile's list, or -1.
@@ -106,8 +108,7 @@ __device__ __forceinline__ void one_entry(const LogitArgs& a, const Tile& s, con
   const int64_t at = row * a.V + v;
   float x = BF16 ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(a.logits)[at]) << 16)
                  : static_cast<const float*>(a.logits)[at];
-  const uint32_t amount = s.words[j];
-  x = s.flags[j / 32] >> (j % 32) & 1 ? adjust(x, amount, r, s, penalties) : penalties.apply(x, amount);
+  x = processed(x, s.words[j], r, s, penalties);
   const uint32_t* mask = reinterpret_cast<const uint32_t*>(a.d.mask);
   const bool allowed = !mask || (mask[row * ((a.V + 31) / 32) + v / 32] >> (v % 32) & 1);
   a.out[at] = allowed ? x * inv : -INFINITY;
@@ -162,7 +163,8 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_ke
     }
     cp_async_commit();
   };
-  for (int i = tid; i < kFlagWords * 32; i += kLogitThreads) s.words[i] = 0;
+  for (int i = tid * 4; i < a.tile + kVec; i += kLogitThreads * 4)
+    *reinterpret_cast<uint4*>(s.words + i) = make_uint4(0, 0, 0, 0);
   if (tid == 0) s.bias_n = 0;
   pdl_wait();
   pdl_trigger();
@@ -182,7 +184,10 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_ke
   penalties.freq = d.frequency ? d.frequency[b] : 0.f;
   penalties.pres = d.presence ? d.presence[b] : 0.f;
   const float inv = d.temperature ? __frcp_rn(d.temperature[b]) : 1.f;
+  const int32_t* bias_ids = d.bias_ids + static_cast<int64_t>(b) * d.bias_count;
   const float* bias = d.bias + static_cast<int64_t>(b) * d.bias_count;
+  const int first_id = tid < d.bias_count ? bias_ids[tid] : 0;
+  const float first_bias = tid < d.bias_count ? bias[tid] : 0.f;
   __syncthreads();
   constexpr int kAhead = 16;  // tokens in flight per thread; the first of them do not wait for the length
   for (int i0 = tid, bound = room; i0 < bound; i0 += kAhead * kLogitThreads, bound = length) {
@@ -200,61 +205,40 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_ke
       else atomicOr(&s.words[v[k]], kPrompt);
     }
   }
-  if (d.bias_ids) {
-    for (int k = tid; k < d.bias_count; k += kLogitThreads) {
-      const int id = d.bias_ids[static_cast<int64_t>(b) * d.bias_count + k];
+  for (int k = tid; k < d.bias_count; k += kLogitThreads) {
+    const uint32_t v = static_cast<uint32_t>(k == tid ? first_id : bias_ids[k]) - static_cast<uint32_t>(v0);
+    if (v < n) {
+      const int at = atomicAdd(&s.bias_n, 1);
+      s.bias_id[at] = static_cast<uint16_t>(v);
+      s.bias_at[at] = static_cast<uint16_t>(k);
+      s.record_bias[kMaxNodes + at] = k == tid ? first_bias : bias[k];
+      atomicOr(&s.words[v], kBias);
+    }
+  }
+  __syncthreads();
+  if (d.drafts) {  // a record of each token that is drafted, by its first node
+    if (tid < a.N) {
+      const int id = s.draft[tid];
       const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(v0);
-      if (v < n) {
-        const int at = atomicAdd(&s.bias_n, 1);
-        s.bias_id[at] = static_cast<uint16_t>(v);
-        s.bias_at[at] = static_cast<uint16_t>(k);
-        atomicOr(&s.words[v], kBias);
+      uint64_t path = 0;
+      for (int j = 0; j < a.N; ++j) path |= static_cast<uint64_t>(s.draft[j] == id) << j;
+      if (v < n && __ffsll(path) - 1 == tid) {
+        const uint32_t w = s.words[v] | kDraft;
+        if (w & kBias) s.record_bias[tid] = s.record_bias[kMaxNodes + last_bias(s, static_cast<int>(v))];
+        s.path[tid] = path;
+        s.record_word[tid] = w;
+        s.words[v] = kDraft | tid;
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
-  const bool records = d.drafts || s.bias_n;  // the same for the whole block
-  if (d.drafts && tid < a.N) {  // each token that is drafted once, with the nodes that carry it
-    const int id = s.draft[tid];
-    const uint32_t v = static_cast<uint32_t>(id) - static_cast<uint32_t>(v0);
-    uint64_t path = 0;
-    for (int j = 0; j < a.N; ++j) path |= static_cast<uint64_t>(s.draft[j] == id) << j;
-    const bool first = v < n && __ffsll(path) - 1 == tid;
-    s.draft_id[tid] = first ? static_cast<int>(v) : -1;
-    s.path[tid] = path;
-    if (first) {
-      const int k = last_bias(s, static_cast<int>(v));
-      s.record_bias[tid] = k < 0 ? 0.f : bias[s.bias_at[k]];
-      atomicOr(&s.words[v], kDraft);
-    }
-  }
-  if (records) __syncthreads();
-  for (int k = tid; k < s.bias_n; k += kLogitThreads) {
-    const int entry = s.bias_id[k];
-    const bool holds = !(s.words[entry] & kDraft) && last_bias(s, entry) == k;
-    s.record_word[kMaxNodes + k] = holds;
-    s.record_bias[kMaxNodes + k] = holds ? bias[s.bias_at[k]] : 0.f;
-  }
-  // words to amounts; drafted and biased entries get a flag
-  for (int j = tid; j < kFlagWords * 32; j += kLogitThreads) {
-    const uint32_t w = s.words[j];
-    const bool rare = w & (kDraft | kBias);
-    if (w != 0 && !rare) s.words[j] = penalties.amount(w, 0);
-    const uint32_t all = __ballot_sync(0xffffffffu, rare);
-    if (lane == 0) s.flags[j / 32] = all;
-  }
-  __syncthreads();
-  if (records) {  // and the records their words
-    if (d.drafts && tid < a.N && s.draft_id[tid] >= 0) {
-      uint32_t& w = s.words[s.draft_id[tid]];
-      s.record_word[tid] = w;
-      w = 1 + tid;
-    }
+  if (s.bias_n) {  // and of each other token that is biased
     for (int k = tid; k < s.bias_n; k += kLogitThreads) {
-      if (!s.record_word[kMaxNodes + k]) continue;
-      uint32_t& w = s.words[s.bias_id[k]];
+      const int entry = s.bias_id[k];
+      const uint32_t w = s.words[entry];
+      if (w & kDraft || last_bias(s, entry) != k) continue;
       s.record_word[kMaxNodes + k] = w;
-      w = 1 + kMaxNodes + k;
+      s.words[entry] = kBias | (kMaxNodes + k);
     }
     __syncthreads();
   }
@@ -267,11 +251,12 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_ke
   }
   // what the warp's rows have to treat: the entries of its parts, which begin at one of eight places
   int listed = 0;
+#pragma unroll 4
   for (int j0 = warp * segment; j0 < (warp + 1) * segment + kVec; j0 += 32) {
     const int j = j0 + lane;
     const bool has = j < (warp + 1) * segment + kVec && s.words[j] != 0;
     const uint32_t all = __ballot_sync(0xffffffffu, has);
-    if (has) s.list[warp][listed + __popc(all & ((1u << lane) - 1))] = j | (s.flags[j / 32] >> (j % 32) & 1) << 15;
+    if (has) s.list[warp][listed + __popc(all & ((1u << lane) - 1))] = j;
     listed += __popc(all);
   }
   __syncwarp();
@@ -298,12 +283,10 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_ke
     __syncwarp();
     // first the few entries that have a word, 32 at a time
     for (int i = lane; i < listed; i += 32) {
-      const uint32_t e = s.list[warp][i];
-      const int j = e & 0x7fff, l = j + v0 - part.v;
+      const int j = s.list[warp][i], l = j + v0 - part.v;
       if (l < part.lo * kVec || l >= part.hi * kVec) continue;
       float* at = reinterpret_cast<float*>(x + swizzled(l >> 2) * 16) + (l & 3);
-      const uint32_t amount = s.words[j];
-      *at = e & 0x8000 ? adjust(*at, amount, r, s, penalties) : penalties.apply(*at, amount);
+      *at = processed(*at, s.words[j], r, s, penalties);
     }
     __syncwarp();
 #pragma unroll
@@ -373,8 +356,9 @@ int qk_process_logits(const qk_logits_desc* desc, const void* logits, int in_dty
   a.vector = (reinterpret_cast<uintptr_t>(logits) & (bf16 ? 15 : 31)) == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0;
   const int lead = a.vector && V % kVec ? kVec - 1 : 0;  // by which a row's accesses may begin before a tile
   const int tiles = (V + lead + a.tile - 1) / a.tile;
-  // A block takes several rows of its request (each repeats the counting), but leaves 8 blocks per SM
-  // where there are as many: tiles of frequent tokens take longer than others.
+  // A block takes several rows of its request (each repeats the counting), but leaves 8 blocks per SM where
+  // there are as many: tiles of frequent tokens take longer than others. 16 x 24 rows of 151937: 89 us at 8,
+  // 95 at 4, 111 at 16.
   int parts = 1;
   while (parts < N && static_cast<int64_t>(B) * tiles * parts < 8 * sm_count()) parts *= 2;
   a.rows_per_block = (N + parts - 1) / parts;
