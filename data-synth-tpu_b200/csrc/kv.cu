@@ -115,30 +115,38 @@ __global__ void read_kernel(const int8_t* __restrict__ codes, const uint16_t* __
   }
 }
 
-// read_kernel for 8 channels per thread (one 8-byte load of codes, one scale; groups of 8 channels or
-// more): the same values, at an eighth of the index arithmetic, which bounded it (8448 slots of 1024
-// channels to BF16: 51 -> 6 us). I: an index type that holds `total`.
-template <typename I>
+struct WideDivider {
+  uint64_t divisor;
+  __device__ uint64_t operator()(uint64_t n) const { return n / divisor; }
+};
+
+// read_kernel for 8 channels per thread (one 8-byte load of codes, one scale; groups of 8, 16 or
+// 32): the same values, at an eighth of the index arithmetic, which bounded it (8448 slots of 1024
+// channels to BF16: 51 -> 6 us). I: an index type that holds `total`; Div: its division by D8 and S.
+template <typename I, typename Div>
 __global__ void __launch_bounds__(256) read8_kernel(const int8_t* __restrict__ codes, const uint16_t* __restrict__ plane,
-                                                    const int32_t* __restrict__ idx, I total, I S, int T, int D8, int G,
-                                                    int group8, int out_bf16, void* __restrict__ out) {
+                                                    const int32_t* __restrict__ idx, I total, Div by_S, Div by_D8, int T, int G,
+                                                    int group8_shift, int out_bf16, void* __restrict__ out) {
   const I stride = static_cast<I>(gridDim.x) * blockDim.x;
   for (I i = static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const I bs = i / D8;
+    const int D8 = static_cast<int>(by_D8.divisor);
+    const I bs = by_D8(i);
     const int col = static_cast<int>(i - bs * D8);
-    const int64_t b = bs / S;
+    const int64_t b = by_S(bs);
     const int t = wrap_clamp(idx[bs], T);
     const uint2 c = *reinterpret_cast<const uint2*>(codes + ((b * T + t) * D8 + col) * 8);
-    const float scale = bf16_to_f32(plane[(b * G + col / group8) * T + t]);
+    const float scale = bf16_to_f32(plane[(b * G + (col >> group8_shift)) * T + t]);
+    // with the sign bit flipped a code c is the byte c + 128: under the exponent of 2^23 it reads
+    // 2^23 + 128 + c, exactly (a conversion runs on a pipe an eighth as wide)
+    const uint32_t u[2] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u};
     float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      f[k] = __fmul_rn(static_cast<float>(static_cast<int8_t>((k < 4 ? c.x : c.y) >> (8 * (k & 3)))), scale);
+      f[k] = __fmul_rn(__uint_as_float(__byte_perm(u[k >> 2], 0x4b000000u, 0x7440 | (k & 3))) - 8388736.f, scale);
     if (out_bf16) {
       uint32_t w[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        w[k] = bf16_bits_rne(f[2 * k]) | static_cast<uint32_t>(bf16_bits_rne(f[2 * k + 1])) << 16;
+      for (int k = 0; k < 4; ++k) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(f[2 * k + 1]), "f"(f[2 * k]));
       reinterpret_cast<uint4*>(out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
       float4* o = reinterpret_cast<float4*>(out) + 2 * static_cast<int64_t>(i);
@@ -230,16 +238,19 @@ int qk_kv_q8_read(const int8_t* codes, const uint16_t* plane, const int32_t* ind
   if (B == 0 || S == 0) return QK_OK;
   QK_REQUIRE(codes && plane && indices && out, "null pointer");
   const int D = kv_heads * head_dim;
-  if (group % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+  if (group >= 8 && pow2_le32(group) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
     const int64_t total = static_cast<int64_t>(B) * S * (D / 8);
     const int grid = grid_for(total, 256);
-    // the stride past the end of a 32-bit index must not wrap
+    const auto launch = [&](auto kernel, auto count, auto by_S, auto by_D8) {
+      kernel<<<grid, 256, 0, as_stream(stream)>>>(codes, plane, indices, count, by_S, by_D8, T, D / group, group / 16,
+                                                  out_dtype == QK_OUT_BF16, out);
+    };
+    // below 2^31 the division is exact and the stride past the end of a 32-bit index does not wrap
     if (total < (1ll << 31))
-      read8_kernel<uint32_t><<<grid, 256, 0, as_stream(stream)>>>(codes, plane, indices, static_cast<uint32_t>(total), S, T, D / 8,
-                                                                 D / group, group / 8, out_dtype == QK_OUT_BF16, out);
+      launch(read8_kernel<uint32_t, Divider>, static_cast<uint32_t>(total), Divider(S), Divider(D / 8));
     else
-      read8_kernel<uint64_t><<<grid, 256, 0, as_stream(stream)>>>(codes, plane, indices, static_cast<uint64_t>(total), S, T, D / 8,
-                                                                 D / group, group / 8, out_dtype == QK_OUT_BF16, out);
+      launch(read8_kernel<uint64_t, WideDivider>, static_cast<uint64_t>(total), WideDivider{static_cast<uint64_t>(S)},
+             WideDivider{static_cast<uint64_t>(D / 8)});
     QK_LAUNCHED("read8_kernel");
     return QK_OK;
   }

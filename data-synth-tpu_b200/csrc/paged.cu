@@ -191,14 +191,36 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a) {
   }
 }
 
-// rint(x / scale) of the codec. The product with the reciprocal is within 2^-22 of the quotient, of
-// at most 127, so it rounds to the same integer unless it lies that close to a half (or is not
-// finite, or the reciprocal overflowed): then, once in some thousand values, the division decides.
-__device__ __forceinline__ float code_of(float x, float scale, float inverse) {
-  const float q = x * inverse;
-  float n = rintf(q);
-  if (!(fabsf(fabsf(q - n) - 0.5f) >= 1.f / 8192)) n = rintf(__fdiv_rn(x, scale));
-  return fminf(fmaxf(n, -127.f), 127.f);
+// rint(x / scale) of the codec, in -127 .. 127, for eight values: bytes of two words. The product with the
+// reciprocal is within 2^-22 of the quotient, of about 127 at most, so it rounds to the same integer unless
+// it lies that close to a half (or is not finite, or the reciprocal overflowed): then, for one warp in
+// some twenty, divisions decide. Adding 1.5 * 2^23 rounds and leaves the code in the sum's low byte: the
+// conversions that this replaces run on a pipe an eighth as wide.
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, float inverse) {
+  constexpr float kRound = 12582912.f;
+  uint32_t t[8];
+  bool near = true;  // an integer, and not near a half
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = x[i] * inverse, sum = fminf(fmaxf(q, -127.f), 127.f) + kRound;
+    t[i] = __float_as_uint(sum);
+    const float off = fabsf(fabsf(q - (sum - kRound)) - 0.5f);
+    near = near && off >= 1.f / 8192 && off < 2.f;
+  }
+  if (!near) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      float n = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) n = k == i ? x[k] : n;
+      n = fminf(fmaxf(rintf(__fdiv_rn(n, scale)), -127.f), 127.f);
+      const uint32_t code = static_cast<uint32_t>(static_cast<int>(static_cast<int8_t>(n)));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[k] = k == i ? code : t[k];
+    }
+  }
+  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
 }
 
 // Codec and scatter: a thread per 8 channels (one 16-byte load of BF16, two of FP32), the
@@ -210,13 +232,14 @@ __global__ void __launch_bounds__(256) write_slots_kernel(const void* __restrict
                                                           int64_t key_stride, int64_t value_stride,
                                                           const int32_t* __restrict__ slots, int8_t* k_codes,
                                                           int8_t* v_codes, uint16_t* k_scale, uint16_t* v_scale,
-                                                          uint32_t total, int D8, int G, int group8, int64_t T,
+                                                          uint32_t total, Divider by_D8, int G, int group8, int64_t T,
                                                           int64_t room) {
   pdl_wait();  // launched as a programmatic dependent: the keys' and values' producer first
   pdl_trigger();
-  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;  // below 2^32: checked by the host
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;  // below 2^31: checked by the host
   const bool in = i < total;
-  const uint32_t item = in ? i / D8 : 0;
+  const int D8 = static_cast<int>(by_D8.divisor);
+  const uint32_t item = in ? by_D8(i) : 0;
   const int col = in ? static_cast<int>(i - item * D8) : 0;
   const bool is_value = item & 1;
   const int64_t token = item >> 1;
@@ -244,17 +267,11 @@ __global__ void __launch_bounds__(256) write_slots_kernel(const void* __restrict
   if (!live) return;
   const float scale = bf16_round(__fdiv_rn(amax, 127.f));
   const float divisor = scale == 0.f ? 1.f : scale, inverse = __frcp_rn(divisor);
-  uint32_t code[2] = {0, 0};
-#pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    const int q = static_cast<int8_t>(code_of(x[t], divisor, inverse));
-    code[t >> 2] |= static_cast<uint32_t>(q & 255) << (8 * (t & 3));
-  }
   int8_t* codes = is_value ? v_codes : k_codes;
-  *reinterpret_cast<uint2*>(codes + (slot * D8 + col) * 8) = make_uint2(code[0], code[1]);
-  if (col % group8 == 0) {
-    const int64_t row = slot / T, t = slot - row * T;
-    (is_value ? v_scale : k_scale)[(row * G + col / group8) * T + t] = bf16_bits_rne(scale);
+  *reinterpret_cast<uint2*>(codes + (slot * D8 + col) * 8) = codes_of(x, divisor, inverse);
+  if ((col & (group8 - 1)) == 0) {
+    const int64_t row = slot < T ? 0 : slot / T, t = slot - row * T;
+    (is_value ? v_scale : k_scale)[(row * G + (col >> (31 - __clz(group8)))) * T + t] = bf16_bits_rne(scale);
   }
 }
 
@@ -305,11 +322,12 @@ int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64
              "codes must be 8-byte aligned");
   const int64_t total = tokens * 2 * (D / 8);
   const int64_t grid = (total + 255) / 256;
-  QK_REQUIRE(grid * 256 < (1ll << 32), "too many tokens in one call");
+  QK_REQUIRE(grid * 256 < (1ll << 31), "too many tokens in one call");
   const auto kernel = in_dtype == QK_OUT_BF16 ? write_slots_kernel<true> : write_slots_kernel<false>;
   const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, as_stream(stream),
                                          key, value, key_stride, value_stride, slots, k_codes, v_codes, k_scale, v_scale,
-                                         static_cast<uint32_t>(total), D / 8, D / group, group / 8, T, static_cast<int64_t>(rows) * T);
+                                         static_cast<uint32_t>(total), Divider(D / 8), D / group, group / 8, T,
+                                         static_cast<int64_t>(rows) * T);
   if (e != cudaSuccess) return cuda_error(e, "write_slots_kernel");
   count_launch();
   return QK_OK;
