@@ -193,31 +193,39 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a) {
 
 // rint(x / scale) of the codec, in -127 .. 127, for eight values: bytes of two words. The product with the
 // reciprocal is within 2^-22 of the quotient, of about 127 at most, so it rounds to the same integer unless
-// it lies that close to a half (or is not finite, or the reciprocal overflowed): then, for one warp in
-// some twenty, divisions decide. Adding 1.5 * 2^23 rounds and leaves the code in the sum's low byte: the
-// conversions that this replaces run on a pipe an eighth as wide.
-__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, float inverse) {
-  constexpr float kRound = 12582912.f;
+// it lies that close to a half. There FP32 values, one in 4096, take the division. A quotient of two BF16
+// numbers near a half is a half, as x and h * scale are multiples of 2^-8 of scale's power of two, or lies
+// 2^-9 away: rounded to multiples of 2^-10 it is the half that it stands for, and rounds to even. Scales
+// whose reciprocal is not normal, or not finite, take the division too.
+// Adding 1.5 * 2^23 rounds and leaves the code in the sum's low byte: the conversions that this replaces
+// run on a pipe an eighth as wide.
+template <bool BF16>
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale) {
+  constexpr float kRound = 12582912.f, kTenth = 12288.f;  // 1.5 * 2^23 and, to multiples of 2^-10, 1.5 * 2^13
+  const float inverse = __frcp_rn(scale);
   uint32_t t[8];
-  bool near = true;  // an integer, and not near a half
+  uint32_t unsure = scale > 0x1p-100f && scale < 0x1p100f ? 0u : 0xffu;  // a bit per value
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = x[i] * inverse, sum = fminf(fmaxf(q, -127.f), 127.f) + kRound;
+    float q = x[i] * inverse;
+    if (BF16) q = (q + kTenth) - kTenth;
+    const float sum = fminf(fmaxf(q, -127.f), 127.f) + kRound;
     t[i] = __float_as_uint(sum);
-    const float off = fabsf(fabsf(q - (sum - kRound)) - 0.5f);
-    near = near && off >= 1.f / 8192 && off < 2.f;
-  }
-  if (!near) {
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      float n = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) n = k == i ? x[k] : n;
-      n = fminf(fmaxf(rintf(__fdiv_rn(n, scale)), -127.f), 127.f);
-      const uint32_t code = static_cast<uint32_t>(static_cast<int>(static_cast<int8_t>(n)));
-#pragma unroll
-      for (int k = 0; k < 8; ++k) t[k] = k == i ? code : t[k];
+    if (!BF16) {
+      const float off = fabsf(fabsf(q - (sum - kRound)) - 0.5f);
+      unsure |= off >= 1.f / 8192 ? 0u : 1u << i;
     }
+  }
+  while (unsure) {
+    const int i = __ffs(unsure) - 1;
+    unsure &= unsure - 1;
+    float n = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) n = k == i ? x[k] : n;
+    n = fminf(fmaxf(rintf(__fdiv_rn(n, scale)), -127.f), 127.f);
+    const uint32_t code = static_cast<uint32_t>(static_cast<int>(static_cast<int8_t>(n)));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = k == i ? code : t[k];
   }
   return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
                     __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
@@ -266,9 +274,9 @@ __global__ void __launch_bounds__(256) write_slots_kernel(const void* __restrict
   for (int o = group8 >> 1; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!live) return;
   const float scale = bf16_round(__fdiv_rn(amax, 127.f));
-  const float divisor = scale == 0.f ? 1.f : scale, inverse = __frcp_rn(divisor);
+  const float divisor = scale == 0.f ? 1.f : scale;
   int8_t* codes = is_value ? v_codes : k_codes;
-  *reinterpret_cast<uint2*>(codes + (slot * D8 + col) * 8) = codes_of(x, divisor, inverse);
+  *reinterpret_cast<uint2*>(codes + (slot * D8 + col) * 8) = codes_of<BF16>(x, divisor);
   if ((col & (group8 - 1)) == 0) {
     const int64_t row = slot < T ? 0 : slot / T, t = slot - row * T;
     (is_value ? v_scale : k_scale)[(row * G + (col >> (31 - __clz(group8)))) * T + t] = bf16_bits_rne(scale);
