@@ -122,7 +122,7 @@ struct WideDivider {
 
 // read_kernel for 8 channels per thread (one 8-byte load of codes, one scale; groups of 8, 16 or
 // 32): the same values, at an eighth of the index arithmetic, which bounded it (8448 slots of 1024
-// channels to BF16: 51 -> 6 us). I: an index type that holds `total`; Div: its division by D8 and S.
+// channels to BF16: 51 -> 5.7 us, 4.7 TB/s, from and to L2 for the most part). I: an index type that holds `total`; Div: its division by D8 and S.
 template <typename I, typename Div>
 __global__ void __launch_bounds__(256) read8_kernel(const int8_t* __restrict__ codes, const uint16_t* __restrict__ plane,
                                                     const int32_t* __restrict__ idx, I total, Div by_S, Div by_D8, int T, int G,

@@ -13,7 +13,8 @@
 // wants and returns of the requests before b itself (B integers from L2) and then writes the
 // slots of 1024 tokens of request b. The last block row computes the new head and count.
 // Ancestor words come from pointer doubling (m |= m[p], p = p[p]): six rounds for 64 nodes.
-// Latency-bound: a few dependent L2 reads and one block-wide sum.
+// Latency-bound, a few dependent L2 reads and one block-wide sum: 64 requests of one token take 3.4 us,
+// 256 trees of 64 nodes 4.6, 61 prompt chunks of 2048 tokens 3.8, where an empty launch takes 2.
 #include "common.cuh"
 
 namespace qk {
@@ -234,7 +235,9 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale) {
 // Codec and scatter: a thread per 8 channels (one 16-byte load of BF16, two of FP32), the
 // group's maximum over its 4 lanes, 8 bytes of codes per thread and one BF16 scale per group.
 // The codes and scales are the append's (scale = bf16(max|x| / 127), code = rint(x / scale) of IEEE
-// quotients), so a token's bytes do not depend on the entry point that wrote it.
+// quotients), so a token's bytes do not depend on the entry point that wrote it. 8111 tokens of 8 heads of
+// 128: 22.0 us from FP32 (84 MB, 3.8 TB/s, 58% of measured HBM) and 22.7 from BF16, bound by the issue of
+// about 150 instructions per 8 channels; 64 tokens: 2.1 us.
 template <bool BF16>
 __global__ void __launch_bounds__(256) write_slots_kernel(const void* __restrict__ key, const void* __restrict__ value,
                                                           int64_t key_stride, int64_t value_stride,

@@ -23,6 +23,17 @@
 //    read as an MN-major operand for V (no transposition).
 //  * 2 warps issue the MMAs, Q K^T and P V: Q and P from TMEM, K and V from shared memory.
 // TMEM: O 256 columns, Q 128, two S/P buffers of 64.
+//
+// Measured with 16 query and 2 KV heads of 256 (join included; the floor is the cache's bytes at the measured
+// HBM rate, from 64 nodes on the products' flop at the measured BF16 rate):
+//   32 requests, 8 nodes, 8192 tokens    51 us, floor 23 (154 MB: 3.0 TB/s)
+//   16 requests, 64 nodes, 16384 tokens 140 us, floor 68 (112 GFLOP: 800 TFLOP/s; 166 us in a loop of seconds,
+//                                       under the power cap)
+//   1 request, 16 nodes, 32768 tokens    32 us, floor 5.5;  1 request, 1 node, 4096 tokens  20 us, floor 0.7
+// What bounds it: at 64 nodes a tile's chain of barriers (copy, decode, S, softmax, P, O; the copies and
+// barriers alone, nothing computed, take 106 of the 140 us) and the decode, which each of a KV head's four
+// row tiles repeats; at few rows the fixed 9 to 14 thousand cycles before the first tile (cold
+// instructions, four dependent reads to the first copy) and the 5 thousand of the last output and the join.
 #include <cuda.h>  // CUtensorMap and its enums; the encoder is looked up at run time
 
 #include "umma.cuh"

@@ -183,6 +183,7 @@ class TreeAttention:
     def __init__(self):
         self._ws = {}
         self._need = {}
+        self._outgrown = []  # a captured graph may still use them
 
     def _workspace(self, device, geometry):
         """The zeroed workspace of the device's current stream, of the size for ``(B, N, hq, kv, hd)``."""
@@ -193,6 +194,8 @@ class TreeAttention:
         key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
         ws = self._ws.get(key)
         if ws is None or ws.numel() < need:
+            if ws is not None:
+                self._outgrown.append(ws)
             ws = self._ws[key] = torch.zeros(need, dtype=torch.uint8, device=device)
         return ws
 
@@ -201,7 +204,8 @@ class TreeAttention:
         values are already in the cache as tokens ``lengths[b] + i``: each sees the prefix
         ``t < lengths[b]`` and the nodes of its word of ``ancestors`` (int64 ``[B, N]``,
         :func:`plan_step`); ``scale`` defaults to ``hd ** -0.5``. Returns BF16 ``[B, N, hq, hd]``,
-        times ``sigmoid(gate)`` where a gate is given; nodes past ``counts[b]`` are zero."""
+        times ``sigmoid(gate)`` where a gate is given; nodes past ``counts[b]`` are zero. Queries must
+        stay within 2^22 and keys within 2^20; a node that sees a draft that is not finite is NaN."""
         if q.dtype != torch.bfloat16 or q.dim() != 4:
             raise TypeError("q must be BF16 [B, N, query_heads, head_dim]")
         shape, device = q.shape, q.device

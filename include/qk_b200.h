@@ -399,7 +399,7 @@ int qk_paged_plan(int32_t* table, const int32_t* held, int32_t* ring, const int3
  * values, tokens key_stride / value_stride values apart, 16-byte aligned) are quantised into slot
  * slots[i] of [0, rows * T); other slots (-1: padding) are dropped. The same codec and the same
  * bytes as qk_kv_q8_append. Two tokens must not name one slot. head_dim a multiple of 32, or 8 or
- * 16. */
+ * 16; tokens * kv_heads * head_dim below 2^33. */
 int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64_t key_stride,
                          int64_t value_stride, const int32_t* slots, int8_t* k_codes, int8_t* v_codes,
                          uint16_t* k_scale, uint16_t* v_scale, int64_t tokens, int rows, int64_t T,
@@ -410,13 +410,15 @@ int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64
  * lengths[b] + i, sees the prefix t < lengths[b] and the nodes j < counts[b] of its ancestor word
  * ancestors[b, i] (uint64 [B, N]); out = softmax(q . k * scale) v over them with k, v = code *
  * scale, times sigmoid(gate) when gate != NULL, rounded once to BF16. Nothing else in the cache has
- * a say, whatever it holds; a node that sees nothing and nodes i >= counts[b] are zero. q BF16
+ * a say, whatever it holds; a node that sees nothing and nodes i >= counts[b] are zero. Keys, values,
+ * queries and weights enter the products with 11 significant bits, sums and statistics are FP32. For
+ * that queries must stay within 2^22 and keys within 2^20 (values may have any finite size); a node
+ * that sees a draft whose key or value is not finite, or 2^121 x 127 and more, is NaN. q BF16
  * [B, N, hq, head_dim] with tokens q_stride values apart (a multiple of 8), gate and out contiguous;
  * hq a multiple of kv_heads, head_dim 64, 128 or 256. The workspace (256-byte aligned) must be
  * zeroed before its first call; calls that share one must not overlap. qk_tree_attention_check
- * synchronises `stream`, reports an earlier call's table entry outside the cache
- * or length outside its table
- * (QK_ERR_INVALID_ARGUMENT; the output is then not valid) or a bounded wait that gave up
+ * synchronises `stream`, reports an earlier call's table entry outside the cache or length outside
+ * its table (QK_ERR_INVALID_ARGUMENT; the output is then not valid) or a bounded wait that gave up
  * (QK_ERR_TIMEOUT), and clears the report. */
 size_t qk_tree_attention_workspace_bytes(int B, int N, int hq, int kv_heads, int head_dim);
 int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes, const int8_t* v_codes,

@@ -219,6 +219,61 @@ def test_write_slots_takes_shapes_and_copies_uneven_strides(cuda_device):
         write_slots({n: t.cpu() for n, t in one.items()}, k, v, slots)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("power", [0, 40, -40, 117, -110, -130])
+def test_write_slots_codes_of_every_quotient(cuda_device, dtype, power):
+    """Every significand of the group's maximum against every significand and power of two of a value, halves
+    of a code among them, in the framework's codec byte for byte; also where scales are subnormal."""
+    import torch
+
+    from qk_b200.attention_cache import quantize
+    from qk_b200.paged import empty_pool, write_slots
+
+    significands = torch.arange(128, 256, dtype=torch.float32) / 128
+    others = (significands[None] * 2.0 ** -torch.arange(9, dtype=torch.float32)[:, None]).reshape(-1)  # 1152
+    others = others[:1116].view(36, 31)
+    top = 127 * significands * 2  # scale: the significand times 2, rounded
+    x = torch.cat([top[:, None, None].expand(128, 36, 1), others[None].expand(128, 36, 31) * top[:, None, None] / 1.99],
+                  dim=2)  # values below the maximum, some past its 127.5th part
+    exact = others[None] * significands[:, None, None] * 128  # and products that are whole and half codes
+    x = torch.stack([x, torch.cat([top[:, None, None].expand(128, 36, 1), exact], dim=2)])
+    x = (x.reshape(-1, 32) * torch.where(torch.arange(2 * 128 * 36) % 2 == 0, 1.0, -1.0)[:, None] * 2.0 ** power)
+    x = x.to(cuda_device).to(torch.bfloat16 if dtype == "bf16" else torch.float32)
+    tokens = x.shape[0] // 2
+    key, value = x.view(2, tokens, 1, 32)
+    cache = empty_pool(tokens // 16, 16, kv_heads=1, head_dim=32, device=cuda_device)
+    write_slots(cache, key, value, torch.arange(tokens, device=cuda_device))
+    for name, y in (("k", key), ("v", value)):
+        codes, scale = quantize(y.reshape(tokens, 32).contiguous(), 32)
+        assert torch.equal(cache[name].view(tokens, 32), codes)
+        assert torch.equal(cache[name + "_scale"].view(-1), scale.view(-1))
+
+
+@pytest.mark.parametrize("batch,selected,time,kv,hd", [(3, 7, 19, 3, 8), (1, 1, 1, 1, 16), (2, 1000, 333, 5, 32), (5, 64, 70, 7, 96),
+                                                       (2, 9, 11, 3, 24)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_reads_of_odd_shapes(cuda_device, batch, selected, time, kv, hd, dtype):
+    import torch
+
+    from qk_b200.attention_cache import CacheConfig, read_quantized
+
+    g = torch.Generator(device=cuda_device).manual_seed(selected)
+    group = min(32, hd)
+    groups = kv * hd // group
+    codes = torch.randint(-128, 128, (batch, time, kv * hd), generator=g, device=cuda_device).to(torch.int8)
+    scale = torch.randn((batch * groups, time), generator=g, device=cuda_device).to(torch.bfloat16)
+    idx = torch.randint(-time - 3, time + 3, (batch, selected), generator=g, device=cuda_device).to(torch.int32)
+    c = CacheConfig(kv_heads=kv, head_dim=hd, query_heads=kv, max_context=time)
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    cache = dict(k=codes, k_scale=scale, v=codes, v_scale=scale)
+    got = read_quantized(cache, "k", idx, c, dt)
+    at = torch.where(idx < 0, idx + time, idx).clamp(0, time - 1).long()
+    rows = torch.arange(batch, device=cuda_device)[:, None]
+    want = codes[rows, at].float().view(batch, selected, groups, group)
+    want = want * scale.view(batch, groups, time).permute(0, 2, 1)[rows, at].float()[..., None]
+    assert torch.equal(got.reshape(-1), want.reshape(-1).to(dt))
+
+
 # ---- tree attention ----------------------------------------------------------------------------
 
 
@@ -493,6 +548,37 @@ def test_tree_attention_strided_queries_and_streams(cuda_device):
             outs.append(tree_attention(q, cache, table, lengths, words, page_size=64))
     torch.cuda.synchronize()
     assert all(torch.equal(o, first) for o in outs)
+
+
+def test_tree_attention_captured_before_a_larger_call(cuda_device):
+    """A graph keeps the workspace that it was captured with, also when a later call needs a larger one."""
+    import torch
+
+    from qk_b200.paged import TreeAttention
+
+    attention = TreeAttention()
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    cache = random_pool(g, 1, 64 * 32, 2, 128)
+    table = torch.randperm(32, device=cuda_device, generator=g).to(torch.int32).view(2, 16)
+    lengths = torch.tensor([900, 77], device=cuda_device, dtype=torch.int32)
+    words = (2 << torch.arange(48, device=cuda_device)).sub(1).expand(2, 48).contiguous()
+    q = torch.randn((2, 48, 8, 128), device=cuda_device, generator=g).to(torch.bfloat16)
+    call = lambda n: attention(q[:, :n], cache, table, lengths, words[:, :n].contiguous(), page_size=64)  # noqa: E731
+    small = call(2)
+    stream, graph = torch.cuda.Stream(cuda_device), torch.cuda.CUDAGraph()
+    few, one = q[:, :2].contiguous(), words[:, :2].contiguous()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        attention(few, cache, table, lengths, one, page_size=64)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            out = attention(few, cache, table, lengths, one, page_size=64)
+        call(48)
+        junk = torch.full((1 << 26,), 255, dtype=torch.uint8, device=cuda_device)  # takes what was given back
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, small) and junk[0] == 255
 
 
 def test_tree_attention_offsets_past_32_bits(cuda_device):

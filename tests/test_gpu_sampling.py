@@ -107,6 +107,32 @@ def test_process_logits_rules(cuda_device, batch, nodes, vocab, room, names, dty
         assert again is x and np.array_equal(to_f32(x), got.astype(np.float32))
 
 
+@pytest.mark.parametrize("vocab", [4089, 4095, 4097, 4104, 5003, 8185, 8191, 9001])
+@pytest.mark.parametrize("nodes", [1, 9, 20])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_process_logits_ends_of_tiles(cuda_device, vocab, nodes, dtype, shift):
+    """Rows that begin at every place of an access, vocabularies that end about a tile's end, logits that
+    begin off an access, and a context with most of the vocabulary in it."""
+    import torch
+
+    from qk_b200.sampling import process_logits
+
+    rng = np.random.default_rng(vocab + nodes)
+    r = rules(rng, 2, nodes, vocab, 2 * vocab, ALL)
+    r["history"] = rng.integers(0, vocab, (2, 2 * vocab))
+    r["history_lengths"][0] = 2 * vocab
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    flat = torch.from_numpy(rng.normal(0, 3, 2 * nodes * vocab + 8).astype(np.float32)).to(cuda_device).to(dt)
+    x = flat[shift:shift + 2 * nodes * vocab].view(2, nodes, vocab)
+    given = {k: torch.from_numpy(v.view(np.int64) if v.dtype == np.uint64 else v).to(cuda_device) for k, v in r.items()}
+    got = to_f32(process_logits(x, **given)).astype(np.float64)
+    want, bound = oracle(to_f32(x).astype(np.float64), r)
+    finite = np.isfinite(want)
+    np.testing.assert_array_equal(got[~finite], want[~finite])
+    assert (np.abs(got[finite] - want[finite]) <= bound[finite]).all()
+
+
 def test_process_logits_two_dimensions_and_repeated_biases(cuda_device):
     """[B, V] logits; of several biases of one token the last holds, however many there are."""
     import torch
