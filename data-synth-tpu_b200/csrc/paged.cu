@@ -7,7 +7,8 @@
 //
 // Plan. With need_b = ceil((length_b + count_b) / P) pages and held_b in the table, request b
 // takes want_b = max(need_b - held_b, 0) pages from the ring of free pages (in request order;
-// it gets all of them or, where the ring or the table's width runs out, none) and returns
+// it gets all of them or, where the ring runs out, none; nor does one that outgrows its table, without
+// keeping pages from those behind it) and returns
 // max(held_b - need_b, 0). Takes come from the ring's head and returns go behind its tail, so
 // no block reads what another writes and every block can work alone: block (c, b) adds up the
 // wants and returns of the requests before b itself (B integers from L2) and then writes the
@@ -43,8 +44,8 @@ struct PlanArgs {
 struct Request {
   int length, count, held;
   int64_t need;
-  bool bad;
-  __device__ int64_t want() const { return need > held ? need - held : 0; }
+  bool bad, roomy;  // roomy: the table has a place for all its pages; one without takes none from the ring
+  __device__ int64_t want() const { return roomy && need > held ? need - held : 0; }
   __device__ int64_t drop() const { return held > need ? held - need : 0; }
 };
 
@@ -58,6 +59,7 @@ __device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
   r.held = min(max(h, 0), a.width);
   r.bad = r.length != n || r.count != c || r.held != h;
   r.need = (static_cast<int64_t>(r.length) + r.count + (1 << a.shift) - 1) >> a.shift;
+  r.roomy = r.need <= a.width;
   return r;
 }
 
@@ -99,7 +101,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a) {
       if (b0 + tid < a.B) r = load_request(a, b0 + tid);
       int64_t total, fitted, dropped;
       const int64_t w = r.want(), before = upto + block_prefix(w, warps, total);
-      block_prefix(before + w <= avail && r.need <= a.width ? w : 0, warps, fitted);
+      block_prefix(before + w <= avail ? w : 0, warps, fitted);
       block_prefix(r.drop(), warps, dropped);
       upto += total;
       taken += fitted;
@@ -122,13 +124,12 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a) {
   block_prefix(want, warps, wants);
   block_prefix(drop, warps, drops);
   const Request r = load_request(a, b);
-  const bool roomy = r.need <= a.width;
-  const bool fits = r.want() == 0 || (wants + r.want() <= avail && roomy);
+  const bool fits = r.want() == 0 || wants + r.want() <= avail;
   const int held = r.held + static_cast<int>((fits ? r.want() : 0) - r.drop());
   int32_t* row = a.table + static_cast<int64_t>(b) * a.width;
   // page p >= r.held of this request comes from the ring, in order
   auto fresh = [&](int p) { return a.ring[(head + wants + (p - r.held)) % a.pages]; };
-  int status = (r.bad ? kPlanBadLength : 0) | (fits ? 0 : roomy ? kPlanNoPages : kPlanTableFull);
+  int status = (r.bad ? kPlanBadLength : 0) | (!r.roomy ? kPlanTableFull : fits ? 0 : kPlanNoPages);
 
   if (blockIdx.x == 0) {
     for (int p = r.held + tid; p < held; p += kPlanThreads) row[p] = fresh(p);

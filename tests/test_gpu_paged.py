@@ -31,7 +31,7 @@ def plan_oracle(table, held, ring, span, lengths, counts, parents, nodes, page):
         need = -(-(length + count) // page)
         have = int(held[b])
         if need > have:
-            asked += need - have
+            asked += need - have if need <= width else 0
             if need > width:
                 status[b] = 2
             elif asked > free:
@@ -131,6 +131,29 @@ def test_plan_reports_bad_input_and_a_narrow_table(cuda_device):
     ring = np.array([0, 1, 2, 3, 9, 9, 9, 9, 8, 9])
     want, _, _ = check_plan(cuda_device, table, held, ring, np.array([8, 6]), lengths, counts, parents, 4, 16)
     assert list(want[5]) == [4, 4, 8, 2, 0]
+
+
+@pytest.mark.parametrize("nodes", [4, 100])
+def test_plan_beside_requests_that_outgrow_their_tables(cuda_device, nodes):
+    """They take no page, and those behind them take the pages that the ring gives up: each page stays with one
+    owner, and none is lost."""
+    rng = np.random.default_rng(nodes)
+    batch, page, width = 40, 16, 9
+    pages = batch * width
+    table, held = np.full((batch, width), -1), np.zeros(batch, np.int64)
+    ring, span = rng.permutation(pages), np.array([pages - 5, pages])
+    lengths = rng.integers(0, width * page + 20, batch)
+    full = 0
+    for _ in range(4):
+        counts = rng.integers(0, nodes + 1, batch)
+        want, table, ring = check_plan(cuda_device, table, held, ring, span, lengths, counts, None, nodes, page)
+        held, span = want[3], want[4]
+        full += int((want[5] == 2).sum())
+        owned = [int(p) for b in range(batch) for p in table[b, :held[b]]]
+        free = [int(ring[(span[0] + j) % pages]) for j in range(span[1])]
+        assert sorted(owned + free) == list(range(pages))
+        lengths = np.where(want[5] == 0, lengths + counts, rng.integers(0, width * page + 20, batch))
+    assert full > 8
 
 
 def test_plan_refusals():
