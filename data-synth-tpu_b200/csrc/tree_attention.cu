@@ -73,7 +73,7 @@ struct TreeArgs {
   const uint16_t* gate;
   float scale_log2;         // |scale| * log2(e) / (kQueryPower * kKeyPower), above zero
   uint32_t q_keep, q_flip;  // Q's bits & keep ^ flip: nothing for a scale of zero, the sign for a negative one
-  int B, N, hq, kv, rep, pages, pages_per_row, width, room, shift, row_tiles, part_rows;  // room: tokens of a table row
+  int B, N, hq, kv, rep, pages, pages_per_row, width, room, shift, row_tiles, part_rows, ctas;  // room: tokens of a table row
   int64_t T;
   uint16_t* out;
   int* status;
@@ -859,7 +859,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
     gate[0] = ld_guarded_v4(a.gate + to);
     gate[1] = ld_guarded_v4(a.gate + to + 8);
   }
-  const Parts parts = a.parts[unit];
+  Parts parts = a.parts[unit];
+  // a first kernel that gave up may have left them unwritten: what is read stays in the workspace
+  parts.first = min(max(parts.first, 0), a.ctas - 1);
+  parts.count = min(parts.count, a.ctas - parts.first);
   const int count = load_request(a, b).count;
   uint4* out = reinterpret_cast<uint4*>(a.out + to);
   if (row - lane >= count * a.rep) {  // nobody in these rows
@@ -1059,6 +1062,7 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   while ((1 << a.shift) < page_size) ++a.shift;
   a.row_tiles = w.row_tiles;
   a.part_rows = w.part_rows;
+  a.ctas = sm_count();
   a.T = T;
   a.out = out;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
