@@ -5,8 +5,8 @@
 //   x -= f * count + p * [count > 0];  x += bias;  x /= temperature;  mask bit 0: x = -inf
 //
 // A logit in, an FP32 value out and one mask bit per entry: 16 requests of 24 rows of 151937 FP32 logits
-// have to move 475 MB, 72 us, and take 89 us (5.4 TB/s); in BF16 80 us. A single row of 151936 takes 6 us,
-// the latency of its four dependent reads. What made the difference (from 160 us):
+// have to move 475 MB, 72 us, and take 88 us (5.4 TB/s, 82% of measured HBM); in BF16 78 us. A single row of
+// 151936 takes 5.3 us, the latency of its dependent reads, and 64 of them 27 (58 MB), the block's counting. What made the difference (from 160 us):
 //  * A block owns a tile of the vocabulary of one request and counts the request's history into a 32-bit
 //    word per entry in shared memory; the words then serve all rows of the request, one per node of a draft
 //    tree (each tile re-reads the history, from L2). Word: bits 0-19 the count of generated tokens, then
@@ -28,7 +28,7 @@ namespace {
 constexpr int kLogitThreads = 256, kLogitWarps = kLogitThreads / 32;
 constexpr int kLogitBlocks = 3;  // per SM: shared memory
 constexpr int kVec = 8;  // entries per access
-constexpr int kMaxBias = 1024, kMaxNodes = 64, kMaxTile = 4096;  // tiles of 2048: 97 us for 89
+constexpr int kMaxBias = 1024, kMaxNodes = 64, kMaxTile = 4096;  // tiles of 2048: 97 us for 88
 constexpr int kMaxHistory = (1 << 20) - 1;
 constexpr uint32_t kCountMask = (1u << 20) - 1, kPrompt = 1u << 20, kDraft = 1u << 21, kBias = 1u << 22;
 
@@ -56,7 +56,7 @@ constexpr int kEntries = kMaxTile + kVec;
 constexpr int kSegment = kMaxTile / kLogitWarps;  // entries per warp and row, at most
 constexpr int kList = kSegment + kVec, kMaskWords = kSegment / 32 + 2;
 // Rows on their way to a warp, and for BF16 the row at hand in FP32.
-constexpr int kStages16 = 2, kStages32 = 2;  // a third of BF16 costs a block per SM: 80 -> 96 us
+constexpr int kStages16 = 2, kStages32 = 2;  // a third of BF16 costs a block per SM: 78 -> 96 us
 constexpr int kRowBytes = std::max(kStages16 * 2 + 4, kStages32 * 4) * kSegment;
 
 struct Tile {
@@ -189,7 +189,9 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_ke
   const int first_id = tid < d.bias_count ? bias_ids[tid] : 0;
   const float first_bias = tid < d.bias_count ? bias[tid] : 0.f;
   __syncthreads();
-  constexpr int kAhead = 16;  // tokens in flight per thread; the first of them do not wait for the length
+  // Tokens in flight per thread; the first of them do not wait for the length. 64 rows of 151936 with histories
+  // of up to 2048: 27 us at 8, 30 at 16; with a branch around each of the 16 instead, 16 x 24 rows 112 for 88.
+  constexpr int kAhead = 8;
   for (int i0 = tid, bound = room; i0 < bound; i0 += kAhead * kLogitThreads, bound = length) {
     uint32_t v[kAhead];
 #pragma unroll
@@ -249,15 +251,25 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_ke
         one_entry<BF16>(a, s, penalties, inv, b, r, v0 + j, j);
     return;
   }
-  // what the warp's rows have to treat: the entries of its parts, which begin at one of eight places
+  // what the warp's rows have to treat: the entries of its parts, which begin at one of eight places. Four
+  // entries per lane; an entry's place follows those of the lanes before it and its lane's own before it.
   int listed = 0;
-#pragma unroll 4
-  for (int j0 = warp * segment; j0 < (warp + 1) * segment + kVec; j0 += 32) {
-    const int j = j0 + lane;
-    const bool has = j < (warp + 1) * segment + kVec && s.words[j] != 0;
-    const uint32_t all = __ballot_sync(0xffffffffu, has);
-    if (has) s.list[warp][listed + __popc(all & ((1u << lane) - 1))] = j;
-    listed += __popc(all);
+  const uint32_t below = (1u << lane) - 1;
+  for (int j0 = warp * segment, end = j0 + segment + kVec; j0 < end; j0 += 128) {
+    const int j = j0 + 4 * lane;
+    const uint4 u = j < end ? lds_v4(s.words + j) : make_uint4(0, 0, 0, 0);
+    if (!__any_sync(0xffffffffu, (u.x | u.y | u.z | u.w) != 0)) continue;
+    uint32_t all[4];
+    int at = listed;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      all[t] = __ballot_sync(0xffffffffu, word(u, t) != 0);
+      at += __popc(all[t] & below);
+      listed += __popc(all[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (word(u, t) != 0) s.list[warp][at++] = static_cast<uint16_t>(j + t);
   }
   __syncwarp();
 
@@ -357,8 +369,8 @@ int qk_process_logits(const qk_logits_desc* desc, const void* logits, int in_dty
   const int lead = a.vector && V % kVec ? kVec - 1 : 0;  // by which a row's accesses may begin before a tile
   const int tiles = (V + lead + a.tile - 1) / a.tile;
   // A block takes several rows of its request (each repeats the counting), but leaves 8 blocks per SM where
-  // there are as many: tiles of frequent tokens take longer than others. 16 x 24 rows of 151937: 89 us at 8,
-  // 95 at 4, 111 at 16.
+  // there are as many: tiles of frequent tokens take longer than others. 16 x 24 rows of 151937: 88 us at 8,
+  // 95 at 4, 96 at 12.
   int parts = 1;
   while (parts < N && static_cast<int64_t>(B) * tiles * parts < 8 * sm_count()) parts *= 2;
   a.rows_per_block = (N + parts - 1) / parts;
