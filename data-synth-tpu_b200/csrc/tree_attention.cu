@@ -201,6 +201,7 @@ __device__ __forceinline__ Walk locate(const TreeArgs& a, int me, int& total, bo
 struct Barriers {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[kStages], p_full[kStages], q_full, o_full;
+  uint64_t swapped[4], bad_read;  // a row's two warps have left their maxima; a unit's record of bad values is read
   uint64_t raw_full[2][kRaw], raw_empty[2][kRaw];  // K, V
 };
 
@@ -297,9 +298,6 @@ __device__ __forceinline__ float power_of(uint32_t bits) {
 __device__ __forceinline__ float inverse_power(float power) {
   return __uint_as_float((254u - (__float_as_uint(power) >> 23)) << 23);
 }
-
-// The two softmax warps of 32 rows.
-__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
 
 // A bounded wait of a whole warp, converged behind it: false for all lanes if one gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
@@ -615,7 +613,7 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t o_cols = tm + kColO + half * (HD / 2);
   Segment seg, next;
-  uint32_t it = 0;
+  uint32_t it = 0, swaps = 0, reads = 0;
   bool more = walk.next(a, next);
   auto busy_of = [&](const Segment& s) { return s.row_tile * kRows + quarter * 32 < s.r.count * a.rep; };
   auto give_q = [&](const Segment& s) {
@@ -676,7 +674,9 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
         float(*tops)[kRows] = ctl.top[it & 1];
         tops[half][quarter * 32 + lane] = top;
         // the pair's scores are both read by then: P may go over either's columns
-        pair_sync(quarter);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.bar.swapped[quarter]);
+        if (!warp_wait(&ctl.bar.swapped[quarter], swaps++ & 1)) return false;
         top = fmaxf(top, tops[half ^ 1][quarter * 32 + lane]);
         const bool grow = top > m + kLazyGrowth;
         if (__any_sync(0xffffffffu, grow)) {
@@ -731,38 +731,42 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
     more = walk.next(a, next);
     if (more) give_q(next);
     if (!warp_wait(&ctl.bar.o_full, seg.index & 1)) return false;
-    if (!busy) continue;
-    tc_fence_after();
-    // The unit's part of O as it is, FP32, channel by channel (32 rows are 128 B): the join divides,
-    // gates and rounds. A quarter of the instructions of doing that here, where nothing hides them.
-    const uint64_t* bad = ctl.bad[seg.index % kBadRing] + half * (HD / 64);
-    const int unit = (seg.b * a.kv + seg.head) * a.row_tiles + seg.row_tile;
-    const int64_t record = static_cast<int64_t>(unit) + blockIdx.x;
-    float* part = a.part + (record * HD + half * (HD / 2)) * a.part_rows + quarter * 32 + lane;
-#pragma unroll 1
-    for (int c = 0; c < HD / 64; ++c) {
-      uint32_t o[32];
-      tmem_ld32(o_cols + c * 32, o);
-      tmem_wait_ld();
-      if (bad[c] & path) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = 0x7fc00000u;
+    if (busy) {
+      tc_fence_after();
+      // The unit's part of O as it is, FP32, channel by channel (32 rows are 128 B): the join divides,
+      // gates and rounds. A quarter of the instructions of doing that here, where nothing hides them.
+      const uint64_t* bad = ctl.bad[seg.index % kBadRing] + half * (HD / 64);
+      const int unit = (seg.b * a.kv + seg.head) * a.row_tiles + seg.row_tile;
+      const int64_t record = static_cast<int64_t>(unit) + blockIdx.x;
+      float* part = a.part + (record * HD + half * (HD / 2)) * a.part_rows + quarter * 32 + lane;
+  #pragma unroll 1
+      for (int c = 0; c < HD / 64; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o_cols + c * 32, o);
+        tmem_wait_ld();
+        if (bad[c] & path) {
+  #pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0x7fc00000u;
+        }
+  #pragma unroll
+        for (int j = 0; j < 32; ++j) part[(c * 32 + j) * a.part_rows] = __uint_as_float(o[j]);
+        __syncwarp();
       }
-#pragma unroll
-      for (int j = 0; j < 32; ++j) part[(c * 32 + j) * a.part_rows] = __uint_as_float(o[j]);
-      __syncwarp();
+      float* stats = a.stats + record * 3 * a.part_rows + quarter * 32 + lane;
+      if (half == 0) stats[0] = m;
+      stats[(1 + half) * a.part_rows] = l;
+      if (seg.t0 == 0 && threadIdx.x == 0)
+        a.parts[unit] = Parts{static_cast<int>(blockIdx.x),
+                              Ranges(total, gridDim.x).owner(seg.start + seg.r.tiles - 1) - static_cast<int>(blockIdx.x) + 1};
+      tc_fence_before();
     }
-    float* stats = a.stats + record * 3 * a.part_rows + quarter * 32 + lane;
-    if (half == 0) stats[0] = m;
-    stats[(1 + half) * a.part_rows] = l;
-    if (seg.t0 == 0 && threadIdx.x == 0)
-      a.parts[unit] = Parts{static_cast<int>(blockIdx.x),
-                            Ranges(total, gridDim.x).owner(seg.start + seg.r.tiles - 1) - static_cast<int>(blockIdx.x) + 1};
-    tc_fence_before();
-    if (seg.r.length < seg.t1 * kTile) {  // the unit saw drafts: its record of bad values is read, clear it
-      const int pairs = min(kSoftmaxWarps / 2, (seg.r.count * a.rep - seg.row_tile * kRows + 31) / 32);
-      asm volatile("bar.sync 5, %0;" ::"r"(64 * pairs) : "memory");
-      if (warp == 0 && lane < 8) ctl.bad[seg.index % kBadRing][lane] = 0;
+    if (seg.r.length < seg.t1 * kTile) {  // the unit saw drafts: when all have read its bad values, clear them
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.bar.bad_read);
+      if (warp == 0) {
+        if (!warp_wait(&ctl.bar.bad_read, reads++ & 1)) return false;
+        if (lane < 8) ctl.bad[seg.index % kBadRing][lane] = 0;
+      }
     }
   }
   return true;
@@ -794,6 +798,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     }
     mbar_init(&ctl.bar.q_full, kSoftmaxWarps);
     mbar_init(&ctl.bar.o_full, 1);
+    mbar_init(&ctl.bar.bad_read, kSoftmaxWarps);
+    for (int i = 0; i < 4; ++i) mbar_init(&ctl.bar.swapped[i], 2);
     fence_mbar_init();
   }
   if (threadIdx.x < kBadRing * 8) ctl.bad[threadIdx.x / 8][threadIdx.x % 8] = 0;
