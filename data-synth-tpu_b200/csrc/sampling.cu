@@ -5,8 +5,9 @@
 //   x -= f * count + p * [count > 0];  x += bias;  x /= temperature;  mask bit 0: x = -inf
 //
 // A logit in, an FP32 value out and one mask bit per entry: 16 requests of 24 rows of 151937 FP32 logits
-// have to move 475 MB, 72 us, and take 88 us (5.4 TB/s, 82% of measured HBM); in BF16 78 us. A single row of
-// 151936 takes 5.3 us, the latency of its dependent reads, and 64 of them 27 (58 MB), the block's counting. What made the difference (from 160 us):
+// have to move 475 MB, 72 us, and take 88 us (5.4 TB/s, 82% of measured HBM); in BF16 78 us. A single row
+// of 151936 takes 5.3 us, the latency of its dependent reads, and 64 of them 27 (58 MB), bound by the issue
+// of the counting. What made the difference (from 160 us):
 //  * A block owns a tile of the vocabulary of one request and counts the request's history into a 32-bit
 //    word per entry in shared memory; the words then serve all rows of the request, one per node of a draft
 //    tree (each tile re-reads the history, from L2). Word: bits 0-19 the count of generated tokens, then

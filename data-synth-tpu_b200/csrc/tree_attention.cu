@@ -803,6 +803,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     fence_mbar_init();
   }
   if (threadIdx.x < kBadRing * 8) ctl.bad[threadIdx.x / 8][threadIdx.x % 8] = 0;
+  // All of the SM's tensor memory, asked for before earlier kernels end: this CTA's 61,440 registers leave
+  // room for no other that could be waiting for some at the same time.
   if (warp == kScoreWarp) tmem_alloc(&ctl.tmem, 512);
   tc_fence_before();
   __syncthreads();

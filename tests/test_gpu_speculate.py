@@ -89,13 +89,13 @@ def test_generated_tokens_are_greedy_choices(cuda_device, drafts):
     assert all(6 <= g <= 36 for g in grown) and all(o[:len(p)] == p for o, p in zip(out, prompts))
     if drafts == "branches":
         assert sum(grown) >= 2 * 6 * batch  # of up to 4 per step
-    judge = SpeculativeGeneration(model, batch, context, nodes=1, page_size=16, vocab=VOCAB)
+    single = SpeculativeGeneration(model, batch, context, nodes=1, page_size=16, vocab=VOCAB)
     one = torch.ones(batch, dtype=torch.int32, device=cuda_device)
     for t in range(max(len(o) for o in out) - 1):
         tokens = torch.tensor([[o[min(t, len(o) - 1)]] for o in out], dtype=torch.int32, device=cuda_device)
-        hidden, _ = judge.forward(tokens, one)
-        judge.cached = judge.cached + one
-        logits = to_f32(torch.matmul(hidden, judge.embedding.t()))
+        hidden, _ = single.forward(tokens, one)
+        single.cached = single.cached + one
+        logits = to_f32(torch.matmul(hidden, single.embedding.t()))
         for b, o in enumerate(out):
             if len(prompts[b]) - 1 <= t < len(o) - 1:
                 assert logits[b, o[t + 1]] >= logits[b].max() - 5e-2 * np.abs(logits[b]).max()
