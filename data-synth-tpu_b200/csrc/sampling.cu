@@ -19,8 +19,6 @@
 //  * Drafted and biased entries have a record, so that no row searches lists or waits for a global read.
 // Counts are integers and the last of several biases of one token holds by its index, so nothing depends on
 // the order of atomics.
-#include <algorithm>
-
 #include "common.cuh"
 
 namespace qk {
@@ -56,13 +54,13 @@ struct Penalties {
 constexpr int kEntries = kMaxTile + kVec;
 constexpr int kSegment = kMaxTile / kLogitWarps;  // entries per warp and row, at most
 constexpr int kList = kSegment + kVec, kMaskWords = kSegment / 32 + 2;
-// Rows on their way to a warp, and for BF16 the row at hand in FP32.
-constexpr int kStages16 = 2, kStages32 = 2;  // a third of BF16 costs a block per SM: 78 -> 96 us
-constexpr int kRowBytes = std::max(kStages16 * 2 + 4, kStages32 * 4) * kSegment;
+// Rows on their way to a warp (a third of BF16 costs a block per SM: 78 -> 96 us); of BF16 they take half of
+// the room, and the row at hand in FP32 the other half.
+constexpr int kStages = 2, kRowBytes = kStages * 4 * kSegment;
 
 struct Tile {
   alignas(16) uint8_t rows[kLogitWarps][kRowBytes];
-  uint32_t masks[kLogitWarps][kStages16][kMaskWords];
+  uint32_t masks[kLogitWarps][kStages][kMaskWords];
   alignas(16) uint32_t words[kEntries];
   uint16_t list[kLogitWarps][kList];  // the entries that have a word
   // Drafted or biased entries have a record: of a drafted token the number of its first node, of others
@@ -124,7 +122,7 @@ struct Part {
   int word;       // of the mask, the first that is copied
   __device__ Part(const LogitArgs& a, int64_t row, int v0, int segment, int warp) : base(row * a.V) {
     v = v0 + kVec - static_cast<int>(base + v0 & (kVec - 1)) + warp * segment;
-    lo = v < 0;  // an access is no longer than what lies before entry 0
+    lo = v < 0;  // by seven entries at most: the first access is not whole
     hi = min(segment, max(a.V - v, 0)) / kVec;
     word = max(v, 0) >> 5;
   }
@@ -137,7 +135,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(kLogitThreads, kLogitBlocks) process_logits_kernel(LogitArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Tile& s = *reinterpret_cast<Tile*>(smem);
-  constexpr int kSize = BF16 ? 2 : 4, kStages = BF16 ? kStages16 : kStages32, kBatch = kSegment / (32 * kVec);
+  constexpr int kSize = BF16 ? 2 : 4, kBatch = kSegment / (32 * kVec);
   // the tiles of the first tokens, usually the most frequent and so the slowest, start first
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int v0 = blockIdx.z * a.tile - kVec;  // of entry 0; below zero in the first tile
