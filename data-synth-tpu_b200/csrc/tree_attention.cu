@@ -422,8 +422,6 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
       uint4 code[SPT];
 #pragma unroll
       for (int i = 0; i < SPT; ++i) code[i] = lds_v4_at((i & 1 ? from_odd : from_even) + slot + i * HD);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_empty[stage]);
       if (tile * kTile + kTile > seg.r.length) {  // drafts, or past the end
         const int total = seg.r.length + seg.r.count;
 #pragma unroll
@@ -472,8 +470,13 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
       }
       fence_proxy_async_smem();
       __syncwarp();
+      // The raw slot goes back only here, where the stores above have used every code. An arrival right behind
+      // the loads does not hold them: the compiler may let them sink below it and the wait for the stage, and
+      // where that wait was long (a unit's first tiles) a warp decoded the tile that had come into the slot
+      // meanwhile: a pass of four over 16 trees of 64 nodes. It costs no time: 16384 tokens take 139.5 us.
       if (lane == 0) {
         mbar_arrive(&full[stage]);
+        mbar_arrive(&raw_empty[stage]);
       }
     }
   }

@@ -1,0 +1,107 @@
+"""The tree attention at full size, with calls in flight behind one another, and at the edges of its number
+formats, against 64 bits on the GPU."""
+
+import numpy as np
+import pytest
+
+from test_gpu_paged import random_pool, random_words
+
+pytestmark = pytest.mark.gpu
+
+
+def dense(q, cache, table, lengths, counts, words, page, gate=None, scale=None):
+    """``softmax(q . k * scale) v`` of every node in 64 bits: FP64 ``[B, N, hq, hd]``. A product with a weight of
+    zero is zero whatever it is multiplied by."""
+    import torch
+
+    batch, nodes, hq, hd = q.shape
+    rows, time, width = cache["k"].shape
+    kv, groups = width // hd, width // 32
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    scale = hd ** -0.5 if scale is None else scale
+    for b in range(batch):
+        n, c = int(lengths[b]), int(counts[b])
+        if c == 0:
+            continue
+        t = torch.arange(n + c, device=q.device)
+        slots = table[b].to(q.device).long()[t // page] * page + t % page
+        r, s = slots // time, slots % time
+        see = torch.ones((c, n + c), dtype=torch.bool, device=q.device)
+        word = words[b, :c].to(q.device).long()
+        see[:, n:] = ((word[:, None] >> torch.arange(c, device=q.device)) & 1).bool()
+        kd, vd = ((cache[m][r, s].view(n + c, groups, 32).double()
+                   * cache[m + "_scale"].view(rows, groups, time)[r, :, s].double()[..., None]).view(n + c, kv, hd)
+                  for m in ("k", "v"))
+        for h in range(kv):
+            heads = slice(h * hq // kv, (h + 1) * hq // kv)
+            x = torch.einsum("nhd,td->nht", q[b, :c, heads].double(), kd[:, h]) * scale
+            x = x.masked_fill(~see[:, None], -torch.inf)
+            w = torch.nan_to_num(torch.softmax(x, -1), nan=0.0)  # a node that sees nothing
+            out[b, :c, heads] = torch.einsum("nht,td->nhd", w, vd[:, h])
+    return out if gate is None else out * torch.sigmoid(gate.double())
+
+
+def request_batch(g, rng, batch, nodes, hq, kv, hd, page, lengths, counts, sharp=1.5, gate=True):
+    """The tensors of a call: ``dict`` of the arguments of tree_attention and counts, ragged as given."""
+    import torch
+
+    width = max(1, int(-(-(max(lengths) + nodes) // page)))
+    cache = random_pool(g, 1, batch * width * page, kv, hd)
+    table = torch.randperm(batch * width, generator=g, device=g.device).to(torch.int32).view(batch, width)
+    q = (torch.randn((batch, nodes, hq, hd), generator=g, device=g.device) * sharp).to(torch.bfloat16)
+    z = torch.randn((batch, nodes, hq, hd), generator=g, device=g.device).to(torch.bfloat16) if gate else None
+    i32 = dict(dtype=torch.int32, device=g.device)
+    words = torch.from_numpy(random_words(rng, batch, nodes).view(np.int64)).to(g.device)
+    return dict(q=q, cache=cache, table=table, lengths=torch.tensor(lengths, **i32), ancestors=words, page_size=page,
+                counts=torch.tensor(counts, **i32), gate=z)
+
+
+def exactly(call):
+    return dense(call["q"], call["cache"], call["table"], call["lengths"], call["counts"], call["ancestors"],
+                 call["page_size"], call["gate"])
+
+
+def off(out, want):
+    """Per (request, node, head): the 2-norm of the difference over that of the wanted row."""
+    return ((out.double() - want).norm(dim=-1) / want.norm(dim=-1).clamp(min=1e-30)).max().item()
+
+
+def where_differs(out, first):
+    """The place of the first differences: request, node, head and the channels there."""
+    bad = (out.view(-1, *out.shape[2:]) != first.view(-1, *out.shape[2:])).nonzero()
+    return f"{len(bad)} values, rows (request and node, head, channel) {bad[:6].tolist()} .. {bad[-3:].tolist()}"
+
+
+# A row's error is the rounding to BF16 (at most 1.7e-3 for a norm, see the test of eleven bits), that of the
+# scores (keys rounded to 11 bits: a relative 2^-12 / sqrt(3) of products that add up to a score of standard
+# deviation s is s * 1.4e-4, which moves weights by as much and rows that few tokens make by all of it) and of
+# weights and values (2.8e-4 together): 2e-3 for s = 1.5, and at s = 9 three deviations of 1.3e-3 more.
+@pytest.mark.parametrize("sharp,most,bound", [(1.5, 16384, 3e-3), (9.0, 3000, 8e-3)])
+def test_wide_trees_in_flight_behind_one_another(cuda_device, sharp, most, bound):
+    """16 trees of up to 64 nodes over ragged prefixes (one empty, one request without nodes): several row tiles
+    per KV head, idle quarters of them, one-tile units next to units of hundreds. Two sets of inputs are right by
+    themselves, and passes that alternate between them with no wait give the same bits every time. With sharp
+    scores the running maxima of single rows grow in the middle of a unit."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    calls, wants = [], []
+    for seed in (1, 2):
+        rng, g = np.random.default_rng(seed), torch.Generator(device=cuda_device).manual_seed(seed)
+        lengths, counts = rng.integers(1, most + 1, 16).tolist(), rng.integers(32, 65, 16).tolist()
+        lengths[0], counts[0], lengths[1], counts[2] = most, 64, 0, 0
+        calls.append(request_batch(g, rng, 16, 64, 16, 2, 256, 64, lengths, counts, sharp))
+        wants.append(exactly(calls[-1]))
+    firsts = []
+    for call, want in zip(calls, wants):
+        firsts.append(tree_attention(**call))
+        torch.cuda.synchronize()
+        assert off(firsts[-1], want) <= bound
+    for _ in range(4):
+        outs = [tree_attention(**calls[i % 2]) for i in range(60)]
+        torch.cuda.synchronize()
+        for i, out in enumerate(outs):
+            assert torch.equal(out, firsts[i % 2]), f"pass {i}: {where_differs(out, firsts[i % 2])}"
+        del outs
+    tree_attention.check_status()
