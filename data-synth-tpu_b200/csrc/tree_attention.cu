@@ -639,12 +639,12 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
     float m = -INFINITY, l = 0.f;
     for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
       if (!warp_wait(&ctl.bar.s_full[it & 1], (it / 2) & 1)) return false;
+      tc_fence_after();  // also where no row is busy: the next unit's Q goes where these products read theirs
       if (busy) {
-        tc_fence_after();
         uint32_t s[kHalf];
         const uint32_t cols = tm + kColS + (it & 1) * kTile;
         tmem_ld32(cols + half * kHalf, s);
-        tmem_wait_ld();
+        tmem_wait_ld(s);
         const int first = tile * kTile + half * kHalf;
         if (first + kHalf > seg.r.length) {  // drafts, or past the end: the row's 32 bits
           const int cut = seg.r.length - first;
@@ -677,9 +677,11 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
         float(*tops)[kRows] = ctl.top[it & 1];
         tops[half][quarter * 32 + lane] = top;
         // the pair's scores are both read by then: P may go over either's columns
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.bar.swapped[quarter]);
         if (!warp_wait(&ctl.bar.swapped[quarter], swaps++ & 1)) return false;
+        tc_fence_after();
         top = fmaxf(top, tops[half ^ 1][quarter * 32 + lane]);
         const bool grow = top > m + kLazyGrowth;
         if (__any_sync(0xffffffffu, grow)) {
@@ -696,7 +698,7 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
             for (int c = 0; c < HD / 64; ++c) {
               uint32_t o[32];
               tmem_ld32(o_cols + c * 32, o);
-              tmem_wait_ld();
+              tmem_wait_ld(o);
 #pragma unroll
               for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
               tmem_st32(o_cols + c * 32, o);
@@ -746,7 +748,7 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
       for (int c = 0; c < HD / 64; ++c) {
         uint32_t o[32];
         tmem_ld32(o_cols + c * 32, o);
-        tmem_wait_ld();
+        tmem_wait_ld(o);
         if (bad[c] & path) {
   #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0x7fc00000u;
