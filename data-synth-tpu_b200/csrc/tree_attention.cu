@@ -54,7 +54,10 @@ static_assert(2 * kSoftmaxRegs + 3 * kOtherRegs <= 5 * 96, "the shares fit the l
 constexpr uint32_t kColO = 0, kColQ = 256, kColS = 384;  // TMEM columns
 constexpr float kLazyGrowth = 8.f;                       // in powers of two
 constexpr uint32_t kHugeScale = 0x7c00;                  // BF16 bits of 2^121: times 127 it leaves FP32's range
-constexpr int kBadRing = 4, kFactors = 4;
+// Units whose records of bad values are alive at once. The value warps write tile n's when tile n - 3's product
+// is done, so all softmax warps have left the unit of tile n - 4 and its record is cleared.
+constexpr int kBadRing = 4;
+constexpr int kFactors = 4;
 // Queries and keys are multiplied by these for FP16: up to 2^22 and 2^20 fit it, and it leaves errors of
 // 2^-19 and 2^-21 to small ones, a few 2^-16 of a score.
 constexpr float kQueryPower = 1.f / 64, kKeyPower = 1.f / 16;
@@ -209,7 +212,7 @@ struct Control {
   Barriers bar;
   float top[2][2][kRows];     // by tile parity: the row maxima that a row's two warps swap
   float power[kFactors][kSide];  // of V per tile and 16 tokens: the power of two that was divided out
-  uint64_t bad[kBadRing][8];  // per unit and channel group: drafts that are not finite there
+  uint64_t bad[kBadRing][8];  // per unit and channel group: drafts whose values are not finite there
   uint32_t tmem;
 };
 
@@ -432,12 +435,15 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
           if (token >= total) {
             scales[i / 2] &= ~mask;
           } else if (token >= seg.r.length && bits >= kHugeScale) {
-            // a draft that is not finite must not reach the rows that do not see it, neither as 0 * inf
-            // nor through its neighbours' power of two: zero here, NaN at the end for those that do (in
-            // a value's group of channels, or for a key in all)
-            for (int g = values ? chunk / 2 : 0; g < (values ? chunk / 2 + 1 : HD / 32); ++g)
-              atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][g]),
-                       1ull << (token - seg.r.length));
+            // A draft that is not finite. A key's scores are NaN, which the mask keeps from rows that do not
+            // see it. A value must not reach those rows, neither as 0 * inf nor through its neighbours' power
+            // of two: zero here, and in its group of channels NaN at the end for the rows that do.
+            if (!values) {
+              scales[i / 2] |= mask & 0x7fff7fffu;
+              continue;
+            }
+            atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][chunk / 2]),
+                     1ull << (token - seg.r.length));
             scales[i / 2] &= ~mask;
           }
         }

@@ -105,3 +105,31 @@ def test_wide_trees_in_flight_behind_one_another(cuda_device, sharp, most, bound
             assert torch.equal(out, firsts[i % 2]), f"pass {i}: {where_differs(out, firsts[i % 2])}"
         del outs
     tree_attention.check_status()
+
+
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_drafts_that_are_not_finite_in_many_short_units(cuda_device, hd, which):
+    """Several requests of one tile per SM, one behind the other: a draft that is not finite makes the nodes that
+    see it NaN, and changes no bit of the requests before and behind it."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    batch, nodes, kv = 7 * torch.cuda.get_device_properties(cuda_device).multi_processor_count // 2, 3, 2
+    rng, g = np.random.default_rng(hd), torch.Generator(device=cuda_device).manual_seed(hd)
+    call = request_batch(g, rng, batch, nodes, 4, kv, hd, 16, rng.integers(0, 13, batch).tolist(), [nodes] * batch)
+    call["ancestors"] = torch.tensor([[1, 3, 5]], device=cuda_device).expand(batch, 3).contiguous()  # node 2 beside 1
+    good = tree_attention(**call)
+    hit = torch.arange(2, batch, 3, device=cuda_device)
+    at = call["lengths"][hit].long() + 1  # node 1's token
+    slots = call["table"][hit, at // 16].long() * 16 + at % 16
+    groups = hd // 32
+    call["cache"][which].view(kv, groups, -1)[1, groups - 1, slots] = float("nan")
+    want = good.clone()
+    touched = slice(None) if which == "k_scale" else slice(hd - 32, hd)
+    want[hit, 1, 2:, touched] = float("nan")  # node 1 of the second KV head's query heads
+    for _ in range(20):
+        out = tree_attention(**call)
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(want))
