@@ -16,11 +16,11 @@
 // One CTA per SM, three kinds of warps joined by mbarriers (every wait bounded):
 //  * 8 softmax warps, two threads per row: Q to TMEM once per unit; then per tile S from TMEM, mask,
 //    running maximum and sum in FP32, P as FP16 back over S's columns. O (FP32, in TMEM) is rescaled
-//    only when a row's maximum grows by more than 2^8: P stays below 2^8, far inside FP16's range.
+//    only when a row's maximum grows by more than 2^8: P, 2^7 at the maximum, stays below 2^15.
 //  * 8 decode warps (4 for K, 4 for V): codes and scales from shared memory, where a copy warp each
 //    brings them by tensor copies two tiles ahead; int8 -> FP16 with the group's scale (rounded once, to
-//    11 bits where BF16 has 8), stored as 128-byte swizzled tiles: K-major for K, and the same bytes
-//    read as an MN-major operand for V (no transposition).
+//    11 bits where BF16 has 8; the join computes what does not fit FP16 again, from the cache), stored as
+//    128-byte swizzled tiles: K-major for K, and the same bytes read as an MN-major operand for V.
 //  * 2 warps issue the MMAs, Q K^T and P V: Q and P from TMEM, K and V from shared memory.
 // TMEM: O 256 columns, Q 128, two S/P buffers of 64.
 //
@@ -57,10 +57,22 @@ constexpr uint32_t kHugeScale = 0x7c00;                  // BF16 bits of 2^121: 
 // Units whose records of bad values are alive at once. The value warps write tile n's when tile n - 3's product
 // is done, so all softmax warps have left the unit of tile n - 4 and its record is cleared.
 constexpr int kBadRing = 4;
-constexpr int kFactors = 4;
 // Queries and keys are multiplied by these for FP16: up to 2^22 and 2^20 fit it, and it leaves errors of
 // 2^-19 and 2^-21 to small ones, a few 2^-16 of a score.
 constexpr float kQueryPower = 1.f / 64, kKeyPower = 1.f / 16;
+// Values are divided by a power of two that a part finds for each 32 channels from the prefix in its first tile:
+// the largest scale there becomes 1 to 2. Scales up to 256 times as large still fit FP16 with their codes, those
+// down to 2^-14 keep all 11 bits, smaller ones leave errors of 127 * 2^-25. Drafts are not asked, for one must not
+// decide for the others: in a tile without prefix the values are divided by 2^-6, which takes those between 2^-13
+// and 2^10. (To ask the prefix's end then instead took code that cost 4 us of 135 where it was not run.)
+constexpr uint32_t kValueSpan = 64;  // of the exponents
+constexpr float kOnlyDrafts = 1.f / 64;
+constexpr float kDraftLimit = 512.f;  // a draft's scale by that power: 127 times this is no longer sure to fit
+// Weights go out as 2^(score - m + kWeightRoom), 2^15 at most: FP16 then keeps weights down to 2^-32 of the largest.
+constexpr float kWeightRoom = 7.f;
+// An output whose 16 channels are smaller than this on average (in the values' power) may have lost bits to FP16's
+// range: 2^11 times the error of 2^-18 above.
+constexpr float kSmall = 1.f / 128;
 constexpr uint32_t kQStage = 2048;  // bytes per softmax warp
 // What a unit costs besides its tiles (Q in, the output out), in tiles of the ranges: 16 requests of 64 nodes over
 // 16384 tokens take 160 us at 2, 145 at 4 and 140 at 6; 32 requests of 8 nodes over 8192 take 53 at 4 and 51 at 6.
@@ -82,6 +94,7 @@ struct TreeArgs {
   int* status;
   float* part;          // [units + CTAs][HD][part_rows] unnormalised O
   float* stats;         // [units + CTAs][3][part_rows] maximum (log2) and two sums
+  float* powers;        // [units + CTAs][HD / 32] what the part's values were divided by
   struct Parts* parts;  // [units]
 };
 
@@ -160,6 +173,11 @@ struct Walk {
   }
 };
 
+// A piece's unit among all, present or not.
+__device__ __forceinline__ int unit_of(const TreeArgs& a, const Segment& s) {
+  return (s.b * a.kv + s.head) * a.row_tiles + s.row_tile;
+}
+
 // The whole work and where range `me` of it begins; every warp finds out for itself (a lane per
 // request, no barrier).
 __device__ __forceinline__ Walk locate(const TreeArgs& a, int me, int& total, bool report) {
@@ -211,8 +229,7 @@ struct Barriers {
 struct Control {
   Barriers bar;
   float top[2][2][kRows];     // by tile parity: the row maxima that a row's two warps swap
-  float power[kFactors][kSide];  // of V per tile and 16 tokens: the power of two that was divided out
-  uint64_t bad[kBadRing][8];  // per unit and channel group: drafts whose values are not finite there
+  uint64_t bad[kBadRing][8];  // per unit and channel group: drafts whose values do not fit FP16 there
   uint32_t tmem;
 };
 
@@ -293,11 +310,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return r;
 }
 
-// The power of two 2^e with the BF16 exponent of `bits` (no sign), e in [-40, 126]: what is divided by
-// it lies below 2 (4 at the top), and FP16 takes it with all its bits down to 2^-14.
-__device__ __forceinline__ float power_of(uint32_t bits) {
-  return __uint_as_float(min(max(bits & 0x7f80u, (127u - 40u) << 7), (127u + 126u) << 7) << 16);
-}
+// A power of two by its exponent, biased as FP32 has it, and the inverse of one.
+__device__ __forceinline__ float power_of(uint32_t biased) { return __uint_as_float(biased << 23); }
 __device__ __forceinline__ float inverse_power(float power) {
   return __uint_as_float((254u - (__float_as_uint(power) >> 23)) << 23);
 }
@@ -385,11 +399,27 @@ __device__ __forceinline__ bool copy_role(const TreeArgs& a, Control& ctl, const
   return ok;
 }
 
+// For the power of two of a part's values: the largest scale, in 32 channels, of the prefix tokens in its first tile,
+// of which `scales` is the first.
+__device__ __forceinline__ uint32_t top_scale(uint32_t scales, int box, uint32_t box_stride, int known) {
+  uint32_t top = 0;
+  const int box_shift = 31 - __clz(box);
+#pragma unroll 1
+  for (int t = 0; t < known; t += 8) {
+    const uint4 u = lds_v4_at(scales + (t >> box_shift) * box_stride + (t & (box - 1)) * 2);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int left = known - t - 2 * w;
+      top = __vmaxu2(top, left > 1 ? word(u, w) & 0x7fff7fffu : left > 0 ? word(u, w) & 0x7fffu : 0u);
+    }
+  }
+  return max(top & 0xffffu, top >> 16);
+}
+
 // 4 decode warps for K and 4 for V, all in one copy of this code: with a copy each the CTA's hot code
 // left the instruction cache. FP16 has the bits but not the range of the cache's BF16 scales. Keys (and
 // queries) go in with a fixed power of two: what matters of them is a score's absolute error. Values
-// count relatively, so a warp divides the power of two of its 16 tokens' largest scale out of them; it
-// comes back through the weights' exponent.
+// count relatively, so a part has a power of its own per 32 channels, by which the join multiplies.
 template <int HD>
 __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uint32_t tiles, uint32_t raw, Walk walk) {
   constexpr int SPT = HD / 32, CHUNKS = HD / 16;  // a thread's share of a tile: 16 channels of SPT tokens
@@ -412,9 +442,20 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
   const int box = min(1 << a.shift, kTile);
   const uint32_t scales_at = raw + 2 * Raw<HD>::kCodes + (values ? Raw<HD>::kScales : 0) +
                              sub / box * Raw<HD>::box_stride(box) + (chunk / 2 * box + (sub & (box - 1))) * 2;
+  const uint32_t group_scales = raw + 2 * Raw<HD>::kCodes + Raw<HD>::kScales + chunk / 2 * box * 2;
+  float inverse = kKeyPower;
   Segment seg;
   uint32_t it = 0;
   while (walk.next(a, seg)) {
+    if (values) {  // outside the loop over tiles, whose code has to stay in the instruction cache
+      if (!warp_wait(&raw_full[it & 1], it >> 1 & 1)) return false;
+      const int known = seg.r.length - seg.t0 * kTile;
+      const uint32_t top = top_scale(group_scales + (it & 1) * Raw<HD>::kBytes, box, Raw<HD>::box_stride(box), min(known, kTile));
+      const float power = top ? power_of(min(max(top >> 7, 127u - kValueSpan), 127u + kValueSpan)) : kOnlyDrafts;
+      inverse = inverse_power(power);
+      if (t < CHUNKS && !(chunk & 1))
+        a.powers[static_cast<int64_t>(unit_of(a, seg) + static_cast<int>(blockIdx.x)) * (HD / 32) + chunk / 2] = power;
+    }
 #pragma unroll 1
     for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
       const uint32_t stage = it & 1, phase = it >> 1 & 1, slot = stage * Raw<HD>::kBytes;
@@ -434,28 +475,19 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
           const uint32_t bits = scales[i / 2] >> (16 * (i & 1)) & 0x7fffu;
           if (token >= total) {
             scales[i / 2] &= ~mask;
-          } else if (token >= seg.r.length && bits >= kHugeScale) {
-            // A draft that is not finite. A key's scores are NaN, which the mask keeps from rows that do not
-            // see it. A value must not reach those rows, neither as 0 * inf nor through its neighbours' power
-            // of two: zero here, and in its group of channels NaN at the end for the rows that do.
-            if (!values) {
-              scales[i / 2] |= mask & 0x7fff7fffu;
-              continue;
-            }
+          } else if (token < seg.r.length) {
+            // a prefix value past FP16's range is infinite in the products, which the join finds
+          } else if (!values) {
+            // the scores of a draft's key that is not finite are NaN, which the mask keeps from rows that do not see it
+            if (bits >= kHugeScale) scales[i / 2] |= mask & 0x7fff7fffu;
+          } else if (!(__uint_as_float(bits << 16) * inverse < kDraftLimit)) {
+            // a draft's value that does not fit must not reach the rows that do not see it as 0 * inf: zero here,
+            // and NaN for the rows that do
             atomicOr(reinterpret_cast<unsigned long long*>(&ctl.bad[seg.index % kBadRing][chunk / 2]),
                      1ull << (token - seg.r.length));
             scales[i / 2] &= ~mask;
           }
         }
-      }
-      float inverse = kKeyPower;
-      if (values) {
-        uint32_t top = scales[0] & 0x7fff7fffu;
-#pragma unroll
-        for (int i = 1; i < SPT / 2; ++i) top = __vmaxu2(top, scales[i] & 0x7fff7fffu);
-        const float power = power_of(__reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16)));
-        inverse = inverse_power(power);
-        if (lane == 0) ctl.power[it % kFactors][t / 32] = power;
       }
 #pragma unroll
       for (int i = 0; i < SPT / 2; ++i)
@@ -662,24 +694,13 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
           for (int j = 0; j < kHalf; ++j)
             if (!(see >> j & 1)) s[j] = 0xff800000u;
         }
-        // The weights go out as 2^(score + e - m), e the exponent that V's 16 tokens had divided out:
-        // times V's FP16 values that is the product with V itself, and m bounds them as stored. Sums
-        // take e off again.
-        float add[2], undo[2], top = -INFINITY;
-        if (!warp_wait(&ctl.bar.v_full[it % kStages], (it / kStages) & 1)) return false;
+        float most = -INFINITY, most2 = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float v = ctl.power[it % kFactors][half * 2 + g];
-          add[g] = static_cast<float>(static_cast<int>(__float_as_uint(v) >> 23) - 127);
-          undo[g] = inverse_power(v);
-          float most = -INFINITY, most2 = -INFINITY;
-#pragma unroll
-          for (int j = 16 * g; j < 16 * g + 16; j += 4) {
-            most = max3(most, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-            most2 = max3(most2, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
-          }
-          top = fmaxf(top, fmaf(fmaxf(most, most2), a.scale_log2, add[g]));
+        for (int j = 0; j < kHalf; j += 4) {
+          most = max3(most, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+          most2 = max3(most2, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
         }
+        float top = fmaxf(most, most2) * a.scale_log2;
         float(*tops)[kRows] = ctl.top[it & 1];
         tops[half][quarter * 32 + lane] = top;
         // the pair's scores are both read by then: P may go over either's columns
@@ -711,25 +732,22 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
             }
           }
         }
-        const float shift = m == -INFINITY ? 0.f : m;
+        const float shift = (m == -INFINITY ? 0.f : m) - kWeightRoom;
         uint32_t p[kHalf / 2];
+        const uint64_t mul2 = pair(a.scale_log2, a.scale_log2), add2m = pair(-shift, -shift);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const uint64_t mul2 = pair(a.scale_log2, a.scale_log2), add2g = pair(add[g] - shift, add[g] - shift);
-          uint64_t sum[2] = {0, 0};
-#pragma unroll
-          for (int j = 8 * g; j < 8 * g + 8; ++j) {
-            float x, y;
-            unpair(fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), mul2, add2g), x, y);
-            x = exp2_fast(x);
-            y = exp2_fast(y);
-            sum[j & 1] = add2(sum[j & 1], pair(x, y));
-            p[j] = pack_f16x2(x, y);
-          }
-          float even, odd;
-          unpair(add2(sum[0], sum[1]), even, odd);
-          l = fmaf(even + odd, undo[g], l);
+        for (int j = 0; j < kHalf / 2; ++j) {
+          float x, y;
+          unpair(fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), mul2, add2m), x, y);
+          x = exp2_fast(x);
+          y = exp2_fast(y);
+          sum[j & 1] = add2(sum[j & 1], pair(x, y));
+          p[j] = pack_f16x2(x, y);
         }
+        float even, odd;
+        unpair(add2(sum[0], sum[1]), even, odd);
+        l += even + odd;
         tmem_st16(cols + half * (kHalf / 2), p);
         tmem_wait_st();
         tc_fence_before();
@@ -747,7 +765,7 @@ __device__ __forceinline__ bool softmax_role(const TreeArgs& a, Control& ctl, ui
       // The unit's part of O as it is, FP32, channel by channel (32 rows are 128 B): the join divides,
       // gates and rounds. A quarter of the instructions of doing that here, where nothing hides them.
       const uint64_t* bad = ctl.bad[seg.index % kBadRing] + half * (HD / 64);
-      const int unit = (seg.b * a.kv + seg.head) * a.row_tiles + seg.row_tile;
+      const int unit = unit_of(a, seg);
       const int64_t record = static_cast<int64_t>(unit) + blockIdx.x;
       float* part = a.part + (record * HD + half * (HD / 2)) * a.part_rows + quarter * 32 + lane;
   #pragma unroll 1
@@ -856,9 +874,126 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
 // what the piece is and then its parts, so everything that can is asked for in the first.
 constexpr int kJoinWarps = 8, kJoinCols = 16;
 
+// Rows whose products may have left FP16's range, over 16 channels (of one group of 32), straight from the cache
+// in FP32: values past the range or far below their part's power, and what is not finite at all. `rows` are lanes,
+// row row0 + lane of a KV head; `zeros` those that came out zero. A warp per row, a lane per token: slow (a row of
+// 16384 tokens takes 1.5 ms), and no cache of ordinary values comes here.
+template <int HD>
+__device__ __forceinline__ void exact_rows(const TreeArgs& a, int b, int head, int row0, int col0, uint32_t rows,
+                                                uint32_t zeros) {
+  constexpr int G = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const Request r = load_request(a, b);
+  const int total = r.length + r.count, page_mask = (1 << a.shift) - 1;
+  const int32_t* table = a.table + static_cast<int64_t>(b) * a.width;
+  const float scale_log2 = a.scale_log2 * (kQueryPower * kKeyPower);
+  // the slot of a token and its first scale among the head's
+  const auto find = [&](int t, int64_t& slot, int64_t& plane) {
+    int page = table[t >> a.shift];
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) page = 0;  // reported by the first kernel
+    slot = (static_cast<int64_t>(page) << a.shift) + (t & page_mask);
+    const int cache_row = page / a.pages_per_row;
+    plane = (static_cast<int64_t>(cache_row) * a.kv + head) * G * a.T + slot - cache_row * a.T;
+  };
+  // the largest scale that a row sees, by whose power of two its sums stay in FP32's range: first of the prefix
+  uint32_t prefix = 0;
+#pragma unroll 4
+  for (int t = lane; t < r.length; t += 32) {
+    int64_t slot, plane;
+    find(t, slot, plane);
+    prefix = max(prefix, a.v_scale[plane + col0 / 32 * a.T] & 0x7fffu);
+  }
+  prefix = __reduce_max_sync(0xffffffffu, prefix);
+  for (; rows; rows &= rows - 1) {
+    const int i = __ffs(rows) - 1, row = row0 + i, node = row / a.rep, query = head * a.rep + row - node * a.rep;
+    const uint64_t path = a.ancestors[static_cast<int64_t>(b) * a.N + node];
+    const uint16_t* q = a.q + (static_cast<int64_t>(b) * a.N + node) * a.q_stride + static_cast<int64_t>(query) * HD;
+    uint32_t top = prefix;
+    bool broken = false;  // by a draft that is not finite
+    for (int t = r.length + lane; t < total; t += 32) {
+      if (!(path >> (t - r.length) & 1)) continue;
+      int64_t slot, plane;
+      find(t, slot, plane);
+      const uint32_t bits = a.v_scale[plane + col0 / 32 * a.T] & 0x7fffu;
+      top = max(top, bits);
+      broken = broken || bits >= kHugeScale;
+      for (int g = 0; g < G; ++g) broken = broken || (a.k_scale[plane + g * a.T] & 0x7fffu) >= kHugeScale;
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    broken = __any_sync(0xffffffffu, broken);
+    const float power = power_of(min(max(top >> 7, 1u), 253u)), inverse = inverse_power(power);
+    float m = -INFINITY, l = 0.f, o[kJoinCols];
+#pragma unroll
+    for (int j = 0; j < kJoinCols; ++j) o[j] = 0.f;
+    const bool done = broken || (top == 0 && (zeros >> i & 1));  // values that are all zero: so is what was found
+    for (int t = done ? total : lane; t < total; t += 32) {
+      if (t >= r.length && !(path >> (t - r.length) & 1)) continue;
+      int64_t slot, plane;
+      find(t, slot, plane);
+      const int64_t code = (slot * a.kv + head) * HD;
+      const uint4 v = *reinterpret_cast<const uint4*>(a.v_codes + code + col0);
+      const float scale = bf16_to_f32(a.v_scale[plane + col0 / 32 * a.T]) * inverse;
+      float x = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 64) {
+        uint4 k[4];
+        float by[2];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) k[h] = *reinterpret_cast<const uint4*>(a.k_codes + code + c + 16 * h);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) by[h] = bf16_to_f32(a.k_scale[plane + (c / 32 + h) * a.T]);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float part = 0.f;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint4 u = *reinterpret_cast<const uint4*>(q + c + 32 * g + 8 * h);
+            u = make_uint4((u.x & a.q_keep) ^ a.q_flip, (u.y & a.q_keep) ^ a.q_flip, (u.z & a.q_keep) ^ a.q_flip,
+                           (u.w & a.q_keep) ^ a.q_flip);
+            float f[8];
+            unpack8(u, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              part = fmaf(f[j], static_cast<float>(static_cast<int8_t>(word(k[2 * g + h / 2], 2 * (h % 2) + j / 4) >> 8 * (j % 4))),
+                          part);
+          }
+          x = fmaf(part, by[g], x);
+        }
+      }
+      x *= scale_log2;
+      const float now = fmaxf(m, x), shift = now == -INFINITY ? 0.f : now;
+      const float keep = exp2f(m - shift), p = exp2f(x - shift);
+      m = now;
+      l = fmaf(l, keep, p);
+#pragma unroll
+      for (int j = 0; j < kJoinCols; ++j)
+        o[j] = fmaf(o[j], keep, p * (static_cast<float>(static_cast<int8_t>(word(v, j / 4) >> 8 * (j % 4))) * scale));
+    }
+    float most = m;
+#pragma unroll
+    for (int s = 16; s; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+    const float share = exp2f(m - (most == -INFINITY ? 0.f : most));
+    l *= share;
+#pragma unroll
+    for (int s = 16; s; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+    const int64_t to = ((static_cast<int64_t>(b) * a.N + node) * a.hq + query) * HD + col0;
+#pragma unroll
+    for (int j = 0; j < kJoinCols; ++j) {
+      float sum = o[j] * share;
+#pragma unroll
+      for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+      if (lane != j) continue;
+      float f = broken ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : sum / l * power;
+      if (a.gate) f *= sigmoid_fast(bf16_to_f32(a.gate[to + j]));
+      a.out[to + j] = bf16_bits_rne(f);
+    }
+    __syncwarp();
+  }
+}
+
 template <int HD, int WARPS>
-__global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs a, int pieces) {
-  __shared__ float red[WARPS > 1 ? WARPS : 1][2][32];
+__global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(const __grid_constant__ TreeArgs a, int pieces) {
+  __shared__ float red[WARPS > 1 ? WARPS : 1][3][32];
   __shared__ float acc[WARPS > 1 ? WARPS : 1][kJoinCols][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int p = WARPS > 1 ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
@@ -889,8 +1024,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
     return;
   }
   const int64_t record = static_cast<int64_t>(unit) + parts.first;
-  // one pass with a running maximum, as over tiles
-  float m = -INFINITY, l = 0.f, o[kJoinCols];
+  // one pass with a running maximum, as over tiles; `power`: the parts' powers by their weight
+  const float* powers = a.powers + record * (HD / 32) + col0 / 32;
+  float m = -INFINITY, l = 0.f, power = 0.f, o[kJoinCols];
 #pragma unroll
   for (int j = 0; j < kJoinCols; ++j) o[j] = 0.f;
 #pragma unroll 2
@@ -898,6 +1034,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
     const float* st = a.stats + (record + i) * 3 * pr + in_tile;
     const float* part = a.part + ((record + i) * HD + col0) * pr + in_tile;
     const float x = st[0], y = st[pr] + st[2 * pr];
+    const float by = powers[i * (HD / 32)];
     float v[kJoinCols];
 #pragma unroll
     for (int j = 0; j < kJoinCols; ++j) v[j] = part[j * pr];
@@ -905,12 +1042,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
     const float keep = exp2_fast(m - shift), w = exp2_fast(x - shift);
     m = top;
     l = fmaf(l, keep, y * w);
+    power = fmaf(power, keep, y * w * by);
 #pragma unroll
-    for (int j = 0; j < kJoinCols; ++j) o[j] = fmaf(o[j], keep, v[j] * w);
+    for (int j = 0; j < kJoinCols; ++j) o[j] = fmaf(o[j], keep, v[j] * (w * by));
   }
   if (WARPS > 1) {
     red[warp][0][lane] = m;
     red[warp][1][lane] = l;
+    red[warp][2][lane] = power;
 #pragma unroll
     for (int j = 0; j < kJoinCols; ++j) acc[warp][j][lane] = o[j];
     __syncthreads();
@@ -919,33 +1058,43 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(TreeArgs 
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red[w][0][lane]);
     const float shift = top == -INFINITY ? 0.f : top;
-    l = 0.f;
+    l = power = 0.f;
 #pragma unroll
     for (int j = 0; j < kJoinCols; ++j) o[j] = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float f = exp2_fast(red[w][0][lane] - shift);
       l = fmaf(red[w][1][lane], f, l);
+      power = fmaf(red[w][2][lane], f, power);
 #pragma unroll
       for (int j = 0; j < kJoinCols; ++j) o[j] = fmaf(acc[w][j][lane], f, o[j]);
     }
   }
-  if (node >= a.N) return;
-  const float inv = node < count && (l > 0.f || l != l) ? 1.f / l : 0.f;
+  const bool sees = node < count && (l > 0.f || l != l);
+  float size = 0.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float f[8], z[8];
-    if (a.gate) unpack8(gate[h], z);
-    uint32_t w[4];
+  for (int j = 0; j < kJoinCols; ++j) size += fabsf(o[j]);
+  const bool lost = sees && !(size >= power * (kSmall * kJoinCols) && size < INFINITY);  // also where something is NaN
+  if (node < a.N && !lost) {
+    const float inv = sees ? 1.f / l : 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f[j] = inv == 0.f ? 0.f : o[h * 8 + j] * inv;
-      if (a.gate && inv != 0.f) f[j] *= sigmoid_fast(z[j]);
+    for (int h = 0; h < 2; ++h) {
+      float f[8], z[8];
+      if (a.gate) unpack8(gate[h], z);
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] = inv == 0.f ? 0.f : o[h * 8 + j] * inv;
+        if (a.gate && inv != 0.f) f[j] *= sigmoid_fast(z[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+      out[h] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
-    out[h] = make_uint4(w[0], w[1], w[2], w[3]);
   }
+  // Last, where nothing has to be kept. Inlined: as a function it made the compiler spill, 20.6 -> 21.6 us for one node.
+  const uint32_t rows = __ballot_sync(0xffffffffu, lost), zeros = __ballot_sync(0xffffffffu, size == 0.f && l == l);
+  if (__builtin_expect(rows != 0, 0)) exact_rows<HD>(a, b, head, row - lane, col0, rows, zeros);
 }
 
 constexpr size_t kHeader = 256;
@@ -975,7 +1124,7 @@ bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64
 struct Layout {
   int row_tiles, part_rows;
   int64_t units, records;
-  size_t parts, part, stats, bytes;
+  size_t parts, part, stats, powers, bytes;
 };
 Layout layout_of(int B, int N, int hq, int kv, int hd) {
   Layout w;
@@ -986,7 +1135,8 @@ Layout layout_of(int B, int N, int hq, int kv, int hd) {
   w.records = w.units + sm_count();
   w.parts = kHeader;
   w.stats = w.parts + (w.units * sizeof(Parts) + 255) / 256 * 256;
-  w.part = w.stats + static_cast<size_t>(w.records) * 3 * w.part_rows * sizeof(float);
+  w.powers = w.stats + static_cast<size_t>(w.records) * 3 * w.part_rows * sizeof(float);
+  w.part = w.powers + (static_cast<size_t>(w.records) * (hd / 32) * sizeof(float) + 255) / 256 * 256;
   w.bytes = w.part + static_cast<size_t>(w.records) * hd * w.part_rows * sizeof(float);
   return w;
 }
@@ -1089,6 +1239,7 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
   a.parts = reinterpret_cast<Parts*>(ws + w.parts);
   a.part = reinterpret_cast<float*>(ws + w.part);
   a.stats = reinterpret_cast<float*>(ws + w.stats);
+  a.powers = reinterpret_cast<float*>(ws + w.powers);
   Maps maps;
   const uint64_t D = static_cast<uint64_t>(kv_heads) * head_dim, slots = static_cast<uint64_t>(rows) * T;
   const uint32_t box = page_size < kTile ? page_size : kTile;

@@ -412,8 +412,11 @@ int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64
  * scale, times sigmoid(gate) when gate != NULL, rounded once to BF16. Nothing else in the cache has
  * a say, whatever it holds; a node that sees nothing and nodes i >= counts[b] are zero. Keys, values,
  * queries and weights enter the products with 11 significant bits, sums and statistics are FP32. For
- * that queries must stay within 2^22 and keys within 2^20 (values may have any finite size); a node
- * that sees a draft whose key or value is not finite, or 2^121 x 127 and more, is NaN. q BF16
+ * that queries must stay within 2^22 and keys within 2^20. Values may have any finite size: an output
+ * (16 channels of a query head) that 11 bits cannot give, because its values differ too much in size
+ * (256 times as large as the first 64 of a stretch, say), is computed in FP32, much more slowly. A node
+ * that sees a draft whose key or value has a scale that is not finite or 2^121 and more is NaN, for a
+ * value in its group of channels. q BF16
  * [B, N, hq, head_dim] with tokens q_stride values apart (a multiple of 8), gate and out contiguous;
  * hq a multiple of kv_heads, head_dim 64, 128 or 256. The workspace (256-byte aligned) must be
  * zeroed before its first call; calls that share one must not overlap. qk_tree_attention_check

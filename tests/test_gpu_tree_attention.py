@@ -133,3 +133,105 @@ def test_drafts_that_are_not_finite_in_many_short_units(cuda_device, hd, which):
         out = tree_attention(**call)
         assert torch.equal(torch.isnan(out), torch.isnan(want))
         assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(want))
+
+
+def group_error(out, want):
+    """The largest relative 2-norm of the error over the 32-channel groups of all rows, besides what BF16 rounds off
+    where its own numbers are subnormal: 2^-134 of each value."""
+    a, b = (x.double().reshape(-1, 32) for x in (out, want))
+    assert not a.isnan().any()
+    return (((a - b).norm(dim=-1) - 32 ** 0.5 * 2.0 ** -134) / b.norm(dim=-1).clamp(min=1e-300)).max().item()
+
+
+# A group of 32 channels: the rounding to BF16 is within 2^-9 of each value; values, weights and scores add 2^-12 /
+# sqrt(3) each, with which the weighted sum's terms err independently: below a third of that for any such group.
+GROUP_BOUND = 4e-3
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("power", [16, 40, 100])
+@pytest.mark.parametrize("length", [0, 30, 300])
+def test_a_large_draft_counts_for_the_nodes_that_see_it_alone(cuda_device, hd, power, length):
+    """A sibling whose value has another finite size, next to its neighbours' tokens, changes no bit of the rows
+    that do not see it; those that do agree with 64 bits."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    rng, g = np.random.default_rng(hd), torch.Generator(device=cuda_device).manual_seed(hd + length)
+    call = request_batch(g, rng, 2, 6, 4, 2, hd, 16, [length, 77], [6, 6])
+    call["ancestors"] = torch.tensor([[1, 3, 5, 11, 21, 37]], device=cuda_device).expand(2, 6).contiguous()
+    good = tree_attention(**call)
+    at = length + 1  # node 1, seen by nodes 1 and 3
+    slot = int(call["table"][0, at // 16]) * 16 + at % 16
+    call["cache"]["v_scale"][:, slot] *= 2.0 ** power
+    out = tree_attention(**call)
+    for node in range(6):
+        assert torch.equal(out[0, node], good[0, node]) == (node not in (1, 3))
+    assert torch.equal(out[1], good[1])
+    assert group_error(out[0, [1, 3]], exactly(call)[0, [1, 3]]) <= GROUP_BOUND
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("power", [12, 24, 60, -60])
+@pytest.mark.parametrize("at", [3, 40, 200])
+def test_a_prefix_token_of_another_size_and_no_weight(cuda_device, hd, power, at):
+    """A value 2^12 to 2^60 times its neighbours (or they that much larger than it), which every node sees with a
+    weight of about exp(-90): it neither takes the other values' bits nor adds anything."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    rng, g = np.random.default_rng(1), torch.Generator(device=cuda_device).manual_seed(hd)
+    call = request_batch(g, rng, 1, 2, 4, 2, hd, 64, [260], [2], gate=False)
+    call["q"] = (call["q"].abs() + 1).clamp(max=3.0)
+    slot = int(call["table"][0, at // 64]) * 64 + at % 64
+    cache = call["cache"]
+    cache["k"][0, slot] = -127
+    cache["k_scale"][:, slot] = 90.0 / 127 / hd ** 0.5
+    others = torch.arange(cache["v_scale"].shape[1], device=cuda_device) != slot
+    cache["v_scale"][:, ~others if power > 0 else others] *= 2.0 ** abs(power)
+    assert group_error(tree_attention(**call), exactly(call)) <= GROUP_BOUND
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["tiny", "huge", "groups", "growing", "falling", "mixed"])
+def test_values_of_many_sizes(cuda_device, hd, kind):
+    """All values of one size, each channel group of its own, sizes that change along the cache or from token to
+    token: every group of channels keeps its bits."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    rng, g = np.random.default_rng(2), torch.Generator(device=cuda_device).manual_seed(hd)
+    call = request_batch(g, rng, 3, 3, 8, 2, hd, 32, [700, 0, 65], [3, 3, 2])
+    plane = call["cache"]["v_scale"]
+    groups, slots = plane.shape
+    t = torch.empty(slots, device=cuda_device)  # a slot's token
+    for b in range(3):
+        t.view(-1, 32)[call["table"][b].long()] = torch.arange(call["table"].shape[1] * 32, device=cuda_device).view(-1, 32).float()
+    size = {"tiny": torch.full((groups, slots), -100.0), "huge": torch.full((groups, slots), 100.0),
+            "groups": (torch.arange(groups) * -14.0 + 30)[:, None].expand(groups, slots),
+            "growing": (t / 8).floor().expand(groups, slots), "falling": -(t / 8).floor().expand(groups, slots),
+            "mixed": torch.randint(-40, 40, (groups, slots), generator=g, device=cuda_device)}[kind]
+    plane.copy_((plane.double() * 2.0 ** size.to(cuda_device).double()).to(torch.bfloat16))
+    assert group_error(tree_attention(**call), exactly(call)) <= GROUP_BOUND
+
+
+def test_rows_past_the_fast_range_in_long_split_requests(cuda_device):
+    """What is computed again is found through the parts of a request that many ranges share, at scales of the
+    scores below and at zero, with values that are all zero beside."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    rng, g = np.random.default_rng(3), torch.Generator(device=cuda_device).manual_seed(3)
+    call = request_batch(g, rng, 1, 4, 16, 2, 256, 64, [6000], [4])
+    call["cache"]["v_scale"][2, 5 * 64 + 7] *= 2.0 ** 30
+    call["cache"]["v_scale"][5] = 0
+    for scale in (None, 0.0, -0.05):
+        out = tree_attention(**call, scale=scale)
+        want = dense(call["q"], call["cache"], call["table"], call["lengths"], call["counts"], call["ancestors"], 64,
+                     call["gate"], scale)
+        assert (out[:, :, :8, 5 * 32:6 * 32] == 0).all()
+        assert group_error(out, want) <= GROUP_BOUND
