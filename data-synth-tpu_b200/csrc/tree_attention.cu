@@ -78,6 +78,10 @@ constexpr uint32_t kQStage = 2048;  // bytes per softmax warp
 // 16384 tokens take 160 us at 2, 145 at 4 and 140 at 6; 32 requests of 8 nodes over 8192 take 53 at 4 and 51 at 6.
 constexpr int kUnitCost = 6;
 
+// What calls on the device reported last, besides the word in their workspaces: a workspace can be gone, or belong
+// to a graph, when somebody asks.
+__device__ int g_tree_status;
+
 struct TreeArgs {
   const uint16_t* q;
   int64_t q_stride;
@@ -121,6 +125,11 @@ __device__ __forceinline__ Request load_request(const TreeArgs& a, int b) {
   r.row_tiles = (r.count * a.rep + kRows - 1) / kRows;
   r.tiles = r.count ? (r.length + r.count + kTile - 1) / kTile : 0;
   return r;
+}
+
+__device__ __forceinline__ void report(const TreeArgs& a, int status) {
+  *a.status = status;
+  atomicExch(&g_tree_status, status);
 }
 
 // The CTAs' ranges of a total of `total` steps: n of them, the first total % n one step longer. All
@@ -180,7 +189,7 @@ __device__ __forceinline__ int unit_of(const TreeArgs& a, const Segment& s) {
 
 // The whole work and where range `me` of it begins; every warp finds out for itself (a lane per
 // request, no barrier).
-__device__ __forceinline__ Walk locate(const TreeArgs& a, int me, int& total, bool report) {
+__device__ __forceinline__ Walk locate(const TreeArgs& a, int me, int& total, bool tell) {
   const int lane = threadIdx.x & 31;
   total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
@@ -188,7 +197,7 @@ __device__ __forceinline__ Walk locate(const TreeArgs& a, int me, int& total, bo
     if (b0 + lane < a.B) {
       const Request r = load_request(a, b0 + lane);
       w = r.work(a.kv);
-      if (r.cut && report) *a.status = QK_ERR_INVALID_ARGUMENT;
+      if (r.cut && tell) report(a, QK_ERR_INVALID_ARGUMENT);
     }
     total += __reduce_add_sync(0xffffffffu, w);
   }
@@ -372,7 +381,7 @@ __device__ __forceinline__ bool copy_role(const TreeArgs& a, Control& ctl, const
     for (int tile = seg.t0; tile < seg.t1; ++tile, ++it) {
       const uint32_t slot = it % kRaw;
       if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) {  // reported, and read as page 0
-        *a.status = QK_ERR_INVALID_ARGUMENT;
+        report(a, QK_ERR_INVALID_ARGUMENT);
         page = 0;
       }
       const int y = (page << a.shift) + ((tile * kTile + mine) & ((1 << a.shift) - 1));  // the slot
@@ -856,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const __gri
     else if (warp == kScoreWarp) ok = score_role<HD>(a, ctl, ktiles, walk);
     else ok = value_role<HD>(a, ctl, vtiles, walk);
   }
-  if (!ok) *a.status = QK_ERR_TIMEOUT;
+  if (!ok) report(a, QK_ERR_TIMEOUT);
   tc_fence_before();
   __syncthreads();
   if (warp == kScoreWarp) {
@@ -1254,13 +1263,14 @@ int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes
 }
 
 int qk_tree_attention_check(const void* workspace, qk_stream_t stream) {
-  QK_REQUIRE(workspace, "null pointer");
   int status = 0;
   cudaStream_t st = as_stream(stream);
-  cudaError_t e = cudaMemcpyAsync(&status, workspace, sizeof(int), cudaMemcpyDeviceToHost, st);
+  void* word = const_cast<void*>(workspace);
+  cudaError_t e = word ? cudaSuccess : cudaGetSymbolAddress(&word, g_tree_status);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&status, word, sizeof(int), cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e == cudaSuccess && status) {
-    e = cudaMemsetAsync(const_cast<void*>(workspace), 0, sizeof(int), st);
+    e = cudaMemsetAsync(word, 0, sizeof(int), st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   }
   if (e != cudaSuccess) return cuda_error(e, "qk_tree_attention_check");

@@ -243,14 +243,11 @@ class TreeAttention:
         return out
 
     def check_status(self, device=None):
-        """Raise what earlier calls on the current stream reported (a table entry outside the
-        cache, a length outside the table, a bounded wait that gave up); synchronises the stream."""
+        """Raise what earlier calls on the device reported, in graphs and on other streams too as far as they have
+        run (a table entry outside the cache, a length outside the table, a bounded wait that gave up);
+        synchronises the current stream."""
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        with torch.cuda.device(device):
-            index = torch.cuda.current_device()
-            ws = self._ws.get((index, torch._C._cuda_getCurrentRawStream(index)))
-            if ws is not None:
-                _lib.call_on(torch.device("cuda", index), "qk_tree_attention_check", ws.data_ptr())
+        _lib.call_on(device, "qk_tree_attention_check", None)
 
 
 tree_attention = TreeAttention()

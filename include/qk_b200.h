@@ -422,7 +422,8 @@ int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64
  * zeroed before its first call; calls that share one must not overlap. qk_tree_attention_check
  * synchronises `stream`, reports an earlier call's table entry outside the cache or length outside
  * its table (QK_ERR_INVALID_ARGUMENT; the output is then not valid) or a bounded wait that gave up
- * (QK_ERR_TIMEOUT), and clears the report. */
+ * (QK_ERR_TIMEOUT), and clears the report: of the calls with this workspace, or with workspace NULL
+ * of all calls on the current device. */
 size_t qk_tree_attention_workspace_bytes(int B, int N, int hq, int kv_heads, int head_dim);
 int qk_tree_attention(const uint16_t* q, int64_t q_stride, const int8_t* k_codes, const int8_t* v_codes,
                       const uint16_t* k_scale, const uint16_t* v_scale, const int32_t* table,

@@ -235,3 +235,46 @@ def test_rows_past_the_fast_range_in_long_split_requests(cuda_device):
                      call["gate"], scale)
         assert (out[:, :, :8, 5 * 32:6 * 32] == 0).all()
         assert group_error(out, want) <= GROUP_BOUND
+
+
+def test_reports_outlive_their_workspace_and_come_out_of_graphs(cuda_device):
+    """A bad page is reported after a larger call has taken a larger workspace, from another stream, and from every
+    replay of a graph, one that was captured without a call before it included; a report is raised once."""
+    import torch
+
+    from qk_b200.paged import TreeAttention
+
+    attend = TreeAttention()
+    rng, g = np.random.default_rng(4), torch.Generator(device=cuda_device).manual_seed(4)
+    call = request_batch(g, rng, 2, 2, 4, 2, 64, 16, [40, 30], [2, 2])
+    large = request_batch(g, rng, 40, 16, 4, 2, 64, 16, [40] * 40, [16] * 40)
+    bad = dict(call, table=call["table"].clone().fill_(1 << 20))
+    attend.check_status()
+    attend(**bad)
+    attend(**large)
+    with pytest.raises(ValueError):
+        attend.check_status()
+    attend.check_status()
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(**bad)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError):
+        attend.check_status()
+    held = dict(call, table=call["table"].clone())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = TreeAttention()(**held)
+    graph.replay()
+    attend.check_status()
+    assert torch.equal(out, attend(**call))
+    held["table"].copy_(bad["table"])
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(ValueError):
+            attend.check_status()
+    held["table"].copy_(call["table"])
+    graph.replay()
+    attend.check_status()
+    assert torch.equal(out, attend(**call))
