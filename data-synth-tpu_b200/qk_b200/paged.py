@@ -178,24 +178,29 @@ def write_slots(cache, key, value, slots):
 
 
 class TreeAttention:
-    """Attention of drafted tokens over a paged Q8 cache, with a workspace per stream."""
+    """Attention of drafted tokens over a paged Q8 cache, with a workspace per stream; calls in a graph have
+    theirs in the graph's memory, so that graphs may be replayed beside one another."""
 
     def __init__(self):
         self._ws = {}
         self._need = {}
-        self._outgrown = []  # a captured graph may still use them
 
     def _workspace(self, device, geometry):
-        """The zeroed workspace of the device's current stream, of the size for ``(B, N, hq, kv, hd)``."""
+        """The workspace of a call on the device's current stream, of the size for ``(B, N, hq, kv, hd)``."""
         need = self._need.get(geometry)
         if need is None:
             with torch.cuda.device(device):
                 need = self._need[geometry] = int(_lib.load().qk_tree_attention_workspace_bytes(*geometry))
+        if torch.cuda.current_device() == device.index:
+            capturing = torch._C._cuda_isCurrentStreamCapturing()
+        else:
+            with torch.cuda.device(device):
+                capturing = torch._C._cuda_isCurrentStreamCapturing()
+        if capturing:
+            return torch.empty(need, dtype=torch.uint8, device=device)
         key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
         ws = self._ws.get(key)
         if ws is None or ws.numel() < need:
-            if ws is not None:
-                self._outgrown.append(ws)
             ws = self._ws[key] = torch.zeros(need, dtype=torch.uint8, device=device)
         return ws
 

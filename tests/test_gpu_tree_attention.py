@@ -278,3 +278,32 @@ def test_reports_outlive_their_workspace_and_come_out_of_graphs(cuda_device):
     graph.replay()
     attend.check_status()
     assert torch.equal(out, attend(**call))
+
+
+def test_graphs_replayed_beside_one_another(cuda_device):
+    """Two graphs, captured one after the other on torch's one capture stream, and calls outside them run on three
+    streams at once: none writes into another's parts."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    calls = []
+    for seed in (5, 6, 7):
+        rng, g = np.random.default_rng(seed), torch.Generator(device=cuda_device).manual_seed(seed)
+        calls.append(request_batch(g, rng, 3, 4, 16, 2, 256, 64, [5000, 400, 3000], [4, 3, 4]))
+    wants = [tree_attention(**c) for c in calls]
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph, call in zip(graphs, calls):
+        with torch.cuda.graph(graph):
+            outs.append([tree_attention(**call) for _ in range(10)])
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            outside = [tree_attention(**calls[2]) for _ in range(10)]
+        torch.cuda.synchronize()
+        for got, want in zip([*outs, outside], wants):
+            assert all(torch.equal(o, want) for o in got)
