@@ -153,10 +153,14 @@ class SpeculativeGeneration:
 
     def prefill(self, prompts):
         """``prompts``: token lists, one per sequence. All but the last token of each go into the cache,
-        ``nodes`` at a time; the last is the first step's node 0."""
+        ``nodes`` at a time; the last is the first step's node 0. What was generated before is forgotten, and
+        all pages are free again."""
         if len(prompts) != self.batch or any(not 0 < len(p) <= self.context for p in prompts):
             raise ValueError("one prompt of 1 to `context` tokens per sequence")
         dev = self.model.device
+        self.table, self.held, self.ring, self.span = empty_tables(self.batch, self.table.shape[1], self.ring.shape[0], dev)
+        self.cached, self.status = torch.zeros_like(self.cached), torch.zeros_like(self.status)
+        self.history.zero_()
         longest = max(len(p) for p in prompts)
         rows = torch.tensor([list(p) + [0] * (longest - len(p)) for p in prompts], dtype=torch.int32)
         self.history[:, :longest] = rows.to(dev)
