@@ -136,7 +136,9 @@ def _cache_geometry(cache, kv, hd, device):
 def _tokens(x, width):
     """``x`` ``[..., kv, hd]`` as rows of ``width`` values: ``(x, stride)``; copied only where its
     tokens are not evenly spaced 16-byte aligned rows."""
-    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+    if x.data_ptr() % 16:  # a contiguous tensor is itself its contiguous(): only a copy moves it
+        return x.clone(memory_format=torch.contiguous_format), width
+    if x.is_contiguous():
         return x, width
     per = 16 // x.element_size()
     lead = x.shape[:-2]
@@ -144,7 +146,7 @@ def _tokens(x, width):
     step = x.stride(-3) if lead else width
     for i in range(len(lead) - 1):
         dense = dense and (lead[i] == 1 or x.stride(i) == step * _count(lead[i + 1:]))
-    if not dense or step < width or step % per or x.data_ptr() % 16:
+    if not dense or step < width or step % per:
         return x.contiguous(), width
     return x, step
 
@@ -235,6 +237,8 @@ class TreeAttention:
             counts = _array(counts, "counts", torch.int32, (batch,), device)
         if gate is not None:
             gate = _array(gate, "gate", torch.bfloat16, shape, device)
+            if gate.data_ptr() % 16:
+                gate = gate.clone()
         if out is None:
             out = torch.empty(shape, dtype=torch.bfloat16, device=device) if stride != hq * hd else torch.empty_like(q)
         elif out.dtype != torch.bfloat16 or out.shape != shape or out.device != device or not out.is_contiguous():

@@ -307,3 +307,29 @@ def test_graphs_replayed_beside_one_another(cuda_device):
         torch.cuda.synchronize()
         for got, want in zip([*outs, outside], wants):
             assert all(torch.equal(o, want) for o in got)
+
+
+def test_views_that_begin_off_sixteen_bytes(cuda_device):
+    """Contiguous tokens, queries and gates at an odd address are copied, not refused."""
+    import torch
+
+    from qk_b200.paged import empty_pool, tree_attention, write_slots
+
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+
+    def shifted(x):
+        flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+        view = flat[1:].view(x.shape)
+        assert view.is_contiguous() and view.data_ptr() % 16
+        return view.copy_(x)
+
+    for dtype in (torch.bfloat16, torch.float32):
+        key, value = (torch.randn((7, 2, 64), device=cuda_device, generator=g).to(dtype) for _ in range(2))
+        slots = torch.arange(7, device=cuda_device)
+        one, two = (empty_pool(2, 16, kv_heads=2, head_dim=64, device=cuda_device) for _ in range(2))
+        write_slots(one, key, value, slots)
+        write_slots(two, shifted(key), shifted(value), slots)
+        assert all(torch.equal(one[n], two[n]) for n in one)
+    call = request_batch(g, np.random.default_rng(8), 2, 3, 4, 2, 64, 16, [20, 9], [3, 2])
+    want = tree_attention(**call)
+    assert torch.equal(tree_attention(**dict(call, q=shifted(call["q"]), gate=shifted(call["gate"]))), want)
