@@ -45,10 +45,12 @@ def accept(tokens, parents, ancestors, counts, choices):
     ``[B, N]`` is the token chosen after each node; node 0 is kept, and a node is where its parent is
     and its token is the choice after the parent. ``best`` is the deepest kept node (the first of
     several), ``path`` marks it and its ancestors, ``ranks`` their places on the path, ``kept`` their
-    number. ``parents`` None: a chain."""
+    number. ``parents`` None: a chain; a parent that is not an earlier node counts as -1, as for
+    :func:`~qk_b200.paged.plan_step`, and those of nodes past ``counts`` may be anything."""
     batch, nodes = tokens.shape
     node = torch.arange(nodes, device=tokens.device)
     up = (node - 1).expand(batch, nodes) if parents is None else parents.long()
+    up = torch.where((up >= -1) & (up < node), up, -1)
     match = (tokens == torch.gather(choices, 1, up.clamp(min=0)).to(tokens.dtype)) & (up >= 0)
     match[:, 0] = True
     bits = (match.long() << node).sum(1, keepdim=True)

@@ -68,3 +68,22 @@ def test_lookup_drafts_follow_the_newest_tokens_last_place():
     tokens, parents, counts = lookup_drafts(history, torch.tensor([len(r) for r in rows]), 4)
     assert parents is None and counts.tolist() == [3, 1, 1, 1]
     assert tokens[0, :3].tolist() == [5, 9, 2] and tokens[1:, 0].tolist() == [3, 4, 6]
+
+
+def test_accept_takes_a_parent_that_is_no_earlier_node_as_none():
+    """As the step plan does: nodes past the counts may name anything, a node that names itself or a later one
+    hangs on nothing and is not kept."""
+    import torch
+
+    from qk_b200.speculate import accept
+
+    parents = torch.tensor([[7, 0, 0, 99, -5], [-1, 0, 3, 3, 2 ** 31 - 1]])
+    counts = torch.tensor([3, 4])
+    tokens = torch.tensor([[4, 1, 2, 0, 0], [4, 1, 2, 3, 0]])
+    choices = torch.tensor([[2, 0, 5, 0, 0], [1, 2, 3, 0, 0]])
+    fixed = parents.clone()
+    fixed[0, 0] = fixed[0, 3] = fixed[0, 4] = fixed[1, 2] = fixed[1, 3] = fixed[1, 4] = -1
+    words = torch.from_numpy(words_of(fixed.numpy(), counts.numpy()))
+    best, path, ranks, kept = accept(tokens, parents, words, counts, choices)
+    assert best.tolist() == [2, 1] and kept.tolist() == [2, 2]
+    assert path.tolist() == [[True, False, True, False, False], [True, True, False, False, False]]
