@@ -113,7 +113,8 @@ class SpeculativeGeneration:
 
     def forward(self, tokens, counts, parents=None):
         """``tokens`` ``[B, nodes]`` (the first ``counts[b]`` of each row) behind the cached ones of
-        every sequence, in a tree of ``parents``: ``(hidden [B * nodes, H], plan)``."""
+        every sequence, in a tree of ``parents``: ``(hidden [B * nodes, H], plan)``. Padding may hold any
+        id; a draft outside the vocabulary is embedded as the nearest one in it, and never accepted."""
         m, cfg, lib, P = self.model, self.model.cfg, _lib.load(), _lib.ptr
         rows, H = self.batch * self.nodes, cfg.hidden
         hq, kv, hd = cfg.query_heads, cfg.kv_heads, cfg.head_dim
@@ -121,7 +122,7 @@ class SpeculativeGeneration:
                          page_size=self.page, parents=parents)
         self.held, self.span = plan.held, plan.span
         self.status |= plan.status
-        x = self.embedding.index_select(0, tokens.reshape(-1).long())
+        x = self.embedding.index_select(0, tokens.reshape(-1).long().clamp(0, self.embedding.shape[0] - 1))
         st = _lib.stream_handle(m.device)
         _lib.check(lib.qk_rms_norm(P(x), P(m.layers[0].attn_norm), rows, H, cfg.eps, P(self.h), st))
         for li, L in enumerate(m.layers):
@@ -159,6 +160,8 @@ class SpeculativeGeneration:
         all pages are free again."""
         if len(prompts) != self.batch or any(not 0 < len(p) <= self.context for p in prompts):
             raise ValueError("one prompt of 1 to `context` tokens per sequence")
+        if any(not 0 <= t < self.embedding.shape[0] for p in prompts for t in p):
+            raise ValueError("a prompt's tokens must lie in the vocabulary")
         dev = self.model.device
         self.table, self.held, self.ring, self.span = empty_tables(self.batch, self.table.shape[1], self.ring.shape[0], dev)
         self.cached, self.status = torch.zeros_like(self.cached), torch.zeros_like(self.status)
