@@ -243,6 +243,8 @@ class TreeAttention:
             out = torch.empty(shape, dtype=torch.bfloat16, device=device) if stride != hq * hd else torch.empty_like(q)
         elif out.dtype != torch.bfloat16 or out.shape != shape or out.device != device or not out.is_contiguous():
             raise ValueError("out must be contiguous BF16 of q's shape")
+        elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+            q, stride = q.clone(memory_format=torch.contiguous_format), hq * hd  # read until the last output is written
         ws = self._workspace(device, (batch, nodes, hq, kv, hd))
         _lib.call_on(device, "qk_tree_attention", q.data_ptr(), stride, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
                      vs.data_ptr(), table.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr(),

@@ -417,8 +417,8 @@ int qk_kv_q8_write_slots(const void* key, const void* value, int in_dtype, int64
  * (256 times as large as the first 64 of a stretch, say), is computed in FP32, much more slowly. A node
  * that sees a draft whose key or value has a scale that is not finite or 2^121 and more is NaN, for a
  * value in its group of channels. q BF16
- * [B, N, hq, head_dim] with tokens q_stride values apart (a multiple of 8), gate and out contiguous;
- * hq a multiple of kv_heads, head_dim 64, 128 or 256. The workspace (256-byte aligned) must be
+ * [B, N, hq, head_dim] with tokens q_stride values apart (a multiple of 8), gate and out contiguous, out
+ * apart from q (it may be gate); hq a multiple of kv_heads, head_dim 64, 128 or 256. The workspace (256-byte aligned) must be
  * zeroed before its first call; calls that share one must not overlap. qk_tree_attention_check
  * synchronises `stream`, reports an earlier call's table entry outside the cache or length outside
  * its table (QK_ERR_INVALID_ARGUMENT; the output is then not valid) or a bounded wait that gave up

@@ -333,3 +333,20 @@ def test_views_that_begin_off_sixteen_bytes(cuda_device):
     call = request_batch(g, np.random.default_rng(8), 2, 3, 4, 2, 64, 16, [20, 9], [3, 2])
     want = tree_attention(**call)
     assert torch.equal(tree_attention(**dict(call, q=shifted(call["q"]), gate=shifted(call["gate"]))), want)
+
+
+def test_outputs_over_queries_or_gates(cuda_device):
+    """The output may be the queries' or the gate's own memory, also where it is computed again."""
+    import torch
+
+    from qk_b200.paged import tree_attention
+
+    call = request_batch(torch.Generator(device=cuda_device).manual_seed(9), np.random.default_rng(9), 2, 3, 4, 2, 64, 16,
+                         [200, 9], [3, 2])
+    slot = int(call["table"][0, 6]) * 16 + 2
+    call["cache"]["v_scale"][:, slot] *= 2.0 ** 40
+    want = tree_attention(**call)
+    for name in ("q", "gate"):
+        own = call[name].clone()
+        out = tree_attention(**dict(call, **{name: own}), out=own)
+        assert out is own and torch.equal(out, want)
