@@ -68,11 +68,12 @@ constexpr float kQueryPower = 1.f / 64, kKeyPower = 1.f / 16;
 constexpr uint32_t kValueSpan = 64;  // of the exponents
 constexpr float kOnlyDrafts = 1.f / 64;
 constexpr float kDraftLimit = 512.f;  // a draft's scale by that power: 127 times this is no longer sure to fit
-// Weights go out as 2^(score - m + kWeightRoom), 2^15 at most: FP16 then keeps weights down to 2^-32 of the largest.
-constexpr float kWeightRoom = 7.f;
-// An output whose 16 channels are smaller than this on average (in the values' power) may have lost bits to FP16's
-// range: 2^11 times the error of 2^-18 above.
-constexpr float kSmall = 1.f / 128;
+// Weights go out as 2^(score - m + kWeightRoom), 2^15 at most: FP16 then keeps weights down to 2^-31 of the largest.
+constexpr float kWeightRoom = 7.f, kMostWeight = 32768.f;
+// Values below 2^-9 of their power may have lost bits to FP16's range: their scales lie below 2^-14, where a half
+// step is 2^-10 of them. They show as outputs smaller than that: an average over n tokens of equal weight is
+// smaller by sqrt(n), and n is at least the sum of the weights by the largest that there can be.
+constexpr float kSmall = 1.f / 512;
 constexpr uint32_t kQStage = 2048;  // bytes per softmax warp
 // What a unit costs besides its tiles (Q in, the output out), in tiles of the ranges: 16 requests of 64 nodes over
 // 16384 tokens take 160 us at 2, 145 at 4 and 140 at 6; 32 requests of 8 nodes over 8192 take 53 at 4 and 51 at 6.
@@ -1083,7 +1084,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 2) tree_join_kernel(const __g
   float size = 0.f;
 #pragma unroll
   for (int j = 0; j < kJoinCols; ++j) size += fabsf(o[j]);
-  const bool lost = sees && !(size >= power * (kSmall * kJoinCols) && size < INFINITY);  // also where something is NaN
+  const float least = power * (kSmall * kJoinCols) * rsqrtf(fmaxf(l * (1.f / kMostWeight), 1.f));
+  const bool lost = sees && !(size >= least && size < INFINITY);  // also where something is NaN
   if (node < a.N && !lost) {
     const float inv = sees ? 1.f / l : 0.f;
 #pragma unroll
