@@ -26,12 +26,12 @@
 //
 // Measured with 16 query and 2 KV heads of 256 (join included; the floor is the cache's bytes at the measured
 // HBM rate, from 64 nodes on the products' flop at the measured BF16 rate):
-//   32 requests, 8 nodes, 8192 tokens    51 us, floor 23 (154 MB: 3.0 TB/s)
-//   16 requests, 64 nodes, 16384 tokens 140 us, floor 68 (112 GFLOP: 800 TFLOP/s; 166 us in a loop of seconds,
+//   32 requests, 8 nodes, 8192 tokens    52 us, floor 23 (154 MB: 3.0 TB/s)
+//   16 requests, 64 nodes, 16384 tokens 137 us, floor 68 (112 GFLOP: 820 TFLOP/s; 159 us in a loop of seconds,
 //                                       under the power cap)
-//   1 request, 16 nodes, 32768 tokens    32 us, floor 5.5;  1 request, 1 node, 4096 tokens  20 us, floor 0.7
+//   1 request, 16 nodes, 32768 tokens    29 us, floor 5.5;  1 request, 1 node, 4096 tokens  18 us, floor 0.7
 // What bounds it: at 64 nodes a tile's chain of barriers (copy, decode, S, softmax, P, O; the copies and
-// barriers alone, nothing computed, take 106 of the 140 us) and the decode, which each of a KV head's four
+// barriers alone, nothing computed, took 106 us of 140) and the decode, which each of a KV head's four
 // row tiles repeats; at few rows the fixed 9 to 14 thousand cycles before the first tile (cold
 // instructions, four dependent reads to the first copy) and the 5 thousand of the last output and the join.
 #include <cuda.h>  // CUtensorMap and its enums; the encoder is looked up at run time
@@ -75,8 +75,9 @@ constexpr float kWeightRoom = 7.f, kMostWeight = 32768.f;
 // smaller by sqrt(n), and n is at least the sum of the weights by the largest that there can be.
 constexpr float kSmall = 1.f / 512;
 constexpr uint32_t kQStage = 2048;  // bytes per softmax warp
-// What a unit costs besides its tiles (Q in, the output out), in tiles of the ranges: 16 requests of 64 nodes over
-// 16384 tokens take 160 us at 2, 145 at 4 and 140 at 6; 32 requests of 8 nodes over 8192 take 53 at 4 and 51 at 6.
+// What a unit costs besides its tiles (Q in, the output out), in tiles of the ranges, at 2 / 4 / 6 / 8: 16 requests of
+// 64 nodes over 16384 tokens take 154 / 141 / 137 / 138 us, 32 of 8 nodes over 8192 60 / 54 / 53 / 53, with 32 / 8
+// heads of 64 16 requests of 64 nodes over 8192 116 / 101 / 102 / 105, of 128 with 16 nodes 73 / 63 / 63 / 64.
 constexpr int kUnitCost = 6;
 
 // What calls on the device reported last, besides the word in their workspaces: a workspace can be gone, or belong
@@ -521,7 +522,8 @@ __device__ __forceinline__ bool decode_role(const TreeArgs& a, Control& ctl, uin
       // The raw slot goes back only here, where the stores above have used every code. An arrival right behind
       // the loads does not hold them: the compiler may let them sink below it and the wait for the stage, and
       // where that wait was long (a unit's first tiles) a warp decoded the tile that had come into the slot
-      // meanwhile: a pass of four over 16 trees of 64 nodes. It costs no time: 16384 tokens take 139.5 us.
+      // meanwhile: in a pass of four over 16 trees of 64 nodes. It costs no time (139.5 us, loads that are volatile
+      // instead 143.7).
       if (lane == 0) {
         mbar_arrive(&full[stage]);
         mbar_arrive(&raw_empty[stage]);
