@@ -1,0 +1,242 @@
+// Quantisation of the FP8 dense path: e4m3 codes and FP32 scales of rows (blocks of 128 columns) and of
+// weights (blocks of 128 x 128), and the residual add + RMSNorm whose output leaves as codes.
+//
+//   most = max(max |x| of the block, 2^-100); scale = most / 448; code = e4m3(448 x / most)
+//
+// All are bound by HBM: one pass, a block of a row in 16 lanes of 8 values each.
+#include "fp8.cuh"
+
+namespace qk {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Eight values from `at` of a row whose first `width` exist; the others are zero.
+template <bool F32, bool ALIGNED>
+__device__ __forceinline__ void load8(const void* row, int at, int width, float (&f)[8]) {
+  if (ALIGNED) {
+    if (at >= width) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    } else if (F32) {
+      const uint4 a = ld_guarded_v4(static_cast<const float*>(row) + at);
+      const uint4 b = ld_guarded_v4(static_cast<const float*>(row) + at + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(word(a, j)), f[4 + j] = __uint_as_float(word(b, j));
+    } else {
+      unpack8(ld_guarded_v4(static_cast<const uint16_t*>(row) + at), f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] = 0.f;
+      if (at + j < width) f[j] = F32 ? static_cast<const float*>(row)[at + j] : bf16_to_f32(static_cast<const uint16_t*>(row)[at + j]);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t most8(const float (&f)[8]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = max(most, magnitude(f[j]));
+  return most;
+}
+
+struct RowsArgs {
+  const void* x;
+  int64_t stride, ld;
+  int64_t rows;
+  int width, blocks;
+  uint8_t* codes;
+  float* scales;  // [blocks][rows]
+};
+
+// Half a warp per block of a row. Consecutive warps take consecutive pairs of blocks.
+template <bool F32, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads) fp8_rows_kernel(RowsArgs a) {
+  const int lane = threadIdx.x & 31, pairs = (a.blocks + 1) / 2;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); u < a.rows * pairs; u += warps) {
+    const int64_t row = u / pairs;
+    const int block = static_cast<int>(u - row * pairs) * 2 + (lane >> 4), at = block * kFp8Block + (lane & 15) * 8;
+    const void* from = F32 ? static_cast<const void*>(static_cast<const float*>(a.x) + row * a.stride)
+                           : static_cast<const void*>(static_cast<const uint16_t*>(a.x) + row * a.stride);
+    float f[8];
+    load8<F32, ALIGNED>(from, at, a.width, f);
+    const uint32_t most = block_most(most8(f));
+    const Fp8Divisor by(most);
+    if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(f), by.codes4(f + 4));
+    if (block < a.blocks && (lane & 15) == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = fp8_scale(most);
+  }
+}
+
+// A CTA per block of 128 x 128 weights: 8 rows by half warps, 16 times over.
+template <bool F32, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads) fp8_blocks_kernel(RowsArgs a) {
+  __shared__ uint32_t red[kThreads / 32];
+  const int lane = threadIdx.x & 31, half = threadIdx.x >> 4;
+  const int at = blockIdx.x * kFp8Block + (lane & 15) * 8;
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kTimes = kFp8Block / (kThreads / 16);
+  float f[kTimes][8];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+    const int64_t row = static_cast<int64_t>(blockIdx.y) * kFp8Block + i * (kThreads / 16) + half;
+    const void* from = F32 ? static_cast<const void*>(static_cast<const float*>(a.x) + row * a.stride)
+                           : static_cast<const void*>(static_cast<const uint16_t*>(a.x) + row * a.stride);
+    load8<F32, ALIGNED>(from, at, row < a.rows ? a.width : 0, f[i]);
+    most = max(most, most8(f[i]));
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) red[threadIdx.x >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) most = max(most, red[w]);
+  const Fp8Divisor by(most);
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+    const int64_t row = static_cast<int64_t>(blockIdx.y) * kFp8Block + i * (kThreads / 16) + half;
+    if (row < a.rows && at < a.width)
+      *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(f[i]), by.codes4(f[i] + 4));
+  }
+  if (threadIdx.x == 0) a.scales[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = fp8_scale(most);
+}
+
+struct NormArgs {
+  const uint16_t *x, *y, *gamma;
+  int64_t rows, ld;
+  int width;
+  float eps;
+  uint16_t* sum;
+  uint8_t* codes;
+  float* scales;
+};
+
+// A CTA per row held in registers. With p = s gamma (exact in FP32) the normed row is r p, r = rsqrt(mean s^2 + eps):
+// r moves no code, so the codes leave without waiting for the sum and r goes into the scales.
+__global__ void __launch_bounds__(kRowBlock) fp8_norm_kernel(NormArgs a) {
+  __shared__ float red[kRowBlock / 32];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  float ss = 0.f;
+  uint32_t most[kRowChunks];
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) {
+    const int at = (threadIdx.x + c * kRowBlock) * 8;
+    most[c] = 0;
+    if ((at & ~255) >= a.width) continue;  // the same for the warp
+    float f[8], g[8];
+    load8<false, true>(a.x + row * a.width, at, a.width, f);
+    load8<false, true>(a.gamma, at, a.width, g);
+    if (a.y) {
+      float h[8];
+      load8<false, true>(a.y + row * a.width, at, a.width, h);
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(__fadd_rn(f[2 * j], h[2 * j]), __fadd_rn(f[2 * j + 1], h[2 * j + 1]));
+      const uint4 s = make_uint4(w[0], w[1], w[2], w[3]);
+      if (at < a.width) *reinterpret_cast<uint4*>(a.sum + row * a.width + at) = s;
+      unpack8(s, f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ss = fmaf(f[j], f[j], ss);
+      f[j] *= g[j];
+    }
+    most[c] = block_most(most8(f));
+    const Fp8Divisor by(most[c]);
+    if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(f), by.codes4(f + 4));
+  }
+  const float r = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(ss, red), static_cast<float>(a.width)), a.eps));
+  if ((lane & 15) == 0) {
+#pragma unroll
+    for (int c = 0; c < kRowChunks; ++c) {
+      const int at = (threadIdx.x + c * kRowBlock) * 8;
+      if (at < a.width) a.scales[static_cast<int64_t>(at / kFp8Block) * a.rows + row] = fp8_scale(most[c]) * r;
+    }
+  }
+}
+
+template <typename Kernel>
+int launch(Kernel kernel, dim3 grid, int threads, cudaStream_t st, const RowsArgs& a, const char* name) {
+  cudaError_t e = launch_dependent(kernel, grid, dim3(threads), 0, st, a);
+  if (e != cudaSuccess) return cuda_error(e, name);
+  count_launch();
+  return QK_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace qk
+
+using namespace qk;
+
+extern "C" {
+
+int qk_fp8_quantize(const void* x, int in_dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t* codes, int64_t ld,
+                    float* scales, qk_stream_t stream) {
+  QK_REQUIRE(in_dtype == QK_OUT_F32 || in_dtype == QK_OUT_BF16, "x must be FP32 or BF16");
+  QK_REQUIRE(rows >= 0 && width >= 1 && width < (1ll << 31) - 256 && x_stride >= width, "invalid rows, width or stride");
+  QK_REQUIRE(ld >= (width + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
+  if (rows == 0) return QK_OK;
+  QK_REQUIRE(x && codes && scales, "null pointer");
+  QK_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
+  const int f32 = in_dtype == QK_OUT_F32, size = f32 ? 4 : 2;
+  QK_REQUIRE((reinterpret_cast<uintptr_t>(x) % size) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3) == 0, "misaligned pointer");
+  RowsArgs a{x, x_stride, ld, rows, static_cast<int>(width), static_cast<int>((width + 127) / 128), codes, scales};
+  const bool aligned = aligned16(x) && x_stride * size % 16 == 0 && width % 8 == 0;
+  const int64_t units = rows * ((a.blocks + 1) / 2), most = 8ll * sm_count();
+  const int64_t ctas = (units + 7) / 8;
+  const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most));
+  cudaStream_t st = as_stream(stream);
+  if (f32) return aligned ? launch(fp8_rows_kernel<true, true>, grid, kThreads, st, a, "fp8_rows_kernel")
+                          : launch(fp8_rows_kernel<true, false>, grid, kThreads, st, a, "fp8_rows_kernel");
+  return aligned ? launch(fp8_rows_kernel<false, true>, grid, kThreads, st, a, "fp8_rows_kernel")
+                 : launch(fp8_rows_kernel<false, false>, grid, kThreads, st, a, "fp8_rows_kernel");
+}
+
+int qk_fp8_quantize_blocks(const void* w, int in_dtype, int64_t w_stride, int64_t rows, int64_t width, uint8_t* codes, int64_t ld,
+                           float* scales, qk_stream_t stream) {
+  QK_REQUIRE(in_dtype == QK_OUT_F32 || in_dtype == QK_OUT_BF16, "w must be FP32 or BF16");
+  QK_REQUIRE(rows >= 0 && width >= 1 && width < (1ll << 31) - 256 && w_stride >= width, "invalid rows, width or stride");
+  QK_REQUIRE(ld >= (width + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
+  QK_REQUIRE(rows <= 65535ll * 128, "too many rows");
+  if (rows == 0) return QK_OK;
+  QK_REQUIRE(w && codes && scales, "null pointer");
+  QK_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
+  const int f32 = in_dtype == QK_OUT_F32, size = f32 ? 4 : 2;
+  QK_REQUIRE((reinterpret_cast<uintptr_t>(w) % size) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3) == 0, "misaligned pointer");
+  RowsArgs a{w, w_stride, ld, rows, static_cast<int>(width), static_cast<int>((width + 127) / 128), codes, scales};
+  const bool aligned = aligned16(w) && w_stride * size % 16 == 0 && width % 8 == 0;
+  const dim3 grid(a.blocks, static_cast<unsigned>((rows + 127) / 128));
+  cudaStream_t st = as_stream(stream);
+  if (f32) return aligned ? launch(fp8_blocks_kernel<true, true>, grid, kThreads, st, a, "fp8_blocks_kernel")
+                          : launch(fp8_blocks_kernel<true, false>, grid, kThreads, st, a, "fp8_blocks_kernel");
+  return aligned ? launch(fp8_blocks_kernel<false, true>, grid, kThreads, st, a, "fp8_blocks_kernel")
+                 : launch(fp8_blocks_kernel<false, false>, grid, kThreads, st, a, "fp8_blocks_kernel");
+}
+
+int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma, int64_t rows, int width, float eps, uint16_t* x_out,
+                    uint8_t* codes, int64_t ld, float* scales, qk_stream_t stream) {
+  QK_REQUIRE(rows >= 0 && rows < (1ll << 31) && width >= 8 && width % 8 == 0 && width <= kMaxRowWidth,
+             "width must be a multiple of 8, 8192 at most");
+  QK_REQUIRE(ld >= (width + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
+  if (rows == 0) return QK_OK;
+  QK_REQUIRE(x && gamma && codes && scales && (!y || x_out), "null pointer");
+  QK_REQUIRE(aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(x_out) && aligned16(codes), "pointers must be 16-byte aligned");
+  NormArgs a{x, y, gamma, rows, ld, width, eps, x_out, codes, scales};
+  cudaError_t e = launch_dependent(fp8_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(kRowBlock), 0, as_stream(stream), a);
+  if (e != cudaSuccess) return cuda_error(e, "fp8_norm_kernel");
+  count_launch();
+  return QK_OK;
+}
+
+}  // extern "C"

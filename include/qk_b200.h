@@ -138,6 +138,43 @@ int qk_linear_bf16(const uint16_t* x, int64_t M, int64_t K, const uint16_t* w, i
  * clears the flag. Synchronises `stream`. */
 int qk_linear_bf16_check(const void* workspace, qk_stream_t stream);
 
+/* ---- FP8 dense path ---------------------------------------------------------------
+ * No counterpart in the reference (its dense projections are BF16, math.py:10-16). A matrix is
+ * e4m3 codes, rows `ld` bytes apart (a multiple of 16; the first 16-byte aligned), with one FP32
+ * scale for each block of 128 columns: of a row for activations (scales [ceil(width / 128)][rows]),
+ * of 128 rows for weights (scales [ceil(rows / 128)][ceil(width / 128)]); the last blocks may be
+ * short. A block whose largest magnitude is m = max(max |x|, 2^-100) has scale m / 448 and codes
+ * e4m3(448 x / m), the quotient rounded to nearest, ties to even; one that holds a NaN is NaN,
+ * beside an infinity every value is NaN too (0 times its scale). */
+
+/* x: FP32 or BF16 (in_dtype), rows x_stride values apart. */
+int qk_fp8_quantize(const void* x, int in_dtype, int64_t x_stride, int64_t rows, int64_t width,
+                    uint8_t* codes, int64_t ld, float* scales, qk_stream_t stream);
+int qk_fp8_quantize_blocks(const void* w, int in_dtype, int64_t w_stride, int64_t rows,
+                           int64_t width, uint8_t* codes, int64_t ld, float* scales,
+                           qk_stream_t stream);
+/* qk_residual_rms_norm (y NULL: qk_rms_norm) with its output quantised: x_out = bf16(x + y), then
+ * with p = x_out * gamma and r = rsqrt(mean(x_out^2) + eps), codes e4m3(448 p / m) and scales
+ * r m / 448, m = max(max |p| of the block, 2^-100). The normed row is not rounded to BF16.
+ * Width a multiple of 8, 8192 at most; all arrays 16-byte aligned; x_out may be x. */
+int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma, int64_t rows,
+                    int width, float eps, uint16_t* x_out, uint8_t* codes, int64_t ld, float* scales,
+                    qk_stream_t stream);
+/* out [M, N] (FP32 or BF16 by out_dtype) = x w^T of x [M, K] (activations) and w [N, K] (weights):
+ * the exact products of the codes, FP32 sums, each block's times its two scales. M may be 0. */
+int qk_fp8_matmul(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t M, int64_t K,
+                  const uint8_t* w, int64_t w_ld, const float* w_scales, int64_t N, int out_dtype,
+                  void* out, qk_stream_t stream);
+/* The gated half of a feed-forward block: h = silu(x gate^T) * (x up^T) in FP32, [M, N], quantised
+ * as activations (codes, rows ld bytes apart, and scales) for the product with the down weights. */
+int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t M, int64_t K,
+                 const uint8_t* gate, int64_t gate_ld, const float* gate_scales, const uint8_t* up,
+                 int64_t up_ld, const float* up_scales, int64_t N, uint8_t* codes, int64_t ld,
+                 float* scales, qk_stream_t stream);
+/* QK_ERR_TIMEOUT if a bounded wait of an earlier FP8 product on the current device gave up (its
+ * output is then not valid), else QK_OK; clears the report. Synchronises `stream`. */
+int qk_fp8_check(qk_stream_t stream);
+
 /* ---- router ------------------------------------------------------------------
  * Replaces the router of qwen38_tpu/math.py:277-281 (routes_and_shared):
  * probs = softmax(f32(x) @ f32(Wr)^T); (w, ids) = top_k(probs, k) (ties: lower index);

@@ -1,0 +1,266 @@
+"""FP8 dense path on the GPU against its definition in 64 bits (plain NumPy): e4m3 codes with an FP32
+scale per block of 128, the residual norm that leaves as codes, the products and the gated block.
+
+Tolerances. Codes are compared exactly where the quotient 448 x / m cannot lie near a border without
+being one: x and m have at most 16 significant bits (BF16, or a product of two), so a quotient that is
+no border is at least 2^-21 of its size from the next, and FP32 decides as 64 bits do. Sums of FP32
+products are off by at most one unit of 2^-23 of the terms' magnitudes per addition: 128 within a block
+(the products of codes are exact) and one per block. Outputs are rounded by half a step on top.
+"""
+
+import numpy as np
+import pytest
+
+from util import to_f32
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 128
+LEAST = 2.0 ** -100
+
+
+def blocks(n):
+    return -(-n // BLOCK)
+
+
+def e4m3(x):
+    """The nearest e4m3 values, ties to even."""
+    _, e = np.frexp(x)
+    step = np.ldexp(1.0, np.maximum(e - 1, -6) - 3)
+    return np.round(x / step) * step
+
+
+def row_most(x):
+    full = np.zeros((x.shape[0], blocks(x.shape[1]) * BLOCK))
+    full[:, :x.shape[1]] = np.abs(x)
+    return np.maximum(full.reshape(x.shape[0], -1, BLOCK).max(2), LEAST)
+
+
+def spread(a, width):
+    """A value per block -> one per column."""
+    return np.repeat(a, BLOCK, axis=-1)[..., :width]
+
+
+def quantized(x):
+    most = row_most(x)
+    return e4m3(x * 448 / spread(most, x.shape[1])), most / 448
+
+
+def values(rows):
+    """The 64-bit values of Fp8Rows, and the codes alone."""
+    codes = to_f32(rows.codes).astype(np.float64)
+    return codes * spread(to_f32(rows.scales).astype(np.float64).T, codes.shape[1]), codes
+
+
+def weight_values(w):
+    codes = to_f32(w.codes).astype(np.float64)
+    scales = spread(to_f32(w.scales).astype(np.float64), codes.shape[1])
+    return codes * np.repeat(scales, BLOCK, axis=0)[:codes.shape[0]]
+
+
+def activations(rows, width, device, seed=0, dtype=None):
+    import torch
+
+    g = torch.Generator(device=device).manual_seed(seed)
+    x = torch.randn((rows, width), generator=g, device=device)
+    x *= torch.exp(torch.randn((rows, 1), generator=g, device=device))
+    return x.to(dtype or torch.bfloat16)
+
+
+def packed(n, k, device, seed=1):
+    from qk_b200.fp8 import pack_fp8
+
+    return pack_fp8(activations(n, k, device, seed) * 0.05)
+
+
+def sum_error(x, w):
+    return (BLOCK + blocks(x.shape[1])) * 2.0 ** -23 * (np.abs(x) @ np.abs(w).T)
+
+
+def check_product(got, x, w, half_step):
+    want, room = x @ w.T, sum_error(x, w)
+    off = np.abs(to_f32(got).astype(np.float64) - want)
+    assert np.all(off <= half_step * (np.abs(want) + room) + room + 1e-38), float(np.max(off / (np.abs(want) + room + 1e-38)))
+
+
+# ---- quantisation -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 128), (3, 127), (5, 129), (64, 2048), (37, 4104), (300, 1111), (2, 40000)])
+def test_rows_are_quantised_by_the_rule(cuda_device, rows, width):
+    from qk_b200.fp8 import quantize_fp8
+
+    x = activations(rows, width, cuda_device, rows + width)
+    x[-1, :BLOCK] = 0
+    got = quantize_fp8(x)
+    codes, scales = quantized(to_f32(x).astype(np.float64))
+    assert got.codes.shape == x.shape and got.scales.shape == (blocks(width), rows)
+    assert np.array_equal(to_f32(got.codes), codes.astype(np.float32))
+    assert np.array_equal(to_f32(got.scales), scales.T.astype(np.float32))
+
+
+@pytest.mark.parametrize("rows,width", [(64, 2048), (33, 1111)])
+def test_fp32_rows(cuda_device, rows, width):
+    """24 bits can lie as near to a border as FP32 can tell: there either neighbour will do."""
+    import torch
+
+    from qk_b200.fp8 import quantize_fp8
+
+    x = activations(rows, width, cuda_device, 3, torch.float32)
+    got = quantize_fp8(x)
+    x = to_f32(x).astype(np.float64)
+    quotient = x * 448 / spread(row_most(x), width)
+    codes = to_f32(got.codes)
+    near = np.abs(e4m3(quotient * (1 + 2.0 ** -21)) - e4m3(quotient * (1 - 2.0 ** -21))) > 0
+    assert np.all((codes == e4m3(quotient)) | near) and near.mean() < 1e-3
+    assert np.array_equal(to_f32(got.scales), (row_most(x) / 448).T.astype(np.float32))
+
+
+def test_ties_go_to_even(cuda_device):
+    """A maximum of 448 makes every short value its own quotient: all borders between codes, exactly."""
+    import torch
+
+    from qk_b200.fp8 import quantize_fp8
+
+    bits = np.arange(1, 0x7e, dtype=np.uint8)
+    grid = torch.from_numpy(bits).view(torch.float8_e4m3fn).float().numpy()
+    border = (grid[1:] + grid[:-1]) / 2
+    for most in (448.0, 448.0 * 1.25, 448.0 * 1.625 * 2 ** -20):
+        x = np.zeros((1, 128), np.float32)
+        x[0, :len(border)] = border * (most / 448)
+        x[0, 127] = most
+        want = quantized(x.astype(np.float64))[0].astype(np.float32)
+        xt = torch.from_numpy(x).to(cuda_device)
+        assert np.array_equal(to_f32(quantize_fp8(xt).codes), want)
+        if torch.equal(xt.to(torch.bfloat16).float(), xt):  # 13 / 8 times a border has a bit too many
+            assert np.array_equal(to_f32(quantize_fp8(xt.to(torch.bfloat16)).codes), want)
+        else:
+            assert most < 1
+
+
+def test_strided_and_shifted_rows(cuda_device):
+    import torch
+
+    from qk_b200.fp8 import quantize_fp8
+
+    wide = activations(20, 1000, cuda_device, 5)
+    for view in (wide[:, 8:520], wide[:, 3:700], wide[::3], wide[:, ::2], wide.t(), wide[:0]):
+        got, want = quantize_fp8(view), quantize_fp8(view.clone(memory_format=torch.contiguous_format))
+        assert torch.equal(got.codes.float(), want.codes.float()) and torch.equal(got.scales, want.scales)
+
+
+def test_extreme_blocks(cuda_device):
+    import torch
+
+    from qk_b200.fp8 import quantize_fp8
+
+    x = torch.ones((6, 256), device=cuda_device)
+    x[0, 3] = float("inf")
+    x[1, 5] = float("nan")
+    x[2] = 3e38          # near FP32's end
+    x[3] = 2.0 ** -126   # far below what counts
+    x[4, :128] = 0
+    x[5, 7] = -float("inf")
+    got = quantize_fp8(x)
+    codes, scales = got.codes.float(), got.scales
+    value = codes * scales.t().repeat_interleave(128, 1)
+    assert not torch.isfinite(value[0, :128]).any() and not torch.isfinite(value[5, :128]).any()
+    assert torch.isnan(value[1, :128]).all()
+    assert (codes[2] == 448).all() and torch.isfinite(value[2]).all()
+    assert (value[3] == 0).all() and (value[4, :128] == 0).all()
+    assert (value[[0, 1, 4, 5], 128:] == 1).all()  # their other blocks
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (128, 128), (127, 130), (300, 1111), (9216, 2048)])
+def test_weights_are_quantised_by_blocks(cuda_device, n, k):
+    from qk_b200.fp8 import pack_fp8
+
+    w = activations(n, k, cuda_device, n)
+    got = pack_fp8(w)
+    w = to_f32(w).astype(np.float64)
+    full = np.zeros((blocks(n) * BLOCK, blocks(k) * BLOCK))
+    full[:n, :k] = np.abs(w)
+    most = np.maximum(full.reshape(blocks(n), BLOCK, blocks(k), BLOCK).max((1, 3)), LEAST)
+    by = np.repeat(spread(most, k), BLOCK, axis=0)[:n]
+    assert np.array_equal(to_f32(got.codes), e4m3(w * 448 / by).astype(np.float32))
+    assert np.array_equal(to_f32(got.scales), (most / 448).astype(np.float32))
+
+
+# ---- norm -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,width", [(1, 8), (3, 136), (8, 2048), (5, 8192), (700, 2048), (257, 1000)])
+@pytest.mark.parametrize("add", [False, True])
+def test_norm_leaves_as_codes(cuda_device, rows, width, add):
+    import torch
+
+    from qk_b200.fp8 import rms_norm_fp8
+
+    x = activations(rows, width, cuda_device, 1)
+    y = activations(rows, width, cuda_device, 2) if add else None
+    gamma = (1 + 0.3 * torch.randn(width, device=cuda_device)).to(torch.bfloat16)
+    x[-1] = 0
+    if add:
+        y[-1] = 0
+    got, total = rms_norm_fp8(x, gamma, 1e-5, residual=y)
+    if add:
+        assert torch.equal(total, (x.float() + y.float()).to(torch.bfloat16))
+        x = total
+    else:
+        assert total is None
+    x, gamma = to_f32(x).astype(np.float64), to_f32(gamma).astype(np.float64)
+    codes, scales = quantized(x * gamma)
+    assert np.array_equal(to_f32(got.codes), codes.astype(np.float32))
+    scales = (scales / np.sqrt((x ** 2).mean(1) + 1e-5)[:, None]).T
+    # the sum of squares: at most 45 additions one behind another, the mean, the root, two products
+    assert np.all(np.abs(to_f32(got.scales) - scales) <= 2.0 ** -18 * scales)
+
+
+# ---- products ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 128, 128), (1, 2048, 9216), (3, 100, 7), (8, 4096, 2048), (16, 2048, 300),
+                                   (31, 1111, 1000), (64, 4096, 2048), (65, 640, 520), (128, 16384, 256), (129, 257, 255),
+                                   (200, 384, 136), (333, 1111, 1000), (1000, 2048, 2304)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_matmul(cuda_device, m, k, n, f32):
+    import torch
+
+    from qk_b200.fp8 import check_status, fp8_matmul, quantize_fp8
+
+    x, w = activations(m, k, cuda_device, m), packed(n, k, cuda_device)
+    dtype = torch.float32 if f32 else torch.bfloat16
+    got = fp8_matmul(x, w, output_dtype=dtype)
+    again = fp8_matmul(quantize_fp8(x), w, output_dtype=dtype)
+    check_status(cuda_device)
+    assert torch.equal(got, again) and got.dtype == dtype and got.shape == (m, n)
+    check_product(got, values(quantize_fp8(x))[0], weight_values(w), 2.0 ** -24 if f32 else 2.0 ** -8)
+
+
+@pytest.mark.parametrize("m,k,inner", [(1, 2048, 512), (4, 128, 128), (16, 300, 200), (33, 1111, 100), (64, 2048, 512),
+                                       (100, 512, 1000), (129, 256, 257), (300, 2048, 640)])
+def test_gated(cuda_device, m, k, inner):
+    import torch
+
+    from qk_b200.fp8 import check_status, fp8_matmul, gated_ffn_fp8, gated_fp8, quantize_fp8
+
+    x, gate, up = activations(m, k, cuda_device, m) * 0.5, packed(inner, k, cuda_device, 2), packed(inner, k, cuda_device, 3)
+    down = packed(192, inner, cuda_device, 4)
+    got = gated_fp8(x, gate, up)
+    xv, gv, uv = values(quantize_fp8(x))[0], weight_values(gate), weight_values(up)
+    g, u = xv @ gv.T, xv @ uv.T
+    silu = g / (1 + np.exp(-g))
+    h = silu * u
+    # |silu'| stays below 1.1; exponential and quotient within 2^-16
+    error = 1.1 * np.abs(u) * sum_error(xv, gv) + np.abs(silu) * sum_error(xv, uv) + 2.0 ** -16 * np.abs(h)
+    most = row_most(h)
+    worst = np.array([[error[r, b * BLOCK:(b + 1) * BLOCK].max() for b in range(blocks(inner))] for r in range(m)])
+    assert np.all(np.abs(to_f32(got.scales).T - most / 448) <= (worst + 2.0 ** -22 * most) / 448)
+    value, codes = values(got)
+    _, e = np.frexp(codes)
+    step = np.ldexp(1.0, np.maximum(e - 1, -6) - 3) * spread(to_f32(got.scales).astype(np.float64).T, inner)
+    assert np.all(np.abs(value - h) <= step / 2 * (1 + 2.0 ** -20) + 2 * error)
+    out = gated_ffn_fp8(x, gate, up, down)
+    assert torch.equal(out, fp8_matmul(got, down))
+    check_status(cuda_device)
+    check_product(out, value, weight_values(down), 2.0 ** -8)
