@@ -3,384 +3,145 @@
 //   out[m, n] = sum_b xs[b, m] ws[n / 128, b] sum_{k in block b} xc[m, k] wc[n, k]
 //
 // and the gated pair of them, h = silu(x Wg^T) * (x Wu^T), quantised as the next product reads it.
-//
-// One CTA per SM works through tiles of 128 rows by 256 columns (gated: 128 of the gate and the same 128 of up).
-// A block of 128 columns of K is one row of the 128-byte swizzle and four MMAs (M 128, N 256, K 32); its sum goes to
-// one of two buffers of 256 TMEM columns, and eight warps add it, times the block's two scales, to FP32 sums in
-// their registers (a row and 128 columns per thread) while the tensor core fills the other buffer.
-#include <cuda.h>  // CUtensorMap and its enums; the encoder is looked up at run time
-
-#include "fp8.cuh"
+#include "fp8_narrow.cuh"
+#include "fp8_wide.cuh"
 
 namespace qk {
 namespace {
 
-// What kernels on the device reported last: a bounded wait that gave up.
-__device__ int g_fp8_status;
-
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
-      : "memory");
-}
-
-// Instruction descriptor of kind::f8f6f4: e4m3 A and B, both K-major, FP32 D, M = 128.
-__device__ __forceinline__ uint32_t idesc_e4m3_m128(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
-
-__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
-  return one != 0;
-}
-
-// A bounded wait of a whole warp, converged behind it: false for all lanes if one gave up.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
-}
-
-__device__ __forceinline__ void sts_v4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ uint4 lds_v4_at(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_at(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-
-// ---- wide form ------------------------------------------------------------------------------
-
-constexpr int kTileM = 128, kTileN = 256;
-constexpr int kStages = 4, kBuffers = 2;
-constexpr uint32_t kBytesA = kTileM * kFp8Block, kBytesB = kTileN * kFp8Block, kStageBytes = kBytesA + kBytesB;
-constexpr int kFirstSum = 4, kSumWarps = 8, kThreads = (kFirstSum + kSumWarps) * 32;
-constexpr uint32_t kStaging = 4096;  // bytes per summing warp
-// Registers per thread: 168 at launch for 3 warpgroups (504 in all).
-constexpr int kSumRegs = 216, kOtherRegs = 72;
-static_assert(2 * kSumRegs + kOtherRegs <= 3 * 168, "the shares fit the launch's registers");
-constexpr int kGroupM = 8;  // tiles of rows that run next to one another, so that they share the weights' tiles in L2
-
-struct WideArgs {
-  int64_t M;
-  int N, blocks, n_blocks;  // blocks of K, blocks of N
-  int tiles_m, tiles_n;
-  const float *xs, *ws, *us;  // [blocks][M], [n_blocks][blocks], and of up
-  void* out;                  // [M][N], or codes [M][ld]
-  int64_t ld;
-  float* out_scales;          // [n_blocks][M]
-  bool f32, vectors;          // of out: FP32, and rows that begin on 16 bytes
-};
-
-struct WideControl {
-  uint64_t full[kStages], empty[kStages], sum_full[kBuffers], sum_empty[kBuffers];
-  uint64_t swapped[4];               // a row's two warps have left their maxima
-  uint32_t tmem;
-};
-
-struct Tile {
-  int m, n;
-};
-__device__ __forceinline__ Tile tile_of(const WideArgs& a, int t) {
-  const int band = kGroupM * a.tiles_n, first = t / band * kGroupM, in = t % band;
-  const int high = min(kGroupM, a.tiles_m - first);
-  return Tile{first + in % high, in / high};
-}
-
-template <bool GATED>
-__device__ __forceinline__ bool wide_copies(const WideArgs& a, WideControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
-                                            const CUtensorMap* u, uint32_t smem) {
-  uint32_t it = 0;
-  bool ok = true;
-  for (int t = blockIdx.x; ok && t < a.tiles_m * a.tiles_n; t += gridDim.x) {
-    const Tile tile = tile_of(a, t);
-    for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t s = it % kStages, at = smem + s * kStageBytes;
-      ok = mbar_wait_bounded(&ctl.empty[s], (it / kStages & 1) ^ 1);
-      if (!ok) break;
-      mbar_expect_tx(&ctl.full[s], kStageBytes);
-      load_box(at, x, b * kFp8Block, tile.m * kTileM, &ctl.full[s]);
-      if (GATED) {
-        load_box(at + kBytesA, w, b * kFp8Block, tile.n * kFp8Block, &ctl.full[s]);
-        load_box(at + kBytesA + kBytesB / 2, u, b * kFp8Block, tile.n * kFp8Block, &ctl.full[s]);
-      } else {
-        load_box(at + kBytesA, w, b * kFp8Block, tile.n * kTileN, &ctl.full[s]);
-      }
-    }
-  }
-  // every copy issued must have landed before the CTA leaves
-  for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait_bounded(&ctl.full[i % kStages], i / kStages & 1);
-  return ok;
-}
-
-__device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ctl, uint32_t smem) {
-  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = idesc_e4m3_m128(kTileN);
-  uint32_t it = 0;
-  for (int t = blockIdx.x; t < a.tiles_m * a.tiles_n; t += gridDim.x) {
-    for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t s = it % kStages, d = it % kBuffers;
-      if (!warp_wait(&ctl.full[s], it / kStages & 1)) return false;
-      if (!warp_wait(&ctl.sum_empty[d], (it / kBuffers & 1) ^ 1)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t ad = sdesc_sw128(smem + s * kStageBytes, 1024u), bd = sdesc_sw128(smem + s * kStageBytes + kBytesA, 1024u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_e4m3(tm + d * kTileN, ad + 2 * k, bd + 2 * k, idesc, k != 0);
-        umma_commit(&ctl.empty[s]);
-        umma_commit(&ctl.sum_full[d]);
-      }
-      __syncwarp();
-    }
-  }
-  return true;
-}
-
-// One block's sums, `count` columns from `col`, times `scale`, added to `acc`.
-template <int COUNT>
-__device__ __forceinline__ void add_block(uint32_t col, float scale, uint64_t* acc) {
-  const uint64_t by = f32x2(scale, scale);
-#pragma unroll
-  for (int c = 0; c < COUNT; c += 32) {
-    uint32_t v[32];
-    tmem_ld32(col + c, v);
-    tmem_wait_ld(v);
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      acc[c / 2 + j] = f32x2_fma(f32x2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), by, acc[c / 2 + j]);
-  }
-}
-
-// 32 rows (a lane each) of 128 columns out, through 4 KB of shared memory, in pieces of 128 bytes a row.
-template <bool F32>
-__device__ __forceinline__ void wide_store(const WideArgs& a, const uint64_t (&acc)[64], uint32_t staging, int64_t row0, int col0) {
-  constexpr int kSize = F32 ? 4 : 2, kColumns = 128 / kSize;
-  const int lane = threadIdx.x & 31;
-  const int rows = static_cast<int>(min(a.M - row0, static_cast<int64_t>(32)));
-#pragma unroll
-  for (int c = 0; c < 128; c += kColumns) {
-    if (col0 + c >= a.N) break;
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x, y;
-        if (F32) {
-          f32x2_split(acc[c / 2 + j * 2 + i / 2], x, y);
-          w[i] = __float_as_uint(i & 1 ? y : x);
-        } else {
-          f32x2_split(acc[c / 2 + j * 4 + i], x, y);
-          w[i] = pack_bf16x2(x, y);
-        }
-      }
-      sts_v4(staging + lane * 128 + ((j ^ lane) & 7) * 16, w[0], w[1], w[2], w[3]);
-    }
-    __syncwarp();
-    uint8_t* out = static_cast<uint8_t*>(a.out) + (row0 * a.N + col0 + c) * kSize;
-    if (a.vectors && col0 + c + kColumns <= a.N) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + lane / 8;
-        if (r < rows)
-          *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * a.N * kSize + (lane & 7) * 16) =
-              lds_v4_at(staging + r * 128 + ((lane ^ r) & 7) * 16);
-      }
-    } else {
-      for (int r = 0; r < rows; ++r) {
-        const uint32_t v = lds_at(staging + r * 128 + ((lane / 4 ^ r) & 7) * 16 + (lane & 3) * 4);
-        uint8_t* at = out + static_cast<int64_t>(r) * a.N * kSize + lane * 4;
-        if (F32) {
-          if (col0 + c + lane < a.N) *reinterpret_cast<uint32_t*>(at) = v;
-        } else {
-          if (col0 + c + 2 * lane < a.N) *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(v);
-          if (col0 + c + 2 * lane + 1 < a.N) *reinterpret_cast<uint16_t*>(at + 2) = static_cast<uint16_t>(v >> 16);
-        }
-      }
-    }
-  }
-}
-
-// silu(g) u
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
-
-template <bool GATED>
-__device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, uint32_t staging) {
-  const int warp = (threadIdx.x >> 5) - kFirstSum, quarter = warp & 3, half = warp >> 2, lane = threadIdx.x & 31;
-  const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  uint32_t it = 0, swaps = 0;
-  for (int t = blockIdx.x; t < a.tiles_m * a.tiles_n; t += gridDim.x) {
-    const Tile tile = tile_of(a, t);
-    const int64_t row0 = static_cast<int64_t>(tile.m) * kTileM + quarter * 32, row = row0 + lane;
-    // a thread's columns: 128 of the tile's 256, or 64 of the gate's and the same of up's
-    const int n_block = GATED ? tile.n : min(tile.n * 2 + half, a.n_blocks - 1);
-    const float* ws = a.ws + static_cast<int64_t>(n_block) * a.blocks;
-    const float* us = GATED ? a.us + static_cast<int64_t>(n_block) * a.blocks : nullptr;
-    const float* xs = a.xs + min(row, a.M - 1);
-    uint64_t acc[64];
-#pragma unroll
-    for (int j = 0; j < 64; ++j) acc[j] = 0;
-    float x = xs[0], w = ws[0], u = GATED ? us[0] : 0.f;
-    for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t d = it % kBuffers, cols = tm + d * kTileN;
-      const float by_w = x * w, by_u = x * u;
-      if (b + 1 < a.blocks) {
-        x = xs[(b + 1) * a.M];
-        w = ws[b + 1];
-        if (GATED) u = us[b + 1];
-      }
-      if (!warp_wait(&ctl.sum_full[d], it / kBuffers & 1)) return false;
-      tc_fence_after();
-      if (GATED) {
-        add_block<64>(cols + half * 64, by_w, acc);
-        add_block<64>(cols + 128 + half * 64, by_u, acc + 32);
-      } else {
-        add_block<128>(cols + half * 128, by_w, acc);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.sum_empty[d]);
-    }
-    if (!GATED) {
-      if (a.f32) wide_store<true>(a, acc, staging + warp * kStaging, row0, tile.n * kTileN + half * 128);
-      else wide_store<false>(a, acc, staging + warp * kStaging, row0, tile.n * kTileN + half * 128);
-      continue;
-    }
-    // A thread has half of its row's block of 128: two threads swap their maxima. No rounding before the codes'.
-    float h[64];
-    uint32_t most = 0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      float g0, g1, u0, u1;
-      f32x2_split(acc[j], g0, g1);
-      f32x2_split(acc[32 + j], u0, u1);
-      h[2 * j] = gated(g0, u0);
-      h[2 * j + 1] = gated(g1, u1);
-      most = max(most, max(magnitude(h[2 * j]), magnitude(h[2 * j + 1])));
-    }
-    const uint32_t swap = staging + (swaps & 1) * 1024 + quarter * 128 + lane * 4;
-    asm volatile("st.shared.u32 [%0], %1;" ::"r"(swap + half * 512), "r"(most) : "memory");
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.swapped[quarter]);
-    if (!warp_wait(&ctl.swapped[quarter], swaps & 1)) return false;
-    most = max(most, lds_at(swap + (half ^ 1) * 512));
-    ++swaps;
-    if (row < a.M) {
-      const Fp8Divisor by(most);
-      const int col = tile.n * kFp8Block + half * 64;
-      uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.ld + col;
-#pragma unroll
-      for (int j = 0; j < 64; j += 16)
-        if (col + j < a.N)
-          *reinterpret_cast<uint4*>(out + j) =
-              make_uint4(by.codes4(h + j), by.codes4(h + j + 4), by.codes4(h + j + 8), by.codes4(h + j + 12));
-      if (half == 0) a.out_scales[static_cast<int64_t>(tile.n) * a.M + row] = fp8_scale(most);
-    }
-  }
-  return true;
-}
-
-template <bool GATED>
-__global__ void __launch_bounds__(kThreads, 1)
-    fp8_wide_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap w, const __grid_constant__ CUtensorMap u,
-                    WideArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ WideControl ctl;
-  const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
-  const int warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&ctl.full[i], 1);
-      mbar_init(&ctl.empty[i], 1);
-    }
-    for (int i = 0; i < kBuffers; ++i) {
-      mbar_init(&ctl.sum_full[i], 1);
-      mbar_init(&ctl.sum_empty[i], kSumWarps);
-    }
-    for (int i = 0; i < 4; ++i) mbar_init(&ctl.swapped[i], 2);
-    fence_mbar_init();
-  }
-  if (warp == 1) tmem_alloc(&ctl.tmem, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  pdl_wait();
-  pdl_trigger();
-  bool ok = true;
-  if (warp >= kFirstSum) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
-    ok = wide_sums<GATED>(a, ctl, smem + kStages * kStageBytes);
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 0) {
-      if (threadIdx.x == 0) ok = wide_copies<GATED>(a, ctl, &x, &w, &u, smem);
-    } else if (warp == 1) {
-      ok = wide_products(a, ctl, smem);
-    }
-  }
-  if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(ctl.tmem, 512);
-  }
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// Codes [rows][width], rows `ld` bytes apart, in boxes of `box_rows` x 128 with the 128-byte swizzle; zero past the ends.
-bool encode(CUtensorMap* map, const void* codes, int64_t rows, int64_t width, int64_t ld, uint32_t box_rows) {
-  EncodeTiledFn fn = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
-  const cuuint32_t box[2] = {kFp8Block, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <bool GATED>
-int launch_wide(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const WideArgs& a, cudaStream_t st) {
-  const size_t smem = 1024 + kStages * kStageBytes + kSumWarps * kStaging;
-  const int rc = allow_smem(reinterpret_cast<const void*>(fp8_wide_kernel<GATED>), smem);
-  if (rc) return rc;
-  const int tiles = a.tiles_m * a.tiles_n;
-  cudaError_t e = launch_dependent(fp8_wide_kernel<GATED>, dim3(tiles < sm_count() ? tiles : sm_count()), dim3(kThreads), smem, st,
-                                   x, w, u, a);
-  if (e != cudaSuccess) return cuda_error(e, "fp8_wide_kernel");
-  count_launch();
+int check_weights(int64_t M, int64_t K, const uint8_t* w, int64_t w_ld, const float* ws, int64_t N, const void* out) {
+  QK_REQUIRE(M >= 0 && N >= 1 && K >= 1, "invalid rows, columns or width");
+  QK_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K < (1ll << 31) - 256, "sizes must stay below 2^31 - 256");
+  QK_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) < (1ll << 28), "too many tiles in one call");
+  QK_REQUIRE(w_ld >= K && w_ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart");
+  if (M == 0) return QK_OK;
+  QK_REQUIRE(w && ws && out, "null pointer");
+  QK_REQUIRE(aligned16(w) && (reinterpret_cast<uintptr_t>(ws) & 3) == 0, "codes must be 16-byte aligned, scales 4-byte");
   return QK_OK;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// The conditions that both products have in common.
 int check_operands(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t K, const uint8_t* w, int64_t w_ld, const float* ws,
                    int64_t N, const void* out) {
-  QK_REQUIRE(M >= 0 && N >= 1 && K >= 1, "invalid rows, columns or width");
-  QK_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K < (1ll << 31) - 256, "sizes must stay below 2^31 - 256");
-  QK_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) < (1ll << 31), "too many tiles in one call");
-  QK_REQUIRE(x_ld >= K && x_ld % 16 == 0 && w_ld >= K && w_ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart");
-  if (M == 0) return QK_OK;
-  QK_REQUIRE(x && xs && w && ws && out, "null pointer");
-  QK_REQUIRE(aligned16(x) && aligned16(w), "codes must be 16-byte aligned");
-  QK_REQUIRE(((reinterpret_cast<uintptr_t>(xs) | reinterpret_cast<uintptr_t>(ws)) & 3) == 0, "scales must be 4-byte aligned");
+  const int rc = check_weights(M, K, w, w_ld, ws, N, out);
+  if (rc || M == 0) return rc;
+  QK_REQUIRE(x_ld >= K && x_ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart");
+  QK_REQUIRE(x && xs, "null pointer");
+  QK_REQUIRE(aligned16(x) && (reinterpret_cast<uintptr_t>(xs) & 3) == 0, "codes must be 16-byte aligned, scales 4-byte");
+  return QK_OK;
+}
+
+int check_rows(const void* x, int in_dtype, int64_t stride, int64_t M, int64_t K) {
+  QK_REQUIRE(in_dtype == QK_OUT_F32 || in_dtype == QK_OUT_BF16, "x must be FP32 or BF16");
+  QK_REQUIRE(M >= 0 && K >= 1 && stride >= K, "invalid rows, width or stride");
+  QK_REQUIRE(M == 0 || (x && reinterpret_cast<uintptr_t>(x) % (in_dtype == QK_OUT_F32 ? 4 : 2) == 0), "misaligned or null x");
+  return QK_OK;
+}
+
+// Rows of x from which the wide form is used.
+constexpr int64_t kMostNarrow = 128;
+
+bool narrow(int64_t M) { return M <= kMostNarrow; }
+
+// Half of a feed-forward block (u not NULL, codes out) or a product (u NULL) of codes.
+struct Weights {
+  const uint8_t* codes;
+  int64_t ld;
+  const float* scales;
+};
+
+int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t K, const Weights& w, const Weights* u, int64_t N, bool f32,
+            void* out, int64_t ld, float* out_scales, cudaStream_t st) {
+  const int blocks = static_cast<int>((K + 127) / 128), n_blocks = static_cast<int>((N + 127) / 128);
+  const bool vectors = !u && aligned16(out) && N * (f32 ? 4 : 2) % 16 == 0;
+  CUtensorMap xm, wm, um;
+  bool ok;
+  if (narrow(M)) {
+    const NarrowPlan plan(M, N, blocks);
+    ok = encode(&xm, x, M, K, x_ld, plan.tokens) && encode(&wm, w.codes, N, K, w.ld, 128) && (!u || encode(&um, u->codes, N, K, u->ld, 128));
+    if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
+    NarrowArgs a{};
+    a.M = M;
+    a.N = static_cast<int>(N);
+    a.blocks = blocks;
+    a.xs = xs;
+    a.ws = w.scales;
+    a.us = u ? u->scales : nullptr;
+    a.out = out;
+    a.ld = ld;
+    a.out_scales = out_scales;
+    a.f32 = f32;
+    a.vectors = vectors;
+    return u ? launch_narrow<true>(false, xm, wm, um, a, plan, st) : launch_narrow<false>(false, xm, wm, wm, a, plan, st);
+  }
+  ok = encode(&xm, x, M, K, x_ld, kTileM) && encode(&wm, w.codes, N, K, w.ld, u ? kFp8Block : kTileN) &&
+       (!u || encode(&um, u->codes, N, K, u->ld, kFp8Block));
+  if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
+  WideArgs a{};
+  a.M = M;
+  a.N = static_cast<int>(N);
+  a.blocks = blocks;
+  a.n_blocks = n_blocks;
+  a.tiles_m = static_cast<int>((M + kTileM - 1) / kTileM);
+  a.tiles_n = u ? n_blocks : static_cast<int>((N + kTileN - 1) / kTileN);
+  a.xs = xs;
+  a.ws = w.scales;
+  a.us = u ? u->scales : nullptr;
+  a.out = out;
+  a.ld = ld;
+  a.out_scales = out_scales;
+  a.f32 = f32;
+  a.vectors = vectors;
+  return u ? launch_wide<true>(xm, wm, um, a, st) : launch_wide<false>(xm, wm, wm, a, st);
+}
+
+// The same from rows of BF16 or FP32, which a narrow product of BF16 quantises itself where it can; else into `room`
+// (row_bytes of it).
+size_t row_bytes(int64_t M, int64_t K) {
+  const size_t codes = static_cast<size_t>(M) * ((K + 15) / 16 * 16), scales = static_cast<size_t>(M) * ((K + 127) / 128) * 4;
+  return (codes + 255) / 256 * 256 + (scales + 255) / 256 * 256;
+}
+
+// Whether a product of BF16 rows quantises them itself: by the sizes alone, so that the workspace's size is.
+bool quantises(int in_dtype, int64_t M, int64_t K, int64_t N) {
+  const int blocks = static_cast<int>((K + 127) / 128);
+  return in_dtype == QK_OUT_BF16 && K % 8 == 0 && NarrowPlan(M, N, blocks).quantises(M, blocks);
+}
+size_t room_for(int in_dtype, int64_t M, int64_t K, int64_t N) { return quantises(in_dtype, M, K, N) ? 0 : row_bytes(M, K); }
+
+int product_of_rows(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const Weights& w, const Weights* u, int64_t N,
+                    bool f32, void* out, int64_t ld, float* out_scales, uint8_t* room, cudaStream_t st) {
+  if (quantises(in_dtype, M, K, N)) {
+    QK_REQUIRE(aligned16(x) && x_stride % 8 == 0, "few rows of x must begin on 16 bytes");
+    const int blocks = static_cast<int>((K + 127) / 128);
+    const NarrowPlan plan(M, N, blocks);
+    CUtensorMap wm, um;
+    if (!encode(&wm, w.codes, N, K, w.ld, 128) || (u && !encode(&um, u->codes, N, K, u->ld, 128)))
+      return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
+    NarrowArgs a{};
+    a.M = M;
+    a.N = static_cast<int>(N);
+    a.blocks = blocks;
+    a.x = static_cast<const uint16_t*>(x);
+    a.x_stride = x_stride;
+    a.width = static_cast<int>(K);
+    a.ws = w.scales;
+    a.us = u ? u->scales : nullptr;
+    a.out = out;
+    a.ld = ld;
+    a.out_scales = out_scales;
+    a.f32 = f32;
+    a.vectors = !u && aligned16(out) && N * (f32 ? 4 : 2) % 16 == 0;
+    return u ? launch_narrow<true>(true, wm, wm, um, a, plan, st) : launch_narrow<false>(true, wm, wm, wm, a, plan, st);
+  }
+  const int64_t x_ld = (K + 15) / 16 * 16;
+  float* scales = reinterpret_cast<float*>(room + (static_cast<size_t>(M) * x_ld + 255) / 256 * 256);
+  const int rc = qk_fp8_quantize(x, in_dtype, x_stride, M, K, room, x_ld, scales, st);
+  return rc ? rc : product(room, x_ld, scales, M, K, w, u, N, f32, out, ld, out_scales, st);
+}
+
+int check_room(const void* room, size_t bytes, size_t need) {
+  if (need && (!room || bytes < need)) return set_error(QK_ERR_WORKSPACE, "the FP8 product needs a workspace of %zu bytes, got %zu", need, bytes);
+  QK_REQUIRE((reinterpret_cast<uintptr_t>(room) & 255) == 0, "workspace must be 256-byte aligned");
   return QK_OK;
 }
 
@@ -396,24 +157,9 @@ int qk_fp8_matmul(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t
   QK_REQUIRE(out_dtype == QK_OUT_F32 || out_dtype == QK_OUT_BF16, "out must be FP32 or BF16");
   const int rc = check_operands(x, x_ld, x_scales, M, K, w, w_ld, w_scales, N, out);
   if (rc || M == 0) return rc;
-  const int size = out_dtype == QK_OUT_F32 ? 4 : 2;
-  QK_REQUIRE(reinterpret_cast<uintptr_t>(out) % size == 0, "misaligned out");
-  WideArgs a{};
-  a.M = M;
-  a.N = static_cast<int>(N);
-  a.blocks = static_cast<int>((K + 127) / 128);
-  a.n_blocks = static_cast<int>((N + 127) / 128);
-  a.tiles_m = static_cast<int>((M + kTileM - 1) / kTileM);
-  a.tiles_n = static_cast<int>((N + kTileN - 1) / kTileN);
-  a.xs = x_scales;
-  a.ws = w_scales;
-  a.out = out;
-  a.f32 = out_dtype == QK_OUT_F32;
-  a.vectors = aligned16(out) && N * size % 16 == 0;
-  CUtensorMap xm, wm;
-  if (!encode(&xm, x, M, K, x_ld, kTileM) || !encode(&wm, w, N, K, w_ld, kTileN))
-    return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
-  return launch_wide<false>(xm, wm, wm, a, as_stream(stream));
+  QK_REQUIRE(reinterpret_cast<uintptr_t>(out) % (out_dtype == QK_OUT_F32 ? 4 : 2) == 0, "misaligned out");
+  return product(x, x_ld, x_scales, M, K, Weights{w, w_ld, w_scales}, nullptr, N, out_dtype == QK_OUT_F32, out, 0, nullptr,
+                 as_stream(stream));
 }
 
 int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t M, int64_t K, const uint8_t* gate, int64_t gate_ld,
@@ -424,23 +170,53 @@ int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t 
   if (rc || M == 0) return rc;
   QK_REQUIRE(ld >= (N + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
   QK_REQUIRE(aligned16(codes) && scales && (reinterpret_cast<uintptr_t>(scales) & 3) == 0, "misaligned or null output");
-  WideArgs a{};
-  a.M = M;
-  a.N = static_cast<int>(N);
-  a.blocks = static_cast<int>((K + 127) / 128);
-  a.n_blocks = static_cast<int>((N + 127) / 128);
-  a.tiles_m = static_cast<int>((M + kTileM - 1) / kTileM);
-  a.tiles_n = a.n_blocks;
-  a.xs = x_scales;
-  a.ws = gate_scales;
-  a.us = up_scales;
-  a.out = codes;
-  a.ld = ld;
-  a.out_scales = scales;
-  CUtensorMap xm, gm, um;
-  if (!encode(&xm, x, M, K, x_ld, kTileM) || !encode(&gm, gate, N, K, gate_ld, kFp8Block) || !encode(&um, up, N, K, up_ld, kFp8Block))
-    return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
-  return launch_wide<true>(xm, gm, um, a, as_stream(stream));
+  const Weights u{up, up_ld, up_scales};
+  return product(x, x_ld, x_scales, M, K, Weights{gate, gate_ld, gate_scales}, &u, N, false, codes, ld, scales, as_stream(stream));
+}
+
+size_t qk_fp8_linear_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t N) {
+  return M > 0 && K > 0 && N > 0 ? room_for(in_dtype, M, K, N) : 0;
+}
+
+int qk_fp8_linear(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const uint8_t* w, int64_t w_ld,
+                  const float* w_scales, int64_t N, int out_dtype, void* out, void* workspace, size_t workspace_bytes,
+                  qk_stream_t stream) {
+  QK_REQUIRE(out_dtype == QK_OUT_F32 || out_dtype == QK_OUT_BF16, "out must be FP32 or BF16");
+  int rc = check_rows(x, in_dtype, x_stride, M, K);
+  if (!rc) rc = check_weights(M, K, w, w_ld, w_scales, N, out);
+  if (rc || M == 0) return rc;
+  QK_REQUIRE(reinterpret_cast<uintptr_t>(out) % (out_dtype == QK_OUT_F32 ? 4 : 2) == 0, "misaligned out");
+  rc = check_room(workspace, workspace_bytes, room_for(in_dtype, M, K, N));
+  if (rc) return rc;
+  return product_of_rows(x, in_dtype, x_stride, M, K, Weights{w, w_ld, w_scales}, nullptr, N, out_dtype == QK_OUT_F32, out, 0, nullptr,
+                         static_cast<uint8_t*>(workspace), as_stream(stream));
+}
+
+size_t qk_fp8_ffn_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t inner) {
+  return M > 0 && K > 0 && inner > 0 ? room_for(in_dtype, M, K, inner) + row_bytes(M, inner) : 0;
+}
+
+int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const uint8_t* gate, int64_t gate_ld,
+               const float* gate_scales, const uint8_t* up, int64_t up_ld, const float* up_scales, int64_t inner, const uint8_t* down,
+               int64_t down_ld, const float* down_scales, int64_t N, uint16_t* out, void* workspace, size_t workspace_bytes,
+               qk_stream_t stream) {
+  int rc = check_rows(x, in_dtype, x_stride, M, K);
+  if (!rc) rc = check_weights(M, K, gate, gate_ld, gate_scales, inner, out);
+  if (!rc) rc = check_weights(M, K, up, up_ld, up_scales, inner, out);
+  if (!rc) rc = check_weights(M, inner, down, down_ld, down_scales, N, out);
+  if (rc || M == 0) return rc;
+  QK_REQUIRE((reinterpret_cast<uintptr_t>(out) & 1) == 0, "misaligned out");
+  rc = check_room(workspace, workspace_bytes, room_for(in_dtype, M, K, inner) + row_bytes(M, inner));
+  if (rc) return rc;
+  cudaStream_t st = as_stream(stream);
+  uint8_t* h = static_cast<uint8_t*>(workspace) + room_for(in_dtype, M, K, inner);
+  const int64_t ld = (inner + 15) / 16 * 16;
+  float* h_scales = reinterpret_cast<float*>(h + (static_cast<size_t>(M) * ld + 255) / 256 * 256);
+  const Weights u{up, up_ld, up_scales};
+  rc = product_of_rows(x, in_dtype, x_stride, M, K, Weights{gate, gate_ld, gate_scales}, &u, inner, false, h, ld, h_scales,
+                       static_cast<uint8_t*>(workspace), st);
+  if (rc) return rc;
+  return product(h, ld, h_scales, M, inner, Weights{down, down_ld, down_scales}, nullptr, N, false, out, 0, nullptr, st);
 }
 
 int qk_fp8_check(qk_stream_t stream) {

@@ -1,0 +1,397 @@
+// The narrow FP8 product, for few rows of x (tokens): bound by reading the weights once.
+//
+// The weights are the M = 128 operand and MT tokens the N operand, so a tile of 128 columns of the output is 128 rows
+// of the weights. Its blocks of K are split over a cluster of CTAs, which all stream their part of the weights at
+// once; each adds its blocks' sums, times their scales, in registers (a thread per weight row and half of the
+// tokens), leaves them in shared memory, and the CTAs add up one another's in rank order and write.
+// x comes as codes, by tensor copies beside the weights', or (ROWS: up to 16 rows) as BF16 that every CTA quantises
+// for itself while its weights are on their way: that saves a launch, and the values are the same.
+#pragma once
+
+#include "fp8_product.cuh"
+
+namespace qk {
+namespace {
+
+constexpr int kNarrowStages = 5, kNarrowSumWarps = 8, kNarrowFirstSum = 2;
+constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
+constexpr int kMostSplits = 8;       // the portable cluster size
+constexpr int kInlineRows = 16;      // rows of BF16 that the CTAs quantise themselves
+constexpr int kInlineBlocks = 16;    // and blocks of K per CTA
+
+struct NarrowArgs {
+  int64_t M;
+  int N, blocks, splits, stages;
+  const uint16_t* x;      // BF16 (ROWS), width a multiple of 8
+  int64_t x_stride;
+  int width;
+  const float *xs, *ws, *us;
+  void* out;
+  int64_t ld;             // of the gated codes
+  float* out_scales;
+  bool f32, vectors;
+};
+
+template <int MT, bool GATED>
+struct Narrow {
+  static constexpr int kOperands = GATED ? 2 : 1;
+  static constexpr uint32_t kBytesW = kOperands * 128 * kFp8Block, kBytesX = MT * kFp8Block, kStage = kBytesW + kBytesX;
+  static constexpr int kColumns = kOperands * MT;                           // TMEM columns of a block's sums
+  static constexpr int kBuffers = 256 / kColumns < 2 ? 2 : 256 / kColumns > 8 ? 8 : 256 / kColumns;
+  static constexpr uint32_t kAlloc = kColumns * kBuffers < 32 ? 32 : kColumns * kBuffers;
+  static constexpr uint32_t kPartial = kOperands * MT * 128 * 4;            // a CTA's sums
+  static constexpr int kEach = MT / 2;                                      // tokens per thread
+  static size_t smem(int stages, int inline_blocks) {
+    const size_t ring = stages * (inline_blocks ? kBytesW : kStage) + inline_blocks * kBytesX;
+    return 1024 + (ring > kPartial ? ring : kPartial);
+  }
+};
+
+struct NarrowControl {
+  uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], x_full;
+  uint32_t tmem;
+  alignas(16) float scales[kInlineBlocks * kInlineRows > kNarrowSumWarps * 2 * 64 ? kInlineBlocks * kInlineRows : kNarrowSumWarps * 2 * 64];
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Four floats of the shared memory of the cluster's CTA `rank`, at this CTA's address `addr`.
+__device__ __forceinline__ float4 cluster_ld4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [a];\n}\n"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+template <int MT, bool GATED, bool ROWS>
+__device__ __forceinline__ bool narrow_copies(const NarrowArgs& a, NarrowControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
+                                              const CUtensorMap* u, uint32_t smem, int b0, int b1, int tile, int row0) {
+  using L = Narrow<MT, GATED>;
+  constexpr uint32_t kStage = ROWS ? L::kBytesW : L::kStage;
+  bool ok = true;
+  int it = 0;
+  for (int b = b0; b < b1; ++b, ++it) {
+    const int s = it % a.stages;
+    const uint32_t at = smem + s * kStage;
+    ok = mbar_wait_bounded(&ctl.empty[s], (it / a.stages & 1) ^ 1);
+    if (!ok) break;
+    mbar_expect_tx(&ctl.full[s], kStage);
+    load_box(at, w, b * kFp8Block, tile * 128, &ctl.full[s]);
+    if (GATED) load_box(at + L::kBytesW / 2, u, b * kFp8Block, tile * 128, &ctl.full[s]);
+    if (!ROWS) load_box(at + L::kBytesW, x, b * kFp8Block, row0, &ctl.full[s]);
+  }
+  // every copy issued must have landed before the CTA leaves
+  for (int i = max(it - a.stages, 0); i < it; ++i) mbar_wait_bounded(&ctl.full[i % a.stages], i / a.stages & 1);
+  return ok;
+}
+
+template <int MT, bool GATED, bool ROWS>
+__device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int count) {
+  using L = Narrow<MT, GATED>;
+  constexpr uint32_t kStage = ROWS ? L::kBytesW : L::kStage;
+  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = idesc_e4m3_m128(MT);
+  if (ROWS && !warp_wait(&ctl.x_full, 0)) return false;
+  for (int it = 0; it < count; ++it) {
+    const int s = it % a.stages, d = it % L::kBuffers;
+    if (!warp_wait(&ctl.full[s], it / a.stages & 1)) return false;
+    if (!warp_wait(&ctl.sum_empty[d], (it / L::kBuffers & 1) ^ 1)) return false;
+    tc_fence_after();
+    if (elect_one()) {
+      const uint32_t at = smem + s * kStage;
+      const uint64_t wd = sdesc_sw128(at, 1024u);
+      const uint64_t xd = sdesc_sw128(ROWS ? smem + a.stages * kStage + it * L::kBytesX : at + L::kBytesW, 1024u);
+#pragma unroll
+      for (int o = 0; o < L::kOperands; ++o)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_e4m3(tm + d * L::kColumns + o * MT, wd + o * (128 * kFp8Block >> 4) + 2 * k, xd + 2 * k, idesc, k != 0);
+      umma_commit(&ctl.empty[s]);
+      umma_commit(&ctl.sum_full[d]);
+    }
+    __syncwarp();
+  }
+  return true;
+}
+
+// The CTA's blocks of x, quantised into the operand tiles (rows past M: zeros) and ctl.scales [block][16].
+template <int MT>
+__device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl& ctl, uint32_t tiles, int b0, int count) {
+  const int t = threadIdx.x - kNarrowFirstSum * 32, lane = threadIdx.x & 31, in = lane & 15;
+  const int rows = static_cast<int>(a.M);
+  for (int i = t; i < count * (MT - rows) * 8; i += kNarrowSumWarps * 32) {
+    const int unit = i / 8, b = unit / (MT - rows), row = rows + unit % (MT - rows);
+    sts_v4(tiles + b * (MT * kFp8Block) + row * kFp8Block + (i & 7) * 16, 0, 0, 0, 0);
+  }
+  const int units = count * rows;
+  for (int u0 = t / 32 * 2; u0 < units; u0 += kNarrowSumWarps * 2) {  // uniform in a warp
+    const int unit = u0 + (lane >> 4);
+    const bool live = unit < units;
+    const int b = live ? unit / rows : 0, row = live ? unit - b * rows : 0;
+    const int at = (b0 + b) * kFp8Block + in * 8;
+    float f[8];
+    const uint4 v = live && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0);
+    unpack8(v, f);
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = max(most, magnitude(f[j]));
+    most = block_most(most);
+    const Fp8Divisor by(most);
+    if (live) {
+      const uint32_t to = tiles + b * (MT * kFp8Block) + row * kFp8Block + (((in >> 1) ^ (row & 7)) << 4) + (in & 1) * 8;
+      asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to), "r"(by.codes4(f)), "r"(by.codes4(f + 4)) : "memory");
+      if (in == 0) ctl.scales[b * kInlineRows + row] = fp8_scale(most);
+    }
+  }
+}
+
+template <int MT, bool GATED, bool ROWS>
+__device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int b0, int count, int tile, int row0) {
+  using L = Narrow<MT, GATED>;
+  constexpr int kEach = L::kEach;
+  const int warp = (threadIdx.x >> 5) - kNarrowFirstSum, half = warp >> 2, lane = threadIdx.x & 31;
+  const int quarter = (threadIdx.x >> 5) & 3;  // the TMEM lanes that this warp may read
+  const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kEach;
+  const float* ws = a.ws + static_cast<int64_t>(tile) * a.blocks + b0;
+  const float* us = GATED ? a.us + static_cast<int64_t>(tile) * a.blocks + b0 : nullptr;
+  uint64_t acc[L::kOperands][kEach / 2];
+#pragma unroll
+  for (int o = 0; o < L::kOperands; ++o)
+#pragma unroll
+    for (int j = 0; j < kEach / 2; ++j) acc[o][j] = 0;
+  // codes: a warp brings its tokens' scales of a block to its own two slots, one block ahead
+  float* slots = ctl.scales + warp * 128;
+  float next[kEach > 32 ? 2 : 1];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int c = 0; c < (kEach > 32 ? 2 : 1); ++c) {
+      const int64_t row = row0 + half * kEach + c * 32 + lane;
+      next[c] = i < count && c * 32 + lane < kEach && row < a.M ? a.xs[static_cast<int64_t>(b0 + i) * a.M + row] : 0.f;
+    }
+  };
+  if (!ROWS) fetch(0);
+  float w = ws[0], u = GATED ? us[0] : 0.f;
+  for (int it = 0; it < count; ++it) {
+    const int d = it % L::kBuffers;
+    const float* scales = ctl.scales + it * kInlineRows + half * kEach;
+    if (!ROWS) {
+      float* slot = slots + (it & 1) * 64;
+#pragma unroll
+      for (int c = 0; c < (kEach > 32 ? 2 : 1); ++c) slot[c * 32 + lane] = next[c];
+      __syncwarp();
+      scales = slot;
+      fetch(it + 1);
+    }
+    const float by_w = w, by_u = u;
+    if (it + 1 < count) {
+      w = ws[it + 1];
+      if (GATED) u = us[it + 1];
+    }
+    if (!warp_wait(&ctl.sum_full[d], it / L::kBuffers & 1)) return false;
+    tc_fence_after();
+#pragma unroll
+    for (int o = 0; o < L::kOperands; ++o) {
+      const uint64_t by = o ? f32x2(by_u, by_u) : f32x2(by_w, by_w);
+#pragma unroll
+      for (int c = 0; c < kEach; c += 8) {
+        uint32_t v[8];
+        tmem_ld8(tm + d * L::kColumns + o * MT + c, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
+                     :
+                     : "memory");
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 s = *reinterpret_cast<const float2*>(scales + c + 2 * j);
+          acc[o][c / 2 + j] = f32x2_fma(f32x2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
+                                        f32x2_mul(f32x2(s.x, s.y), by), acc[o][c / 2 + j]);
+        }
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.sum_empty[d]);
+  }
+  // all products are done, so nothing reads or fills the ring any more: [operand][token][weight row]
+  const uint32_t to = smem + (half * kEach * 128 + quarter * 32 + lane) * 4;
+#pragma unroll
+  for (int o = 0; o < L::kOperands; ++o)
+#pragma unroll
+    for (int j = 0; j < kEach / 2; ++j) {
+      float p, q;
+      f32x2_split(acc[o][j], p, q);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (o * MT + 2 * j) * 512), "f"(p) : "memory");
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (o * MT + 2 * j + 1) * 512), "f"(q) : "memory");
+    }
+  return true;
+}
+
+// The cluster's sums, a warp per token and four weight rows per lane, and the output.
+template <int MT, bool GATED>
+__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t smem, int rank, int tile, int row0) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = tile * 128 + lane * 4;
+  const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT)));
+  for (int t = warp * a.splits + rank; t < live; t += (kNarrowThreads / 32) * a.splits) {
+    float f[2][4];
+#pragma unroll
+    for (int o = 0; o < (GATED ? 2 : 1); ++o) {
+      const uint32_t at = smem + ((o * MT + t) * 128 + lane * 4) * 4;
+      float4 s = cluster_ld4(at, 0);
+      for (int r = 1; r < a.splits; ++r) {
+        const float4 v = cluster_ld4(at, r);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+      f[o][0] = s.x, f[o][1] = s.y, f[o][2] = s.z, f[o][3] = s.w;
+    }
+    const int64_t row = row0 + t;
+    if (GATED) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[0][j] = gated(f[0][j], f[1][j]);
+        most = max(most, magnitude(f[0][j]));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (n < a.N) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + row * a.ld + n) = Fp8Divisor(most).codes4(f[0]);
+      if (lane == 0) a.out_scales[static_cast<int64_t>(tile) * a.M + row] = fp8_scale(most);
+    } else if (a.f32) {
+      float* out = static_cast<float*>(a.out) + row * a.N + n;
+      if (a.vectors && n < a.N) *reinterpret_cast<float4*>(out) = make_float4(f[0][0], f[0][1], f[0][2], f[0][3]);
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < a.N) out[j] = f[0][j];
+    } else {
+      uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.N + n;
+      if (a.vectors && n < a.N) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(f[0][0], f[0][1]), pack_bf16x2(f[0][2], f[0][3]));
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < a.N) out[j] = static_cast<uint16_t>(pack_bf16x2(f[0][j], 0.f));
+    }
+  }
+}
+
+// grid: (splits x tiles of 128 weight rows, tiles of MT tokens), clusters of `splits`.
+template <int MT, bool GATED, bool ROWS>
+__global__ void __launch_bounds__(kNarrowThreads, MT > 64 ? 1 : 2)
+    fp8_narrow_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap w, const __grid_constant__ CUtensorMap u,
+                      NarrowArgs a) {
+  using L = Narrow<MT, GATED>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ NarrowControl ctl;
+  const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
+  const int warp = threadIdx.x >> 5, rank = static_cast<int>(cluster_rank());
+  const int tile = static_cast<int>(blockIdx.x) / a.splits, row0 = static_cast<int>(blockIdx.y) * MT;
+  const int b0 = static_cast<int>(static_cast<int64_t>(rank) * a.blocks / a.splits);
+  const int count = static_cast<int>(static_cast<int64_t>(rank + 1) * a.blocks / a.splits) - b0;  // at least one
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kNarrowStages; ++i) {
+      mbar_init(&ctl.full[i], 1);
+      mbar_init(&ctl.empty[i], 1);
+    }
+    for (int i = 0; i < L::kBuffers; ++i) {
+      mbar_init(&ctl.sum_full[i], 1);
+      mbar_init(&ctl.sum_empty[i], kNarrowSumWarps);
+    }
+    mbar_init(&ctl.x_full, kNarrowSumWarps);
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&ctl.tmem, L::kAlloc);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  pdl_trigger();
+  bool ok = true;
+  if (warp == 0) {
+    if (threadIdx.x == 0) ok = narrow_copies<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, b0, b0 + count, tile, row0);
+  } else if (warp == 1) {
+    ok = narrow_products<MT, GATED, ROWS>(a, ctl, smem, count);
+  } else {
+    if (ROWS) {
+      narrow_quantise<MT>(a, ctl, smem + a.stages * L::kBytesW, b0, count);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&ctl.x_full);
+      ok = warp_wait(&ctl.x_full, 0);  // the scales are everybody's
+    }
+    if (ok) ok = narrow_sums<MT, GATED, ROWS>(a, ctl, smem, b0, count, tile, row0);
+  }
+  if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(ctl.tmem, L::kAlloc);
+  }
+  cluster_sync();
+  narrow_join<MT, GATED>(a, smem, rank, tile, row0);
+  cluster_sync();  // the others have read this CTA's sums
+}
+
+// What a call does, by its sizes alone: `splits` CTAs of a cluster per tile, as many as two per SM leave room for.
+struct NarrowPlan {
+  int tokens, splits;
+  NarrowPlan(int64_t M, int64_t N, int blocks) {
+    tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = (tokens > 64 ? 1 : 2) * sm_count() / tiles;
+    splits = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
+    if (splits > blocks) splits = blocks;
+  }
+  int each(int blocks) const { return (blocks + splits - 1) / splits; }
+  // Whether the CTAs can quantise rows of x themselves.
+  bool quantises(int64_t M, int blocks) const { return M <= kInlineRows && each(blocks) <= kInlineBlocks; }
+};
+
+template <int MT, bool GATED, bool ROWS>
+int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, NarrowArgs a, const NarrowPlan& plan, cudaStream_t st) {
+  using L = Narrow<MT, GATED>;
+  const int each = plan.each(a.blocks);
+  const size_t room = MT > 64 ? 220 * 1024 : 108 * 1024;
+  a.splits = plan.splits;
+  a.stages = each < kNarrowStages ? each : kNarrowStages;
+  while (a.stages > 1 && L::smem(a.stages, ROWS ? each : 0) > room) --a.stages;
+  const size_t smem = L::smem(a.stages, ROWS ? each : 0);
+  const void* kernel = reinterpret_cast<const void*>(fp8_narrow_kernel<MT, GATED, ROWS>);
+  const int rc = allow_smem(kernel, smem);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.splits * ((a.N + 127) / 128)), static_cast<unsigned>((a.M + MT - 1) / MT));
+  cfg.blockDim = dim3(kNarrowThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(plan.splits);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_narrow_kernel<MT, GATED, ROWS>, x, w, u, a);
+  if (e != cudaSuccess) return cuda_error(e, "fp8_narrow_kernel");
+  count_launch();
+  return QK_OK;
+}
+
+template <bool GATED>
+int launch_narrow(bool rows, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const NarrowArgs& a, const NarrowPlan& plan,
+                  cudaStream_t st) {
+  if (rows) return launch_narrow<16, GATED, true>(x, w, u, a, plan, st);
+  return plan.tokens == 16   ? launch_narrow<16, GATED, false>(x, w, u, a, plan, st)
+         : plan.tokens == 32 ? launch_narrow<32, GATED, false>(x, w, u, a, plan, st)
+         : plan.tokens == 64 ? launch_narrow<64, GATED, false>(x, w, u, a, plan, st)
+                             : launch_narrow<128, GATED, false>(x, w, u, a, plan, st);
+}
+
+}  // namespace
+}  // namespace qk

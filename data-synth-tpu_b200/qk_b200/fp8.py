@@ -81,9 +81,31 @@ def _matrix(x, name):
     if not x.is_cuda:
         raise ValueError("expected CUDA tensors")
     code = _dtype_code(x)
+    if x.is_contiguous():
+        return x, code, x.shape[1]
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        x = x.contiguous()
+        return x.contiguous(), code, x.shape[1]
     return x, code, max(x.stride(0), x.shape[1])
+
+
+def _aligned(x, name):
+    """The same with rows that begin on 16 bytes if any number of rows of the width can."""
+    x, code, stride = _matrix(x, name)
+    if x.data_ptr() % 16 or stride * x.element_size() % 16:
+        return x.clone(memory_format=torch.contiguous_format), code, x.shape[1]
+    return x, code, stride
+
+
+_needs = {}
+
+
+def _workspace(name, key, device):
+    """``(workspace, bytes)`` of a call on ``device``, from the current stream's memory."""
+    need = _needs.get((name, key))
+    if need is None:
+        with torch.cuda.device(device):
+            need = _needs[name, key] = int(getattr(_lib.load(), name)(*key))
+    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
 def quantize_fp8(x):
@@ -123,26 +145,17 @@ def fp8_weights(codes, scales, device=None):
     return Fp8Weights(codes, _scales(scales, shape, codes.device, "the weights"))
 
 
-def _operands(x, weights, name="weights"):
-    """``weights`` as a product of ``K`` columns reads them: ``(codes, pitch, scales)``."""
-    (n, k), device = weights.codes.shape, weights.codes.device
-    if x is not None and (x.shape[1] != k or x.device != device):
-        raise ValueError(f"{name} must be [N, {x.shape[1]}] on the device of x")
+def _operand(weights, k, device, name):
+    """``weights`` as a product of ``k`` columns on ``device`` reads them: ``(rows, codes, pitch, scales)``."""
     codes, pitch = _codes(weights.codes, name)
-    return codes, pitch, _scales(weights.scales, (_blocks(n), _blocks(k)), device, name)
-
-
-def _source(x):
-    source = x.codes if isinstance(x, Fp8Rows) else x
-    if not isinstance(source, torch.Tensor) or source.dim() != 2 or source.shape[1] < 1:
-        raise ValueError("x must be a matrix or Fp8Rows")
-    return source
+    n, width = codes.shape
+    if width != k or n < 1 or codes.device != device:
+        raise ValueError(f"{name} must be [N, {k}] on the device of x")
+    return n, codes, pitch, _scales(weights.scales, (_blocks(n), _blocks(k)), device, name)
 
 
 def _rows(x):
-    """Activations as a product reads them, quantised if they are not: ``(codes, pitch, scales)``."""
-    if not isinstance(x, Fp8Rows):
-        x = quantize_fp8(x)
+    """Quantised activations as a product reads them: ``(codes, pitch, scales)``."""
     codes, pitch = _codes(x.codes, "x")
     return codes, pitch, _scales(x.scales, (_blocks(codes.shape[1]), codes.shape[0]), codes.device, "x")
 
@@ -161,26 +174,34 @@ def fp8_matmul(x, weights, *, output_dtype=None, out=None):
     dtype = output_dtype or (torch.bfloat16 if out is None else out.dtype)
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("output_dtype must be BF16 or FP32")
-    source = _source(x)
-    w, w_pitch, w_scales = _operands(source, weights)
-    (m, k), n, device = source.shape, w.shape[0], source.device
+    out_code = _lib.QK_OUT_F32 if dtype == torch.float32 else _lib.QK_OUT_BF16
+    if isinstance(x, Fp8Rows):
+        codes, pitch, scales = _rows(x)
+        (m, k), device = codes.shape, codes.device
+        n, w, w_pitch, w_scales = _operand(weights, k, device, "weights")
+        out = _output(out, (m, n), dtype, device)
+        _lib.call_on(device, "qk_fp8_matmul", codes.data_ptr(), pitch, scales.data_ptr(), m, k, w.data_ptr(), w_pitch,
+                     w_scales.data_ptr(), n, out_code, out.data_ptr())
+        return out
+    x, code, stride = _aligned(x, "x")
+    (m, k), device = x.shape, x.device
+    n, w, w_pitch, w_scales = _operand(weights, k, device, "weights")
     out = _output(out, (m, n), dtype, device)
-    codes, pitch, scales = _rows(x)
-    _lib.call_on(device, "qk_fp8_matmul", codes.data_ptr(), pitch, scales.data_ptr(), m, k, w.data_ptr(), w_pitch,
-                 w_scales.data_ptr(), n, _lib.QK_OUT_F32 if dtype == torch.float32 else _lib.QK_OUT_BF16, out.data_ptr())
+    room, need = _workspace("qk_fp8_linear_workspace_bytes", (code, m, k, n), device)
+    _lib.call_on(device, "qk_fp8_linear", x.data_ptr(), code, stride, m, k, w.data_ptr(), w_pitch, w_scales.data_ptr(), n,
+                 out_code, out.data_ptr(), room.data_ptr() if need else None, need)
     return out
 
 
 def gated_fp8(x, gate, up):
     """``silu(x gate^T) * (x up^T)`` as :class:`Fp8Rows` ``[M, I]``, quantised from FP32 by the rule of
     :func:`quantize_fp8`: ``x`` as for :func:`fp8_matmul`, ``gate`` and ``up`` ``[I, K]``."""
-    source = _source(x)
-    g, g_pitch, g_scales = _operands(source, gate, "gate")
-    u, u_pitch, u_scales = _operands(source, up, "up")
-    (m, k), inner, device = source.shape, g.shape[0], source.device
-    if u.shape[0] != inner:
+    codes, pitch, scales = _rows(x if isinstance(x, Fp8Rows) else quantize_fp8(x))
+    (m, k), device = codes.shape, codes.device
+    inner, g, g_pitch, g_scales = _operand(gate, k, device, "gate")
+    n, u, u_pitch, u_scales = _operand(up, k, device, "up")
+    if n != inner:
         raise ValueError("gate and up must be [I, K]")
-    codes, pitch, scales = _rows(x)
     h = _empty_codes(m, inner, device)
     h_scales = torch.empty((_blocks(inner), m), dtype=torch.float32, device=device)
     _lib.call_on(device, "qk_fp8_gated", codes.data_ptr(), pitch, scales.data_ptr(), m, k, g.data_ptr(), g_pitch,
@@ -192,9 +213,21 @@ def gated_fp8(x, gate, up):
 def gated_ffn_fp8(x, gate, up, down, *, out=None):
     """A gated feed-forward block, ``(silu(x gate^T) * (x up^T)) down^T`` as BF16 ``[M, H]``: the product
     of :func:`gated_fp8` with ``down`` ``[H, I]``."""
-    if down.codes.dim() != 2 or down.codes.shape[1] != gate.codes.shape[0]:
-        raise ValueError("down must be [H, I] for gate and up [I, K]")
-    return fp8_matmul(gated_fp8(x, gate, up), down, out=out, output_dtype=torch.bfloat16)
+    if isinstance(x, Fp8Rows):
+        return fp8_matmul(gated_fp8(x, gate, up), down, out=out, output_dtype=torch.bfloat16)
+    x, code, stride = _aligned(x, "x")
+    (m, k), device = x.shape, x.device
+    inner, g, g_pitch, g_scales = _operand(gate, k, device, "gate")
+    n, u, u_pitch, u_scales = _operand(up, k, device, "up")
+    if n != inner:
+        raise ValueError("gate and up must be [I, K]")
+    n, d, d_pitch, d_scales = _operand(down, inner, device, "down")
+    out = _output(out, (m, n), torch.bfloat16, device)
+    room, need = _workspace("qk_fp8_ffn_workspace_bytes", (code, m, k, inner), device)
+    _lib.call_on(device, "qk_fp8_ffn", x.data_ptr(), code, stride, m, k, g.data_ptr(), g_pitch, g_scales.data_ptr(),
+                 u.data_ptr(), u_pitch, u_scales.data_ptr(), inner, d.data_ptr(), d_pitch, d_scales.data_ptr(), n, out.data_ptr(),
+                 room.data_ptr() if need else None, need)
+    return out
 
 
 def rms_norm_fp8(x, gamma, eps=1e-6, *, residual=None):

@@ -171,6 +171,23 @@ int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t 
                  const uint8_t* gate, int64_t gate_ld, const float* gate_scales, const uint8_t* up,
                  int64_t up_ld, const float* up_scales, int64_t N, uint8_t* codes, int64_t ld,
                  float* scales, qk_stream_t stream);
+/* The product from rows of BF16 or FP32 (in_dtype, x_stride values apart), quantised in the call by
+ * the rule of qk_fp8_quantize: the values of qk_fp8_quantize and qk_fp8_matmul. The workspace
+ * (256-byte aligned) holds the codes and scales where a launch of its own makes them; where none is
+ * needed (few rows of BF16), rows of x must begin on 16 bytes. */
+size_t qk_fp8_linear_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t N);
+int qk_fp8_linear(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K,
+                  const uint8_t* w, int64_t w_ld, const float* w_scales, int64_t N, int out_dtype,
+                  void* out, void* workspace, size_t workspace_bytes, qk_stream_t stream);
+/* A gated feed-forward block, out [M, N] BF16 = (silu(x gate^T) * (x up^T)) down^T with gate and up
+ * [inner, K], down [N, inner]: the values of qk_fp8_quantize, qk_fp8_gated and qk_fp8_matmul. Rows of
+ * x must begin on 16 bytes where qk_fp8_linear_workspace_bytes(in_dtype, M, K, inner) is 0. */
+size_t qk_fp8_ffn_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t inner);
+int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K,
+               const uint8_t* gate, int64_t gate_ld, const float* gate_scales, const uint8_t* up,
+               int64_t up_ld, const float* up_scales, int64_t inner, const uint8_t* down,
+               int64_t down_ld, const float* down_scales, int64_t N, uint16_t* out, void* workspace,
+               size_t workspace_bytes, qk_stream_t stream);
 /* QK_ERR_TIMEOUT if a bounded wait of an earlier FP8 product on the current device gave up (its
  * output is then not valid), else QK_OK; clears the report. Synchronises `stream`. */
 int qk_fp8_check(qk_stream_t stream);
