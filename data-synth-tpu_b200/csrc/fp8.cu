@@ -52,24 +52,52 @@ struct RowsArgs {
   float* scales;  // [blocks][rows]
 };
 
-// Half a warp per block of a row. Consecutive warps take consecutive pairs of blocks.
-template <bool F32, bool ALIGNED>
+// Half a warp per block of a row; a warp has a row and 2 U consecutive blocks, all asked for at once, a CTA eight rows,
+// so that it writes whole sectors of scales. Rows that do not begin on 16 bytes (or FP32 or BF16 of odd widths) are
+// read a value per lane and turned around through shared memory, which is a twelfth of the cache lookups of eight
+// neighbouring values per lane.
+template <bool F32, bool ALIGNED, int U>
 __global__ void __launch_bounds__(kThreads) fp8_rows_kernel(RowsArgs a) {
-  const int lane = threadIdx.x & 31, pairs = (a.blocks + 1) / 2;
+  __shared__ __align__(16) uint8_t turned[ALIGNED ? 1 : kThreads / 16][ALIGNED ? 1 : kFp8Block];
+  const int lane = threadIdx.x & 31, in = lane & 15;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int block0 = blockIdx.y * (2 * U) + (lane >> 4);
   pdl_wait();
   pdl_trigger();
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); u < a.rows * pairs; u += warps) {
-    const int64_t row = u / pairs;
-    const int block = static_cast<int>(u - row * pairs) * 2 + (lane >> 4), at = block * kFp8Block + (lane & 15) * 8;
-    const void* from = F32 ? static_cast<const void*>(static_cast<const float*>(a.x) + row * a.stride)
-                           : static_cast<const void*>(static_cast<const uint16_t*>(a.x) + row * a.stride);
-    float f[8];
-    load8<F32, ALIGNED>(from, at, a.width, f);
-    const uint32_t most = block_most(most8(f));
+  if (row >= a.rows) return;
+  const void* from = F32 ? static_cast<const void*>(static_cast<const float*>(a.x) + row * a.stride)
+                         : static_cast<const void*>(static_cast<const uint16_t*>(a.x) + row * a.stride);
+  float f[U][8];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = (block0 + 2 * u) * kFp8Block;
+    if (ALIGNED) {
+      load8<F32, true>(from, at + in * 8, a.width, f[u]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = at + j * 16 + in;
+        f[u][j] = 0.f;
+        if (k < a.width) f[u][j] = F32 ? static_cast<const float*>(from)[k] : bf16_to_f32(static_cast<const uint16_t*>(from)[k]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int block = block0 + 2 * u, at = block * kFp8Block + in * 8;
+    const uint32_t most = block_most(most8(f[u]));
     const Fp8Divisor by(most);
-    if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(f), by.codes4(f + 4));
-    if (block < a.blocks && (lane & 15) == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = fp8_scale(most);
+    uint2 codes = make_uint2(by.codes4(f[u]), by.codes4(f[u] + 4));
+    if (!ALIGNED) {
+      uint8_t* mine = turned[threadIdx.x >> 4];
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mine[j * 16 + in] = static_cast<uint8_t>((j < 4 ? codes.x : codes.y) >> (8 * (j & 3)));
+      __syncwarp();
+      codes = *reinterpret_cast<const uint2*>(mine + in * 8);
+    }
+    if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = codes;
+    if (block < a.blocks && in == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = fp8_scale(most);
   }
 }
 
@@ -117,8 +145,39 @@ struct NormArgs {
   float* scales;
 };
 
-// A CTA per row held in registers. With p = s gamma (exact in FP32) the normed row is r p, r = rsqrt(mean s^2 + eps):
-// r moves no code, so the codes leave without waiting for the sum and r goes into the scales.
+// Eight values of a row's s and p = s gamma from `at`: the sum is kept, p comes out, the squares are added to `ss`.
+__device__ __forceinline__ void norm8(const NormArgs& a, int64_t row, int at, const uint4& x, const uint4& y, const uint4& gamma, float (&p)[8],
+                                      float& ss) {
+  float g[8];
+  unpack8(x, p);
+  unpack8(gamma, g);
+  if (a.y) {
+    float h[8];
+    unpack8(y, h);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(__fadd_rn(p[2 * j], h[2 * j]), __fadd_rn(p[2 * j + 1], h[2 * j + 1]));
+    const uint4 s = make_uint4(w[0], w[1], w[2], w[3]);
+    if (at < a.width) *reinterpret_cast<uint4*>(a.sum + row * a.width + at) = s;
+    unpack8(s, p);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    ss = fmaf(p[j], p[j], ss);
+    p[j] *= g[j];
+  }
+}
+
+__device__ __forceinline__ uint4 load16(const uint16_t* p, int at, int width) {
+  return at < width ? ld_guarded_v4(p + at) : make_uint4(0, 0, 0, 0);
+}
+// x and y may be written as the sum: not through the read-only path.
+__device__ __forceinline__ uint4 load16_rw(const uint16_t* p, int at, int width) {
+  return at < width ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0, 0, 0, 0);
+}
+
+// With p = s gamma (exact in FP32) the normed row is r p, r = rsqrt(mean s^2 + eps): r moves no code, so the codes
+// leave without waiting for the sum of squares and r goes into the scales. Few rows: a CTA each.
 __global__ void __launch_bounds__(kRowBlock) fp8_norm_kernel(NormArgs a) {
   __shared__ float red[kRowBlock / 32];
   const int64_t row = blockIdx.x;
@@ -132,27 +191,13 @@ __global__ void __launch_bounds__(kRowBlock) fp8_norm_kernel(NormArgs a) {
     const int at = (threadIdx.x + c * kRowBlock) * 8;
     most[c] = 0;
     if ((at & ~255) >= a.width) continue;  // the same for the warp
-    float f[8], g[8];
-    load8<false, true>(a.x + row * a.width, at, a.width, f);
-    load8<false, true>(a.gamma, at, a.width, g);
-    if (a.y) {
-      float h[8];
-      load8<false, true>(a.y + row * a.width, at, a.width, h);
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(__fadd_rn(f[2 * j], h[2 * j]), __fadd_rn(f[2 * j + 1], h[2 * j + 1]));
-      const uint4 s = make_uint4(w[0], w[1], w[2], w[3]);
-      if (at < a.width) *reinterpret_cast<uint4*>(a.sum + row * a.width + at) = s;
-      unpack8(s, f);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ss = fmaf(f[j], f[j], ss);
-      f[j] *= g[j];
-    }
-    most[c] = block_most(most8(f));
+    const uint4 x = load16_rw(a.x + row * a.width, at, a.width), g = load16(a.gamma, at, a.width);
+    const uint4 y = a.y ? load16_rw(a.y + row * a.width, at, a.width) : x;
+    float p[8];
+    norm8(a, row, at, x, y, g, p, ss);
+    most[c] = block_most(most8(p));
     const Fp8Divisor by(most[c]);
-    if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(f), by.codes4(f + 4));
+    if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(p), by.codes4(p + 4));
   }
   const float r = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(ss, red), static_cast<float>(a.width)), a.eps));
   if ((lane & 15) == 0) {
@@ -164,9 +209,50 @@ __global__ void __launch_bounds__(kRowBlock) fp8_norm_kernel(NormArgs a) {
   }
 }
 
+// Many rows: a warp each, four loads of either addend in flight, no barrier. The sums are in another order.
+constexpr int kNormAhead = 4;
+__global__ void __launch_bounds__(kThreads) fp8_norm_rows_kernel(NormArgs a) {
+  __shared__ float scale[kThreads / 32][kMaxRowWidth / kFp8Block];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  if (row >= a.rows) return;
+  float* mine = scale[threadIdx.x >> 5];
+  float ss = 0.f;
+#pragma unroll 1
+  for (int at0 = 0; at0 < a.width; at0 += kNormAhead * 256) {
+    uint4 x[kNormAhead], y[kNormAhead];
+#pragma unroll
+    for (int c = 0; c < kNormAhead; ++c) {
+      const int at = at0 + c * 256 + lane * 8;
+      x[c] = load16_rw(a.x + row * a.width, at, a.width);
+      y[c] = a.y ? load16_rw(a.y + row * a.width, at, a.width) : x[c];
+    }
+#pragma unroll
+    for (int c = 0; c < kNormAhead; ++c) {
+      const int at = at0 + c * 256 + lane * 8;
+      if (at0 + c * 256 >= a.width) break;  // the same for the warp
+      float p[8];
+      norm8(a, row, at, x[c], y[c], load16(a.gamma, at, a.width), p, ss);
+      const uint32_t most = block_most(most8(p));
+      const Fp8Divisor by(most);
+      if (at < a.width) {
+        *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(p), by.codes4(p + 4));
+        if ((lane & 15) == 0) mine[at / kFp8Block] = fp8_scale(most);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float r = rsqrtf(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.width)), a.eps));
+  __syncwarp();
+  for (int b = lane; b < (a.width + kFp8Block - 1) / kFp8Block; b += 32) a.scales[static_cast<int64_t>(b) * a.rows + row] = mine[b] * r;
+}
+
 template <typename Kernel>
-int launch(Kernel kernel, dim3 grid, int threads, cudaStream_t st, const RowsArgs& a, const char* name) {
-  cudaError_t e = launch_dependent(kernel, grid, dim3(threads), 0, st, a);
+int launch(Kernel kernel, dim3 grid, cudaStream_t st, const RowsArgs& a, const char* name) {
+  cudaError_t e = launch_dependent(kernel, grid, dim3(kThreads), 0, st, a);
   if (e != cudaSuccess) return cuda_error(e, name);
   count_launch();
   return QK_OK;
@@ -193,14 +279,19 @@ int qk_fp8_quantize(const void* x, int in_dtype, int64_t x_stride, int64_t rows,
   QK_REQUIRE((reinterpret_cast<uintptr_t>(x) % size) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3) == 0, "misaligned pointer");
   RowsArgs a{x, x_stride, ld, rows, static_cast<int>(width), static_cast<int>((width + 127) / 128), codes, scales};
   const bool aligned = aligned16(x) && x_stride * size % 16 == 0 && width % 8 == 0;
-  const int64_t units = rows * ((a.blocks + 1) / 2), most = 8ll * sm_count();
-  const int64_t ctas = (units + 7) / 8;
-  const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most));
+  const int64_t ctas = (rows + 7) / 8;
+  QK_REQUIRE(ctas < (1ll << 31) && a.blocks <= 65535 * 8, "too many rows or columns");
   cudaStream_t st = as_stream(stream);
-  if (f32) return aligned ? launch(fp8_rows_kernel<true, true>, grid, kThreads, st, a, "fp8_rows_kernel")
-                          : launch(fp8_rows_kernel<true, false>, grid, kThreads, st, a, "fp8_rows_kernel");
-  return aligned ? launch(fp8_rows_kernel<false, true>, grid, kThreads, st, a, "fp8_rows_kernel")
-                 : launch(fp8_rows_kernel<false, false>, grid, kThreads, st, a, "fp8_rows_kernel");
+  // four blocks per half warp where there is work for all SMs all the same
+  const bool many = ctas * a.blocks >= 64ll * sm_count() || a.blocks > 65535 * 2;
+  const dim3 grid(static_cast<unsigned>(ctas), many ? (a.blocks + 7) / 8 : (a.blocks + 1) / 2);
+  const char* name = "fp8_rows_kernel";
+  if (f32) {
+    if (aligned) return many ? launch(fp8_rows_kernel<true, true, 4>, grid, st, a, name) : launch(fp8_rows_kernel<true, true, 1>, grid, st, a, name);
+    return many ? launch(fp8_rows_kernel<true, false, 4>, grid, st, a, name) : launch(fp8_rows_kernel<true, false, 1>, grid, st, a, name);
+  }
+  if (aligned) return many ? launch(fp8_rows_kernel<false, true, 4>, grid, st, a, name) : launch(fp8_rows_kernel<false, true, 1>, grid, st, a, name);
+  return many ? launch(fp8_rows_kernel<false, false, 4>, grid, st, a, name) : launch(fp8_rows_kernel<false, false, 1>, grid, st, a, name);
 }
 
 int qk_fp8_quantize_blocks(const void* w, int in_dtype, int64_t w_stride, int64_t rows, int64_t width, uint8_t* codes, int64_t ld,
@@ -218,10 +309,10 @@ int qk_fp8_quantize_blocks(const void* w, int in_dtype, int64_t w_stride, int64_
   const bool aligned = aligned16(w) && w_stride * size % 16 == 0 && width % 8 == 0;
   const dim3 grid(a.blocks, static_cast<unsigned>((rows + 127) / 128));
   cudaStream_t st = as_stream(stream);
-  if (f32) return aligned ? launch(fp8_blocks_kernel<true, true>, grid, kThreads, st, a, "fp8_blocks_kernel")
-                          : launch(fp8_blocks_kernel<true, false>, grid, kThreads, st, a, "fp8_blocks_kernel");
-  return aligned ? launch(fp8_blocks_kernel<false, true>, grid, kThreads, st, a, "fp8_blocks_kernel")
-                 : launch(fp8_blocks_kernel<false, false>, grid, kThreads, st, a, "fp8_blocks_kernel");
+  if (f32) return aligned ? launch(fp8_blocks_kernel<true, true>, grid, st, a, "fp8_blocks_kernel")
+                          : launch(fp8_blocks_kernel<true, false>, grid, st, a, "fp8_blocks_kernel");
+  return aligned ? launch(fp8_blocks_kernel<false, true>, grid, st, a, "fp8_blocks_kernel")
+                 : launch(fp8_blocks_kernel<false, false>, grid, st, a, "fp8_blocks_kernel");
 }
 
 int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma, int64_t rows, int width, float eps, uint16_t* x_out,
@@ -233,7 +324,9 @@ int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma,
   QK_REQUIRE(x && gamma && codes && scales && (!y || x_out), "null pointer");
   QK_REQUIRE(aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(x_out) && aligned16(codes), "pointers must be 16-byte aligned");
   NormArgs a{x, y, gamma, rows, ld, width, eps, x_out, codes, scales};
-  cudaError_t e = launch_dependent(fp8_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(kRowBlock), 0, as_stream(stream), a);
+  cudaError_t e = rows >= 8ll * sm_count()
+                      ? launch_dependent(fp8_norm_rows_kernel, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(kThreads), 0, as_stream(stream), a)
+                      : launch_dependent(fp8_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(kRowBlock), 0, as_stream(stream), a);
   if (e != cudaSuccess) return cuda_error(e, "fp8_norm_kernel");
   count_launch();
   return QK_OK;

@@ -73,8 +73,8 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
     a.vectors = vectors;
     return u ? launch_narrow<true>(false, xm, wm, um, a, plan, st) : launch_narrow<false>(false, xm, wm, wm, a, plan, st);
   }
-  ok = encode(&xm, x, M, K, x_ld, kTileM) && encode(&wm, w.codes, N, K, w.ld, u ? kFp8Block : kTileN) &&
-       (!u || encode(&um, u->codes, N, K, u->ld, kFp8Block));
+  ok = encode(&xm, x, M, K, x_ld, kHalf) && encode(&wm, w.codes, N, K, w.ld, kHalf / 2) &&
+       (!u || encode(&um, u->codes, N, K, u->ld, kHalf / 2));
   if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
   WideArgs a{};
   a.M = M;

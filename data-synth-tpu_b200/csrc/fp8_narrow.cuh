@@ -53,14 +53,6 @@ struct NarrowControl {
   alignas(16) float scales[kInlineBlocks * kInlineRows > kNarrowSumWarps * 2 * 64 ? kInlineBlocks * kInlineRows : kNarrowSumWarps * 2 * 64];
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // Four floats of the shared memory of the cluster's CTA `rank`, at this CTA's address `addr`.
 __device__ __forceinline__ float4 cluster_ld4(uint32_t addr, uint32_t rank) {
   float4 v;

@@ -1,9 +1,12 @@
 // The wide FP8 product, for many rows of x.
 //
-// One CTA per SM works through tiles of 128 rows by 256 columns (gated: 128 of the gate and the same 128 of up).
-// A block of 128 columns of K is one row of the 128-byte swizzle and four MMAs (M 128, N 256, K 32); its sum goes to
-// one of two buffers of 256 TMEM columns, and eight warps add it, times the block's two scales, to FP32 sums in
-// their registers (a row and 128 columns per thread) while the tensor core fills the other buffer.
+// Pairs of CTAs, one per SM, work through tiles of 256 rows by 256 columns (gated: 128 of the gate and the same 128
+// of up): each CTA brings 128 rows of x and 128 of the weights, and one MMA over the pair (M 256, N 128, K 32) reads
+// both. A block of 128 columns of K is one row of the 128-byte swizzle and twice four MMAs, for either half of the
+// columns; their sums go to one of two buffers of 128 TMEM columns for that half (in each CTA its 128 rows), and the
+// half's four warps per CTA add them, times the block's two scales, to FP32 sums in their registers (a row and 128
+// columns per thread) while the tensor core fills the three others. A buffer's round trip (MMAs, commit, sums,
+// release) is what bounds the kernel: with two buffers of 256 columns it took 307 us where this takes .
 #pragma once
 
 #include "fp8_product.cuh"
@@ -11,11 +14,12 @@
 namespace qk {
 namespace {
 
-constexpr int kTileM = 128, kTileN = 256;
-constexpr int kStages = 4, kBuffers = 2;
-constexpr uint32_t kBytesA = kTileM * kFp8Block, kBytesB = kTileN * kFp8Block, kStageBytes = kBytesA + kBytesB;
+constexpr int kTileM = 256, kTileN = 256, kHalf = 128;  // a pair's tile, and a CTA's rows of either operand
+constexpr int kStages = 5, kBuffers = 2;
+constexpr uint32_t kBytesA = kHalf * kFp8Block, kStageBytes = 2 * kBytesA;  // of one CTA
 constexpr int kFirstSum = 4, kSumWarps = 8, kThreads = (kFirstSum + kSumWarps) * 32;
 constexpr uint32_t kStaging = 4096;  // bytes per summing warp
+constexpr int kAhead = 4;            // blocks whose scales of x are on their way
 // Registers per thread: 168 at launch for 3 warpgroups (504 in all).
 constexpr int kSumRegs = 216, kOtherRegs = 72;
 static_assert(2 * kSumRegs + kOtherRegs <= 3 * 168, "the shares fit the launch's registers");
@@ -33,7 +37,7 @@ struct WideArgs {
 };
 
 struct WideControl {
-  uint64_t full[kStages], empty[kStages], sum_full[kBuffers], sum_empty[kBuffers];
+  uint64_t full[kStages], empty[kStages], sum_full[kBuffers][2], sum_empty[kBuffers][2];
   uint64_t swapped[4];               // a row's two warps have left their maxima
   uint32_t tmem;
 };
@@ -47,65 +51,106 @@ __device__ __forceinline__ Tile tile_of(const WideArgs& a, int t) {
   return Tile{first + in % high, in / high};
 }
 
+// The address of `bar` in the pair's first CTA, which issues the MMAs.
+__device__ __forceinline__ uint32_t leaders(const uint64_t* bar) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(bar)));
+  return r;
+}
+
+__device__ __forceinline__ void load_box_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive once on `bar` in both CTAs when all MMAs issued so far by this thread are complete.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+
+// An arrival that orders nothing but what came before by itself: the loads from tensor memory are complete (wait::ld).
+// With .release.cluster, which waits for this thread's stores to be seen in the cluster, the round trip of a buffer
+// took 1.4 us and 16384 x 2048 by 9216 580 us (now 307).
+__device__ __forceinline__ void cluster_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Both CTAs: their rows of x and of the weights. The bytes count on the leader's barrier.
 template <bool GATED>
 __device__ __forceinline__ bool wide_copies(const WideArgs& a, WideControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
-                                            const CUtensorMap* u, uint32_t smem) {
+                                            const CUtensorMap* u, uint32_t smem, int rank) {
   uint32_t it = 0;
   bool ok = true;
-  for (int t = blockIdx.x; ok && t < a.tiles_m * a.tiles_n; t += gridDim.x) {
+  const CUtensorMap* b_map = GATED && rank ? u : w;
+  for (int t = blockIdx.x / 2; ok && t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     const Tile tile = tile_of(a, t);
+    const int a_row = tile.m * kTileM + rank * kHalf, b_row = GATED ? tile.n * kFp8Block : tile.n * kTileN + rank * 64;
     for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t s = it % kStages, at = smem + s * kStageBytes;
+      const uint32_t s = it % kStages, at = smem + s * kStageBytes, bar = leaders(&ctl.full[s]);
       ok = mbar_wait_bounded(&ctl.empty[s], (it / kStages & 1) ^ 1);
       if (!ok) break;
-      mbar_expect_tx(&ctl.full[s], kStageBytes);
-      load_box(at, x, b * kFp8Block, tile.m * kTileM, &ctl.full[s]);
-      if (GATED) {
-        load_box(at + kBytesA, w, b * kFp8Block, tile.n * kFp8Block, &ctl.full[s]);
-        load_box(at + kBytesA + kBytesB / 2, u, b * kFp8Block, tile.n * kFp8Block, &ctl.full[s]);
-      } else {
-        load_box(at + kBytesA, w, b * kFp8Block, tile.n * kTileN, &ctl.full[s]);
-      }
+      if (rank == 0) mbar_expect_tx(&ctl.full[s], 2 * kStageBytes);
+      load_box_pair(at, x, b * kFp8Block, a_row, bar);
+      load_box_pair(at + kBytesA, b_map, b * kFp8Block, b_row, bar);
+      load_box_pair(at + kBytesA + kBytesA / 2, b_map, b * kFp8Block, b_row + (GATED ? 64 : 128), bar);
     }
   }
-  // every copy issued must have landed before the CTA leaves
-  for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait_bounded(&ctl.full[i % kStages], i / kStages & 1);
+  // Every copy issued must have landed before the CTA leaves: when the MMAs that read it are done.
+  for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait_bounded(&ctl.empty[i % kStages], i / kStages & 1);
   return ok;
 }
 
+// The leader's MMA warp.
 __device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ctl, uint32_t smem) {
-  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = idesc_e4m3_m128(kTileN);
+  // kind::f8f6f4, e4m3 A and B, both K-major, FP32 D, M = 256, N = 128
+  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = (1u << 4) | (128 >> 3) << 17 | (kTileM >> 4) << 24;
   uint32_t it = 0;
-  for (int t = blockIdx.x; t < a.tiles_m * a.tiles_n; t += gridDim.x) {
+  for (int t = blockIdx.x / 2; t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     for (int b = 0; b < a.blocks; ++b, ++it) {
       const uint32_t s = it % kStages, d = it % kBuffers;
-      if (!warp_wait(&ctl.full[s], it / kStages & 1)) return false;
-      if (!warp_wait(&ctl.sum_empty[d], (it / kBuffers & 1) ^ 1)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t ad = sdesc_sw128(smem + s * kStageBytes, 1024u), bd = sdesc_sw128(smem + s * kStageBytes + kBytesA, 1024u);
+      const uint64_t ad = sdesc_sw128(smem + s * kStageBytes, 1024u), bd = sdesc_sw128(smem + s * kStageBytes + kBytesA, 1024u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_e4m3(tm + d * kTileN, ad + 2 * k, bd + 2 * k, idesc, k != 0);
-        umma_commit(&ctl.empty[s]);
-        umma_commit(&ctl.sum_full[d]);
+      for (int h = 0; h < 2; ++h) {
+        if (!warp_wait(&ctl.sum_empty[d][h], (it / kBuffers & 1) ^ 1)) return false;
+        if (h == 0 && !warp_wait(&ctl.full[s], it / kStages & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_e4m3_pair(tm + d * kTileN + h * 128, ad + 2 * k, bd + h * (kBytesA / 2 >> 4) + 2 * k, idesc, k != 0);
+          if (h) umma_commit_pair(&ctl.empty[s]);
+          umma_commit_pair(&ctl.sum_full[d][h]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
   }
   return true;
 }
 
-// One block's sums, `count` columns from `col`, times `scale`, added to `acc`.
+// One block's sums, 64 columns at a time, times `by`, added to `acc`.
 template <int COUNT>
 __device__ __forceinline__ void add_block(uint32_t col, float scale, uint64_t* acc) {
   const uint64_t by = f32x2(scale, scale);
 #pragma unroll
-  for (int c = 0; c < COUNT; c += 32) {
-    uint32_t v[32];
-    tmem_ld32(col + c, v);
-    tmem_wait_ld(v);
+  for (int c = 0; c < COUNT; c += 64) {
+    uint32_t v[64];
+    tmem_get64(col + c, v);
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int j = 0; j < 32; ++j)
       acc[c / 2 + j] = f32x2_fma(f32x2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), by, acc[c / 2 + j]);
   }
 }
@@ -162,41 +207,48 @@ __device__ __forceinline__ void wide_store(const WideArgs& a, const uint64_t (&a
 }
 
 template <bool GATED>
-__device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, uint32_t staging) {
+__device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, uint32_t staging, int rank) {
   const int warp = (threadIdx.x >> 5) - kFirstSum, quarter = warp & 3, half = warp >> 2, lane = threadIdx.x & 31;
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t released[kBuffers] = {leaders(&ctl.sum_empty[0][half]), leaders(&ctl.sum_empty[1][half])};
+  const uint32_t scales = staging + kSumWarps * kStaging + (threadIdx.x - kFirstSum * 32) * 4;  // this thread's, kAhead slots
   uint32_t it = 0, swaps = 0;
-  for (int t = blockIdx.x; t < a.tiles_m * a.tiles_n; t += gridDim.x) {
+  for (int t = blockIdx.x / 2; t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     const Tile tile = tile_of(a, t);
-    const int64_t row0 = static_cast<int64_t>(tile.m) * kTileM + quarter * 32, row = row0 + lane;
+    const int64_t row0 = static_cast<int64_t>(tile.m) * kTileM + rank * kHalf + quarter * 32, row = row0 + lane;
     // a thread's columns: 128 of the tile's 256, or 64 of the gate's and the same of up's
     const int n_block = GATED ? tile.n : min(tile.n * 2 + half, a.n_blocks - 1);
     const float* ws = a.ws + static_cast<int64_t>(n_block) * a.blocks;
     const float* us = GATED ? a.us + static_cast<int64_t>(n_block) * a.blocks : nullptr;
     const float* xs = a.xs + min(row, a.M - 1);
+    auto fetch = [&](int b) {  // a thread brings its row's scale of a block to its own slot, so nobody else waits for it
+      if (b < a.blocks)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scales + (b % kAhead) * (kSumWarps * 128)),
+                     "l"(xs + static_cast<int64_t>(b) * a.M)
+                     : "memory");
+      cp_async_commit();
+    };
+    for (int b = 0; b < kAhead; ++b) fetch(b);
     uint64_t acc[64];
 #pragma unroll
     for (int j = 0; j < 64; ++j) acc[j] = 0;
-    float x = xs[0], w = ws[0], u = GATED ? us[0] : 0.f;
     for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t d = it % kBuffers, cols = tm + d * kTileN;
-      const float by_w = x * w, by_u = x * u;
-      if (b + 1 < a.blocks) {
-        x = xs[(b + 1) * a.M];
-        w = ws[b + 1];
-        if (GATED) u = us[b + 1];
-      }
-      if (!warp_wait(&ctl.sum_full[d], it / kBuffers & 1)) return false;
+      const uint32_t d = it % kBuffers, cols = tm + d * kTileN + half * 128;
+      const float w = __ldg(ws + b), u = GATED ? __ldg(us + b) : 0.f;
+      cp_async_wait<kAhead - 1>();
+      const float x = __uint_as_float(lds_at(scales + (b % kAhead) * (kSumWarps * 128)));
+      fetch(b + kAhead);
+      if (!warp_wait(&ctl.sum_full[d][half], it / kBuffers & 1)) return false;
       tc_fence_after();
       if (GATED) {
-        add_block<64>(cols + half * 64, by_w, acc);
-        add_block<64>(cols + 128 + half * 64, by_u, acc + 32);
+        add_block<64>(cols, x * w, acc);
+        add_block<64>(cols + 64, x * u, acc + 32);
       } else {
-        add_block<128>(cols + half * 128, by_w, acc);
+        add_block<128>(cols, x * w, acc);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.sum_empty[d]);
+      if (lane == 0) cluster_arrive(released[d]);
     }
     if (!GATED) {
       if (a.f32) wide_store<true>(a, acc, staging + warp * kStaging, row0, tile.n * kTileN + half * 128);
@@ -238,60 +290,68 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, u
 }
 
 template <bool GATED>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     fp8_wide_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap w, const __grid_constant__ CUtensorMap u,
                     WideArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ WideControl ctl;
   const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
-  const int warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5, rank = static_cast<int>(cluster_rank());
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&ctl.full[i], 1);
       mbar_init(&ctl.empty[i], 1);
     }
     for (int i = 0; i < kBuffers; ++i) {
-      mbar_init(&ctl.sum_full[i], 1);
-      mbar_init(&ctl.sum_empty[i], kSumWarps);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&ctl.sum_full[i][h], 1);
+        mbar_init(&ctl.sum_empty[i][h], kSumWarps);  // half of the warps of either CTA
+      }
     }
     for (int i = 0; i < 4; ++i) mbar_init(&ctl.swapped[i], 2);
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(&ctl.tmem, 512);
+  // Both CTAs' tensor memory. They hold it while they wait for one another, but no other CTA that could wait for some
+  // fits beside one of these: they have all but 1,024 of an SM's registers.
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&ctl.tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // the barriers of both are there
   tc_fence_after();
   pdl_wait();
   pdl_trigger();
   bool ok = true;
   if (warp >= kFirstSum) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
-    ok = wide_sums<GATED>(a, ctl, smem + kStages * kStageBytes);
+    ok = wide_sums<GATED>(a, ctl, smem + kStages * kStageBytes, rank);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 0) {
-      if (threadIdx.x == 0) ok = wide_copies<GATED>(a, ctl, &x, &w, &u, smem);
-    } else if (warp == 1) {
+      if (threadIdx.x == 0) ok = wide_copies<GATED>(a, ctl, &x, &w, &u, smem, rank);
+    } else if (warp == 1 && rank == 0) {
       ok = wide_products(a, ctl, smem);
     }
   }
   if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // neither reads the other's shared or tensor memory any more
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(ctl.tmem, 512);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(ctl.tmem));
   }
 }
 
 template <bool GATED>
 int launch_wide(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const WideArgs& a, cudaStream_t st) {
-  const size_t smem = 1024 + kStages * kStageBytes + kSumWarps * kStaging;
+  const size_t smem = 1024 + kStages * kStageBytes + kSumWarps * kStaging + kAhead * kSumWarps * 128;
   const int rc = allow_smem(reinterpret_cast<const void*>(fp8_wide_kernel<GATED>), smem);
   if (rc) return rc;
-  const int tiles = a.tiles_m * a.tiles_n;
-  cudaError_t e = launch_dependent(fp8_wide_kernel<GATED>, dim3(tiles < sm_count() ? tiles : sm_count()), dim3(kThreads), smem, st,
-                                   x, w, u, a);
+  const int tiles = a.tiles_m * a.tiles_n, pairs = sm_count() / 2;
+  cudaError_t e = launch_dependent(fp8_wide_kernel<GATED>, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kThreads), smem, st, x, w, u, a);
   if (e != cudaSuccess) return cuda_error(e, "fp8_wide_kernel");
   count_launch();
   return QK_OK;

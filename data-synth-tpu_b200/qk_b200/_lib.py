@@ -244,21 +244,34 @@ def stream_handle(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_bound = {}  # name -> entry point
+_cuda = None  # torch._C, once there is a CUDA tensor to call for
+
+
 def call_on(device, name, *args):
     """``name(*args, stream)`` with ``device`` current, on its current stream: for entry points that
     take plain addresses (``Tensor.data_ptr()`` or None) and the stream last. Leaner than a device
     guard and stream object of its own: a decode step makes many calls of a few microseconds."""
-    import torch
-
+    global _cuda
     if device.type != "cuda":
         raise ValueError("expected CUDA tensors")
-    index = torch.cuda.current_device() if device.index is None else device.index
-    fn = getattr(_lib or load(), name)
-    if torch.cuda.current_device() == index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if _cuda is None:
+        import torch
+
+        torch.cuda.current_device()  # initialises CUDA
+        _cuda = torch._C
+    current = _cuda._cuda_getDevice()
+    index = current if device.index is None else device.index
+    fn = _bound.get(name)
+    if fn is None:
+        fn = _bound[name] = getattr(load(), name)
+    if current == index:
+        status = fn(*args, _cuda._cuda_getCurrentRawStream(index))
     else:
+        import torch
+
         with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            status = fn(*args, _cuda._cuda_getCurrentRawStream(index))
     if status != QK_OK:
         check(status)
 

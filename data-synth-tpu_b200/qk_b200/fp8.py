@@ -19,10 +19,10 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .attention_cache import _dtype_code
 
 BLOCK = 128
 _E4M3 = torch.float8_e4m3fn
+_TYPES = {torch.bfloat16: _lib.QK_OUT_BF16, torch.float32: _lib.QK_OUT_F32}
 
 
 class Fp8Rows(NamedTuple):
@@ -43,26 +43,30 @@ def _blocks(n):
     return -(-n // BLOCK)
 
 
-def _empty_codes(rows, width, device):
-    """Codes ``[rows, width]`` whose rows begin on 16 bytes."""
+def _empty_rows(like, rows, width):
+    """:class:`Fp8Rows` to be written, on the device of ``like``; rows of codes begin on 16 bytes."""
     pitch = (width + 15) // 16 * 16
-    codes = torch.empty((rows, pitch), dtype=_E4M3, device=device)
-    return codes if pitch == width else codes[:, :width]
+    codes = like.new_empty((rows, pitch), dtype=_E4M3)
+    return (Fp8Rows(codes if pitch == width else codes[:, :width], like.new_empty((_blocks(width), rows), dtype=torch.float32)),
+            pitch)
 
 
 def _codes(codes, name):
     """Codes as the products read them, and the bytes from row to row; copied only where their rows
     are not evenly spaced on 16-byte boundaries."""
-    if codes.dim() != 2 or codes.dtype != _E4M3:
+    if codes.dtype != _E4M3 or codes.dim() != 2:
         raise TypeError(f"{name} must hold float8_e4m3fn codes, a matrix")
     if not codes.is_cuda:
         raise ValueError("expected CUDA tensors")
     rows, width = codes.shape
-    pitch = codes.stride(0) if rows > 1 else max(codes.stride(0), (width + 15) // 16 * 16)
-    if codes.data_ptr() % 16 or pitch % 16 or pitch < width or (width > 1 and codes.stride(1) != 1):
-        fresh = _empty_codes(rows, width, codes.device)
+    pitch = codes.stride(0)
+    if rows == 1 and pitch < width:
+        pitch = (width + 15) // 16 * 16
+    if pitch % 16 or pitch < width or codes.data_ptr() % 16 or (width > 1 and codes.stride(1) != 1):
+        pitch = (width + 15) // 16 * 16
+        fresh = codes.new_empty((rows, pitch))[:, :width]
         fresh.copy_(codes)
-        codes, pitch = fresh, fresh.stride(0)
+        return fresh, pitch
     return codes, pitch
 
 
@@ -78,9 +82,11 @@ def _matrix(x, name):
     """``x`` BF16 or FP32 ``[rows, width]`` with dense rows: ``(x, type code, stride)``."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"{name} must be a BF16 or FP32 matrix")
+    code = _TYPES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be BF16 or FP32")
     if not x.is_cuda:
         raise ValueError("expected CUDA tensors")
-    code = _dtype_code(x)
     if x.is_contiguous():
         return x, code, x.shape[1]
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
@@ -89,7 +95,7 @@ def _matrix(x, name):
 
 
 def _aligned(x, name):
-    """The same with rows that begin on 16 bytes if any number of rows of the width can."""
+    """The same with rows that begin on 16 bytes if those of a fresh tensor do."""
     x, code, stride = _matrix(x, name)
     if x.data_ptr() % 16 or stride * x.element_size() % 16:
         return x.clone(memory_format=torch.contiguous_format), code, x.shape[1]
@@ -113,23 +119,23 @@ def quantize_fp8(x):
     the largest magnitude ``m`` (at least 2^-100) has the scale ``m / 448`` and the codes
     ``e4m3(448 x / m)``. A block that holds an infinity or a NaN has no finite values."""
     x, code, stride = _matrix(x, "x")
-    (rows, width), device = x.shape, x.device
-    codes = _empty_codes(rows, width, device)
-    scales = torch.empty((_blocks(width), rows), dtype=torch.float32, device=device)
-    _lib.call_on(device, "qk_fp8_quantize", x.data_ptr(), code, stride, rows, width, codes.data_ptr(), codes.stride(0),
-                 scales.data_ptr())
-    return Fp8Rows(codes, scales)
+    rows, width = x.shape
+    out, pitch = _empty_rows(x, rows, width)
+    _lib.call_on(x.device, "qk_fp8_quantize", x.data_ptr(), code, stride, rows, width, out.codes.data_ptr(), pitch,
+                 out.scales.data_ptr())
+    return out
 
 
 def pack_fp8(weight):
     """``weight`` BF16 or FP32 ``[N, K]`` -> :class:`Fp8Weights`, by the rule of :func:`quantize_fp8`
     for blocks of 128 x 128."""
     weight, code, stride = _matrix(weight, "weight")
-    (rows, width), device = weight.shape, weight.device
-    codes = _empty_codes(rows, width, device)
-    scales = torch.empty((_blocks(rows), _blocks(width)), dtype=torch.float32, device=device)
-    _lib.call_on(device, "qk_fp8_quantize_blocks", weight.data_ptr(), code, stride, rows, width, codes.data_ptr(),
-                 codes.stride(0), scales.data_ptr())
+    rows, width = weight.shape
+    pitch = (width + 15) // 16 * 16
+    codes = weight.new_empty((rows, pitch), dtype=_E4M3)[:, :width]
+    scales = weight.new_empty((_blocks(rows), _blocks(width)), dtype=torch.float32)
+    _lib.call_on(weight.device, "qk_fp8_quantize_blocks", weight.data_ptr(), code, stride, rows, width, codes.data_ptr(),
+                 pitch, scales.data_ptr())
     return Fp8Weights(codes, scales)
 
 
@@ -202,12 +208,11 @@ def gated_fp8(x, gate, up):
     n, u, u_pitch, u_scales = _operand(up, k, device, "up")
     if n != inner:
         raise ValueError("gate and up must be [I, K]")
-    h = _empty_codes(m, inner, device)
-    h_scales = torch.empty((_blocks(inner), m), dtype=torch.float32, device=device)
+    h, h_pitch = _empty_rows(codes, m, inner)
     _lib.call_on(device, "qk_fp8_gated", codes.data_ptr(), pitch, scales.data_ptr(), m, k, g.data_ptr(), g_pitch,
-                 g_scales.data_ptr(), u.data_ptr(), u_pitch, u_scales.data_ptr(), inner, h.data_ptr(), h.stride(0),
-                 h_scales.data_ptr())
-    return Fp8Rows(h, h_scales)
+                 g_scales.data_ptr(), u.data_ptr(), u_pitch, u_scales.data_ptr(), inner, h.codes.data_ptr(), h_pitch,
+                 h.scales.data_ptr())
+    return h
 
 
 def gated_ffn_fp8(x, gate, up, down, *, out=None):
@@ -242,15 +247,21 @@ def rms_norm_fp8(x, gamma, eps=1e-6, *, residual=None):
         raise ValueError("gamma and residual must be on the device of x")
     if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != x.shape):
         raise ValueError("residual must be BF16 of x's shape")
-    x, gamma, residual = (None if t is None else t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16
-                          else t.contiguous() for t in (x, gamma, residual))
-    codes = _empty_codes(rows, width, device)
-    scales = torch.empty((_blocks(width), rows), dtype=torch.float32, device=device)
-    total = None if residual is None else torch.empty_like(x)
-    _lib.call_on(device, "qk_fp8_rms_norm", x.data_ptr(), None if residual is None else residual.data_ptr(), gamma.data_ptr(),
-                 rows, width, eps, None if total is None else total.data_ptr(), codes.data_ptr(), codes.stride(0),
-                 scales.data_ptr())
-    return Fp8Rows(codes, scales), total
+    x, gamma = _dense(x), _dense(gamma)
+    out, pitch = _empty_rows(x, rows, width)
+    total = y = None
+    if residual is not None:
+        residual = _dense(residual)
+        total = torch.empty_like(x)
+        y, kept = residual.data_ptr(), total.data_ptr()
+    _lib.call_on(device, "qk_fp8_rms_norm", x.data_ptr(), y, gamma.data_ptr(), rows, width, eps, kept if y else None,
+                 out.codes.data_ptr(), pitch, out.scales.data_ptr())
+    return out, total
+
+
+def _dense(t):
+    """``t`` contiguous and 16-byte aligned."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def check_status(device=None):
