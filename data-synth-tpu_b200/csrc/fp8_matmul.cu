@@ -56,7 +56,7 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
   CUtensorMap xm, wm, um;
   bool ok;
   if (narrow(M)) {
-    const NarrowPlan plan(M, N, blocks);
+    const NarrowPlan plan(M, N, blocks, u != nullptr);
     ok = encode(&xm, x, M, K, x_ld, plan.tokens) && encode(&wm, w.codes, N, K, w.ld, 128) && (!u || encode(&um, u->codes, N, K, u->ld, 128));
     if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
     NarrowArgs a{};
@@ -102,18 +102,20 @@ size_t row_bytes(int64_t M, int64_t K) {
 }
 
 // Whether a product of BF16 rows quantises them itself: by the sizes alone, so that the workspace's size is.
-bool quantises(int in_dtype, int64_t M, int64_t K, int64_t N) {
+bool quantises(int in_dtype, int64_t M, int64_t K, int64_t N, bool gated) {
   const int blocks = static_cast<int>((K + 127) / 128);
-  return in_dtype == QK_OUT_BF16 && K % 8 == 0 && NarrowPlan(M, N, blocks).quantises(M, blocks);
+  return in_dtype == QK_OUT_BF16 && K % 8 == 0 && NarrowPlan(M, N, blocks, gated).quantises(M, blocks);
 }
-size_t room_for(int in_dtype, int64_t M, int64_t K, int64_t N) { return quantises(in_dtype, M, K, N) ? 0 : row_bytes(M, K); }
+size_t room_for(int in_dtype, int64_t M, int64_t K, int64_t N, bool gated) {
+  return quantises(in_dtype, M, K, N, gated) ? 0 : row_bytes(M, K);
+}
 
 int product_of_rows(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const Weights& w, const Weights* u, int64_t N,
                     bool f32, void* out, int64_t ld, float* out_scales, uint8_t* room, cudaStream_t st) {
-  if (quantises(in_dtype, M, K, N)) {
+  if (quantises(in_dtype, M, K, N, u != nullptr)) {
     QK_REQUIRE(aligned16(x) && x_stride % 8 == 0, "few rows of x must begin on 16 bytes");
     const int blocks = static_cast<int>((K + 127) / 128);
-    const NarrowPlan plan(M, N, blocks);
+    const NarrowPlan plan(M, N, blocks, u != nullptr);
     CUtensorMap wm, um;
     if (!encode(&wm, w.codes, N, K, w.ld, 128) || (u && !encode(&um, u->codes, N, K, u->ld, 128)))
       return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
@@ -175,7 +177,7 @@ int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t 
 }
 
 size_t qk_fp8_linear_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t N) {
-  return M > 0 && K > 0 && N > 0 ? room_for(in_dtype, M, K, N) : 0;
+  return M > 0 && K > 0 && N > 0 ? room_for(in_dtype, M, K, N, false) : 0;
 }
 
 int qk_fp8_linear(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const uint8_t* w, int64_t w_ld,
@@ -186,14 +188,14 @@ int qk_fp8_linear(const void* x, int in_dtype, int64_t x_stride, int64_t M, int6
   if (!rc) rc = check_weights(M, K, w, w_ld, w_scales, N, out);
   if (rc || M == 0) return rc;
   QK_REQUIRE(reinterpret_cast<uintptr_t>(out) % (out_dtype == QK_OUT_F32 ? 4 : 2) == 0, "misaligned out");
-  rc = check_room(workspace, workspace_bytes, room_for(in_dtype, M, K, N));
+  rc = check_room(workspace, workspace_bytes, room_for(in_dtype, M, K, N, false));
   if (rc) return rc;
   return product_of_rows(x, in_dtype, x_stride, M, K, Weights{w, w_ld, w_scales}, nullptr, N, out_dtype == QK_OUT_F32, out, 0, nullptr,
                          static_cast<uint8_t*>(workspace), as_stream(stream));
 }
 
 size_t qk_fp8_ffn_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t inner) {
-  return M > 0 && K > 0 && inner > 0 ? room_for(in_dtype, M, K, inner) + row_bytes(M, inner) : 0;
+  return M > 0 && K > 0 && inner > 0 ? room_for(in_dtype, M, K, inner, true) + row_bytes(M, inner) : 0;
 }
 
 int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const uint8_t* gate, int64_t gate_ld,
@@ -206,10 +208,10 @@ int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t
   if (!rc) rc = check_weights(M, inner, down, down_ld, down_scales, N, out);
   if (rc || M == 0) return rc;
   QK_REQUIRE((reinterpret_cast<uintptr_t>(out) & 1) == 0, "misaligned out");
-  rc = check_room(workspace, workspace_bytes, room_for(in_dtype, M, K, inner) + row_bytes(M, inner));
+  rc = check_room(workspace, workspace_bytes, room_for(in_dtype, M, K, inner, true) + row_bytes(M, inner));
   if (rc) return rc;
   cudaStream_t st = as_stream(stream);
-  uint8_t* h = static_cast<uint8_t*>(workspace) + room_for(in_dtype, M, K, inner);
+  uint8_t* h = static_cast<uint8_t*>(workspace) + room_for(in_dtype, M, K, inner, true);
   const int64_t ld = (inner + 15) / 16 * 16;
   float* h_scales = reinterpret_cast<float*>(h + (static_cast<size_t>(M) * ld + 255) / 256 * 256);
   const Weights u{up, up_ld, up_scales};

@@ -3,7 +3,7 @@
 // The weights are the M = 128 operand and MT tokens the N operand, so a tile of 128 columns of the output is 128 rows
 // of the weights. Its blocks of K are split over a cluster of CTAs, which all stream their part of the weights at
 // once; each adds its blocks' sums, times their scales, in registers (a thread per weight row and half of the
-// tokens), leaves them in shared memory, and the CTAs add up one another's in rank order and write.
+// tokens) and sends every token's to the CTA that owns it, which adds them in rank order and writes.
 // x comes as codes, by tensor copies beside the weights', or (ROWS: up to 16 rows) as BF16 that every CTA quantises
 // for itself while its weights are on their way: that saves a launch, and the values are the same.
 #pragma once
@@ -22,6 +22,7 @@ constexpr int kInlineBlocks = 16;    // and blocks of K per CTA
 struct NarrowArgs {
   int64_t M;
   int N, blocks, splits, stages;
+  uint32_t ring;          // bytes of the copies' ring and x's tiles
   const uint16_t* x;      // BF16 (ROWS), width a multiple of 8
   int64_t x_stride;
   int width;
@@ -39,47 +40,60 @@ struct Narrow {
   static constexpr int kColumns = kOperands * MT;                           // TMEM columns of a block's sums
   static constexpr int kBuffers = 256 / kColumns < 2 ? 2 : 256 / kColumns > 8 ? 8 : 256 / kColumns;
   static constexpr uint32_t kAlloc = kColumns * kBuffers < 32 ? 32 : kColumns * kBuffers;
-  static constexpr uint32_t kPartial = kOperands * MT * 128 * 4;            // a CTA's sums
   static constexpr int kEach = MT / 2;                                      // tokens per thread
-  static size_t smem(int stages, int inline_blocks) {
-    const size_t ring = stages * (inline_blocks ? kBytesW : kStage) + inline_blocks * kBytesX;
-    return 1024 + (ring > kPartial ? ring : kPartial);
+  static constexpr bool kTwo = kColumns <= 64;                              // two CTAs per SM
+  // shared memory: the ring (and x's tiles), then [CTA of the cluster][token it owns][operand][weight row] sums
+  static uint32_t ring(int stages, int inline_blocks) {
+    return stages * (inline_blocks ? kBytesW : kStage) + inline_blocks * kBytesX;
+  }
+  static size_t smem(int stages, int inline_blocks, int splits) {
+    return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits) * ((MT + splits - 1) / splits) * kOperands * 512;
   }
 };
 
 struct NarrowControl {
-  uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], x_full;
+  uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], x_full, joined;
   uint32_t tmem;
   alignas(16) float scales[kInlineBlocks * kInlineRows > kNarrowSumWarps * 2 * 64 ? kInlineBlocks * kInlineRows : kNarrowSumWarps * 2 * 64];
 };
 
-// Four floats of the shared memory of the cluster's CTA `rank`, at this CTA's address `addr`.
-__device__ __forceinline__ float4 cluster_ld4(uint32_t addr, uint32_t rank) {
-  float4 v;
-  asm volatile(
-      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [a];\n}\n"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-      : "r"(addr), "r"(rank)
-      : "memory");
-  return v;
+// The address of this CTA's `addr` in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t in_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// A store to another CTA's shared memory that counts its bytes on that CTA's barrier: no fence, no barrier of the
+// cluster. (Partial sums read from the others' shared memory between two cluster barriers, whose release waits for
+// every store of the CTA: 0.7 and 1 us of 10.)
+__device__ __forceinline__ void send(uint32_t addr, float v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar)
+               : "memory");
 }
 
 template <int MT, bool GATED, bool ROWS>
-__device__ __forceinline__ bool narrow_copies(const NarrowArgs& a, NarrowControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
-                                              const CUtensorMap* u, uint32_t smem, int b0, int b1, int tile, int row0) {
+__device__ __forceinline__ void narrow_copy(const NarrowArgs& a, NarrowControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
+                                            const CUtensorMap* u, uint32_t smem, int it, int b0, int tile, int row0) {
   using L = Narrow<MT, GATED>;
   constexpr uint32_t kStage = ROWS ? L::kBytesW : L::kStage;
+  const int s = it % a.stages, b = b0 + it;
+  const uint32_t at = smem + s * kStage;
+  mbar_expect_tx(&ctl.full[s], kStage);
+  load_box(at, w, b * kFp8Block, tile * 128, &ctl.full[s]);
+  if (GATED) load_box(at + L::kBytesW / 2, u, b * kFp8Block, tile * 128, &ctl.full[s]);
+  if (!ROWS) load_box(at + L::kBytesW, x, b * kFp8Block, row0, &ctl.full[s]);
+}
+
+// The copies behind the first a.stages.
+template <int MT, bool GATED, bool ROWS>
+__device__ __forceinline__ bool narrow_copies(const NarrowArgs& a, NarrowControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
+                                              const CUtensorMap* u, uint32_t smem, int b0, int count, int tile, int row0) {
   bool ok = true;
-  int it = 0;
-  for (int b = b0; b < b1; ++b, ++it) {
-    const int s = it % a.stages;
-    const uint32_t at = smem + s * kStage;
-    ok = mbar_wait_bounded(&ctl.empty[s], (it / a.stages & 1) ^ 1);
+  int it = min(count, a.stages);
+  for (; it < count; ++it) {
+    ok = mbar_wait_bounded(&ctl.empty[it % a.stages], (it / a.stages & 1) ^ 1);
     if (!ok) break;
-    mbar_expect_tx(&ctl.full[s], kStage);
-    load_box(at, w, b * kFp8Block, tile * 128, &ctl.full[s]);
-    if (GATED) load_box(at + L::kBytesW / 2, u, b * kFp8Block, tile * 128, &ctl.full[s]);
-    if (!ROWS) load_box(at + L::kBytesW, x, b * kFp8Block, row0, &ctl.full[s]);
+    narrow_copy<MT, GATED, ROWS>(a, ctl, x, w, u, smem, it, b0, tile, row0);
   }
   // every copy issued must have landed before the CTA leaves
   for (int i = max(it - a.stages, 0); i < it; ++i) mbar_wait_bounded(&ctl.full[i % a.stages], i / a.stages & 1);
@@ -114,15 +128,12 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
   return true;
 }
 
-// The CTA's blocks of x, quantised into the operand tiles (rows past M: zeros) and ctl.scales [block][16].
+// The CTA's blocks of x, quantised into the operand tiles and ctl.scales [block][16]. Rows past M hold whatever the
+// memory held: they make columns of the product that nobody reads.
 template <int MT>
 __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl& ctl, uint32_t tiles, int b0, int count) {
   const int t = threadIdx.x - kNarrowFirstSum * 32, lane = threadIdx.x & 31, in = lane & 15;
   const int rows = static_cast<int>(a.M);
-  for (int i = t; i < count * (MT - rows) * 8; i += kNarrowSumWarps * 32) {
-    const int unit = i / 8, b = unit / (MT - rows), row = rows + unit % (MT - rows);
-    sts_v4(tiles + b * (MT * kFp8Block) + row * kFp8Block + (i & 7) * 16, 0, 0, 0, 0);
-  }
   const int units = count * rows;
   for (int u0 = t / 32 * 2; u0 < units; u0 += kNarrowSumWarps * 2) {  // uniform in a warp
     const int unit = u0 + (lane >> 4);
@@ -146,7 +157,8 @@ __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowContr
 }
 
 template <int MT, bool GATED, bool ROWS>
-__device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int b0, int count, int tile, int row0) {
+__device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& ctl, uint32_t sums, int b0, int count, int tile, int row0,
+                                            int rank) {
   using L = Narrow<MT, GATED>;
   constexpr int kEach = L::kEach;
   const int warp = (threadIdx.x >> 5) - kNarrowFirstSum, half = warp >> 2, lane = threadIdx.x & 31;
@@ -212,36 +224,47 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& 
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl.sum_empty[d]);
   }
-  // all products are done, so nothing reads or fills the ring any more: [operand][token][weight row]
-  const uint32_t to = smem + (half * kEach * 128 + quarter * 32 + lane) * 4;
+  // to the tokens' owners
+  cluster_wait();
+  const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT)));
+  const int owned = (MT + a.splits - 1) / a.splits, first = half * kEach;
+  int owner = first % a.splits, place = first / a.splits;
 #pragma unroll
-  for (int o = 0; o < L::kOperands; ++o)
+  for (int j = 0; j < kEach; ++j) {
+    if (first + j < live) {
+      const uint32_t to = in_rank(sums, owner) + ((rank * owned + place) * L::kOperands * 128 + quarter * 32 + lane) * 4;
+      const uint32_t bar = in_rank(smem_addr(&ctl.joined), owner);
 #pragma unroll
-    for (int j = 0; j < kEach / 2; ++j) {
-      float p, q;
-      f32x2_split(acc[o][j], p, q);
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (o * MT + 2 * j) * 512), "f"(p) : "memory");
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (o * MT + 2 * j + 1) * 512), "f"(q) : "memory");
+      for (int o = 0; o < L::kOperands; ++o) {
+        float p, q;
+        f32x2_split(acc[o][j / 2], p, q);
+        send(to + o * 512, j & 1 ? q : p, bar);
+      }
     }
+    if (++owner == a.splits) owner = 0, ++place;
+  }
   return true;
 }
 
-// The cluster's sums, a warp per token and four weight rows per lane, and the output.
+// The sums of the tokens that this CTA owns, a warp per token and four weight rows per lane, and the output.
 template <int MT, bool GATED>
-__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t smem, int rank, int tile, int row0) {
+__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t sums, int rank, int tile, int row0) {
+  using L = Narrow<MT, GATED>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = tile * 128 + lane * 4;
-  const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT)));
-  for (int t = warp * a.splits + rank; t < live; t += (kNarrowThreads / 32) * a.splits) {
+  const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT))), owned = (MT + a.splits - 1) / a.splits;
+  for (int i = warp;; i += kNarrowThreads / 32) {
+    const int t = i * a.splits + rank;
+    if (t >= live) break;
     float f[2][4];
 #pragma unroll
-    for (int o = 0; o < (GATED ? 2 : 1); ++o) {
-      const uint32_t at = smem + ((o * MT + t) * 128 + lane * 4) * 4;
-      float4 s = cluster_ld4(at, 0);
-      for (int r = 1; r < a.splits; ++r) {
-        const float4 v = cluster_ld4(at, r);
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    for (int o = 0; o < L::kOperands; ++o) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[o][j] = 0.f;
+      for (int r = 0; r < a.splits; ++r) {
+        const uint4 v = lds_v4_at(sums + (((r * owned + i) * L::kOperands + o) * 128 + lane * 4) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[o][j] += __uint_as_float(word(v, j));
       }
-      f[o][0] = s.x, f[o][1] = s.y, f[o][2] = s.z, f[o][3] = s.w;
     }
     const int64_t row = row0 + t;
     if (GATED) {
@@ -274,7 +297,7 @@ __device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t smem, 
 
 // grid: (splits x tiles of 128 weight rows, tiles of MT tokens), clusters of `splits`.
 template <int MT, bool GATED, bool ROWS>
-__global__ void __launch_bounds__(kNarrowThreads, MT > 64 ? 1 : 2)
+__global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 1)
     fp8_narrow_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap w, const __grid_constant__ CUtensorMap u,
                       NarrowArgs a) {
   using L = Narrow<MT, GATED>;
@@ -285,8 +308,14 @@ __global__ void __launch_bounds__(kNarrowThreads, MT > 64 ? 1 : 2)
   const int tile = static_cast<int>(blockIdx.x) / a.splits, row0 = static_cast<int>(blockIdx.y) * MT;
   const int b0 = static_cast<int>(static_cast<int64_t>(rank) * a.blocks / a.splits);
   const int count = static_cast<int>(static_cast<int64_t>(rank + 1) * a.blocks / a.splits) - b0;  // at least one
+  const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT)));
+  const int mine = live > rank ? (live - rank + a.splits - 1) / a.splits : 0;  // tokens that this CTA owns
+  const uint32_t sums = smem + a.ring;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kNarrowStages; ++i) {
+    prefetch_map(&w);
+    if (GATED) prefetch_map(&u);
+    if (!ROWS) prefetch_map(&x);
+    for (int i = 0; i < a.stages; ++i) {
       mbar_init(&ctl.full[i], 1);
       mbar_init(&ctl.empty[i], 1);
     }
@@ -295,19 +324,28 @@ __global__ void __launch_bounds__(kNarrowThreads, MT > 64 ? 1 : 2)
       mbar_init(&ctl.sum_empty[i], kNarrowSumWarps);
     }
     mbar_init(&ctl.x_full, kNarrowSumWarps);
+    mbar_init(&ctl.joined, 1);
     fence_mbar_init();
+    mbar_expect_tx(&ctl.joined, a.splits * mine * L::kOperands * 512);
+    pdl_wait();
+    // the first copies are on their way while the others set up
+    for (int i = 0; i < min(count, a.stages); ++i) narrow_copy<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, i, b0, tile, row0);
   }
   if (warp == 1) tmem_alloc(&ctl.tmem, L::kAlloc);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  cluster_arrive_relaxed();  // this CTA's barriers are there: the others may send from now on
   pdl_wait();
   pdl_trigger();
   bool ok = true;
   if (warp == 0) {
-    if (threadIdx.x == 0) ok = narrow_copies<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, b0, b0 + count, tile, row0);
+    if (threadIdx.x == 0) ok = narrow_copies<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, b0, count, tile, row0);
+    __syncwarp();
+    cluster_wait();
   } else if (warp == 1) {
     ok = narrow_products<MT, GATED, ROWS>(a, ctl, smem, count);
+    cluster_wait();
   } else {
     if (ROWS) {
       narrow_quantise<MT>(a, ctl, smem + a.stages * L::kBytesW, b0, count);
@@ -316,26 +354,27 @@ __global__ void __launch_bounds__(kNarrowThreads, MT > 64 ? 1 : 2)
       if ((threadIdx.x & 31) == 0) mbar_arrive(&ctl.x_full);
       ok = warp_wait(&ctl.x_full, 0);  // the scales are everybody's
     }
-    if (ok) ok = narrow_sums<MT, GATED, ROWS>(a, ctl, smem, b0, count, tile, row0);
+    if (ok) ok = narrow_sums<MT, GATED, ROWS>(a, ctl, sums, b0, count, tile, row0, rank);
+    if (!ok) cluster_wait();
   }
-  if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(ctl.tmem, L::kAlloc);
   }
-  cluster_sync();
-  narrow_join<MT, GATED>(a, smem, rank, tile, row0);
-  cluster_sync();  // the others have read this CTA's sums
+  // Also a CTA that gave up stays until the others' sums are there, or they have given up too.
+  if (!warp_wait(&ctl.joined, 0)) ok = false;
+  if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
+  narrow_join<MT, GATED>(a, sums, rank, tile, row0);
 }
 
 // What a call does, by its sizes alone: `splits` CTAs of a cluster per tile, as many as two per SM leave room for.
 struct NarrowPlan {
   int tokens, splits;
-  NarrowPlan(int64_t M, int64_t N, int blocks) {
-    tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = (tokens > 64 ? 1 : 2) * sm_count() / tiles;
+  NarrowPlan(int64_t M, int64_t N, int blocks, bool gated) {
+    tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 || gated ? 64 : 128;
+    const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = (tokens * (gated ? 2 : 1) > 64 ? 1 : 2) * sm_count() / tiles;
     splits = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
     if (splits > blocks) splits = blocks;
   }
@@ -348,11 +387,13 @@ template <int MT, bool GATED, bool ROWS>
 int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, NarrowArgs a, const NarrowPlan& plan, cudaStream_t st) {
   using L = Narrow<MT, GATED>;
   const int each = plan.each(a.blocks);
-  const size_t room = MT > 64 ? 220 * 1024 : 108 * 1024;
+  const size_t room = L::kTwo ? 108 * 1024 : 220 * 1024;
+  const int tiles_of_x = ROWS ? each : 0;
   a.splits = plan.splits;
   a.stages = each < kNarrowStages ? each : kNarrowStages;
-  while (a.stages > 1 && L::smem(a.stages, ROWS ? each : 0) > room) --a.stages;
-  const size_t smem = L::smem(a.stages, ROWS ? each : 0);
+  while (a.stages > 1 && L::smem(a.stages, tiles_of_x, a.splits) > room) --a.stages;
+  a.ring = L::ring(a.stages, tiles_of_x);
+  const size_t smem = L::smem(a.stages, tiles_of_x, a.splits);
   const void* kernel = reinterpret_cast<const void*>(fp8_narrow_kernel<MT, GATED, ROWS>);
   const int rc = allow_smem(kernel, smem);
   if (rc) return rc;
@@ -379,10 +420,11 @@ template <bool GATED>
 int launch_narrow(bool rows, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const NarrowArgs& a, const NarrowPlan& plan,
                   cudaStream_t st) {
   if (rows) return launch_narrow<16, GATED, true>(x, w, u, a, plan, st);
-  return plan.tokens == 16   ? launch_narrow<16, GATED, false>(x, w, u, a, plan, st)
-         : plan.tokens == 32 ? launch_narrow<32, GATED, false>(x, w, u, a, plan, st)
-         : plan.tokens == 64 ? launch_narrow<64, GATED, false>(x, w, u, a, plan, st)
-                             : launch_narrow<128, GATED, false>(x, w, u, a, plan, st);
+  if (plan.tokens == 16) return launch_narrow<16, GATED, false>(x, w, u, a, plan, st);
+  if (plan.tokens == 32) return launch_narrow<32, GATED, false>(x, w, u, a, plan, st);
+  if constexpr (!GATED)
+    if (plan.tokens == 128) return launch_narrow<128, GATED, false>(x, w, u, a, plan, st);
+  return launch_narrow<64, GATED, false>(x, w, u, a, plan, st);
 }
 
 }  // namespace

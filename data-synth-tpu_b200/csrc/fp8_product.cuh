@@ -59,8 +59,17 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// The two halves of a cluster barrier; the first orders nothing (barriers are made visible by their own fence).
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive_relaxed();
+  cluster_wait();
 }
 
 // silu(g) u
