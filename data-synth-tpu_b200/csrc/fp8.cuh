@@ -61,8 +61,11 @@ struct Fp8Divisor {
   }
 };
 
+// most / 448, rounded to nearest: a quotient corrected by its remainder as above (an infinite one has none).
 __device__ __forceinline__ float fp8_scale(uint32_t most_bits) {
-  return __fdiv_rn(__uint_as_float(max(most_bits, kFp8LeastBits)), kFp8Most);
+  const float m = __uint_as_float(max(most_bits, kFp8LeastBits)), q = m * (1.f / kFp8Most);
+  const float r = fmaf(fmaf(-q, kFp8Most, m), 1.f / kFp8Most, q);
+  return most_bits == 0x7f800000u ? q : r;
 }
 
 // The largest of 16 lanes' (a block's: 8 values each) magnitudes, in all of them.

@@ -126,6 +126,7 @@ int product_of_rows(const void* x, int in_dtype, int64_t x_stride, int64_t M, in
     a.x = static_cast<const uint16_t*>(x);
     a.x_stride = x_stride;
     a.width = static_cast<int>(K);
+    while (1 << a.row_shift < M) ++a.row_shift;
     a.ws = w.scales;
     a.us = u ? u->scales : nullptr;
     a.out = out;

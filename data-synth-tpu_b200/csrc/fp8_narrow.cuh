@@ -25,7 +25,7 @@ struct NarrowArgs {
   uint32_t ring;          // bytes of the copies' ring and x's tiles
   const uint16_t* x;      // BF16 (ROWS), width a multiple of 8
   int64_t x_stride;
-  int width;
+  int width, row_shift;   // the power of two of rows, M or more
   const float *xs, *ws, *us;
   void* out;
   int64_t ld;             // of the gated codes
@@ -43,16 +43,19 @@ struct Narrow {
   static constexpr int kEach = MT / 2;                                      // tokens per thread
   static constexpr bool kTwo = kColumns <= 64;                              // two CTAs per SM
   // shared memory: the ring (and x's tiles), then [CTA of the cluster][token it owns][operand][weight row] sums
+  // (whose own sums go where the ring was)
+  static constexpr uint32_t kToken = kOperands * 512, kSums = MT * kToken;
   static uint32_t ring(int stages, int inline_blocks) {
-    return stages * (inline_blocks ? kBytesW : kStage) + inline_blocks * kBytesX;
+    const uint32_t bytes = stages * (inline_blocks ? kBytesW : kStage) + inline_blocks * kBytesX;
+    return bytes > kSums ? bytes : kSums;
   }
   static size_t smem(int stages, int inline_blocks, int splits) {
-    return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits) * ((MT + splits - 1) / splits) * kOperands * 512;
+    return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits) * ((MT + splits - 1) / splits) * kToken;
   }
 };
 
 struct NarrowControl {
-  uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], x_full, joined;
+  uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], x_full, stored, joined;
   uint32_t tmem;
   alignas(16) float scales[kInlineBlocks * kInlineRows > kNarrowSumWarps * 2 * 64 ? kInlineBlocks * kInlineRows : kNarrowSumWarps * 2 * 64];
 };
@@ -63,11 +66,12 @@ __device__ __forceinline__ uint32_t in_rank(uint32_t addr, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-// A store to another CTA's shared memory that counts its bytes on that CTA's barrier: no fence, no barrier of the
-// cluster. (Partial sums read from the others' shared memory between two cluster barriers, whose release waits for
-// every store of the CTA: 0.7 and 1 us of 10.)
-__device__ __forceinline__ void send(uint32_t addr, float v, uint32_t bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar)
+// A copy to another CTA's shared memory that counts its bytes on that CTA's barrier: no fence, no barrier of the
+// cluster. (Sums read from the others' shared memory between two cluster barriers, whose release waits for every
+// store of the CTA, took 0.7 and 1 us of 10; a store per value 1.3 us for 64 tokens, most of it cold instructions.)
+__device__ __forceinline__ void send(uint32_t to, uint32_t from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "r"(from),
+               "r"(bytes), "r"(bar)
                : "memory");
 }
 
@@ -105,25 +109,27 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
   using L = Narrow<MT, GATED>;
   constexpr uint32_t kStage = ROWS ? L::kBytesW : L::kStage;
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = idesc_e4m3_m128(MT);
+  const uint64_t wd0 = sdesc_sw128(smem, 1024u), xd0 = sdesc_sw128(smem + (ROWS ? a.stages * kStage : L::kBytesW), 1024u);
   if (ROWS && !warp_wait(&ctl.x_full, 0)) return false;
+  int s = 0, d = 0;
+  uint32_t full = 0, freed = 1;
   for (int it = 0; it < count; ++it) {
-    const int s = it % a.stages, d = it % L::kBuffers;
-    if (!warp_wait(&ctl.full[s], it / a.stages & 1)) return false;
-    if (!warp_wait(&ctl.sum_empty[d], (it / L::kBuffers & 1) ^ 1)) return false;
+    if (it >= L::kBuffers && !warp_wait(&ctl.sum_empty[d], freed)) return false;
+    if (!warp_wait(&ctl.full[s], full)) return false;
     tc_fence_after();
     if (elect_one()) {
-      const uint32_t at = smem + s * kStage;
-      const uint64_t wd = sdesc_sw128(at, 1024u);
-      const uint64_t xd = sdesc_sw128(ROWS ? smem + a.stages * kStage + it * L::kBytesX : at + L::kBytesW, 1024u);
+      const uint64_t wd = wd0 + s * (kStage >> 4), xd = xd0 + (ROWS ? it * (L::kBytesX >> 4) : s * (kStage >> 4));
 #pragma unroll
       for (int o = 0; o < L::kOperands; ++o)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           umma_e4m3(tm + d * L::kColumns + o * MT, wd + o * (128 * kFp8Block >> 4) + 2 * k, xd + 2 * k, idesc, k != 0);
-      umma_commit(&ctl.empty[s]);
+      if (it + a.stages < count) umma_commit(&ctl.empty[s]);
       umma_commit(&ctl.sum_full[d]);
     }
     __syncwarp();
+    if (++s == a.stages) s = 0, full ^= 1;
+    if (++d == L::kBuffers) d = 0, freed ^= 1;
   }
   return true;
 }
@@ -132,23 +138,21 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
 // memory held: they make columns of the product that nobody reads.
 template <int MT>
 __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl& ctl, uint32_t tiles, int b0, int count) {
-  const int t = threadIdx.x - kNarrowFirstSum * 32, lane = threadIdx.x & 31, in = lane & 15;
-  const int rows = static_cast<int>(a.M);
-  const int units = count * rows;
-  for (int u0 = t / 32 * 2; u0 < units; u0 += kNarrowSumWarps * 2) {  // uniform in a warp
-    const int unit = u0 + (lane >> 4);
-    const bool live = unit < units;
-    const int b = live ? unit / rows : 0, row = live ? unit - b * rows : 0;
+  const int lane = threadIdx.x & 31, in = lane & 15;
+  const int half = (threadIdx.x - kNarrowFirstSum * 32) >> 4;  // 16 half warps: a row and every 16 / rows-th block each
+  const int row = half & ((1 << a.row_shift) - 1);
+  const bool live = row < a.M;
+#pragma unroll 1
+  for (int b = half >> a.row_shift; b - (half >> a.row_shift) < count; b += 16 >> a.row_shift) {  // as often in the whole warp
     const int at = (b0 + b) * kFp8Block + in * 8;
     float f[8];
-    const uint4 v = live && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0);
-    unpack8(v, f);
+    unpack8(live && b < count && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0), f);
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) most = max(most, magnitude(f[j]));
     most = block_most(most);
     const Fp8Divisor by(most);
-    if (live) {
+    if (live && b < count) {
       const uint32_t to = tiles + b * (MT * kFp8Block) + row * kFp8Block + (((in >> 1) ^ (row & 7)) << 4) + (in & 1) * 8;
       asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to), "r"(by.codes4(f)), "r"(by.codes4(f + 4)) : "memory");
       if (in == 0) ctl.scales[b * kInlineRows + row] = fp8_scale(most);
@@ -157,8 +161,7 @@ __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowContr
 }
 
 template <int MT, bool GATED, bool ROWS>
-__device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& ctl, uint32_t sums, int b0, int count, int tile, int row0,
-                                            int rank) {
+__device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int b0, int count, int tile, int row0) {
   using L = Narrow<MT, GATED>;
   constexpr int kEach = L::kEach;
   const int warp = (threadIdx.x >> 5) - kNarrowFirstSum, half = warp >> 2, lane = threadIdx.x & 31;
@@ -224,37 +227,43 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& 
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl.sum_empty[d]);
   }
-  // to the tokens' owners
-  cluster_wait();
-  const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT)));
-  const int owned = (MT + a.splits - 1) / a.splits, first = half * kEach;
-  int owner = first % a.splits, place = first / a.splits;
+  // All products are done, so nothing reads or fills the ring any more: [token][operand][weight row] goes there.
+  const uint32_t to = smem + half * kEach * L::kToken + (quarter * 32 + lane) * 4;
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    if (first + j < live) {
-      const uint32_t to = in_rank(sums, owner) + ((rank * owned + place) * L::kOperands * 128 + quarter * 32 + lane) * 4;
-      const uint32_t bar = in_rank(smem_addr(&ctl.joined), owner);
+  for (int j = 0; j < kEach; ++j)
 #pragma unroll
-      for (int o = 0; o < L::kOperands; ++o) {
-        float p, q;
-        f32x2_split(acc[o][j / 2], p, q);
-        send(to + o * 512, j & 1 ? q : p, bar);
-      }
+    for (int o = 0; o < L::kOperands; ++o) {
+      float p, q;
+      f32x2_split(acc[o][j / 2], p, q);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + j * L::kToken + o * 512), "f"(j & 1 ? q : p) : "memory");
     }
-    if (++owner == a.splits) owner = 0, ++place;
-  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&ctl.stored);
+  return true;
+}
+
+// A warp per owner sends it its tokens.
+template <int MT, bool GATED>
+__device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int owned, int live, int rank) {
+  using L = Narrow<MT, GATED>;
+  const int owner = (threadIdx.x >> 5) - kNarrowFirstSum, tokens = min(owned, live - owner * owned);
+  if (owner >= a.splits || tokens <= 0) return true;
+  if (!warp_wait(&ctl.stored, 0)) return false;
+  if (elect_one())
+    send(in_rank(smem + a.ring + rank * owned * L::kToken, owner), smem + owner * owned * L::kToken, tokens * L::kToken,
+         in_rank(smem_addr(&ctl.joined), owner));
+  __syncwarp();
   return true;
 }
 
 // The sums of the tokens that this CTA owns, a warp per token and four weight rows per lane, and the output.
 template <int MT, bool GATED>
-__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t sums, int rank, int tile, int row0) {
+__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t sums, int owned, int mine, int64_t first, int tile) {
   using L = Narrow<MT, GATED>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = tile * 128 + lane * 4;
-  const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT))), owned = (MT + a.splits - 1) / a.splits;
-  for (int i = warp;; i += kNarrowThreads / 32) {
-    const int t = i * a.splits + rank;
-    if (t >= live) break;
+#pragma unroll 1
+  for (int i = warp; i < mine; i += kNarrowThreads / 32) {
     float f[2][4];
 #pragma unroll
     for (int o = 0; o < L::kOperands; ++o) {
@@ -266,7 +275,7 @@ __device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t sums, 
         for (int j = 0; j < 4; ++j) f[o][j] += __uint_as_float(word(v, j));
       }
     }
-    const int64_t row = row0 + t;
+    const int64_t row = first + i;
     if (GATED) {
       uint32_t most = 0;
 #pragma unroll
@@ -309,8 +318,8 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
   const int b0 = static_cast<int>(static_cast<int64_t>(rank) * a.blocks / a.splits);
   const int count = static_cast<int>(static_cast<int64_t>(rank + 1) * a.blocks / a.splits) - b0;  // at least one
   const int live = static_cast<int>(min(a.M - row0, static_cast<int64_t>(MT)));
-  const int mine = live > rank ? (live - rank + a.splits - 1) / a.splits : 0;  // tokens that this CTA owns
-  const uint32_t sums = smem + a.ring;
+  // the tokens that a CTA owns, in their order
+  const int owned = (live + a.splits - 1) / a.splits, mine = min(max(live - rank * owned, 0), owned);
   if (threadIdx.x == 0) {
     prefetch_map(&w);
     if (GATED) prefetch_map(&u);
@@ -324,9 +333,10 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
       mbar_init(&ctl.sum_empty[i], kNarrowSumWarps);
     }
     mbar_init(&ctl.x_full, kNarrowSumWarps);
+    mbar_init(&ctl.stored, kNarrowSumWarps);
     mbar_init(&ctl.joined, 1);
     fence_mbar_init();
-    mbar_expect_tx(&ctl.joined, a.splits * mine * L::kOperands * 512);
+    mbar_expect_tx(&ctl.joined, a.splits * mine * L::kToken);
     pdl_wait();
     // the first copies are on their way while the others set up
     for (int i = 0; i < min(count, a.stages); ++i) narrow_copy<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, i, b0, tile, row0);
@@ -354,8 +364,10 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
       if ((threadIdx.x & 31) == 0) mbar_arrive(&ctl.x_full);
       ok = warp_wait(&ctl.x_full, 0);  // the scales are everybody's
     }
-    if (ok) ok = narrow_sums<MT, GATED, ROWS>(a, ctl, sums, b0, count, tile, row0, rank);
-    if (!ok) cluster_wait();
+    if (ok) ok = narrow_sums<MT, GATED, ROWS>(a, ctl, smem, b0, count, tile, row0);
+    __syncwarp();
+    cluster_wait();
+    if (ok) ok = narrow_send<MT, GATED>(a, ctl, smem, owned, live, rank);
   }
   tc_fence_before();
   __syncthreads();
@@ -363,10 +375,12 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
     tc_fence_after();
     tmem_dealloc(ctl.tmem, L::kAlloc);
   }
-  // Also a CTA that gave up stays until the others' sums are there, or they have given up too.
   if (!warp_wait(&ctl.joined, 0)) ok = false;
   if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
-  narrow_join<MT, GATED>(a, sums, rank, tile, row0);
+  cluster_arrive_relaxed();  // what the others sent has been read from their memory
+  narrow_join<MT, GATED>(a, smem + a.ring, owned, mine, row0 + static_cast<int64_t>(rank) * owned, tile);
+  __syncwarp();
+  cluster_wait();
 }
 
 // What a call does, by its sizes alone: `splits` CTAs of a cluster per tile, as many as two per SM leave room for.

@@ -113,29 +113,27 @@ __device__ __forceinline__ bool wide_copies(const WideArgs& a, WideControl& ctl,
   return ok;
 }
 
-// The leader's MMA warp.
-__device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ctl, uint32_t smem) {
-  // kind::f8f6f4, e4m3 A and B, both K-major, FP32 D, M = 256, N = 128
-  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = (1u << 4) | (128 >> 3) << 17 | (kTileM >> 4) << 24;
-  uint32_t it = 0;
+// The leader's MMA warps, one for each half of the columns.
+__device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ctl, uint32_t smem, const int h) {
+  constexpr uint32_t idesc = (1u << 4) | (128 >> 3) << 17 | (kTileM >> 4) << 24;
+  const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
+  const uint64_t ad0 = sdesc_sw128(smem, 1024u), bd0 = sdesc_sw128(smem + kBytesA + h * (kBytesA / 2), 1024u);
+  uint32_t s = 0, full = 0, d = 0, freed = 1;
   for (int t = blockIdx.x / 2; t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
-    for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t s = it % kStages, d = it % kBuffers;
-      const uint64_t ad = sdesc_sw128(smem + s * kStageBytes, 1024u), bd = sdesc_sw128(smem + s * kStageBytes + kBytesA, 1024u);
+    for (int b = 0; b < a.blocks; ++b) {
+      if (!warp_wait(&ctl.sum_empty[d][h], freed)) return false;
+      if (!warp_wait(&ctl.full[s], full)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t ad = ad0 + s * (kStageBytes >> 4), bd = bd0 + s * (kStageBytes >> 4);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (!warp_wait(&ctl.sum_empty[d][h], (it / kBuffers & 1) ^ 1)) return false;
-        if (h == 0 && !warp_wait(&ctl.full[s], it / kStages & 1)) return false;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_e4m3_pair(tm + d * kTileN + h * 128, ad + 2 * k, bd + h * (kBytesA / 2 >> 4) + 2 * k, idesc, k != 0);
-          if (h) umma_commit_pair(&ctl.empty[s]);
-          umma_commit_pair(&ctl.sum_full[d][h]);
-        }
-        __syncwarp();
+        for (int k = 0; k < 4; ++k) umma_e4m3_pair(tm + d * kTileN + h * 128, ad + 2 * k, bd + 2 * k, idesc, k != 0);
+        umma_commit_pair(&ctl.empty[s]);
+        umma_commit_pair(&ctl.sum_full[d][h]);
       }
+      __syncwarp();
+      if (++s == kStages) s = 0, full ^= 1;
+      if (++d == kBuffers) d = 0, freed ^= 1;
     }
   }
   return true;
@@ -300,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&ctl.full[i], 1);
-      mbar_init(&ctl.empty[i], 1);
+      mbar_init(&ctl.empty[i], 2);
     }
     for (int i = 0; i < kBuffers; ++i) {
       for (int h = 0; h < 2; ++h) {
@@ -332,7 +330,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     if (warp == 0) {
       if (threadIdx.x == 0) ok = wide_copies<GATED>(a, ctl, &x, &w, &u, smem, rank);
     } else if (warp == 1 && rank == 0) {
-      ok = wide_products(a, ctl, smem);
+      ok = wide_products(a, ctl, smem, 0);
+    } else if (warp == 2 && rank == 0) {
+      ok = wide_products(a, ctl, smem, 1);
     }
   }
   if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
