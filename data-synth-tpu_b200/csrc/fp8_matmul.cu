@@ -37,10 +37,10 @@ int check_rows(const void* x, int in_dtype, int64_t stride, int64_t M, int64_t K
   return QK_OK;
 }
 
-// Rows of x from which the wide form is used.
-constexpr int64_t kMostNarrow = 128;
-
-bool narrow(int64_t M) { return M <= kMostNarrow; }
+// The narrow form is used for up to 128 rows, and for more where its tiles of 128 x 128 are so few that their blocks of K
+// are split: K 4096, N 2048 takes 10.7 us for 256 rows and 15.0 for 512 (the wide form 16.6 for both), but K 2048,
+// N 9216 15.1 for 192 (11.1). For 128 rows they take 11.6 and 11.1 of that, of K 8192, N 8192 25 and 31.
+bool narrow(int64_t M, int64_t N) { return M <= 128 || ((M + 127) / 128) * ((N + 127) / 128) <= sm_count() / 2; }
 
 // Half of a feed-forward block (u not NULL, codes out) or a product (u NULL) of codes.
 struct Weights {
@@ -55,7 +55,7 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
   const bool vectors = !u && aligned16(out) && N * (f32 ? 4 : 2) % 16 == 0;
   CUtensorMap xm, wm, um;
   bool ok;
-  if (narrow(M)) {
+  if (narrow(M, N)) {
     const NarrowPlan plan(M, N, blocks, u != nullptr);
     ok = encode(&xm, x, M, K, x_ld, plan.tokens) && encode(&wm, w.codes, N, K, w.ld, 128) && (!u || encode(&um, u->codes, N, K, u->ld, 128));
     if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");

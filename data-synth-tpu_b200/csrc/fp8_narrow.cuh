@@ -4,8 +4,8 @@
 // of the weights. Its blocks of K are split over a cluster of CTAs, which all stream their part of the weights at
 // once; each adds its blocks' sums, times their scales, in registers (a thread per weight row and half of the
 // tokens) and sends every token's to the CTA that owns it, which adds them in rank order and writes.
-// x comes as codes, by tensor copies beside the weights', or (ROWS: up to 16 rows) as BF16 that every CTA quantises
-// for itself while its weights are on their way: that saves a launch, and the values are the same.
+// x comes as codes, by tensor copies beside the weights', or (ROWS) as BF16 that every CTA quantises for itself while
+// its weights are on their way: that saves a launch, and the values are the same.
 #pragma once
 
 #include "fp8_product.cuh"
@@ -13,11 +13,11 @@
 namespace qk {
 namespace {
 
-constexpr int kNarrowStages = 5, kNarrowSumWarps = 8, kNarrowFirstSum = 2;
+constexpr int kNarrowStages = 8, kNarrowSumWarps = 8, kNarrowFirstSum = 2;
 constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
 constexpr int kMostSplits = 8;       // the portable cluster size
-constexpr int kInlineRows = 16;      // rows of BF16 that the CTAs quantise themselves
-constexpr int kInlineBlocks = 16;    // and blocks of K per CTA
+// Blocks of rows of BF16 that a CTA quantises itself, at most. A half warp takes about 0.6 us for one, all latency.
+constexpr int kInlineRows = 16, kInline = 64;
 
 struct NarrowArgs {
   int64_t M;
@@ -41,7 +41,7 @@ struct Narrow {
   static constexpr int kBuffers = 256 / kColumns < 2 ? 2 : 256 / kColumns > 8 ? 8 : 256 / kColumns;
   static constexpr uint32_t kAlloc = kColumns * kBuffers < 32 ? 32 : kColumns * kBuffers;
   static constexpr int kEach = MT / 2;                                      // tokens per thread
-  static constexpr bool kTwo = kColumns <= 64;                              // two CTAs per SM
+  static constexpr bool kTwo = kColumns <= 64;                              // room for two CTAs per SM
   // shared memory: the ring (and x's tiles), then [CTA of the cluster][token it owns][operand][weight row] sums
   // (whose own sums go where the ring was)
   static constexpr uint32_t kToken = kOperands * 512, kSums = MT * kToken;
@@ -57,7 +57,7 @@ struct Narrow {
 struct NarrowControl {
   uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], x_full, stored, joined;
   uint32_t tmem;
-  alignas(16) float scales[kInlineBlocks * kInlineRows > kNarrowSumWarps * 2 * 64 ? kInlineBlocks * kInlineRows : kNarrowSumWarps * 2 * 64];
+  alignas(16) float scales[kNarrowSumWarps * 2 * 64];  // of x: a warp's two slots of 64 tokens, or (ROWS) [block][MT]
 };
 
 // The address of this CTA's `addr` in the cluster's CTA `rank`.
@@ -134,28 +134,29 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
   return true;
 }
 
-// The CTA's blocks of x, quantised into the operand tiles and ctl.scales [block][16]. Rows past M hold whatever the
+// The CTA's blocks of x, quantised into the operand tiles and ctl.scales [block][MT]. Rows past M hold whatever the
 // memory held: they make columns of the product that nobody reads.
 template <int MT>
 __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl& ctl, uint32_t tiles, int b0, int count) {
   const int lane = threadIdx.x & 31, in = lane & 15;
-  const int half = (threadIdx.x - kNarrowFirstSum * 32) >> 4;  // 16 half warps: a row and every 16 / rows-th block each
-  const int row = half & ((1 << a.row_shift) - 1);
-  const bool live = row < a.M;
+  // 16 half warps: each takes every 16th of (block, row) pairs
+  const int half = (threadIdx.x - kNarrowFirstSum * 32) >> 4, units = count << a.row_shift;
 #pragma unroll 1
-  for (int b = half >> a.row_shift; b - (half >> a.row_shift) < count; b += 16 >> a.row_shift) {  // as often in the whole warp
+  for (int first = half & ~1; first < units; first += 16) {  // as often in the whole warp
+    const int unit = first + (half & 1), row = unit & ((1 << a.row_shift) - 1), b = unit >> a.row_shift;
     const int at = (b0 + b) * kFp8Block + in * 8;
+    const bool live = row < a.M && b < count;
     float f[8];
-    unpack8(live && b < count && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0), f);
+    unpack8(live && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0), f);
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) most = max(most, magnitude(f[j]));
     most = block_most(most);
     const Fp8Divisor by(most);
-    if (live && b < count) {
+    if (live) {
       const uint32_t to = tiles + b * (MT * kFp8Block) + row * kFp8Block + (((in >> 1) ^ (row & 7)) << 4) + (in & 1) * 8;
       asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to), "r"(by.codes4(f)), "r"(by.codes4(f + 4)) : "memory");
-      if (in == 0) ctl.scales[b * kInlineRows + row] = fp8_scale(most);
+      if (in == 0) ctl.scales[b * MT + row] = fp8_scale(most);
     }
   }
 }
@@ -188,7 +189,7 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& 
   float w = ws[0], u = GATED ? us[0] : 0.f;
   for (int it = 0; it < count; ++it) {
     const int d = it % L::kBuffers;
-    const float* scales = ctl.scales + it * kInlineRows + half * kEach;
+    const float* scales = ctl.scales + it * MT + half * kEach;
     if (!ROWS) {
       float* slot = slots + (it & 1) * 64;
 #pragma unroll
@@ -383,18 +384,23 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
   cluster_wait();
 }
 
-// What a call does, by its sizes alone: `splits` CTAs of a cluster per tile, as many as two per SM leave room for.
+// What a call does, by its sizes alone: a cluster's CTAs share a tile's blocks of K, as many as give every SM one CTA
+// at most (one row of 2048 x 9216, 72 tiles: 1 / 2 / 3 / 4 CTAs take 7.4 / 5.9 / 6.3 / 8.4 us, of 4096 x 2048, 16
+// tiles: 4 / 6 / 8 take 4.8 / 4.7 / 4.4). A cluster lies within a group of SMs: of 4 there is room for 33 where a CTA
+// takes an SM for itself, of 8 for 15, and one cluster too many costs a second round (64 rows of 4096 x 2048 with
+// eight: 7.2 us where two fit an SM, 11.1 else). So all but the largest leave room for a second, and those have four.
 struct NarrowPlan {
   int tokens, splits;
   NarrowPlan(int64_t M, int64_t N, int blocks, bool gated) {
     tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 || gated ? 64 : 128;
-    const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = (tokens * (gated ? 2 : 1) > 64 ? 1 : 2) * sm_count() / tiles;
+    const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = sm_count() / tiles;
     splits = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
+    if (tokens * (gated ? 2 : 1) > 64) splits = tiles * 4 <= sm_count() * 7 / 8 ? 4 : splits > 2 ? 2 : splits;
     if (splits > blocks) splits = blocks;
   }
   int each(int blocks) const { return (blocks + splits - 1) / splits; }
   // Whether the CTAs can quantise rows of x themselves.
-  bool quantises(int64_t M, int blocks) const { return M <= kInlineRows && each(blocks) <= kInlineBlocks; }
+  bool quantises(int64_t M, int blocks) const { return M <= kInlineRows && M * each(blocks) <= kInline; }
 };
 
 template <int MT, bool GATED, bool ROWS>

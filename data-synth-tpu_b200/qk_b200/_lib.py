@@ -245,27 +245,34 @@ def stream_handle(device=None):
 
 
 _bound = {}  # name -> entry point
-_cuda = None  # torch._C, once there is a CUDA tensor to call for
+_cuda = None  # torch._C, once CUDA is in use
 
 
 def call_on(device, name, *args):
     """``name(*args, stream)`` with ``device`` current, on its current stream: for entry points that
     take plain addresses (``Tensor.data_ptr()`` or None) and the stream last. Leaner than a device
     guard and stream object of its own: a decode step makes many calls of a few microseconds."""
-    global _cuda
     if device.type != "cuda":
         raise ValueError("expected CUDA tensors")
-    if _cuda is None:
+    index = device.index
+    if index is None:
+        import torch
+
+        index = torch.cuda.current_device()
+    call_at(index, name, *args)
+
+
+def call_at(index, name, *args):
+    """:func:`call_on` for the device of number ``index`` (``Tensor.get_device()``)."""
+    global _cuda
+    fn = _bound.get(name)
+    if fn is None:
         import torch
 
         torch.cuda.current_device()  # initialises CUDA
         _cuda = torch._C
-    current = _cuda._cuda_getDevice()
-    index = current if device.index is None else device.index
-    fn = _bound.get(name)
-    if fn is None:
         fn = _bound[name] = getattr(load(), name)
-    if current == index:
+    if _cuda._cuda_getDevice() == index:
         status = fn(*args, _cuda._cuda_getCurrentRawStream(index))
     else:
         import torch
