@@ -17,6 +17,9 @@ math.py:277-284 and the routed FFN, engine.py:193-204), with a plain pre-norm re
     ids, w += (shared, sigmoid(h2 . w_shared_router))            (qk_append_shared_route)
     x  = x + experts(h2, ids, w)                                (qk_moe_forward, routed + shared)
 
+With ``dense="fp8"`` the attention projections are FP8 with a scale for each block of 128: the attention
+norm leaves as codes (qk_fp8_rms_norm) for qk_fp8_matmul, and o goes through qk_fp8_linear.
+
 Every step of a layer is one launch (the MoE call is five), the whole step is captured in a
 CUDA graph, and nothing is allocated per step. Weights are synthetic: BF16 projections
 N(0, 0.02), FP32 router N(0, 0.02), and expert blocks of random code bytes with one FP16
@@ -34,6 +37,7 @@ import torch
 
 from . import _lib
 from .attention_cache import CacheConfig
+from .fp8 import Fp8Weights, pack_fp8
 from .parallel import expert_shape, put_expert_bytes
 from .quant import BLOCK_LAYOUTS, GGML_TYPE, normalize_qtype
 
@@ -69,6 +73,7 @@ class StackConfig:
     down_qtype: str | None = None  # None: the same as qtype; "Q8_0": the checkpoints' type mix
     context: int = 8192
     page: int = 256
+    dense: str = "bf16"  # the attention projections' weights: "bf16", or "fp8" in blocks of 128 x 128
 
 
 # FP16 block-scale bytes inside one raw block and the scale giving a ~0.02 value spread:
@@ -104,6 +109,8 @@ class LayerWeights:
 
         self.w_qkv = normal((2 * hq * hd + 2 * kv * hd, H))
         self.w_o = normal((H, hq * hd))
+        if cfg.dense == "fp8":
+            self.w_qkv, self.w_o = pack_fp8(self.w_qkv), pack_fp8(self.w_o)
         self.attn_norm = torch.ones(H, dtype=torch.bfloat16, device=device)
         self.ffn_norm = torch.ones(H, dtype=torch.bfloat16, device=device)
         self.q_norm = torch.ones(hd, dtype=torch.bfloat16, device=device)
@@ -123,7 +130,39 @@ class LayerWeights:
         return sum(t.numel() for t in self.experts.values()) // self.experts["gate"].shape[0]
 
     def dense_bytes(self):
-        return sum(t.numel() * t.element_size() for t in (self.w_qkv, self.w_o, self.router, self.shared_router))
+        projections = [t for w in (self.w_qkv, self.w_o) for t in (w if isinstance(w, Fp8Weights) else (w,))]
+        return sum(t.numel() * t.element_size() for t in (*projections, self.router, self.shared_router))
+
+
+class Fp8Projections:
+    """The attention projections of ``rows`` rows with FP8 weights, and the buffers between them."""
+
+    def __init__(self, cfg, rows, device):
+        H, wide = cfg.hidden, cfg.query_heads * cfg.head_dim
+        self.rows, self.hidden, self.wide, self.eps = rows, H, wide, cfg.eps
+        self.codes = torch.empty((rows, (H + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)
+        self.scales = torch.empty(((H + 127) // 128, rows), dtype=torch.float32, device=device)
+        with torch.cuda.device(device):
+            self.room = int(_lib.load().qk_fp8_linear_workspace_bytes(_lib.QK_OUT_BF16, rows, wide, H))
+        self.ws = torch.empty(max(self.room, 16), dtype=torch.uint8, device=device)
+
+    def norm(self, x, y, gamma, st):
+        """``x += y`` (None: nothing), and its norm as codes."""
+        P = _lib.ptr
+        _lib.check(_lib.load().qk_fp8_rms_norm(P(x), P(y), P(gamma), self.rows, self.hidden, self.eps, P(x), P(self.codes),
+                                               self.codes.stride(0), P(self.scales), st))
+
+    def qkv(self, w, out, st):
+        P = _lib.ptr
+        _lib.check(_lib.load().qk_fp8_matmul(P(self.codes), self.codes.stride(0), P(self.scales), self.rows, self.hidden,
+                                             P(w.codes), w.codes.stride(0), P(w.scales), w.codes.shape[0], _lib.QK_OUT_BF16,
+                                             P(out), st))
+
+    def out(self, o, w, out, st):
+        P = _lib.ptr
+        _lib.check(_lib.load().qk_fp8_linear(P(o), _lib.QK_OUT_BF16, self.wide, self.rows, self.wide, P(w.codes),
+                                             w.codes.stride(0), P(w.scales), self.hidden, _lib.QK_OUT_BF16, P(out), P(self.ws),
+                                             self.room, st))
 
 
 class SyntheticDecoder:
@@ -136,6 +175,8 @@ class SyntheticDecoder:
     graph-capturable)."""
 
     def __init__(self, cfg, device, seed=1, group=None):
+        if cfg.dense not in ("bf16", "fp8"):
+            raise ValueError("dense must be bf16 or fp8")
         self.cfg = cfg
         self.device = torch.device(device)
         self.group = group
@@ -177,7 +218,7 @@ class DecodeState:
 
     def __init__(self, model, batch, seed, global_batch=None):
         cfg, dev = model.cfg, model.device
-        self.model, self.batch = model, batch
+        self.model, self.batch, self.fp8 = model, batch, None
         self.global_batch = batch if global_batch is None else global_batch
         H, hq, kv, hd, T = cfg.hidden, cfg.query_heads, cfg.kv_heads, cfg.head_dim, cfg.context
         g = torch.Generator(device=dev).manual_seed(seed)
@@ -212,8 +253,10 @@ class DecodeState:
         self.logits = torch.empty((batch, cfg.experts), dtype=torch.float32, device=dev)
         # the attention projections: this library's tcgen05 pass up to 256 rows, a library GEMM
         # beyond (their zeroed workspaces are reused by every call)
-        self.own_linear = batch <= 256
-        if self.own_linear:
+        self.own_linear = batch <= 256 and cfg.dense == "bf16"
+        if cfg.dense == "fp8":
+            self.fp8 = Fp8Projections(cfg, batch, dev)
+        elif self.own_linear:
             from .packed import linear_workspace
 
             self.lin_qkv = (self.qkv.shape[1], linear_workspace(batch, H, self.qkv.shape[1], dev))
@@ -244,10 +287,15 @@ class DecodeState:
         T = cfg.context
         nl = len(m.layers)
         # the first layer's attention norm; every later one runs with the residual add before it
-        _lib.check(lib.qk_rms_norm(P(self.x), P(m.layers[0].attn_norm), B, H, cfg.eps, P(self.h), st))
+        if self.fp8:
+            self.fp8.norm(self.x, None, m.layers[0].attn_norm, st)
+        else:
+            _lib.check(lib.qk_rms_norm(P(self.x), P(m.layers[0].attn_norm), B, H, cfg.eps, P(self.h), st))
         for li, L in enumerate(m.layers):
             cache = self.caches[li]
-            if self.own_linear:
+            if self.fp8:
+                self.fp8.qkv(L.w_qkv, self.qkv, st)
+            elif self.own_linear:
                 n, ws = self.lin_qkv
                 _lib.check(lib.qk_linear_bf16(P(self.h), B, H, P(L.w_qkv), n, P(self.qkv), P(ws), ws.numel(), st))
             else:
@@ -262,7 +310,9 @@ class DecodeState:
                 P(self.q), P(cache["k"]), P(cache["v"]), P(cache["k_scale"]), P(cache["v_scale"]), P(self.indices),
                 None, P(self.positions), P(self.gate), B, T, T, hq, kv, hd, P(self.o),
                 P(self.attn_ws) if self.attn_ws_bytes else None, self.attn_ws_bytes, st))
-            if self.own_linear:
+            if self.fp8:
+                self.fp8.out(self.o, L.w_o, self.a, st)
+            elif self.own_linear:
                 n, ws = self.lin_o
                 _lib.check(lib.qk_linear_bf16(P(self.o), B, hq * hd, P(L.w_o), n, P(self.a), P(ws), ws.numel(), st))
             else:
@@ -286,7 +336,9 @@ class DecodeState:
             else:
                 self.ep(L.experts["gate"], L.experts["up"], L.experts["down"], self.h, ids_all, self.w_all,
                         out=self.y)
-            if li + 1 < nl:  # the residual add and the next layer's attention norm
+            if li + 1 < nl and self.fp8:
+                self.fp8.norm(self.x, self.y, m.layers[li + 1].attn_norm, st)
+            elif li + 1 < nl:  # the residual add and the next layer's attention norm
                 _lib.check(lib.qk_residual_rms_norm(P(self.x), P(self.y), P(m.layers[li + 1].attn_norm), B, H,
                                                     cfg.eps, P(self.x), P(self.h), st))
             else:
@@ -302,8 +354,10 @@ class DecodeState:
         # library GEMMs above 256 rows)
         attn = 2 if self.attn_ws_bytes else 1
         moe = 5 if self.ep is None else 8
-        own = 2 if self.own_linear else 0
-        return self.model.cfg.layers * (6 + attn + moe + own) + 1, self.model.cfg.layers * (2 - own)
+        own, gemms = (2, 0) if self.own_linear else (0, 2)
+        if self.fp8:  # quantisation of the attention's output where the product does not do it
+            own, gemms = 3 if self.fp8.room else 2, 0
+        return self.model.cfg.layers * (6 + attn + moe + own) + 1, self.model.cfg.layers * gemms
 
     def close(self):
         if self.ep is not None:

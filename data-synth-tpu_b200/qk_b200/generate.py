@@ -7,7 +7,7 @@ share of the expert-parallel model):
 
 * **Prefill** (``engine.py:449-500`` ``forward_chunk``): the whole prompt of every sequence
   is one chunk of ``batch * prompt`` tokens. Per layer: RMSNorm, the q | gate, k, v
-  projection (cuBLAS), per-head q/k RMSNorm and rotary at each token's position
+  projection (cuBLAS; with ``dense="fp8"`` qk_fp8_rms_norm and qk_fp8_matmul), per-head q/k RMSNorm and rotary at each token's position
   (``qk_qk_norm_rope``), the chunk's keys and values quantised into the Q8 cache
   (``qk_kv_q8_append_chunk``), causal attention of the chunk over the dequantised cache
   (``qk_kv_q8_read`` feeding PyTorch's fused attention; the cache's own keys and values, as
@@ -31,7 +31,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .decoder import checked_argmax
+from .decoder import Fp8Projections, checked_argmax
 
 
 class StaticGeneration:
@@ -90,6 +90,7 @@ class StaticGeneration:
         read_idx = torch.arange(W, dtype=torch.int32, device=dev).expand(B, W).contiguous()
         kd = torch.empty((B, W, kv * hd), **bf)
         vd = torch.empty((B, W, kv * hd), **bf)
+        fp8 = Fp8Projections(cfg, n, dev) if cfg.dense == "fp8" else None
         if m.world == 1:
             need = int(lib.qk_moe_workspace_bytes(m.desc, n))
             ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
@@ -103,8 +104,12 @@ class StaticGeneration:
                                                   device=dev)
         for li, L in enumerate(m.layers):
             cache = st.caches[li]
-            _lib.check(lib.qk_rms_norm(P(x), P(L.attn_norm), n, H, cfg.eps, P(h), s))
-            torch.matmul(h, L.w_qkv.t(), out=qkv)
+            if fp8:
+                fp8.norm(x, None, L.attn_norm, s)
+                fp8.qkv(L.w_qkv, qkv, s)
+            else:
+                _lib.check(lib.qk_rms_norm(P(x), P(L.attn_norm), n, H, cfg.eps, P(h), s))
+                torch.matmul(h, L.w_qkv.t(), out=qkv)
             _lib.check(lib.qk_qk_norm_rope(P(qkv), P(L.q_norm), P(L.k_norm), P(m.inv_freq), P(positions), n, hq, kv,
                                            hd, cfg.rotary_dim, cfg.eps, P(q), P(gate), P(k), P(v), s))
             _lib.check(lib.qk_kv_q8_append_chunk(P(k), P(v), _lib.QK_OUT_BF16, P(start), None, P(cache["k"]),
@@ -122,7 +127,10 @@ class StaticGeneration:
             o = torch.nn.functional.scaled_dot_product_attention(qh, kh, vh, is_causal=True)
             del kh, vh
             o = o.transpose(1, 2).reshape(n, hq, hd) * torch.sigmoid(gate)
-            torch.matmul(o.reshape(n, hq * hd), L.w_o.t(), out=a)
+            if fp8:
+                fp8.out(o, L.w_o, a, s)
+            else:
+                torch.matmul(o.reshape(n, hq * hd), L.w_o.t(), out=a)
             _lib.check(lib.qk_residual_add(P(x), P(a), n * H, P(x), s))
             _lib.check(lib.qk_rms_norm(P(x), P(L.ffn_norm), n, H, cfg.eps, P(h), s))
             _lib.check(lib.qk_router_topk(P(h), P(L.router), None, n, H, cfg.experts, cfg.top_k, P(ids), P(w), None,

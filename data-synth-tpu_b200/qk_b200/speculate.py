@@ -20,6 +20,7 @@ import torch
 
 from . import _lib
 from .decoder import checked_argmax
+from .fp8 import Fp8Weights, fp8_matmul
 from .packed import linear_bf16, linear_workspace
 from .paged import empty_pool, empty_tables, plan_step, tree_attention, write_slots
 from .sampling import process_logits
@@ -104,6 +105,8 @@ class SpeculativeGeneration:
                                   device=dev)
 
     def _linear(self, x, w, out):
+        if isinstance(w, Fp8Weights):
+            return fp8_matmul(x, w, out=out)
         if x.shape[0] > 256:  # a library product beyond the decode batches of the tcgen05 pass
             return torch.matmul(x, w.t(), out=out)
         key = tuple(w.shape)

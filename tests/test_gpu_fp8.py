@@ -264,3 +264,100 @@ def test_gated(cuda_device, m, k, inner):
     assert torch.equal(out, fp8_matmul(got, down))
     check_status(cuda_device)
     check_product(out, value, weight_values(down), 2.0 ** -8)
+
+
+# ---- together, and as the decoder uses them ----------------------------------------------------
+
+
+def test_a_layer_of_fp8_operators_matches_its_parts(cuda_device):
+    """Norm, projection, residual norm and feed-forward one behind another, as a dense layer runs them:
+    each operator's output is checked against 64 bits from the operator's own input."""
+    import torch
+
+    from qk_b200.fp8 import check_status, fp8_matmul, gated_ffn_fp8, gated_fp8, rms_norm_fp8
+
+    rows, hidden, inner = 24, 512, 640
+    x = activations(rows, hidden, cuda_device, 7)
+    gamma = (1 + 0.1 * torch.randn(hidden, device=cuda_device)).to(torch.bfloat16)
+    w, gate, up = packed(hidden, hidden, cuda_device), packed(inner, hidden, cuda_device, 2), packed(inner, hidden, cuda_device, 3)
+    down = packed(hidden, inner, cuda_device, 4)
+    h, _ = rms_norm_fp8(x, gamma)
+    y = fp8_matmul(h, w)
+    check_product(y, values(h)[0], weight_values(w), 2.0 ** -8)
+    h, x1 = rms_norm_fp8(x, gamma, residual=y)
+    assert torch.equal(x1, (x.float() + y.float()).to(torch.bfloat16))
+    out = gated_ffn_fp8(h, gate, up, down)
+    check_product(out, values(gated_fp8(h, gate, up))[0], weight_values(down), 2.0 ** -8)
+    check_status(cuda_device)
+
+
+def decoder_of(device, dense):
+    from qk_b200.decoder import StackConfig, SyntheticDecoder
+
+    return SyntheticDecoder(StackConfig(layers=2, experts=16, top_k=2, qtype="Q4_K", context=96, dense=dense), device, seed=5)
+
+
+@pytest.mark.parametrize("batch", [1, 3, 40])
+def test_decode_step_with_fp8_projections(cuda_device, batch):
+    """The step's projections are the products of its own inputs, and a captured step gives the eager one's bits."""
+    import torch
+
+    model = decoder_of(cuda_device, "fp8")
+    state = model.state(batch, seed=2)
+    x0 = state.x.clone()
+    state.step()
+    eager = state.x.clone()
+    L = model.layers[-1]
+    codes = to_f32(state.fp8.codes).astype(np.float64)
+    h = codes * spread(to_f32(state.fp8.scales).astype(np.float64).T, codes.shape[1])
+    check_product(state.qkv, h, weight_values(L.w_qkv), 2.0 ** -8)
+    o = to_f32(state.o).reshape(batch, -1).astype(np.float64)
+    oc, os = quantized(o)
+    check_product(state.a, oc * spread(os.astype(np.float32).astype(np.float64), o.shape[1]), weight_values(L.w_o), 2.0 ** -8)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize(cuda_device)
+    with torch.cuda.graph(graph):
+        state.step()
+    state.x.copy_(x0)
+    graph.replay()
+    torch.cuda.synchronize(cuda_device)
+    assert torch.equal(state.x.view(torch.int16), eager.view(torch.int16))
+
+
+def test_prefill_with_fp8_projections_matches_steps(cuda_device):
+    """As for BF16 projections: one pass over the prompt and token by token agree."""
+    import torch
+
+    from qk_b200.generate import StaticGeneration
+
+    model = decoder_of(cuda_device, "fp8")
+    batch, prompt = 3, 64
+    gen = StaticGeneration(model, batch, prompt, 8, vocab=1000, seed=1)
+    gen.prefill()
+    ref = StaticGeneration(model, batch, prompt, 8, vocab=1000, seed=1)
+    for t in range(prompt):
+        ref.state.x.copy_(ref.embedding.index_select(0, ref.prompt_ids[:, t]))
+        ref.state.positions.fill_(t)
+        ref.state.step()
+    ref._choose(0)
+    torch.cuda.synchronize(cuda_device)
+    a, b = to_f32(gen.logits), to_f32(ref.logits)
+    # a code of 4 bits may go the other way for a last bit of its input: twice the room of BF16 projections
+    assert np.abs(a - b).max() < 0.1 * np.abs(b).max()
+    out = gen.decode().cpu().numpy()
+    assert out.min() >= 0 and out.max() < 1000 and int(gen.nonfinite.item()) == 0
+    gen.close()
+    ref.close()
+
+
+def test_speculative_generation_with_fp8_projections(cuda_device):
+    from qk_b200.speculate import SpeculativeGeneration
+
+    model = decoder_of(cuda_device, "fp8")
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, 600, n).tolist() for n in (5, 17)]
+    gen = SpeculativeGeneration(model, 2, 64, nodes=4, page_size=16, vocab=600)
+    gen.prefill(prompts)
+    rows = gen.generate(6)
+    for row, prompt in zip(rows, prompts):
+        assert row[:len(prompt)] == prompt and len(row) > len(prompt) + 5 and all(0 <= t < 600 for t in row)
