@@ -415,7 +415,7 @@ int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap&
   a.ring = L::ring(a.stages, tiles_of_x);
   const size_t smem = L::smem(a.stages, tiles_of_x, a.splits);
   const void* kernel = reinterpret_cast<const void*>(fp8_narrow_kernel<MT, GATED, ROWS>);
-  const int rc = allow_smem(kernel, smem);
+  const int rc = allow_smem(kernel, smem > 64 * 1024 ? smem : 64 * 1024);  // with the static part, 48 KB are soon passed
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(plan.splits * ((a.N + 127) / 128)), static_cast<unsigned>((a.M + MT - 1) / MT));

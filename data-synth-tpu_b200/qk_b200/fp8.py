@@ -74,12 +74,20 @@ def _quantised(codes, scales, by_rows, name):
 
 
 def _weights(weights, k, index, name):
-    """``weights`` of a product of ``k`` columns on device ``index``: ``(rows, codes, pitch, scales)``."""
-    codes, pitch, scales = _quantised(weights[0], weights[1], False, name)
+    """``weights`` of a product of ``k`` columns on device ``index``: ``(rows, address, bytes from row to row,
+    address of the scales)``, and the tensors, which have to live until the call is made."""
+    codes, scales = weights
+    if codes.dtype is not _E4M3 or k % 16 or not (codes.is_contiguous() and scales.is_contiguous()) or scales.dtype is not _F32 \
+            or codes.data_ptr() % 16 or scales.get_device() != index:
+        codes, pitch, scales = _quantised(codes, scales, False, name)
+    else:
+        pitch = k
     n, width = codes.shape
     if width != k or n < 1 or codes.get_device() != index:
         raise ValueError(f"{name} must be [N, {k}] on the device of x")
-    return n, codes, pitch, scales
+    if scales.shape != ((n + 127) // 128, (k + 127) // 128):
+        raise ValueError(f"the scales of {name} do not match its codes, one for each block of 128")
+    return n, codes.data_ptr(), pitch, scales.data_ptr(), (codes, scales)
 
 
 def _matrix(x, name):
@@ -173,17 +181,17 @@ def fp8_matmul(x, weights, *, output_dtype=None, out=None):
         codes, pitch, scales = _quantised(x.codes, x.scales, True, "x")
         m, k = codes.shape
         index = codes.get_device()
-        n, w, w_pitch, w_scales = _weights(weights, k, index, "weights")
+        n, w, w_pitch, w_scales, _keep = _weights(weights, k, index, "weights")
         out = _output(out, m, n, dtype, codes.device)
-        _lib.call_at(index, "qk_fp8_matmul", codes.data_ptr(), pitch, scales.data_ptr(), m, k, w.data_ptr(), w_pitch,
-                     w_scales.data_ptr(), n, out_code, out.data_ptr())
+        _lib.call_at(index, "qk_fp8_matmul", codes.data_ptr(), pitch, scales.data_ptr(), m, k, w, w_pitch, w_scales, n,
+                     out_code, out.data_ptr())
         return out
     x, code, stride, index = _matrix(x, "x")
     m, k = x.shape
-    n, w, w_pitch, w_scales = _weights(weights, k, index, "weights")
+    n, w, w_pitch, w_scales, _keep = _weights(weights, k, index, "weights")
     out = _output(out, m, n, dtype, x.device)
     x, stride, room, need = _room("qk_fp8_linear_workspace_bytes", index, code, m, k, n, x, stride)
-    _lib.call_at(index, "qk_fp8_linear", x.data_ptr(), code, stride, m, k, w.data_ptr(), w_pitch, w_scales.data_ptr(), n,
+    _lib.call_at(index, "qk_fp8_linear", x.data_ptr(), code, stride, m, k, w, w_pitch, w_scales, n,
                  out_code, out.data_ptr(), room.data_ptr() if need else None, need)
     return out
 
@@ -195,13 +203,13 @@ def gated_fp8(x, gate, up):
     codes, pitch, scales = _quantised(x.codes, x.scales, True, "x")
     m, k = codes.shape
     index = codes.get_device()
-    inner, g, g_pitch, g_scales = _weights(gate, k, index, "gate")
-    n, u, u_pitch, u_scales = _weights(up, k, index, "up")
+    inner, g, g_pitch, g_scales, _keep_g = _weights(gate, k, index, "gate")
+    n, u, u_pitch, u_scales, _keep_u = _weights(up, k, index, "up")
     if n != inner:
         raise ValueError("gate and up must be [I, K]")
     h, h_pitch = _empty_rows(m, inner, codes.device)
-    _lib.call_at(index, "qk_fp8_gated", codes.data_ptr(), pitch, scales.data_ptr(), m, k, g.data_ptr(), g_pitch,
-                 g_scales.data_ptr(), u.data_ptr(), u_pitch, u_scales.data_ptr(), inner, h.codes.data_ptr(), h_pitch,
+    _lib.call_at(index, "qk_fp8_gated", codes.data_ptr(), pitch, scales.data_ptr(), m, k, g, g_pitch, g_scales,
+                 u, u_pitch, u_scales, inner, h.codes.data_ptr(), h_pitch,
                  h.scales.data_ptr())
     return h
 
@@ -213,16 +221,15 @@ def gated_ffn_fp8(x, gate, up, down, *, out=None):
         return fp8_matmul(gated_fp8(x, gate, up), down, out=out, output_dtype=torch.bfloat16)
     x, code, stride, index = _matrix(x, "x")
     m, k = x.shape
-    inner, g, g_pitch, g_scales = _weights(gate, k, index, "gate")
-    n, u, u_pitch, u_scales = _weights(up, k, index, "up")
+    inner, g, g_pitch, g_scales, _keep_g = _weights(gate, k, index, "gate")
+    n, u, u_pitch, u_scales, _keep_u = _weights(up, k, index, "up")
     if n != inner:
         raise ValueError("gate and up must be [I, K]")
-    n, d, d_pitch, d_scales = _weights(down, inner, index, "down")
+    n, d, d_pitch, d_scales, _keep_d = _weights(down, inner, index, "down")
     out = _output(out, m, n, torch.bfloat16, x.device)
     x, stride, room, need = _room("qk_fp8_ffn_workspace_bytes", index, code, m, k, inner, x, stride)
-    _lib.call_at(index, "qk_fp8_ffn", x.data_ptr(), code, stride, m, k, g.data_ptr(), g_pitch, g_scales.data_ptr(),
-                 u.data_ptr(), u_pitch, u_scales.data_ptr(), inner, d.data_ptr(), d_pitch, d_scales.data_ptr(), n, out.data_ptr(),
-                 room.data_ptr() if need else None, need)
+    _lib.call_at(index, "qk_fp8_ffn", x.data_ptr(), code, stride, m, k, g, g_pitch, g_scales, u, u_pitch, u_scales, inner, d,
+                 d_pitch, d_scales, n, out.data_ptr(), room.data_ptr() if need else None, need)
     return out
 
 

@@ -361,3 +361,28 @@ def test_speculative_generation_with_fp8_projections(cuda_device):
     rows = gen.generate(6)
     for row, prompt in zip(rows, prompts):
         assert row[:len(prompt)] == prompt and len(row) > len(prompt) + 5 and all(0 <= t < 600 for t in row)
+
+
+def test_products_of_many_sizes(cuda_device):
+    """Sizes at random: every number of tokens, splits of K and buffers, both forms."""
+    import random
+
+    import torch
+
+    from qk_b200.fp8 import check_status, fp8_matmul, gated_ffn_fp8, gated_fp8, quantize_fp8
+
+    rng = random.Random(11)
+    for i in range(60):
+        m = rng.choice([1, 2, 5, 9, 16, 17, 30, 33, 64, 65, 100, 128, 129, 260])
+        k = rng.choice([16, 128, 8 * rng.randint(1, 700), rng.randint(1, 3000)])
+        n = rng.choice([rng.randint(1, 600), 128 * rng.randint(1, 40), 9216])
+        x, w = activations(m, k, cuda_device, i), packed(n, k, cuda_device, i)
+        rows = quantize_fp8(x)
+        got = fp8_matmul(x, w)
+        assert torch.equal(got, fp8_matmul(rows, w)), (m, k, n)
+        check_product(got, values(rows)[0], weight_values(w), 2.0 ** -8)
+        if n * k < 1 << 20:
+            down = packed(rng.randint(1, 300), n, cuda_device, i)
+            out = gated_ffn_fp8(x, w, w, down)
+            assert torch.equal(out, fp8_matmul(gated_fp8(rows, w, w), down)), (m, k, n)
+    check_status(cuda_device)
