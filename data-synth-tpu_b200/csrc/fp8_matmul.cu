@@ -90,8 +90,14 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
   a.ld = ld;
   a.out_scales = out_scales;
   a.f32 = f32;
-  a.vectors = vectors;
-  return u ? launch_wide<true>(xm, wm, um, a, st) : launch_wide<false>(xm, wm, wm, a, st);
+  a.copies = vectors || u;
+  CUtensorMap om = xm;
+  if (u) ok = encode(&om, out, CU_TENSOR_MAP_DATA_TYPE_UINT8, M, N, ld, 32, 64, CU_TENSOR_MAP_SWIZZLE_64B);
+  else if (vectors)
+    ok = encode(&om, out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, M, N, N * (f32 ? 4 : 2), 32, f32 ? 32 : 64,
+                CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the output");
+  return u ? launch_wide<true>(xm, wm, um, om, a, st) : launch_wide<false>(xm, wm, wm, om, a, st);
 }
 
 // The same from rows of BF16 or FP32, which a narrow product of BF16 quantises itself where it can; else into `room`

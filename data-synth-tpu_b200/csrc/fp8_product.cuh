@@ -79,16 +79,21 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Codes [rows][width], rows `ld` bytes apart, in boxes of `box_rows` x 128 with the 128-byte swizzle; zero past the ends.
-bool encode(CUtensorMap* map, const void* codes, int64_t rows, int64_t width, int64_t ld, uint32_t box_rows) {
+// A matrix [rows][width] whose rows are `pitch` bytes apart, in boxes of box_rows x box_width; zero past the ends.
+bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, int64_t rows, int64_t width, int64_t pitch, uint32_t box_rows,
+            uint32_t box_width, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
   if (!fn) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
-  const cuuint32_t box[2] = {kFp8Block, box_rows};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+  const cuuint32_t box[2] = {box_width, box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Codes as operands: boxes of one block of 128 columns in the 128-byte swizzle.
+bool encode(CUtensorMap* map, const void* codes, int64_t rows, int64_t width, int64_t ld, uint32_t box_rows) {
+  return encode(map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, rows, width, ld, box_rows, kFp8Block, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -15,10 +15,10 @@ namespace qk {
 namespace {
 
 constexpr int kTileM = 256, kTileN = 256, kHalf = 128;  // a pair's tile, and a CTA's rows of either operand
-constexpr int kStages = 5, kBuffers = 2;
+constexpr int kStages = 4, kBuffers = 2;
 constexpr uint32_t kBytesA = kHalf * kFp8Block, kStageBytes = 2 * kBytesA;  // of one CTA
 constexpr int kFirstSum = 4, kSumWarps = 8, kThreads = (kFirstSum + kSumWarps) * 32;
-constexpr uint32_t kStaging = 4096;  // bytes per summing warp
+constexpr uint32_t kPiece = 4096, kStaging = 2 * kPiece;  // bytes of 32 rows of 128 on their way out, per summing warp
 constexpr int kAhead = 4;            // blocks whose scales of x are on their way
 // Registers per thread: 168 at launch for 3 warpgroups (504 in all).
 constexpr int kSumRegs = 216, kOtherRegs = 72;
@@ -33,7 +33,7 @@ struct WideArgs {
   void* out;                  // [M][N], or codes [M][ld]
   int64_t ld;
   float* out_scales;          // [n_blocks][M]
-  bool f32, vectors;          // of out: FP32, and rows that begin on 16 bytes
+  bool f32, copies;           // of out: FP32; rows that begin on 16 bytes, so that tensor copies can write them
 };
 
 struct WideControl {
@@ -153,15 +153,34 @@ __device__ __forceinline__ void add_block(uint32_t col, float scale, uint64_t* a
   }
 }
 
-// 32 rows (a lane each) of 128 columns out, through 4 KB of shared memory, in pieces of 128 bytes a row.
+// A piece of staged output out, by a copy that runs beside the next tile's products. (Plain stores held the warps until
+// memory had taken them, all SMs' at the same time: 60 us of 350.)
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, uint32_t from) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(from)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until all but the last `N` pieces that this thread sent have been read from shared memory.
+template <int N>
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
+// 32 rows (a lane each) of 128 columns out, through shared memory, in pieces of 128 bytes a row, two of which alternate.
 template <bool F32>
-__device__ __forceinline__ void wide_store(const WideArgs& a, const uint64_t (&acc)[64], uint32_t staging, int64_t row0, int col0) {
+__device__ __forceinline__ void wide_store(const WideArgs& a, const CUtensorMap* map, const uint64_t (&acc)[64], uint32_t staging,
+                                           int64_t row0, int col0) {
   constexpr int kSize = F32 ? 4 : 2, kColumns = 128 / kSize;
   const int lane = threadIdx.x & 31;
   const int rows = static_cast<int>(min(a.M - row0, static_cast<int64_t>(32)));
+  if (rows <= 0) return;
 #pragma unroll
   for (int c = 0; c < 128; c += kColumns) {
     if (col0 + c >= a.N) break;
+    const uint32_t piece = staging + (c / kColumns & 1) * kPiece;
+    if (lane == 0 && c == 0) stores_read<0>();  // the last tile's
+    if (lane == 0 && c >= 2 * kColumns) stores_read<1>();
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -177,39 +196,37 @@ __device__ __forceinline__ void wide_store(const WideArgs& a, const uint64_t (&a
           w[i] = pack_bf16x2(x, y);
         }
       }
-      sts_v4(staging + lane * 128 + ((j ^ lane) & 7) * 16, w[0], w[1], w[2], w[3]);
+      sts_v4(piece + lane * 128 + ((j ^ lane) & 7) * 16, w[0], w[1], w[2], w[3]);
+    }
+    if (a.copies) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) store_box(map, col0 + c, static_cast<int>(row0), piece);
+      continue;
     }
     __syncwarp();
     uint8_t* out = static_cast<uint8_t*>(a.out) + (row0 * a.N + col0 + c) * kSize;
-    if (a.vectors && col0 + c + kColumns <= a.N) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + lane / 8;
-        if (r < rows)
-          *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * a.N * kSize + (lane & 7) * 16) =
-              lds_v4_at(staging + r * 128 + ((lane ^ r) & 7) * 16);
-      }
-    } else {
-      for (int r = 0; r < rows; ++r) {
-        const uint32_t v = lds_at(staging + r * 128 + ((lane / 4 ^ r) & 7) * 16 + (lane & 3) * 4);
-        uint8_t* at = out + static_cast<int64_t>(r) * a.N * kSize + lane * 4;
-        if (F32) {
-          if (col0 + c + lane < a.N) *reinterpret_cast<uint32_t*>(at) = v;
-        } else {
-          if (col0 + c + 2 * lane < a.N) *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(v);
-          if (col0 + c + 2 * lane + 1 < a.N) *reinterpret_cast<uint16_t*>(at + 2) = static_cast<uint16_t>(v >> 16);
-        }
+    for (int r = 0; r < rows; ++r) {
+      const uint32_t v = lds_at(piece + r * 128 + ((lane / 4 ^ r) & 7) * 16 + (lane & 3) * 4);
+      uint8_t* at = out + static_cast<int64_t>(r) * a.N * kSize + lane * 4;
+      if (F32) {
+        if (col0 + c + lane < a.N) *reinterpret_cast<uint32_t*>(at) = v;
+      } else {
+        if (col0 + c + 2 * lane < a.N) *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(v);
+        if (col0 + c + 2 * lane + 1 < a.N) *reinterpret_cast<uint16_t*>(at + 2) = static_cast<uint16_t>(v >> 16);
       }
     }
   }
 }
 
 template <bool GATED>
-__device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, uint32_t staging, int rank) {
+__device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, const CUtensorMap* out_map, uint32_t staging, int rank) {
   const int warp = (threadIdx.x >> 5) - kFirstSum, quarter = warp & 3, half = warp >> 2, lane = threadIdx.x & 31;
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t released[kBuffers] = {leaders(&ctl.sum_empty[0][half]), leaders(&ctl.sum_empty[1][half])};
   const uint32_t scales = staging + kSumWarps * kStaging + (threadIdx.x - kFirstSum * 32) * 4;  // this thread's, kAhead slots
+  const uint32_t swaps_at = scales - (threadIdx.x - kFirstSum * 32) * 4 + kAhead * kSumWarps * 128;
+  staging += warp * kStaging;
   uint32_t it = 0, swaps = 0;
   for (int t = blockIdx.x / 2; t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     const Tile tile = tile_of(a, t);
@@ -249,8 +266,8 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, u
       if (lane == 0) cluster_arrive(released[d]);
     }
     if (!GATED) {
-      if (a.f32) wide_store<true>(a, acc, staging + warp * kStaging, row0, tile.n * kTileN + half * 128);
-      else wide_store<false>(a, acc, staging + warp * kStaging, row0, tile.n * kTileN + half * 128);
+      if (a.f32) wide_store<true>(a, out_map, acc, staging, row0, tile.n * kTileN + half * 128);
+      else wide_store<false>(a, out_map, acc, staging, row0, tile.n * kTileN + half * 128);
       continue;
     }
     // A thread has half of its row's block of 128: two threads swap their maxima. No rounding before the codes'.
@@ -265,32 +282,35 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, u
       h[2 * j + 1] = gated(g1, u1);
       most = max(most, max(magnitude(h[2 * j]), magnitude(h[2 * j + 1])));
     }
-    const uint32_t swap = staging + (swaps & 1) * 1024 + quarter * 128 + lane * 4;
+    const uint32_t swap = swaps_at + (swaps & 1) * 1024 + quarter * 128 + lane * 4;
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(swap + half * 512), "r"(most) : "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl.swapped[quarter]);
     if (!warp_wait(&ctl.swapped[quarter], swaps & 1)) return false;
     most = max(most, lds_at(swap + (half ^ 1) * 512));
     ++swaps;
-    if (row < a.M) {
-      const Fp8Divisor by(most);
-      const int col = tile.n * kFp8Block + half * 64;
-      uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.ld + col;
+    const Fp8Divisor by(most);
+    if (lane == 0) stores_read<0>();  // the last tile's
+    __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 64; j += 16)
-        if (col + j < a.N)
-          *reinterpret_cast<uint4*>(out + j) =
-              make_uint4(by.codes4(h + j), by.codes4(h + j + 4), by.codes4(h + j + 8), by.codes4(h + j + 12));
-      if (half == 0) a.out_scales[static_cast<int64_t>(tile.n) * a.M + row] = fp8_scale(most);
-    }
+    for (int j = 0; j < 4; ++j)
+      sts_v4(staging + lane * 64 + ((j ^ lane >> 1) & 3) * 16,  // in the 64-byte swizzle
+             by.codes4(h + 16 * j), by.codes4(h + 16 * j + 4), by.codes4(h + 16 * j + 8),
+             by.codes4(h + 16 * j + 12));
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && row0 < a.M && tile.n * kFp8Block + half * 64 < a.N)
+      store_box(out_map, tile.n * kFp8Block + half * 64, static_cast<int>(row0), staging);
+    if (half == 0 && row < a.M) a.out_scales[static_cast<int64_t>(tile.n) * a.M + row] = fp8_scale(most);
   }
+  if (lane == 0) stores_read<0>();  // the CTA's shared memory lives until then
   return true;
 }
 
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     fp8_wide_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap w, const __grid_constant__ CUtensorMap u,
-                    WideArgs a) {
+                    const __grid_constant__ CUtensorMap out, WideArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ WideControl ctl;
   const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
@@ -324,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   bool ok = true;
   if (warp >= kFirstSum) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
-    ok = wide_sums<GATED>(a, ctl, smem + kStages * kStageBytes, rank);
+    ok = wide_sums<GATED>(a, ctl, &out, smem + kStages * kStageBytes, rank);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 0) {
@@ -346,12 +366,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 }
 
 template <bool GATED>
-int launch_wide(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const WideArgs& a, cudaStream_t st) {
-  const size_t smem = 1024 + kStages * kStageBytes + kSumWarps * kStaging + kAhead * kSumWarps * 128;
+int launch_wide(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& out, const WideArgs& a, cudaStream_t st) {
+  const size_t smem = 1024 + kStages * kStageBytes + kSumWarps * kStaging + kAhead * kSumWarps * 128 + 2048;
   const int rc = allow_smem(reinterpret_cast<const void*>(fp8_wide_kernel<GATED>), smem);
   if (rc) return rc;
   const int tiles = a.tiles_m * a.tiles_n, pairs = sm_count() / 2;
-  cudaError_t e = launch_dependent(fp8_wide_kernel<GATED>, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kThreads), smem, st, x, w, u, a);
+  cudaError_t e = launch_dependent(fp8_wide_kernel<GATED>, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kThreads), smem, st, x, w, u, out, a);
   if (e != cudaSuccess) return cuda_error(e, "fp8_wide_kernel");
   count_launch();
   return QK_OK;
