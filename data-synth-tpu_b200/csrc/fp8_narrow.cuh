@@ -322,9 +322,12 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
   // the tokens that a CTA owns, in their order
   const int owned = (live + a.splits - 1) / a.splits, mine = min(max(live - rank * owned, 0), owned);
   if (threadIdx.x == 0) {
-    prefetch_map(&w);
-    if (GATED) prefetch_map(&u);
     if (!ROWS) prefetch_map(&x);
+    // the weights' way from memory to L2 runs beside the kernel ahead
+    for (int i = 0; i < min(count, a.stages); ++i) {
+      prefetch_box(&w, (b0 + i) * kFp8Block, tile * 128);
+      if (GATED) prefetch_box(&u, (b0 + i) * kFp8Block, tile * 128);
+    }
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(&ctl.full[i], 1);
       mbar_init(&ctl.empty[i], 1);

@@ -18,6 +18,12 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// Brings a box into L2 only: also before the kernels ahead have ended, for whatever they write is seen by later loads.
+__device__ __forceinline__ void prefetch_box(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
+               : "memory");
+}
+
 // Instruction descriptor of kind::f8f6f4: e4m3 A and B, both K-major, FP32 D, M = 128.
 __device__ __forceinline__ uint32_t idesc_e4m3_m128(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
 
