@@ -164,7 +164,7 @@ __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowContr
 template <int MT, bool GATED, bool ROWS>
 __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int b0, int count, int tile, int row0) {
   using L = Narrow<MT, GATED>;
-  constexpr int kEach = L::kEach;
+  constexpr int kEach = L::kEach, kLoad = kEach < 32 ? kEach : 32;
   const int warp = (threadIdx.x >> 5) - kNarrowFirstSum, half = warp >> 2, lane = threadIdx.x & 31;
   const int quarter = (threadIdx.x >> 5) & 3;  // the TMEM lanes that this warp may read
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kEach;
@@ -209,15 +209,11 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& 
     for (int o = 0; o < L::kOperands; ++o) {
       const uint64_t by = o ? f32x2(by_u, by_u) : f32x2(by_w, by_w);
 #pragma unroll
-      for (int c = 0; c < kEach; c += 8) {
-        uint32_t v[8];
-        tmem_ld8(tm + d * L::kColumns + o * MT + c, v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
-                     :
-                     : "memory");
+      for (int c = 0; c < kEach; c += kLoad) {
+        uint32_t v[kLoad];
+        tmem_get<kLoad>(tm + d * L::kColumns + o * MT + c, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kLoad / 2; ++j) {
           const float2 s = *reinterpret_cast<const float2*>(scales + c + 2 * j);
           acc[o][c / 2 + j] = f32x2_fma(f32x2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
                                         f32x2_mul(f32x2(s.x, s.y), by), acc[o][c / 2 + j]);
