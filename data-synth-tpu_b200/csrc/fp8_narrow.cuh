@@ -16,8 +16,9 @@ namespace {
 constexpr int kNarrowStages = 8, kNarrowSumWarps = 8, kNarrowFirstSum = 2;
 constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
 constexpr int kMostSplits = 8;       // the portable cluster size
-// Blocks of rows of BF16 that a CTA quantises itself, at most. A half warp takes about 0.6 us for one, all latency.
-constexpr int kInlineRows = 16, kInline = 64;
+// Rows of BF16, and blocks of them, that a CTA quantises itself, at most: 32 rows of 4096 x 2048 (128 blocks per CTA) take
+// 7.2 us, with a launch of its own for that 7.5 and 4 us more of the host, 32 of 2048 x 9216 (256) 11.4 and 9.4.
+constexpr int kInlineRows = 64, kInline = 128;
 
 struct NarrowArgs {
   int64_t M;
@@ -55,7 +56,7 @@ struct Narrow {
 };
 
 struct NarrowControl {
-  uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], x_full, stored, joined;
+  uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], stored, joined;
   uint32_t tmem;
   alignas(16) float scales[kNarrowSumWarps * 2 * 64];  // of x: a warp's two slots of 64 tokens, or (ROWS) [block][MT]
 };
@@ -110,7 +111,6 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
   constexpr uint32_t kStage = ROWS ? L::kBytesW : L::kStage;
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = idesc_e4m3_m128(MT);
   const uint64_t wd0 = sdesc_sw128(smem, 1024u), xd0 = sdesc_sw128(smem + (ROWS ? a.stages * kStage : L::kBytesW), 1024u);
-  if (ROWS && !warp_wait(&ctl.x_full, 0)) return false;
   int s = 0, d = 0;
   uint32_t full = 0, freed = 1;
   for (int it = 0; it < count; ++it) {
@@ -139,24 +139,43 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
 template <int MT>
 __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl& ctl, uint32_t tiles, int b0, int count) {
   const int lane = threadIdx.x & 31, in = lane & 15;
-  // 16 half warps: each takes every 16th of (block, row) pairs
+  // 16 half warps: each takes every 16th of (block, row) pairs, kAtOnce of them at a time
+  constexpr int kAtOnce = 4;
   const int half = (threadIdx.x - kNarrowFirstSum * 32) >> 4, units = count << a.row_shift;
+  const int mask = (1 << a.row_shift) - 1;
 #pragma unroll 1
-  for (int first = half & ~1; first < units; first += 16) {  // as often in the whole warp
-    const int unit = first + (half & 1), row = unit & ((1 << a.row_shift) - 1), b = unit >> a.row_shift;
-    const int at = (b0 + b) * kFp8Block + in * 8;
-    const bool live = row < a.M && b < count;
-    float f[8];
-    unpack8(live && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0), f);
-    uint32_t most = 0;
+  for (int first = half & ~1; first < units; first += 16 * kAtOnce) {  // as often in the whole warp
+    uint4 v[kAtOnce];
+    uint32_t most[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, magnitude(f[j]));
-    most = block_most(most);
-    const Fp8Divisor by(most);
-    if (live) {
-      const uint32_t to = tiles + b * (MT * kFp8Block) + row * kFp8Block + (((in >> 1) ^ (row & 7)) << 4) + (in & 1) * 8;
-      asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to), "r"(by.codes4(f)), "r"(by.codes4(f + 4)) : "memory");
-      if (in == 0) ctl.scales[b * MT + row] = fp8_scale(most);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int unit = first + (half & 1) + 16 * i, row = unit & mask, b = unit >> a.row_shift, at = (b0 + b) * kFp8Block + in * 8;
+      v[i] = row < a.M && b < count && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      float f[8];
+      unpack8(v[i], f);
+      most[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most[i] = max(most[i], magnitude(f[j]));
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int unit = first + (half & 1) + 16 * i, row = unit & mask, b = unit >> a.row_shift;
+      float f[8];
+      unpack8(v[i], f);
+      const Fp8Divisor by(most[i]);
+      const uint32_t lo = by.codes4(f), hi = by.codes4(f + 4);
+      if (row < a.M && b < count) {
+        const uint32_t to = tiles + b * (MT * kFp8Block) + row * kFp8Block + (((in >> 1) ^ (row & 7)) << 4) + (in & 1) * 8;
+        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to), "r"(lo), "r"(hi) : "memory");
+        if (in == 0) ctl.scales[b * MT + row] = fp8_scale(most[i]);
+      }
     }
   }
 }
@@ -332,7 +351,6 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
       mbar_init(&ctl.sum_full[i], 1);
       mbar_init(&ctl.sum_empty[i], kNarrowSumWarps);
     }
-    mbar_init(&ctl.x_full, kNarrowSumWarps);
     mbar_init(&ctl.stored, kNarrowSumWarps);
     mbar_init(&ctl.joined, 1);
     fence_mbar_init();
@@ -342,11 +360,15 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
     for (int i = 0; i < min(count, a.stages); ++i) narrow_copy<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, i, b0, tile, row0);
   }
   if (warp == 1) tmem_alloc(&ctl.tmem, L::kAlloc);
+  pdl_wait();
+  if (ROWS && warp >= kNarrowFirstSum) {
+    narrow_quantise<MT>(a, ctl, smem + a.stages * L::kBytesW, b0, count);
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   cluster_arrive_relaxed();  // this CTA's barriers are there: the others may send from now on
-  pdl_wait();
   pdl_trigger();
   bool ok = true;
   if (warp == 0) {
@@ -357,14 +379,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
     ok = narrow_products<MT, GATED, ROWS>(a, ctl, smem, count);
     cluster_wait();
   } else {
-    if (ROWS) {
-      narrow_quantise<MT>(a, ctl, smem + a.stages * L::kBytesW, b0, count);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(&ctl.x_full);
-      ok = warp_wait(&ctl.x_full, 0);  // the scales are everybody's
-    }
-    if (ok) ok = narrow_sums<MT, GATED, ROWS>(a, ctl, smem, b0, count, tile, row0);
+    ok = narrow_sums<MT, GATED, ROWS>(a, ctl, smem, b0, count, tile, row0);
     __syncwarp();
     cluster_wait();
     if (ok) ok = narrow_send<MT, GATED>(a, ctl, smem, owned, live, rank);
@@ -399,7 +414,11 @@ struct NarrowPlan {
   }
   int each(int blocks) const { return (blocks + splits - 1) / splits; }
   // Whether the CTAs can quantise rows of x themselves.
-  bool quantises(int64_t M, int blocks) const { return M <= kInlineRows && M * each(blocks) <= kInline; }
+  bool quantises(int64_t M, int blocks) const {
+    int rows = 1;
+    while (rows < M && rows < kInlineRows) rows *= 2;
+    return M <= kInlineRows && rows * each(blocks) <= kInline;
+  }
 };
 
 template <int MT, bool GATED, bool ROWS>
@@ -438,12 +457,13 @@ int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap&
 template <bool GATED>
 int launch_narrow(bool rows, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const NarrowArgs& a, const NarrowPlan& plan,
                   cudaStream_t st) {
-  if (rows) return launch_narrow<16, GATED, true>(x, w, u, a, plan, st);
-  if (plan.tokens == 16) return launch_narrow<16, GATED, false>(x, w, u, a, plan, st);
-  if (plan.tokens == 32) return launch_narrow<32, GATED, false>(x, w, u, a, plan, st);
+  if (plan.tokens == 16)
+    return rows ? launch_narrow<16, GATED, true>(x, w, u, a, plan, st) : launch_narrow<16, GATED, false>(x, w, u, a, plan, st);
+  if (plan.tokens == 32)
+    return rows ? launch_narrow<32, GATED, true>(x, w, u, a, plan, st) : launch_narrow<32, GATED, false>(x, w, u, a, plan, st);
   if constexpr (!GATED)
     if (plan.tokens == 128) return launch_narrow<128, GATED, false>(x, w, u, a, plan, st);
-  return launch_narrow<64, GATED, false>(x, w, u, a, plan, st);
+  return rows ? launch_narrow<64, GATED, true>(x, w, u, a, plan, st) : launch_narrow<64, GATED, false>(x, w, u, a, plan, st);
 }
 
 }  // namespace
