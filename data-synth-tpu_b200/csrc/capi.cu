@@ -2,6 +2,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 #include "common.cuh"
 
@@ -40,30 +41,30 @@ int sm_count() {
 }
 
 int allow_smem(const void* kernel, size_t bytes) {
-  // The attribute is per (kernel, device) and is a ceiling: remember the largest value
-  // set so far and raise it when a launch needs more (never lower it).
-  static thread_local const void* done_kernel[256];
-  static thread_local int done_dev[256];
-  static thread_local size_t done_bytes[256];
-  static thread_local int n_done = 0;
+  // The attribute is per (kernel, device) and is a ceiling: remember the largest value set so far and raise it when a
+  // launch needs more (never lower it). One memory for all host threads: with one each, a thread's first call of a
+  // kernel lowered the ceiling that another had raised.
+  struct Ceiling {
+    const void* kernel;
+    int dev;
+    size_t bytes;
+  };
+  static std::mutex mutex;
+  static Ceiling done[512];
+  static int n_done = 0;
   if (bytes <= 48 * 1024) return QK_OK;  // below the default limit: nothing to opt into
   int dev = 0;
   cudaGetDevice(&dev);
-  int slot = -1;
-  for (int i = 0; i < n_done; ++i)
-    if (done_kernel[i] == kernel && done_dev[i] == dev) {
-      if (done_bytes[i] >= bytes) return QK_OK;
-      slot = i;
-    }
+  std::lock_guard<std::mutex> lock(mutex);
+  Ceiling* slot = nullptr;
+  for (int i = 0; i < n_done && !slot; ++i)
+    if (done[i].kernel == kernel && done[i].dev == dev) slot = &done[i];
+  if (slot && slot->bytes >= bytes) return QK_OK;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(bytes));
   if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute");
-  if (slot < 0 && n_done < 256) slot = n_done++;
-  if (slot >= 0) {
-    done_kernel[slot] = kernel;
-    done_dev[slot] = dev;
-    done_bytes[slot] = bytes;
-  }
+  if (!slot && n_done < 512) slot = &done[n_done++];
+  if (slot) *slot = Ceiling{kernel, dev, bytes};
   return QK_OK;
 }
 
