@@ -18,7 +18,7 @@ constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
 constexpr int kMostSplits = 8;       // the portable cluster size
 // Rows of BF16, and blocks of them, that a CTA quantises itself, at most: 32 rows of 4096 x 2048 (128 blocks per CTA) take
 // 7.2 us, with a launch of its own for that 7.5 and 4 us more of the host, 32 of 2048 x 9216 (256) 11.4 and 9.4.
-constexpr int kInlineRows = 64, kInline = 128;
+constexpr int kInlineRows = 64, kInline = 128, kInlineTokens = 256;  // kInlineTokens: of their tiles in shared memory
 
 struct NarrowArgs {
   int64_t M;
@@ -54,6 +54,8 @@ struct Narrow {
     return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits) * ((MT + splits - 1) / splits) * kToken;
   }
 };
+
+static_assert(kInlineTokens <= kNarrowSumWarps * 2 * 64, "a scale for each");
 
 struct NarrowControl {
   uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], stored, joined;
@@ -417,7 +419,7 @@ struct NarrowPlan {
   bool quantises(int64_t M, int blocks) const {
     int rows = 1;
     while (rows < M && rows < kInlineRows) rows *= 2;
-    return M <= kInlineRows && rows * each(blocks) <= kInline;
+    return M <= kInlineRows && rows * each(blocks) <= kInline && tokens * each(blocks) <= kInlineTokens;
   }
 };
 

@@ -221,7 +221,9 @@ def test_norm_leaves_as_codes(cuda_device, rows, width, add):
 
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 128, 128), (1, 2048, 9216), (3, 100, 7), (8, 4096, 2048), (16, 2048, 300),
                                    (31, 1111, 1000), (64, 4096, 2048), (65, 640, 520), (128, 16384, 256), (129, 257, 255),
-                                   (200, 384, 136), (333, 1111, 1000), (1000, 2048, 2304)])
+                                   (200, 384, 136), (333, 1111, 1000), (1000, 2048, 2304),
+                                   # more tiles than SMs: a CTA has all of K, more blocks than it can quantise
+                                   (1, 8192, 19000), (2, 16384, 19100), (40, 2176, 19000)])
 @pytest.mark.parametrize("f32", [False, True])
 def test_matmul(cuda_device, m, k, n, f32):
     import torch
@@ -386,3 +388,187 @@ def test_products_of_many_sizes(cuda_device):
             out = gated_ffn_fp8(x, w, w, down)
             assert torch.equal(out, fp8_matmul(gated_fp8(rows, w, w), down)), (m, k, n)
     check_status(cuda_device)
+
+
+# ---- refusals, layouts, streams, graphs -----------------------------------------------------------
+
+
+def test_mismatched_operands_are_refused(cuda_device):
+    import torch
+
+    from qk_b200.fp8 import Fp8Rows, Fp8Weights, fp8_matmul, fp8_weights, gated_ffn_fp8, quantize_fp8, rms_norm_fp8
+
+    x, w = activations(3, 256, cuda_device), packed(128, 256, cuda_device)
+    rows = quantize_fp8(x)
+    with pytest.raises(ValueError):
+        fp8_matmul(x[:, :128], w)
+    with pytest.raises(ValueError):
+        fp8_matmul(x, Fp8Weights(w.codes, w.scales.t()))
+    with pytest.raises(ValueError):
+        fp8_matmul(x, Fp8Weights(w.codes.cpu(), w.scales))
+    with pytest.raises(ValueError):
+        fp8_matmul(Fp8Rows(rows.codes, rows.scales.t()), w)
+    with pytest.raises(ValueError):
+        fp8_matmul(x, w, out=torch.empty((3, 128), device=cuda_device), output_dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        fp8_matmul(x, w, out=torch.empty((128, 3), dtype=torch.bfloat16, device=cuda_device).t())
+    with pytest.raises(ValueError):
+        gated_ffn_fp8(x, w, packed(120, 256, cuda_device), w)
+    with pytest.raises(ValueError):
+        gated_ffn_fp8(x, w, w, w)
+    with pytest.raises(ValueError):
+        rms_norm_fp8(x, x[0].clone(), residual=x[:2])
+    with pytest.raises(ValueError):
+        fp8_weights(w.codes, w.scales[:, :1])
+
+
+def test_layouts_of_operands(cuda_device):
+    """Views, odd pitches, misaligned beginnings, scales of another type: the values decide."""
+    import torch
+
+    from qk_b200.fp8 import Fp8Rows, Fp8Weights, fp8_matmul, fp8_weights, gated_ffn_fp8, quantize_fp8, rms_norm_fp8
+
+    x, w = activations(9, 384, cuda_device), packed(200, 384, cuda_device)
+    want = fp8_matmul(x, w)
+    wide = torch.zeros((9, 1000), dtype=torch.bfloat16, device=cuda_device)
+    for at in (0, 8, 5):
+        wide[:, at:at + 384] = x
+        assert torch.equal(fp8_matmul(wide[:, at:at + 384], w), want)
+    assert torch.equal(fp8_matmul(x.t().contiguous().t(), w), want)
+    store = torch.zeros(200 * 401 + 7, dtype=torch.uint8, device=cuda_device)
+    odd = store[7:].view(200, 401)[:, :384]
+    odd.copy_(w.codes.view(torch.uint8))
+    assert torch.equal(fp8_matmul(x, Fp8Weights(odd.view(torch.float8_e4m3fn), w.scales.double().t().contiguous().t())), want)
+    laid = fp8_weights(odd.cpu(), w.scales.cpu(), cuda_device)
+    assert torch.equal(fp8_matmul(x, laid), want) and laid.codes.stride(0) % 16 == 0
+    rows = quantize_fp8(x)
+    assert torch.equal(fp8_matmul(Fp8Rows(rows.codes[::2], rows.scales[:, ::2]), w), want[::2])
+    out = torch.empty((9, 200), device=cuda_device)
+    assert fp8_matmul(x.float(), w, out=out) is out and torch.equal(out.to(torch.bfloat16), want)
+    assert fp8_matmul(x[:0], w).shape == (0, 200) and gated_ffn_fp8(x[:0], w, w, packed(8, 200, cuda_device)).shape == (0, 8)
+    gamma = torch.ones(385, dtype=torch.bfloat16, device=cuda_device)[1:]
+    got, _ = rms_norm_fp8(wide[:, 5:389], gamma)
+    same, _ = rms_norm_fp8(x, gamma.clone())
+    assert torch.equal(got.codes.float(), same.codes.float()) and torch.equal(got.scales, same.scales)
+    assert rms_norm_fp8(x[:0], gamma)[0].codes.shape == (0, 384)
+
+
+def test_non_finite_values_stay_in_their_rows(cuda_device):
+    import torch
+
+    from qk_b200.fp8 import fp8_matmul, gated_ffn_fp8
+
+    for m in (4, 70, 600, 2000):  # the last in the wide form
+        x, w = activations(m, 512, cuda_device), packed(700, 512, cuda_device)
+        down = packed(64, 700, cuda_device)
+        want, ffn = fp8_matmul(x, w), gated_ffn_fp8(x, w, w, down)
+        x[1, 200] = float("nan")
+        x[m - 1, 3] = float("inf")
+        for got, good in ((fp8_matmul(x, w), want), (gated_ffn_fp8(x, w, w, down), ffn)):
+            assert torch.isnan(got[1]).all() and torch.isnan(got[m - 1]).all()
+            keep = [i for i in range(m) if i not in (1, m - 1)]
+            assert torch.equal(got[keep], good[keep])
+
+
+def test_rows_do_not_depend_on_their_neighbours(cuda_device):
+    """Padding rows, whatever they hold, and the number of rows within a form change no bit of the others."""
+    import torch
+
+    from qk_b200.fp8 import fp8_matmul
+
+    x, w = activations(64, 640, cuda_device), packed(1000, 640, cuda_device)
+    want = fp8_matmul(x, w)
+    y = x.clone()
+    y[40:] = float("nan")
+    assert torch.equal(fp8_matmul(y, w)[:40], want[:40])
+    assert torch.equal(fp8_matmul(x[:50], w), want[:50])
+
+
+def test_other_streams_threads_and_graphs(cuda_device):
+    """Calls on several streams and from several threads at once, and two graphs replayed beside one another."""
+    import threading
+
+    import torch
+
+    from qk_b200.fp8 import check_status, fp8_matmul, gated_ffn_fp8
+
+    w, gate, down = packed(2048, 512, cuda_device), packed(640, 512, cuda_device, 2), packed(512, 640, cuda_device, 3)
+    sizes = (1, 3, 20, 64, 100, 300)
+    xs = [activations(m, 512, cuda_device, m) for m in sizes]
+
+    def both(x):
+        return fp8_matmul(x, w), gated_ffn_fp8(x, gate, gate, down)
+
+    want = [both(x) for x in xs]
+    torch.cuda.synchronize(cuda_device)
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream(cuda_device)
+        with torch.cuda.stream(stream):
+            for _ in range(40):
+                got = both(xs[i])
+                if not all(torch.equal(g, e) for g, e in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    graphs, outs = [], []
+    for x in xs[2:4]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([both(x) for _ in range(10)])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(cuda_device) for _ in graphs]
+    for _ in range(10):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize(cuda_device)
+    for got, expected in zip(outs, want[2:4]):
+        for pair in got:
+            assert all(torch.equal(g, e) for g, e in zip(pair, expected))
+    check_status(cuda_device)
+
+
+def test_products_are_repeatable(cuda_device):
+    """Sums are joined in a fixed order: equal calls give equal bits, wide and narrow."""
+    import torch
+
+    from qk_b200.fp8 import fp8_matmul, gated_fp8, quantize_fp8
+
+    for m, k, n in ((1, 4096, 2048), (64, 2048, 9216), (2000, 2048, 2304)):
+        x, w = quantize_fp8(activations(m, k, cuda_device)), packed(n, k, cuda_device)
+        want, h = fp8_matmul(x, w, output_dtype=torch.float32), gated_fp8(x, w, w)
+        for _ in range(30):
+            assert torch.equal(fp8_matmul(x, w, output_dtype=torch.float32), want)
+            again = gated_fp8(x, w, w)
+            assert torch.equal(again.codes.view(torch.uint8), h.codes.view(torch.uint8)) and torch.equal(again.scales, h.scales)
+
+
+def test_offsets_past_31_bits(cuda_device):
+    """Rows whose values, codes and outputs lie more than 2^31 elements from the first."""
+    import torch
+
+    from qk_b200.fp8 import fp8_matmul, quantize_fp8, rms_norm_fp8
+
+    rows, width = 600_000, 4096  # 2.5e9 values
+    x = torch.zeros((rows, width), dtype=torch.bfloat16, device=cuda_device)
+    tail = activations(300, width, cuda_device)
+    x[-300:] = tail
+    got, want = quantize_fp8(x), quantize_fp8(tail)
+    assert torch.equal(got.codes[-300:].float(), want.codes.float()) and torch.equal(got.scales[:, -300:], want.scales)
+    w = packed(130, width, cuda_device)
+    out = fp8_matmul(got, w)
+    assert torch.equal(out[-300:], fp8_matmul(quantize_fp8(tail), w)) or np.abs(
+        to_f32(out[-300:]) - to_f32(fp8_matmul(want, w))).max() <= 2.0 ** -7 * np.abs(to_f32(out[-300:])).max()
+    assert not out[:1000].any()
+    gamma = torch.ones(width, dtype=torch.bfloat16, device=cuda_device)
+    normed, total = rms_norm_fp8(x, gamma, residual=x)
+    small, _ = rms_norm_fp8(tail, gamma, residual=tail)
+    assert torch.equal(normed.codes[-300:].float(), small.codes.float())
+    assert torch.equal(total[-300:], (tail.float() * 2).to(torch.bfloat16))
