@@ -50,17 +50,18 @@ struct Narrow {
     const uint32_t bytes = stages * (inline_blocks ? kBytesW : kStage) + inline_blocks * kBytesX;
     return bytes > kSums ? bytes : kSums;
   }
-  static size_t smem(int stages, int inline_blocks, int splits) {
-    return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits) * ((MT + splits - 1) / splits) * kToken;
+  static size_t smem(int stages, int inline_blocks, int splits, int live) {
+    return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits) * ((live + splits - 1) / splits) * kToken;
   }
 };
 
-static_assert(kInlineTokens <= kNarrowSumWarps * 2 * 64, "a scale for each");
-
+template <int MT>
 struct NarrowControl {
   uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], stored, joined;
   uint32_t tmem;
-  alignas(16) float scales[kNarrowSumWarps * 2 * 64];  // of x: a warp's two slots of 64 tokens, or (ROWS) [block][MT]
+  static constexpr int kSlot = MT > 64 ? 64 : 32;
+  alignas(16) float scales[kNarrowSumWarps * 2 * kSlot];  // of x: a warp's two slots of its tokens, or (ROWS) [block][MT]
+  static_assert(kInlineTokens <= kNarrowSumWarps * 2 * kSlot, "a scale for each");
 };
 
 // The address of this CTA's `addr` in the cluster's CTA `rank`.
@@ -79,7 +80,7 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t from, uint32_t bytes,
 }
 
 template <int MT, bool GATED, bool ROWS>
-__device__ __forceinline__ void narrow_copy(const NarrowArgs& a, NarrowControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
+__device__ __forceinline__ void narrow_copy(const NarrowArgs& a, NarrowControl<MT>& ctl, const CUtensorMap* x, const CUtensorMap* w,
                                             const CUtensorMap* u, uint32_t smem, int it, int b0, int tile, int row0) {
   using L = Narrow<MT, GATED>;
   constexpr uint32_t kStage = ROWS ? L::kBytesW : L::kStage;
@@ -93,7 +94,7 @@ __device__ __forceinline__ void narrow_copy(const NarrowArgs& a, NarrowControl& 
 
 // The copies behind the first a.stages.
 template <int MT, bool GATED, bool ROWS>
-__device__ __forceinline__ bool narrow_copies(const NarrowArgs& a, NarrowControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
+__device__ __forceinline__ bool narrow_copies(const NarrowArgs& a, NarrowControl<MT>& ctl, const CUtensorMap* x, const CUtensorMap* w,
                                               const CUtensorMap* u, uint32_t smem, int b0, int count, int tile, int row0) {
   bool ok = true;
   int it = min(count, a.stages);
@@ -108,7 +109,7 @@ __device__ __forceinline__ bool narrow_copies(const NarrowArgs& a, NarrowControl
 }
 
 template <int MT, bool GATED, bool ROWS>
-__device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int count) {
+__device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowControl<MT>& ctl, uint32_t smem, int count) {
   using L = Narrow<MT, GATED>;
   constexpr uint32_t kStage = ROWS ? L::kBytesW : L::kStage;
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0), idesc = idesc_e4m3_m128(MT);
@@ -139,7 +140,7 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
 // The CTA's blocks of x, quantised into the operand tiles and ctl.scales [block][MT]. Rows past M hold whatever the
 // memory held: they make columns of the product that nobody reads.
 template <int MT>
-__device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl& ctl, uint32_t tiles, int b0, int count) {
+__device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl<MT>& ctl, uint32_t tiles, int b0, int count) {
   const int lane = threadIdx.x & 31, in = lane & 15;
   // 16 half warps: each takes every 16th of (block, row) pairs, kAtOnce of them at a time
   constexpr int kAtOnce = 4;
@@ -183,7 +184,7 @@ __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowContr
 }
 
 template <int MT, bool GATED, bool ROWS>
-__device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int b0, int count, int tile, int row0) {
+__device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl<MT>& ctl, uint32_t smem, int b0, int count, int tile, int row0) {
   using L = Narrow<MT, GATED>;
   constexpr int kEach = L::kEach, kLoad = kEach < 32 ? kEach : 32;
   const int warp = (threadIdx.x >> 5) - kNarrowFirstSum, half = warp >> 2, lane = threadIdx.x & 31;
@@ -197,7 +198,8 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& 
 #pragma unroll
     for (int j = 0; j < kEach / 2; ++j) acc[o][j] = 0;
   // codes: a warp brings its tokens' scales of a block to its own two slots, one block ahead
-  float* slots = ctl.scales + warp * 128;
+  constexpr int kSlot = NarrowControl<MT>::kSlot;
+  float* slots = ctl.scales + warp * (2 * kSlot);
   float next[kEach > 32 ? 2 : 1];
   auto fetch = [&](int i) {
 #pragma unroll
@@ -212,7 +214,7 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& 
     const int d = it % L::kBuffers;
     const float* scales = ctl.scales + it * MT + half * kEach;
     if (!ROWS) {
-      float* slot = slots + (it & 1) * 64;
+      float* slot = slots + (it & 1) * kSlot;
 #pragma unroll
       for (int c = 0; c < (kEach > 32 ? 2 : 1); ++c) slot[c * 32 + lane] = next[c];
       __syncwarp();
@@ -263,7 +265,7 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl& 
 
 // A warp per owner sends it its tokens.
 template <int MT, bool GATED>
-__device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl& ctl, uint32_t smem, int owned, int live, int rank) {
+__device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl<MT>& ctl, uint32_t smem, int owned, int live, int rank) {
   using L = Narrow<MT, GATED>;
   const int owner = (threadIdx.x >> 5) - kNarrowFirstSum, tokens = min(owned, live - owner * owned);
   if (owner >= a.splits || tokens <= 0) return true;
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
                       NarrowArgs a) {
   using L = Narrow<MT, GATED>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ NarrowControl ctl;
+  __shared__ NarrowControl<MT> ctl;
   const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, rank = static_cast<int>(cluster_rank());
   const int tile = static_cast<int>(blockIdx.x) / a.splits, row0 = static_cast<int>(blockIdx.y) * MT;
@@ -427,13 +429,13 @@ template <int MT, bool GATED, bool ROWS>
 int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, NarrowArgs a, const NarrowPlan& plan, cudaStream_t st) {
   using L = Narrow<MT, GATED>;
   const int each = plan.each(a.blocks);
-  const size_t room = L::kTwo ? 108 * 1024 : 220 * 1024;
-  const int tiles_of_x = ROWS ? each : 0;
+  const size_t room = L::kTwo ? 109 * 1024 : 220 * 1024;
+  const int tiles_of_x = ROWS ? each : 0, live = static_cast<int>(a.M < MT ? a.M : MT);
   a.splits = plan.splits;
   a.stages = each < kNarrowStages ? each : kNarrowStages;
-  while (a.stages > 1 && L::smem(a.stages, tiles_of_x, a.splits) > room) --a.stages;
+  while (a.stages > 1 && L::smem(a.stages, tiles_of_x, a.splits, live) > room) --a.stages;
   a.ring = L::ring(a.stages, tiles_of_x);
-  const size_t smem = L::smem(a.stages, tiles_of_x, a.splits);
+  const size_t smem = L::smem(a.stages, tiles_of_x, a.splits, live);
   const void* kernel = reinterpret_cast<const void*>(fp8_narrow_kernel<MT, GATED, ROWS>);
   const int rc = allow_smem(kernel, smem > 64 * 1024 ? smem : 64 * 1024);  // with the static part, 48 KB are soon passed
   if (rc) return rc;
