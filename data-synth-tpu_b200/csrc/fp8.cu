@@ -36,13 +36,6 @@ __device__ __forceinline__ void load8(const void* row, int at, int width, float 
   }
 }
 
-__device__ __forceinline__ uint32_t most8(const float (&f)[8]) {
-  uint32_t most = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) most = max(most, magnitude(f[j]));
-  return most;
-}
-
 struct RowsArgs {
   const void* x;
   int64_t stride, ld;
@@ -68,25 +61,42 @@ __global__ void __launch_bounds__(kThreads) fp8_rows_kernel(RowsArgs a) {
   const void* from = F32 ? static_cast<const void*>(static_cast<const float*>(a.x) + row * a.stride)
                          : static_cast<const void*>(static_cast<const uint16_t*>(a.x) + row * a.stride);
   float f[U][8];
+  uint32_t most[U];
+  if constexpr (ALIGNED && !F32) {
+    uint4 v[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int at = (block0 + 2 * u) * kFp8Block;
-    if (ALIGNED) {
-      load8<F32, true>(from, at + in * 8, a.width, f[u]);
-    } else {
+    for (int u = 0; u < U; ++u) {
+      const int at = (block0 + 2 * u) * kFp8Block + in * 8;
+      v[u] = at < a.width ? ld_guarded_v4(static_cast<const uint16_t*>(from) + at) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int k = at + j * 16 + in;
-        f[u][j] = 0.f;
-        if (k < a.width) f[u][j] = F32 ? static_cast<const float*>(from)[k] : bf16_to_f32(static_cast<const uint16_t*>(from)[k]);
+    for (int u = 0; u < U; ++u) {
+      most[u] = most8(v[u]);
+      unpack8(v[u], f[u]);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = (block0 + 2 * u) * kFp8Block;
+      if (ALIGNED) {
+        load8<F32, true>(from, at + in * 8, a.width, f[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int k = at + j * 16 + in;
+          f[u][j] = 0.f;
+          if (k < a.width) f[u][j] = F32 ? static_cast<const float*>(from)[k] : bf16_to_f32(static_cast<const uint16_t*>(from)[k]);
+        }
       }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) most[u] = most8(f[u]);
   }
+  block_most(most);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int block = block0 + 2 * u, at = block * kFp8Block + in * 8;
-    const uint32_t most = block_most(most8(f[u]));
-    const Fp8Divisor by(most);
+    const Fp8Divisor by(most[u]);
     uint2 codes = make_uint2(by.codes4(f[u]), by.codes4(f[u] + 4));
     if (!ALIGNED) {
       uint8_t* mine = turned[threadIdx.x >> 4];
@@ -97,7 +107,7 @@ __global__ void __launch_bounds__(kThreads) fp8_rows_kernel(RowsArgs a) {
       codes = *reinterpret_cast<const uint2*>(mine + in * 8);
     }
     if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = codes;
-    if (block < a.blocks && in == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = fp8_scale(most);
+    if (block < a.blocks && in == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = fp8_scale(most[u]);
   }
 }
 

@@ -68,11 +68,44 @@ __device__ __forceinline__ float fp8_scale(uint32_t most_bits) {
   return most_bits == 0x7f800000u ? q : r;
 }
 
-// The largest of 16 lanes' (a block's: 8 values each) magnitudes, in all of them.
-__device__ __forceinline__ uint32_t block_most(uint32_t most) {
+// The larger magnitude of two and of three FP32, NaN above everything (its bits too), in one instruction each.
+__device__ __forceinline__ float abs_max(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+__device__ __forceinline__ float abs_max(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+// The bits of the largest magnitude of eight values, as FP32 and as packed BF16 (whose magnitudes are in the order of
+// their bits).
+__device__ __forceinline__ uint32_t most8(const float (&f)[8]) {
+  return __float_as_uint(abs_max(abs_max(f[0], f[1], f[2]), abs_max(f[3], f[4], f[5]), abs_max(f[6], f[7])));
+}
+__device__ __forceinline__ uint32_t most8(const uint4& v) {
+  constexpr uint32_t m = 0x7fff7fffu;
+  const uint32_t w = __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return max(w << 16, w & 0xffff0000u);
+}
+
+// The largest of 16 lanes' (a block's: 8 values each) magnitudes, in all of them, for N blocks per half warp at once.
+template <int N>
+__device__ __forceinline__ void block_most(uint32_t (&most)[N]) {
+  if (threadIdx.x & 16) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  return most;
+    for (int i = 0; i < N; ++i) most[i] = __reduce_max_sync(0xffff0000u, most[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) most[i] = __reduce_max_sync(0x0000ffffu, most[i]);
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ uint32_t block_most(uint32_t most) {
+  uint32_t m[1] = {most};
+  block_most(m);
+  return m[0];
 }
 
 }  // namespace qk

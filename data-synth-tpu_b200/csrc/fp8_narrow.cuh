@@ -156,17 +156,8 @@ __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowContr
       v[i] = row < a.M && b < count && at < a.width ? ld_guarded_v4(a.x + row * a.x_stride + at) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      float f[8];
-      unpack8(v[i], f);
-      most[i] = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most[i] = max(most[i], magnitude(f[j]));
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+    for (int i = 0; i < kAtOnce; ++i) most[i] = most8(v[i]);
+    block_most(most);
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const int unit = first + (half & 1) + 16 * i, row = unit & mask, b = unit >> a.row_shift;
