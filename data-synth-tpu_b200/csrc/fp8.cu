@@ -156,25 +156,24 @@ struct NormArgs {
 };
 
 // Eight values of a row's s and p = s gamma from `at`: the sum is kept, p comes out, the squares are added to `ss`.
-__device__ __forceinline__ void norm8(const NormArgs& a, int64_t row, int at, const uint4& x, const uint4& y, const uint4& gamma, float (&p)[8],
-                                      float& ss) {
-  float g[8];
-  unpack8(x, p);
-  unpack8(gamma, g);
+__device__ __forceinline__ void norm8(const NormArgs& a, int64_t row, int at, uint4 x, const uint4& y, const uint4& gamma, float (&p)[8],
+                                      uint64_t& ss) {
   if (a.y) {
-    float h[8];
-    unpack8(y, h);
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(__fadd_rn(p[2 * j], h[2 * j]), __fadd_rn(p[2 * j + 1], h[2 * j + 1]));
-    const uint4 s = make_uint4(w[0], w[1], w[2], w[3]);
-    if (at < a.width) *reinterpret_cast<uint4*>(a.sum + row * a.width + at) = s;
-    unpack8(s, p);
+    for (int j = 0; j < 4; ++j) {
+      float u, v;
+      f32x2_split(f32x2_add(f32x2_of(word(x, j)), f32x2_of(word(y, j))), u, v);
+      w[j] = pack_bf16x2(u, v);
+    }
+    x = make_uint4(w[0], w[1], w[2], w[3]);
+    if (at < a.width) *reinterpret_cast<uint4*>(a.sum + row * a.width + at) = x;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    ss = fmaf(p[j], p[j], ss);
-    p[j] *= g[j];
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t s = f32x2_of(word(x, j));
+    ss = f32x2_fma(s, s, ss);
+    f32x2_split(f32x2_mul(s, f32x2_of(word(gamma, j))), p[2 * j], p[2 * j + 1]);
   }
 }
 
@@ -194,7 +193,7 @@ __global__ void __launch_bounds__(kRowBlock) fp8_norm_kernel(NormArgs a) {
   const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  float ss = 0.f;
+  uint64_t ss = 0;
   uint32_t most[kRowChunks];
 #pragma unroll
   for (int c = 0; c < kRowChunks; ++c) {
@@ -209,7 +208,9 @@ __global__ void __launch_bounds__(kRowBlock) fp8_norm_kernel(NormArgs a) {
     const Fp8Divisor by(most[c]);
     if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(p), by.codes4(p + 4));
   }
-  const float r = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(ss, red), static_cast<float>(a.width)), a.eps));
+  float even, odd;
+  f32x2_split(ss, even, odd);
+  const float r = rsqrtf(__fadd_rn(__fdiv_rn(block_sum(even + odd, red), static_cast<float>(a.width)), a.eps));
   if ((lane & 15) == 0) {
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) {
@@ -219,9 +220,11 @@ __global__ void __launch_bounds__(kRowBlock) fp8_norm_kernel(NormArgs a) {
   }
 }
 
-// Many rows: a warp each, four loads of either addend in flight, no barrier. The sums are in another order.
-constexpr int kNormAhead = 4;
-__global__ void __launch_bounds__(kThreads) fp8_norm_rows_kernel(NormArgs a) {
+// Many rows: a warp each, kNormAhead loads of either addend in flight, no barrier. The sums are in another order.
+// 64 registers, for four CTAs per SM: 4096 rows of 8192 take 43 us (76 registers: 51), 16384 of 2048 40 (41). Rows of 512
+// and less have two loads: 16384 of 512 take 13 us, with four 17.
+template <int kNormAhead>
+__global__ void __launch_bounds__(kThreads, 4) fp8_norm_rows_kernel(NormArgs a) {
   __shared__ float scale[kThreads / 32][kMaxRowWidth / kFp8Block];
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -229,33 +232,42 @@ __global__ void __launch_bounds__(kThreads) fp8_norm_rows_kernel(NormArgs a) {
   pdl_trigger();
   if (row >= a.rows) return;
   float* mine = scale[threadIdx.x >> 5];
-  float ss = 0.f;
+  uint64_t ss = 0;
 #pragma unroll 1
   for (int at0 = 0; at0 < a.width; at0 += kNormAhead * 256) {
-    uint4 x[kNormAhead], y[kNormAhead];
+    uint4 x[kNormAhead], y[kNormAhead], g[kNormAhead];
 #pragma unroll
     for (int c = 0; c < kNormAhead; ++c) {
       const int at = at0 + c * 256 + lane * 8;
       x[c] = load16_rw(a.x + row * a.width, at, a.width);
       y[c] = a.y ? load16_rw(a.y + row * a.width, at, a.width) : x[c];
+      g[c] = load16(a.gamma, at, a.width);
     }
+    float p[kNormAhead][8];
+    uint32_t most[kNormAhead];
 #pragma unroll
     for (int c = 0; c < kNormAhead; ++c) {
       const int at = at0 + c * 256 + lane * 8;
-      if (at0 + c * 256 >= a.width) break;  // the same for the warp
-      float p[8];
-      norm8(a, row, at, x[c], y[c], load16(a.gamma, at, a.width), p, ss);
-      const uint32_t most = block_most(most8(p));
-      const Fp8Divisor by(most);
+      norm8(a, row, at, x[c], y[c], g[c], p[c], ss);
+      most[c] = most8(p[c]);
+    }
+    block_most(most);
+#pragma unroll
+    for (int c = 0; c < kNormAhead; ++c) {
+      const int at = at0 + c * 256 + lane * 8;
+      const Fp8Divisor by(most[c]);
       if (at < a.width) {
-        *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(p), by.codes4(p + 4));
-        if ((lane & 15) == 0) mine[at / kFp8Block] = fp8_scale(most);
+        *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(p[c]), by.codes4(p[c] + 4));
+        if ((lane & 15) == 0) mine[at / kFp8Block] = fp8_scale(most[c]);
       }
     }
   }
+  float even, odd;
+  f32x2_split(ss, even, odd);
+  float sum = even + odd;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float r = rsqrtf(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.width)), a.eps));
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float r = rsqrtf(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.width)), a.eps));
   __syncwarp();
   for (int b = lane; b < (a.width + kFp8Block - 1) / kFp8Block; b += 32) a.scales[static_cast<int64_t>(b) * a.rows + row] = mine[b] * r;
 }
@@ -334,9 +346,11 @@ int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma,
   QK_REQUIRE(x && gamma && codes && scales && (!y || x_out), "null pointer");
   QK_REQUIRE(aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(x_out) && aligned16(codes), "pointers must be 16-byte aligned");
   NormArgs a{x, y, gamma, rows, ld, width, eps, x_out, codes, scales};
-  cudaError_t e = rows >= 8ll * sm_count()
-                      ? launch_dependent(fp8_norm_rows_kernel, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(kThreads), 0, as_stream(stream), a)
-                      : launch_dependent(fp8_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(kRowBlock), 0, as_stream(stream), a);
+  const dim3 warps(static_cast<unsigned>((rows + 7) / 8));
+  cudaStream_t st = as_stream(stream);
+  cudaError_t e = rows < 8ll * sm_count() ? launch_dependent(fp8_norm_kernel, dim3(static_cast<unsigned>(rows)), dim3(kRowBlock), 0, st, a)
+                  : width > 512           ? launch_dependent(fp8_norm_rows_kernel<4>, warps, dim3(kThreads), 0, st, a)
+                                          : launch_dependent(fp8_norm_rows_kernel<2>, warps, dim3(kThreads), 0, st, a);
   if (e != cudaSuccess) return cuda_error(e, "fp8_norm_kernel");
   count_launch();
   return QK_OK;
