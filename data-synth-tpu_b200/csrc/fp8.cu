@@ -36,6 +36,15 @@ __device__ __forceinline__ void load8(const void* row, int at, int width, float 
   }
 }
 
+// Eight codes, of which `left` belong to the row: nothing is written past its width.
+__device__ __forceinline__ void store8(uint8_t* to, uint2 codes, int left) {
+  if (left >= 8) {
+    *reinterpret_cast<uint2*>(to) = codes;
+  } else {
+    for (int j = 0; j < left; ++j) to[j] = static_cast<uint8_t>((j < 4 ? codes.x : codes.y) >> (8 * (j & 3)));
+  }
+}
+
 struct RowsArgs {
   const void* x;
   int64_t stride, ld;
@@ -106,7 +115,7 @@ __global__ void __launch_bounds__(kThreads) fp8_rows_kernel(RowsArgs a) {
       __syncwarp();
       codes = *reinterpret_cast<const uint2*>(mine + in * 8);
     }
-    if (at < a.width) *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = codes;
+    store8(a.codes + row * a.ld + at, codes, a.width - at);
     if (block < a.blocks && in == 0) a.scales[static_cast<int64_t>(block) * a.rows + row] = fp8_scale(most[u]);
   }
 }
@@ -139,8 +148,7 @@ __global__ void __launch_bounds__(kThreads) fp8_blocks_kernel(RowsArgs a) {
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int64_t row = static_cast<int64_t>(blockIdx.y) * kFp8Block + i * (kThreads / 16) + half;
-    if (row < a.rows && at < a.width)
-      *reinterpret_cast<uint2*>(a.codes + row * a.ld + at) = make_uint2(by.codes4(f[i]), by.codes4(f[i] + 4));
+    if (row < a.rows) store8(a.codes + row * a.ld + at, make_uint2(by.codes4(f[i]), by.codes4(f[i] + 4)), a.width - at);
   }
   if (threadIdx.x == 0) a.scales[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = fp8_scale(most);
 }
@@ -293,7 +301,7 @@ int qk_fp8_quantize(const void* x, int in_dtype, int64_t x_stride, int64_t rows,
                     float* scales, qk_stream_t stream) {
   QK_REQUIRE(in_dtype == QK_OUT_F32 || in_dtype == QK_OUT_BF16, "x must be FP32 or BF16");
   QK_REQUIRE(rows >= 0 && width >= 1 && width < (1ll << 31) - 256 && x_stride >= width, "invalid rows, width or stride");
-  QK_REQUIRE(ld >= (width + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
+  QK_REQUIRE(ld >= width && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
   if (rows == 0) return QK_OK;
   QK_REQUIRE(x && codes && scales, "null pointer");
   QK_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
@@ -320,7 +328,7 @@ int qk_fp8_quantize_blocks(const void* w, int in_dtype, int64_t w_stride, int64_
                            float* scales, qk_stream_t stream) {
   QK_REQUIRE(in_dtype == QK_OUT_F32 || in_dtype == QK_OUT_BF16, "w must be FP32 or BF16");
   QK_REQUIRE(rows >= 0 && width >= 1 && width < (1ll << 31) - 256 && w_stride >= width, "invalid rows, width or stride");
-  QK_REQUIRE(ld >= (width + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
+  QK_REQUIRE(ld >= width && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
   QK_REQUIRE(rows <= 65535ll * 128, "too many rows");
   if (rows == 0) return QK_OK;
   QK_REQUIRE(w && codes && scales, "null pointer");
@@ -341,7 +349,7 @@ int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma,
                     uint8_t* codes, int64_t ld, float* scales, qk_stream_t stream) {
   QK_REQUIRE(rows >= 0 && rows < (1ll << 31) && width >= 8 && width % 8 == 0 && width <= kMaxRowWidth,
              "width must be a multiple of 8, 8192 at most");
-  QK_REQUIRE(ld >= (width + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
+  QK_REQUIRE(ld >= width && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
   if (rows == 0) return QK_OK;
   QK_REQUIRE(x && gamma && codes && scales && (!y || x_out), "null pointer");
   QK_REQUIRE(aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(x_out) && aligned16(codes), "pointers must be 16-byte aligned");

@@ -177,7 +177,7 @@ int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t 
   int rc = check_operands(x, x_ld, x_scales, M, K, gate, gate_ld, gate_scales, N, codes);
   if (!rc) rc = check_operands(x, x_ld, x_scales, M, K, up, up_ld, up_scales, N, codes);
   if (rc || M == 0) return rc;
-  QK_REQUIRE(ld >= (N + 15) / 16 * 16 && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
+  QK_REQUIRE(ld >= N && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
   QK_REQUIRE(aligned16(codes) && scales && (reinterpret_cast<uintptr_t>(scales) & 3) == 0, "misaligned or null output");
   const Weights u{up, up_ld, up_scales};
   return product(x, x_ld, x_scales, M, K, Weights{gate, gate_ld, gate_scales}, &u, N, false, codes, ld, scales, as_stream(stream));

@@ -295,7 +295,11 @@ __device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t sums, 
         most = max(most, magnitude(f[0][j]));
       }
       most = __reduce_max_sync(0xffffffffu, most);
-      if (n < a.N) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + row * a.ld + n) = Fp8Divisor(most).codes4(f[0]);
+      const uint32_t codes = Fp8Divisor(most).codes4(f[0]);
+      uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.ld + n;
+      if (n + 4 <= a.N) *reinterpret_cast<uint32_t*>(out) = codes;
+      else
+        for (int j = 0; n + j < a.N; ++j) out[j] = static_cast<uint8_t>(codes >> (8 * j));
       if (lane == 0) a.out_scales[static_cast<int64_t>(tile) * a.M + row] = fp8_scale(most);
     } else if (a.f32) {
       float* out = static_cast<float*>(a.out) + row * a.N + n;

@@ -290,17 +290,25 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, c
     most = max(most, lds_at(swap + (half ^ 1) * 512));
     ++swaps;
     const Fp8Divisor by(most);
+    const int col = tile.n * kFp8Block + half * 64;
     if (lane == 0) stores_read<0>();  // the last tile's
     __syncwarp();
+    uint32_t codes[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      sts_v4(staging + lane * 64 + ((j ^ lane >> 1) & 3) * 16,  // in the 64-byte swizzle
-             by.codes4(h + 16 * j), by.codes4(h + 16 * j + 4), by.codes4(h + 16 * j + 8),
-             by.codes4(h + 16 * j + 12));
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0 && row0 < a.M && tile.n * kFp8Block + half * 64 < a.N)
-      store_box(out_map, tile.n * kFp8Block + half * 64, static_cast<int>(row0), staging);
+    for (int j = 0; j < 16; ++j) codes[j] = by.codes4(h + 4 * j);
+    if (col + 64 <= a.N || a.N % 16 == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        sts_v4(staging + lane * 64 + ((j ^ lane >> 1) & 3) * 16, codes[4 * j], codes[4 * j + 1], codes[4 * j + 2], codes[4 * j + 3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && row0 < a.M && col < a.N) store_box(out_map, col, static_cast<int>(row0), staging);  // 64-byte swizzle
+    } else if (row < a.M) {  // a copy writes 16 bytes at a time, also past the end of a row
+      uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.ld + col;
+#pragma unroll
+      for (int j = 0; j < 64; ++j)
+        if (col + j < a.N) out[j] = static_cast<uint8_t>(codes[j / 4] >> (8 * (j & 3)));
+    }
     if (half == 0 && row < a.M) a.out_scales[static_cast<int64_t>(tile.n) * a.M + row] = fp8_scale(most);
   }
   if (lane == 0) stores_read<0>();  // the CTA's shared memory lives until then

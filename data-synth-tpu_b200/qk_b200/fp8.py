@@ -46,9 +46,8 @@ def _blocks(n):
 def _empty_rows(rows, width, device):
     """:class:`Fp8Rows` to be written; rows of codes begin on 16 bytes."""
     pitch = (width + 15) // 16 * 16
-    codes = torch.empty_strided((rows, pitch), (pitch, 1), dtype=_E4M3, device=device)
-    scales = torch.empty_strided(((width + 127) // 128, rows), (rows, 1), dtype=_F32, device=device)
-    return Fp8Rows(codes if pitch == width else codes[:, :width], scales), pitch
+    codes = torch.empty_strided((rows, width), (pitch, 1), dtype=_E4M3, device=device)
+    return Fp8Rows(codes, torch.empty_strided(((width + 127) // 128, rows), (rows, 1), dtype=_F32, device=device)), pitch
 
 
 def _quantised(codes, scales, by_rows, name):
@@ -66,8 +65,7 @@ def _quantised(codes, scales, by_rows, name):
     pitch, step = codes.stride()
     if pitch % 16 or pitch < width or step != 1 or codes.data_ptr() % 16:
         pitch = (width + 15) // 16 * 16
-        fresh = torch.empty_strided((rows, pitch), (pitch, 1), dtype=_E4M3, device=codes.device)[:, :width]
-        codes = fresh.copy_(codes)
+        codes = torch.empty_strided((rows, width), (pitch, 1), dtype=_E4M3, device=codes.device).copy_(codes)
     if scales.dtype != _F32 or scales.get_device() != index:
         scales = scales.to(device=codes.device, dtype=_F32)
     return codes, pitch, scales if scales.is_contiguous() else scales.contiguous()
@@ -144,7 +142,7 @@ def pack_fp8(weight):
     weight, code, stride, index = _matrix(weight, "weight")
     rows, width = weight.shape
     pitch = (width + 15) // 16 * 16
-    codes = torch.empty((rows, pitch), dtype=_E4M3, device=weight.device)[:, :width]
+    codes = torch.empty_strided((rows, width), (pitch, 1), dtype=_E4M3, device=weight.device)
     scales = torch.empty((_blocks(rows), _blocks(width)), dtype=_F32, device=weight.device)
     _lib.call_at(index, "qk_fp8_quantize_blocks", weight.data_ptr(), code, stride, rows, width, codes.data_ptr(), pitch,
                  scales.data_ptr())

@@ -140,12 +140,13 @@ int qk_linear_bf16_check(const void* workspace, qk_stream_t stream);
 
 /* ---- FP8 dense path ---------------------------------------------------------------
  * No counterpart in the reference (its dense projections are BF16, math.py:10-16). A matrix is
- * e4m3 codes, rows `ld` bytes apart (a multiple of 16; the first 16-byte aligned), with one FP32
- * scale for each block of 128 columns: of a row for activations (scales [ceil(width / 128)][rows]),
- * of 128 rows for weights (scales [ceil(rows / 128)][ceil(width / 128)]); the last blocks may be
- * short. A block whose largest magnitude is m = max(max |x|, 2^-100) has scale m / 448 and codes
- * e4m3(448 x / m), the quotient rounded to nearest, ties to even; one that holds a NaN is NaN,
- * beside an infinity every value is NaN too (0 times its scale). */
+ * e4m3 codes, rows `ld` bytes apart (a multiple of 16; the first 16-byte aligned; nothing past the
+ * width is read or written), with one FP32 scale for each block of 128 columns: of a row for
+ * activations (scales [ceil(width / 128)][rows]), of 128 rows for weights (scales
+ * [ceil(rows / 128)][ceil(width / 128)]); the last blocks may be short. A block whose largest
+ * magnitude is m = max(max |x|, 2^-100) has scale m / 448 and codes e4m3(448 x / m), the quotient
+ * rounded to nearest, ties to even; one that holds a NaN is NaN, beside an infinity every value is
+ * NaN too (0 times its scale). */
 
 /* x: FP32 or BF16 (in_dtype), rows x_stride values apart. */
 int qk_fp8_quantize(const void* x, int in_dtype, int64_t x_stride, int64_t rows, int64_t width,

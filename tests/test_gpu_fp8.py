@@ -572,3 +572,34 @@ def test_offsets_past_31_bits(cuda_device):
     small, _ = rms_norm_fp8(tail, gamma, residual=tail)
     assert torch.equal(normed.codes[-300:].float(), small.codes.float())
     assert torch.equal(total[-300:], (tail.float() * 2).to(torch.bfloat16))
+
+
+def test_nothing_is_written_past_the_rows(cuda_device):
+    """Codes, scales and outputs in buffers of other bytes: those between and behind the rows stay."""
+    import torch
+
+    from qk_b200 import _lib
+    from qk_b200.fp8 import quantize_fp8
+
+    def guarded(rows, ld, kind):
+        store = torch.full(((rows + 1) * ld,), 0xAA, dtype=torch.uint8, device=cuda_device)
+        return store, store.view(rows + 1, ld), kind
+
+    P, st = _lib.ptr, _lib.stream_handle(cuda_device)
+    for m, k, n in ((3, 133, 77), (40, 264, 130), (300, 1111, 1001), (2000, 300, 1290)):
+        x, w = activations(m, k, cuda_device), packed(n, k, cuda_device)
+        rows, ld = quantize_fp8(x), (max(k, n) + 47) // 16 * 16
+        for name in ("qk_fp8_quantize", "qk_fp8_quantize_blocks"):
+            store, codes, _ = guarded(m, ld, name)
+            scales = torch.full((((k + 127) // 128) * m + 8,), 7.0, device=cuda_device)
+            _lib.call(name, P(x), 1, k, m, k, P(store), ld, P(scales), st)
+            assert (codes[:m, k:] == 0xAA).all() and (codes[m] == 0xAA).all() and (scales[-8:] == 7).all(), name
+        store, codes, _ = guarded(m, ld, "gated")
+        scales = torch.full((((n + 127) // 128) * m + 8,), 7.0, device=cuda_device)
+        args = [P(rows.codes), rows.codes.stride(0), P(rows.scales), m, k] + [P(w.codes), w.codes.stride(0), P(w.scales)] * 2
+        _lib.call("qk_fp8_gated", *args, n, P(store), ld, P(scales), st)
+        assert (codes[:m, n:] == 0xAA).all() and (codes[m] == 0xAA).all() and (scales[-8:] == 7).all()
+        for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1)):
+            out = torch.full((m * n + 64,), 7.0, dtype=dtype, device=cuda_device)
+            _lib.call("qk_fp8_matmul", *args[:8], n, code, P(out), st)
+            assert (out[m * n:] == 7).all()
