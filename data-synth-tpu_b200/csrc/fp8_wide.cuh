@@ -5,8 +5,17 @@
 // both. A block of 128 columns of K is one row of the 128-byte swizzle and twice four MMAs, for either half of the
 // columns; their sums go to one of two buffers of 128 TMEM columns for that half (in each CTA its 128 rows), and the
 // half's four warps per CTA add them, times the block's two scales, to FP32 sums in their registers (a row and 128
-// columns per thread) while the tensor core fills the three others. A buffer's round trip (MMAs, commit, sums,
-// release) is what bounds the kernel: with two buffers of 256 columns it took 307 us where this takes .
+// columns per thread) while the tensor core fills the three others. A warp issues each half's MMAs: one for both took
+// about 900 cycles a block for its waits and issues, more than the products.
+//
+// Measured (B200, 1.9 GHz, in bursts / in a loop of seconds under the power cap):
+//   x 16384 x 2048 of codes, 9216 columns, BF16 out   285 / 330 us, 2170 / 1870 TFLOP/s
+//   4096 x 8192, 8192 columns                         235 / 273 us, 2340 / 2010 TFLOP/s
+//   gated, 8192 x 2048, 6144 columns of each          225 / 235 us, 1830 / 1750 TFLOP/s
+// What bounds it: without the additions to the sums the first takes 258 us, without them and the output 210, without the
+// exchange of buffers too 188 (3300 TFLOP/s): the sums' instructions, a buffer's round trip and shared memory (x's tile
+// is read once for either half), in this order, and in long loops the power. One buffer of 256 columns for both halves
+// saves that second read, but takes 317 us; sixteen warps for the sums take 360, five or six stages nothing less.
 #pragma once
 
 #include "fp8_product.cuh"
@@ -83,7 +92,7 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
 
 // An arrival that orders nothing but what came before by itself: the loads from tensor memory are complete (wait::ld).
 // With .release.cluster, which waits for this thread's stores to be seen in the cluster, the round trip of a buffer
-// took 1.4 us and 16384 x 2048 by 9216 580 us (now 307).
+// took 1.4 us and 16384 x 2048 by 9216 580 us, where this took 307.
 __device__ __forceinline__ void cluster_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
