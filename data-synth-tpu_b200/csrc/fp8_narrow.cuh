@@ -8,8 +8,8 @@
 // its weights are on their way: that saves a launch, and the values are the same.
 //
 // Measured in a graph of calls over weights larger than L2 (floor: the weights' bytes at the measured HBM rate):
-//   1 row of BF16, 2048 x 9216        5.5 us, floor 2.9 (18.9 MB: 3.4 TB/s);  8 rows 6.4, 32 rows (two launches) 9.4
-//   64 rows of BF16, 4096 x 2048      8.6 us, floor 1.4 (two launches; from codes 6.6);  1 row 4.0, floor 1.3
+//   1 row of BF16, 2048 x 9216        5.5 us, floor 2.9 (18.9 MB: 3.4 TB/s);  8 rows 6.4, 32 rows 10.3
+//   64 rows of BF16, 4096 x 2048      10.9 us, floor 1.4 (from codes 6.6);  1 row 4.0, floor 1.3
 //   gated, 32 rows of codes, 2048 x 2 x 6144   10.5 us, floor 3.9
 // What bounds it is latency: the set-up, the first copy from memory (2 us), then for each block the issue of its MMAs
 // (about 300 cycles), its sums and, at the end, the exchange and the output, most of it instructions that run once
@@ -24,9 +24,11 @@ namespace {
 constexpr int kNarrowStages = 8, kNarrowSumWarps = 8, kNarrowFirstSum = 2;
 constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
 constexpr int kMostSplits = 8;       // the portable cluster size
-// Rows of BF16, and blocks of them, that a CTA quantises itself, at most: 32 rows of 4096 x 2048 (128 blocks per CTA) take
-// 7.2 us, with a launch of its own for that 7.5 and 4 us more of the host, 32 of 2048 x 9216 (256) 11.4 and 9.4.
-constexpr int kInlineRows = 64, kInline = 128, kInlineTokens = 256;  // kInlineTokens: of their tiles in shared memory
+// Rows of BF16, and blocks of them, that a CTA quantises itself, at most (gated: half, their rings are short). 32 rows of
+// 4096 x 2048 (128 blocks per CTA) take 7.2 us, with a launch of its own for that 7.5; 32 of 2048 x 9216 (256) 10.3 and
+// 9.5, 64 of 4096 x 2048 (256) 10.9 and 8.6, but that launch takes the host 4 us more, which is where such calls end:
+// by wall clock 11.1 and 13.5, 11.1 and 13.3. Gated, 192 blocks (32 rows of 2048 x 6144) cost 3 us and save 1.
+constexpr int kInlineRows = 64, kInline = 256, kInlineTokens = 256;  // kInlineTokens: of their tiles in shared memory
 
 struct NarrowArgs {
   int64_t M;
@@ -147,11 +149,10 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
 
 // The CTA's blocks of x, quantised into the operand tiles and ctl.scales [block][MT]. Rows past M hold whatever the
 // memory held: they make columns of the product that nobody reads.
-template <int MT>
+template <int MT, int kAtOnce>
 __device__ __forceinline__ void narrow_quantise(const NarrowArgs& a, NarrowControl<MT>& ctl, uint32_t tiles, int b0, int count) {
   const int lane = threadIdx.x & 31, in = lane & 15;
   // 16 half warps: each takes every 16th of (block, row) pairs, kAtOnce of them at a time
-  constexpr int kAtOnce = 4;
   const int half = (threadIdx.x - kNarrowFirstSum * 32) >> 4, units = count << a.row_shift;
   const int mask = (1 << a.row_shift) - 1;
 #pragma unroll 1
@@ -369,7 +370,8 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
   if (warp == 1) tmem_alloc(&ctl.tmem, L::kAlloc);
   pdl_wait();
   if (ROWS && warp >= kNarrowFirstSum) {
-    narrow_quantise<MT>(a, ctl, smem + a.stages * L::kBytesW, b0, count);
+    if (MT > 16 && count << a.row_shift > 64) narrow_quantise<MT, 8>(a, ctl, smem + a.stages * L::kBytesW, b0, count);
+    else narrow_quantise<MT, 4>(a, ctl, smem + a.stages * L::kBytesW, b0, count);
     fence_proxy_async_smem();
   }
   tc_fence_before();
@@ -411,20 +413,21 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
 // takes an SM for itself, of 8 for 15, and one cluster too many costs a second round (64 rows of 4096 x 2048 with
 // eight: 7.2 us where two fit an SM, 11.1 else). So all but the largest leave room for a second, and those have four.
 struct NarrowPlan {
-  int tokens, splits;
+  int tokens, splits, most;  // most: blocks of rows that a CTA quantises itself
   NarrowPlan(int64_t M, int64_t N, int blocks, bool gated) {
     tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 || gated ? 64 : 128;
     const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = sm_count() / tiles;
     splits = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
     if (tokens * (gated ? 2 : 1) > 64) splits = tiles * 4 <= sm_count() * 7 / 8 ? 4 : splits > 2 ? 2 : splits;
     if (splits > blocks) splits = blocks;
+    most = gated ? kInline / 2 : kInline;
   }
   int each(int blocks) const { return (blocks + splits - 1) / splits; }
   // Whether the CTAs can quantise rows of x themselves.
   bool quantises(int64_t M, int blocks) const {
     int rows = 1;
     while (rows < M && rows < kInlineRows) rows *= 2;
-    return M <= kInlineRows && rows * each(blocks) <= kInline && tokens * each(blocks) <= kInlineTokens;
+    return M <= kInlineRows && rows * each(blocks) <= most && tokens * each(blocks) <= kInlineTokens;
   }
 };
 
