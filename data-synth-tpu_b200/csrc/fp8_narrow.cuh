@@ -28,7 +28,7 @@ constexpr int kMostSplits = 8;       // the portable cluster size
 // 4096 x 2048 (128 blocks per CTA) take 7.2 us, with a launch of its own for that 7.5; 32 of 2048 x 9216 (256) 10.3 and
 // 9.5, 64 of 4096 x 2048 (256) 10.9 and 8.6, but that launch takes the host 4 us more, which is where such calls end:
 // by wall clock 11.1 and 13.5, 11.1 and 13.3. Gated, 192 blocks (32 rows of 2048 x 6144) cost 3 us and save 1.
-constexpr int kInlineRows = 64, kInline = 256, kInlineTokens = 256;  // kInlineTokens: of their tiles in shared memory
+constexpr int kInline = 256, kInlineTokens = 256;  // kInlineTokens: of their tiles in shared memory
 
 struct NarrowArgs {
   int64_t M;
@@ -412,22 +412,38 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
 // tiles: 4 / 6 / 8 take 4.8 / 4.7 / 4.4). A cluster lies within a group of SMs: of 4 there is room for 33 where a CTA
 // takes an SM for itself, of 8 for 15, and one cluster too many costs a second round (64 rows of 4096 x 2048 with
 // eight: 7.2 us where two fit an SM, 11.1 else). So all but the largest leave room for a second, and those have four.
+// Tokens per tile: all of them up to 64 (gated 32). Beyond, tiles of 64 (32) or of twice as many, which read the
+// weights less often but have only one CTA per SM: a product takes about 3.7 us and 0.5 for each of a CTA's blocks with
+// the first, 5.8 and 0.56 with the second, so the first are taken where a CTA gets up to four blocks more (96 rows of
+// 4096 x 2048: 7.8 and 9.3 us, 512 of 1024 x 1000 5.7 and 7.4; but 128 of 2048 x 9216 12.4 and 11.4. Gated, 128 rows
+// of 2048 x 512 11.9 and 16.1 with the down product, of 2048 x 6144 29.6 and 30.7).
 struct NarrowPlan {
-  int tokens, splits, most;  // most: blocks of rows that a CTA quantises itself
+  int tokens, splits, rows, most;  // rows: that a CTA quantises itself, at most, and (most) blocks of them
   NarrowPlan(int64_t M, int64_t N, int blocks, bool gated) {
-    tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 || gated ? 64 : 128;
-    const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = sm_count() / tiles;
-    splits = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
-    if (tokens * (gated ? 2 : 1) > 64) splits = tiles * 4 <= sm_count() * 7 / 8 ? 4 : splits > 2 ? 2 : splits;
-    if (splits > blocks) splits = blocks;
+    const int small = gated ? 32 : 64;
+    tokens = M <= 16 ? 16 : M <= 32 ? 32 : small;
+    splits = splits_of(M, N, blocks, gated);
+    if (M > small) {
+      const int few = each(blocks), with_few = splits;
+      tokens = 2 * small;
+      splits = splits_of(M, N, blocks, gated);
+      if (few <= each(blocks) + 4) tokens = small, splits = with_few;
+    }
+    rows = small;
     most = gated ? kInline / 2 : kInline;
+  }
+  int splits_of(int64_t M, int64_t N, int blocks, bool gated) const {
+    const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = sm_count() / tiles;
+    int n = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
+    if (tokens * (gated ? 2 : 1) > 64) n = tiles * 4 <= sm_count() * 7 / 8 ? 4 : n > 2 ? 2 : n;
+    return n < blocks ? n : blocks;
   }
   int each(int blocks) const { return (blocks + splits - 1) / splits; }
   // Whether the CTAs can quantise rows of x themselves.
   bool quantises(int64_t M, int blocks) const {
-    int rows = 1;
-    while (rows < M && rows < kInlineRows) rows *= 2;
-    return M <= kInlineRows && rows * each(blocks) <= most && tokens * each(blocks) <= kInlineTokens;
+    int power = 1;
+    while (power < M && power < rows) power *= 2;
+    return M <= rows && power * each(blocks) <= most && tokens * each(blocks) <= kInlineTokens;
   }
 };
 
@@ -471,9 +487,12 @@ int launch_narrow(bool rows, const CUtensorMap& x, const CUtensorMap& w, const C
     return rows ? launch_narrow<16, GATED, true>(x, w, u, a, plan, st) : launch_narrow<16, GATED, false>(x, w, u, a, plan, st);
   if (plan.tokens == 32)
     return rows ? launch_narrow<32, GATED, true>(x, w, u, a, plan, st) : launch_narrow<32, GATED, false>(x, w, u, a, plan, st);
-  if constexpr (!GATED)
-    if (plan.tokens == 128) return launch_narrow<128, GATED, false>(x, w, u, a, plan, st);
-  return rows ? launch_narrow<64, GATED, true>(x, w, u, a, plan, st) : launch_narrow<64, GATED, false>(x, w, u, a, plan, st);
+  if constexpr (GATED) {
+    return launch_narrow<64, true, false>(x, w, u, a, plan, st);  // more rows than a CTA quantises
+  } else {
+    if (plan.tokens == 128) return launch_narrow<128, false, false>(x, w, u, a, plan, st);
+    return rows ? launch_narrow<64, false, true>(x, w, u, a, plan, st) : launch_narrow<64, false, false>(x, w, u, a, plan, st);
+  }
 }
 
 }  // namespace
