@@ -303,7 +303,8 @@ extern "C" {
 int qk_fp8_quantize(const void* x, int in_dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t* codes, int64_t ld,
                     float* scales, qk_stream_t stream) {
   QK_REQUIRE(in_dtype == QK_OUT_F32 || in_dtype == QK_OUT_BF16, "x must be FP32 or BF16");
-  QK_REQUIRE(rows >= 0 && width >= 1 && width < (1ll << 31) - 256 && x_stride >= width, "invalid rows, width or stride");
+  QK_REQUIRE(rows >= 0 && rows < (1ll << 34) && width >= 1 && width < (1ll << 31) - 256 && x_stride >= width,
+             "invalid rows, width or stride");
   QK_REQUIRE(ld >= width && ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart and not overlap");
   if (rows == 0) return QK_OK;
   QK_REQUIRE(x && codes && scales, "null pointer");
@@ -313,7 +314,7 @@ int qk_fp8_quantize(const void* x, int in_dtype, int64_t x_stride, int64_t rows,
   RowsArgs a{x, x_stride, ld, rows, static_cast<int>(width), static_cast<int>((width + 127) / 128), codes, scales};
   const bool aligned = aligned16(x) && x_stride * size % 16 == 0 && width % 8 == 0;
   const int64_t ctas = (rows + 7) / 8;
-  QK_REQUIRE(ctas < (1ll << 31) && a.blocks <= 65535 * 8, "too many rows or columns");
+  QK_REQUIRE(ctas < (1ll << 31) && a.blocks <= 65535 * 8, "too many rows or columns");  // what a grid holds
   cudaStream_t st = as_stream(stream);
   // four blocks per half warp where there is work for all SMs all the same
   const bool many = ctas * a.blocks >= 64ll * sm_count() || a.blocks > 65535 * 2;

@@ -9,10 +9,15 @@
 namespace qk {
 namespace {
 
+// Sizes that a call takes: every product of two of them fits 64 bits, and a grid holds the tiles.
+bool sizes_fit(int64_t M, int64_t K, int64_t N) {
+  constexpr int64_t kMost = (1ll << 31) - 256;
+  return M < kMost && N < kMost && K < kMost && ((M + 127) / 128) * ((N + 127) / 128) < (1ll << 28);
+}
+
 int check_weights(int64_t M, int64_t K, const uint8_t* w, int64_t w_ld, const float* ws, int64_t N, const void* out) {
   QK_REQUIRE(M >= 0 && N >= 1 && K >= 1, "invalid rows, columns or width");
-  QK_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K < (1ll << 31) - 256, "sizes must stay below 2^31 - 256");
-  QK_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) < (1ll << 28), "too many tiles in one call");
+  QK_REQUIRE(sizes_fit(M, K, N), "sizes must stay below 2^31 - 256 and tiles of 128 x 128 below 2^28");
   QK_REQUIRE(w_ld >= K && w_ld % 16 == 0, "rows of codes must be a multiple of 16 bytes apart");
   if (M == 0) return QK_OK;
   QK_REQUIRE(w && ws && out, "null pointer");
@@ -184,7 +189,7 @@ int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t 
 }
 
 size_t qk_fp8_linear_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t N) {
-  return M > 0 && K > 0 && N > 0 ? room_for(in_dtype, M, K, N, false) : 0;
+  return M > 0 && K > 0 && N > 0 && sizes_fit(M, K, N) ? room_for(in_dtype, M, K, N, false) : 0;
 }
 
 int qk_fp8_linear(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const uint8_t* w, int64_t w_ld,
@@ -202,7 +207,7 @@ int qk_fp8_linear(const void* x, int in_dtype, int64_t x_stride, int64_t M, int6
 }
 
 size_t qk_fp8_ffn_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t inner) {
-  return M > 0 && K > 0 && inner > 0 ? room_for(in_dtype, M, K, inner, true) + row_bytes(M, inner) : 0;
+  return M > 0 && K > 0 && inner > 0 && sizes_fit(M, K, inner) ? room_for(in_dtype, M, K, inner, true) + row_bytes(M, inner) : 0;
 }
 
 int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K, const uint8_t* gate, int64_t gate_ld,

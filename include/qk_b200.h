@@ -162,7 +162,8 @@ int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma,
                     int width, float eps, uint16_t* x_out, uint8_t* codes, int64_t ld, float* scales,
                     qk_stream_t stream);
 /* out [M, N] (FP32 or BF16 by out_dtype) = x w^T of x [M, K] (activations) and w [N, K] (weights):
- * the exact products of the codes, FP32 sums, each block's times its two scales. M may be 0. */
+ * the exact products of the codes, FP32 sums, each block's times its two scales. M may be 0; out
+ * shares no memory with x. */
 int qk_fp8_matmul(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t M, int64_t K,
                   const uint8_t* w, int64_t w_ld, const float* w_scales, int64_t N, int out_dtype,
                   void* out, qk_stream_t stream);
@@ -175,14 +176,15 @@ int qk_fp8_gated(const uint8_t* x, int64_t x_ld, const float* x_scales, int64_t 
 /* The product from rows of BF16 or FP32 (in_dtype, x_stride values apart), quantised in the call by
  * the rule of qk_fp8_quantize: the values of qk_fp8_quantize and qk_fp8_matmul. The workspace
  * (256-byte aligned) holds the codes and scales where a launch of its own makes them; where none is
- * needed (few rows of BF16), rows of x must begin on 16 bytes. */
+ * needed (up to 64 rows of BF16, K a multiple of 8), rows of x must begin on 16 bytes. Sizes that a
+ * call refuses need 0 bytes. out shares no memory with x. */
 size_t qk_fp8_linear_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t N);
 int qk_fp8_linear(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K,
                   const uint8_t* w, int64_t w_ld, const float* w_scales, int64_t N, int out_dtype,
                   void* out, void* workspace, size_t workspace_bytes, qk_stream_t stream);
 /* A gated feed-forward block, out [M, N] BF16 = (silu(x gate^T) * (x up^T)) down^T with gate and up
- * [inner, K], down [N, inner]: the values of qk_fp8_quantize, qk_fp8_gated and qk_fp8_matmul. Rows of
- * x must begin on 16 bytes where qk_fp8_linear_workspace_bytes(in_dtype, M, K, inner) is 0. */
+ * [inner, K], down [N, inner]: the values of qk_fp8_quantize, qk_fp8_gated and qk_fp8_matmul. Up to
+ * 32 rows of BF16 with K a multiple of 8 must begin on 16 bytes (others may). out may be x. */
 size_t qk_fp8_ffn_workspace_bytes(int in_dtype, int64_t M, int64_t K, int64_t inner);
 int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t K,
                const uint8_t* gate, int64_t gate_ld, const float* gate_scales, const uint8_t* up,

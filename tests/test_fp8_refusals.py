@@ -105,3 +105,25 @@ def test_python_calls_refuse():
             call()
     with pytest.raises(ValueError):
         SyntheticDecoder(StackConfig(layers=0, dense="fp4"), "cpu")
+
+
+@pytest.mark.parametrize("m,k,n", [(0, 128, 128), (-5, 128, 128), (4, 0, 128), (4, 128, -1), (1 << 62, 1 << 62, 4), (1 << 62, 128, 1 << 62),
+                                   ((1 << 63) - 1, 128, (1 << 63) - 1), (4, (1 << 63) - 1, 4)])
+def test_sizes_that_no_call_takes_need_no_workspace(m, k, n):
+    from qk_b200 import _lib
+
+    lib = _lib.load()
+    for dtype in (0, 1):
+        assert lib.qk_fp8_linear_workspace_bytes(dtype, m, k, n) == 0
+        assert lib.qk_fp8_ffn_workspace_bytes(dtype, m, k, n) == 0
+
+
+@pytest.mark.parametrize("name,at", [("qk_fp8_quantize", 3), ("qk_fp8_quantize_blocks", 3), ("qk_fp8_rms_norm", 3), ("qk_fp8_matmul", 3),
+                                     ("qk_fp8_matmul", 4), ("qk_fp8_matmul", 8), ("qk_fp8_linear", 3), ("qk_fp8_gated", 11),
+                                     ("qk_fp8_ffn", 15)])
+def test_the_largest_sizes_are_refused(name, at):
+    from qk_b200 import _lib
+
+    args = list(GOOD[name])
+    args[at] = (1 << 63) - 1
+    assert getattr(_lib.load(), name)(*args) == _lib.QK_ERR_INVALID_ARGUMENT, _lib.last_error()
