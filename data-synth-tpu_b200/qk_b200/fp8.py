@@ -169,17 +169,22 @@ def fp8_weights(codes, scales, device=None):
     return Fp8Weights(codes, scales)
 
 
-def _output(out, m, n, dtype, index):
+def _output(out, m, n, dtype, index, x=None):
     if out is None:
         return _empty((m, n), (n, 1), dtype, index)
     if out.dtype != dtype or out.shape != (m, n) or out.get_device() != index or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {dtype} {[m, n]} on the device of x")
+    if x is not None and m:
+        first, size = x.data_ptr(), ((m - 1) * x.stride(0) + x.shape[1]) * x.element_size()
+        if first < out.data_ptr() + out.nbytes and out.data_ptr() < first + size:
+            raise ValueError("out must not share memory with x, which is read while out is written")
     return out
 
 
 def fp8_matmul(x, weights, *, output_dtype=None, out=None):
     """``x @ weights.T`` as ``[M, N]`` BF16 (default) or FP32 (``output_dtype``). ``x`` is BF16 or FP32
-    ``[M, K]``, quantised in the call, or :class:`Fp8Rows`. Products of codes are exact, sums FP32."""
+    ``[M, K]``, quantised in the call, or :class:`Fp8Rows`. Products of codes are exact, sums FP32. ``out``
+    must not share memory with ``x``."""
     dtype = output_dtype or (torch.bfloat16 if out is None else out.dtype)
     out_code = _TYPES.get(dtype)
     if out_code is None:
@@ -189,14 +194,14 @@ def fp8_matmul(x, weights, *, output_dtype=None, out=None):
         m, k = codes.shape
         index = codes.get_device()
         n, w, w_pitch, w_scales, _keep = _weights(weights, k, index, "weights")
-        out = _output(out, m, n, dtype, index)
+        out = _output(out, m, n, dtype, index, codes)
         _lib.call_at(index, "qk_fp8_matmul", codes.data_ptr(), pitch, scales.data_ptr(), m, k, w, w_pitch, w_scales, n,
                      out_code, out.data_ptr())
         return out
     x, code, stride, index = _matrix(x, "x")
     m, k = x.shape
     n, w, w_pitch, w_scales, _keep = _weights(weights, k, index, "weights")
-    out = _output(out, m, n, dtype, index)
+    out = _output(out, m, n, dtype, index, x)
     x, stride, room, need = _room("qk_fp8_linear_workspace_bytes", index, code, m, k, n, x, stride)
     _lib.call_at(index, "qk_fp8_linear", x.data_ptr(), code, stride, m, k, w, w_pitch, w_scales, n,
                  out_code, out.data_ptr(), room.data_ptr() if need else None, need)
@@ -223,7 +228,7 @@ def gated_fp8(x, gate, up):
 
 def gated_ffn_fp8(x, gate, up, down, *, out=None):
     """A gated feed-forward block, ``(silu(x gate^T) * (x up^T)) down^T`` as BF16 ``[M, H]``: the product
-    of :func:`gated_fp8` with ``down`` ``[H, I]``."""
+    of :func:`gated_fp8` with ``down`` ``[H, I]``. ``out`` may be ``x``."""
     if isinstance(x, Fp8Rows):
         return fp8_matmul(gated_fp8(x, gate, up), down, out=out, output_dtype=torch.bfloat16)
     x, code, stride, index = _matrix(x, "x")

@@ -422,6 +422,25 @@ def test_mismatched_operands_are_refused(cuda_device):
         fp8_weights(w.codes, w.scales[:, :1])
 
 
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_outputs_over_their_inputs(m, cuda_device):
+    """A product refuses an ``out`` that shares memory with ``x``; a feed-forward block may write over it."""
+    import torch
+
+    from qk_b200.fp8 import fp8_matmul, gated_ffn_fp8
+
+    w = packed(256, 256, cuda_device)
+    store = torch.empty((m + 1) * 256, dtype=torch.bfloat16, device=cuda_device)
+    x = store[:m * 256].view(m, 256)
+    x.copy_(activations(m, 256, cuda_device))
+    for out in (x, store[256:].view(m, 256), store[8:8 + m * 256].view(m, 256)):
+        if m > 1 or out.data_ptr() < x.data_ptr() + 512:
+            with pytest.raises(ValueError):
+                fp8_matmul(x, w, out=out)
+    want = gated_ffn_fp8(x, w, w, w)
+    assert gated_ffn_fp8(x, w, w, w, out=x) is x and torch.equal(x, want)
+
+
 def test_layouts_of_operands(cuda_device):
     """Views, odd pitches, misaligned beginnings, scales of another type: the values decide."""
     import torch
