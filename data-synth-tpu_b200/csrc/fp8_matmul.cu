@@ -42,10 +42,24 @@ int check_rows(const void* x, int in_dtype, int64_t stride, int64_t M, int64_t K
   return QK_OK;
 }
 
-// The narrow form is used for up to 128 rows, and for more where its tiles of 128 x 128 are so few that their blocks of K
-// are split: K 4096, N 2048 takes 10.7 us for 256 rows and 15.0 for 512 (the wide form 16.6 for both), but K 2048,
-// N 9216 15.1 for 192 (11.1). For 128 rows they take 11.6 and 11.1 of that, of K 8192, N 8192 25 and 31.
-bool narrow(int64_t M, int64_t N) { return M <= 128 || ((M + 127) / 128) * ((N + 127) / 128) <= sm_count() / 2; }
+// Which form a call takes: the one with the smaller of these costs, about its ns in a graph (fitted to 65 to 4096 rows, K 256 to
+// 8192, N 128 to 12288); up to 64 rows (gated 32) the narrow one, whose CTAs may quantise them. The wide form has tiles
+// of 256 x 256, or half as wide where that fills no more rounds of the pairs of SMs. Both sides, us, narrow / half / whole:
+// 128 rows of 2048 x 9216 11.5 / 8.8 / 11.3, 256 of 4096 x 2048 10.7 / 13.0 / 16.6, 512 15.0 / 13.1 / 16.8, 1024 of
+// 8192 x 2048 40 / 23 / 30, 512 of 2048 x 9216 28 / 14.5 / 12.2, 2048 of 4096 x 2048 45 / 23.6 / 18. A gated pair with
+// its down product, narrow / wide: 256 rows of 2048 x 512 12.8 / 17.3, 128 of 2048 x 6144 29.6 / 26.4.
+struct WidePlan {
+  bool half;
+  int64_t cost;
+  WidePlan(int64_t M, int64_t N, int blocks, bool gated) {
+    const int64_t pairs = sm_count() / 2, m = (M + 255) / 256, n = (N + 127) / 128;
+    const int64_t halves = (m * n + pairs - 1) / pairs, wholes = gated ? halves : (m * ((n + 1) / 2) + pairs - 1) / pairs;
+    const int64_t cost_half = 3200 + blocks * (halves == 1 ? 330 : 400 * halves);
+    const int64_t cost_whole = 4000 + blocks * (wholes > 1 ? 570 * wholes : gated ? 500 : 450);
+    half = !gated && cost_half < cost_whole;
+    cost = half ? cost_half : cost_whole;
+  }
+};
 
 // Half of a feed-forward block (u not NULL, codes out) or a product (u NULL) of codes.
 struct Weights {
@@ -60,8 +74,9 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
   const bool vectors = !u && aligned16(out) && N * (f32 ? 4 : 2) % 16 == 0;
   CUtensorMap xm, wm, um;
   bool ok;
-  if (narrow(M, N)) {
-    const NarrowPlan plan(M, N, blocks, u != nullptr);
+  const NarrowPlan plan(M, N, blocks, u != nullptr);
+  const WidePlan wide(M, N, blocks, u != nullptr);
+  if (M <= plan.rows || plan.cost <= wide.cost) {
     ok = encode(&xm, x, M, K, x_ld, plan.tokens) && encode(&wm, w.codes, N, K, w.ld, 128) && (!u || encode(&um, u->codes, N, K, u->ld, 128));
     if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
     NarrowArgs a{};
@@ -78,8 +93,8 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
     a.vectors = vectors;
     return u ? launch_narrow<true>(false, xm, wm, um, a, plan, st) : launch_narrow<false>(false, xm, wm, wm, a, plan, st);
   }
-  ok = encode(&xm, x, M, K, x_ld, kHalf) && encode(&wm, w.codes, N, K, w.ld, kHalf / 2) &&
-       (!u || encode(&um, u->codes, N, K, u->ld, kHalf / 2));
+  ok = encode(&xm, x, M, K, x_ld, kHalf) && encode(&wm, w.codes, N, K, w.ld, wide.half ? 32 : 64) &&
+       (!u || encode(&um, u->codes, N, K, u->ld, 64));
   if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
   WideArgs a{};
   a.M = M;
@@ -87,7 +102,7 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
   a.blocks = blocks;
   a.n_blocks = n_blocks;
   a.tiles_m = static_cast<int>((M + kTileM - 1) / kTileM);
-  a.tiles_n = u ? n_blocks : static_cast<int>((N + kTileN - 1) / kTileN);
+  a.tiles_n = u || wide.half ? n_blocks : static_cast<int>((N + 255) / 256);
   a.xs = xs;
   a.ws = w.scales;
   a.us = u ? u->scales : nullptr;
@@ -102,7 +117,8 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
     ok = encode(&om, out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, M, N, N * (f32 ? 4 : 2), 32, f32 ? 32 : 64,
                 CU_TENSOR_MAP_SWIZZLE_128B);
   if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the output");
-  return u ? launch_wide<true>(xm, wm, um, om, a, st) : launch_wide<false>(xm, wm, wm, om, a, st);
+  if (u) return launch_wide<true, 128>(xm, wm, um, om, a, st);
+  return wide.half ? launch_wide<false, 64>(xm, wm, wm, om, a, st) : launch_wide<false, 128>(xm, wm, wm, om, a, st);
 }
 
 // The same from rows of BF16 or FP32, which a narrow product of BF16 quantises itself where it can; else into `room`

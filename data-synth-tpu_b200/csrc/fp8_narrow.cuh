@@ -413,30 +413,31 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
 // takes an SM for itself, of 8 for 15, and one cluster too many costs a second round (64 rows of 4096 x 2048 with
 // eight: 7.2 us where two fit an SM, 11.1 else). So all but the largest leave room for a second, and those have four.
 // Tokens per tile: all of them up to 64 (gated 32). Beyond, tiles of 64 (32) or of twice as many, which read the
-// weights less often but have only one CTA per SM: a product takes about 3.7 us and 0.5 for each of a CTA's blocks with
-// the first, 5.8 and 0.56 with the second, so the first are taken where a CTA gets up to four blocks more (96 rows of
-// 4096 x 2048: 7.8 and 9.3 us, 512 of 1024 x 1000 5.7 and 7.4; but 128 of 2048 x 9216 12.4 and 11.4. Gated, 128 rows
+// weights less often but have only one CTA per SM: the ones with the smaller cost, about the ns of a call in a graph
+// (96 rows of 4096 x 2048: 7.8 and 9.3 us, 512 of 1024 x 1000 5.7 and 7.4; but 256 of 4096 x 2048 11.9 and 10.7. Gated, 128 rows
 // of 2048 x 512 11.9 and 16.1 with the down product, of 2048 x 6144 29.6 and 30.7).
 struct NarrowPlan {
   int tokens, splits, rows, most;  // rows: that a CTA quantises itself, at most, and (most) blocks of them
+  int64_t cost;
   NarrowPlan(int64_t M, int64_t N, int blocks, bool gated) {
-    const int small = gated ? 32 : 64;
-    tokens = M <= 16 ? 16 : M <= 32 ? 32 : small;
-    splits = splits_of(M, N, blocks, gated);
-    if (M > small) {
-      const int few = each(blocks), with_few = splits;
-      tokens = 2 * small;
-      splits = splits_of(M, N, blocks, gated);
-      if (few <= each(blocks) + 4) tokens = small, splits = with_few;
-    }
-    rows = small;
+    rows = gated ? 32 : 64;
     most = gated ? kInline / 2 : kInline;
+    split(M <= 16 ? 16 : M <= 32 ? 32 : rows, M, N, blocks, gated);
+    if (M > rows) {
+      const NarrowPlan few = *this;
+      split(2 * rows, M, N, blocks, gated);
+      if (few.cost <= cost) *this = few;
+    }
   }
-  int splits_of(int64_t M, int64_t N, int blocks, bool gated) const {
+  void split(int of, int64_t M, int64_t N, int blocks, bool gated) {
+    tokens = of;
+    const bool large = tokens * (gated ? 2 : 1) > 64;
     const int64_t tiles = (N + 127) / 128 * ((M + tokens - 1) / tokens), room = sm_count() / tiles;
-    int n = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
-    if (tokens * (gated ? 2 : 1) > 64) n = tiles * 4 <= sm_count() * 7 / 8 ? 4 : n > 2 ? 2 : n;
-    return n < blocks ? n : blocks;
+    splits = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
+    if (large) splits = tiles * 4 <= sm_count() * 7 / 8 ? 4 : splits > 2 ? 2 : splits;
+    if (splits > blocks) splits = blocks;
+    const int64_t work = each(blocks) * ((tiles * splits + sm_count() - 1) / sm_count());  // blocks that an SM goes through
+    cost = gated ? (large ? 6500 : 4000) + 600 * work : large ? 5800 + 560 * work : 3500 + 540 * work;
   }
   int each(int blocks) const { return (blocks + splits - 1) / splits; }
   // Whether the CTAs can quantise rows of x themselves.

@@ -7,6 +7,10 @@
 // half's four warps per CTA add them, times the block's two scales, to FP32 sums in their registers (a row and 128
 // columns per thread) while the tensor core fills the three others. A warp issues each half's MMAs: one for both took
 // about 900 cycles a block for its waits and issues, more than the products.
+// Where the tiles of 256 x 256 do not fill the pairs, they are half as wide (HALF 64), with four buffers of 64 columns
+// for either half: 1024 rows of 4096 x 2048 13.5 us (whole 17.3), 256 of 2048 x 9216 9.0 (11.4). A block of such a tile
+// takes 0.29 us alone (whole 0.38, in a full round 0.57). The halves having every other block of 128 columns instead takes
+// 0.25, but 0.7 more at the end, where they join their sums; summing a block while the next is read 0.30.
 //
 // Measured (B200, 1.9 GHz, in bursts / in a loop of seconds under the power cap):
 //   x 16384 x 2048 of codes, 9216 columns, BF16 out   285 / 330 us, 2170 / 1870 TFLOP/s
@@ -23,9 +27,14 @@
 namespace qk {
 namespace {
 
-constexpr int kTileM = 256, kTileN = 256, kHalf = 128;  // a pair's tile, and a CTA's rows of either operand
-constexpr int kStages = 4, kBuffers = 2;
-constexpr uint32_t kBytesA = kHalf * kFp8Block, kStageBytes = 2 * kBytesA;  // of one CTA
+constexpr int kTileM = 256, kHalf = 128;  // rows of a pair's tile, and a CTA's of x
+constexpr uint32_t kBytesA = kHalf * kFp8Block;
+// What follows from HALF, the columns of either half of a tile: 128 or 64.
+template <int HALF>
+struct Wide {
+  static constexpr int kTileN = 2 * HALF, kBuffers = 512 / kTileN, kStages = HALF == 128 ? 4 : 6;
+  static constexpr uint32_t kBytesB = HALF * kFp8Block, kStageBytes = kBytesA + kBytesB;  // of one CTA
+};
 constexpr int kFirstSum = 4, kSumWarps = 8, kThreads = (kFirstSum + kSumWarps) * 32;
 constexpr uint32_t kPiece = 4096, kStaging = 2 * kPiece;  // bytes of 32 rows of 128 on their way out, per summing warp
 constexpr int kAhead = 4;            // blocks whose scales of x are on their way
@@ -46,7 +55,7 @@ struct WideArgs {
 };
 
 struct WideControl {
-  uint64_t full[kStages], empty[kStages], sum_full[kBuffers][2], sum_empty[kBuffers][2];
+  uint64_t full[6], empty[6], sum_full[4][2], sum_empty[4][2];
   uint64_t swapped[4];               // a row's two warps have left their maxima
   uint32_t tmem;
 };
@@ -98,35 +107,39 @@ __device__ __forceinline__ void cluster_arrive(uint32_t bar) {
 }
 
 // Both CTAs: their rows of x and of the weights. The bytes count on the leader's barrier.
-template <bool GATED>
+template <bool GATED, int HALF>
 __device__ __forceinline__ bool wide_copies(const WideArgs& a, WideControl& ctl, const CUtensorMap* x, const CUtensorMap* w,
                                             const CUtensorMap* u, uint32_t smem, int rank) {
-  uint32_t it = 0;
+  using L = Wide<HALF>;
+  uint32_t it = 0, s = 0, lap = 0;
   bool ok = true;
   const CUtensorMap* b_map = GATED && rank ? u : w;
   for (int t = blockIdx.x / 2; ok && t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     const Tile tile = tile_of(a, t);
-    const int a_row = tile.m * kTileM + rank * kHalf, b_row = GATED ? tile.n * kFp8Block : tile.n * kTileN + rank * 64;
+    const int a_row = tile.m * kTileM + rank * kHalf, b_row = GATED ? tile.n * kFp8Block : tile.n * L::kTileN + rank * (HALF / 2);
     for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t s = it % kStages, at = smem + s * kStageBytes, bar = leaders(&ctl.full[s]);
-      ok = mbar_wait_bounded(&ctl.empty[s], (it / kStages & 1) ^ 1);
+      const uint32_t at = smem + s * L::kStageBytes, bar = leaders(&ctl.full[s]);
+      ok = mbar_wait_bounded(&ctl.empty[s], lap ^ 1);
       if (!ok) break;
-      if (rank == 0) mbar_expect_tx(&ctl.full[s], 2 * kStageBytes);
+      if (rank == 0) mbar_expect_tx(&ctl.full[s], 2 * L::kStageBytes);
       load_box_pair(at, x, b * kFp8Block, a_row, bar);
       load_box_pair(at + kBytesA, b_map, b * kFp8Block, b_row, bar);
-      load_box_pair(at + kBytesA + kBytesA / 2, b_map, b * kFp8Block, b_row + (GATED ? 64 : 128), bar);
+      load_box_pair(at + kBytesA + L::kBytesB / 2, b_map, b * kFp8Block, b_row + (GATED ? 64 : HALF), bar);
+      if (++s == L::kStages) s = 0, lap ^= 1;
     }
   }
   // Every copy issued must have landed before the CTA leaves: when the MMAs that read it are done.
-  for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait_bounded(&ctl.empty[i % kStages], i / kStages & 1);
+  for (uint32_t i = it > L::kStages ? it - L::kStages : 0; i < it; ++i) mbar_wait_bounded(&ctl.empty[i % L::kStages], i / L::kStages & 1);
   return ok;
 }
 
 // The leader's MMA warps, one for each half of the columns.
+template <int HALF>
 __device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ctl, uint32_t smem, const int h) {
-  constexpr uint32_t idesc = (1u << 4) | (128 >> 3) << 17 | (kTileM >> 4) << 24;
+  using L = Wide<HALF>;
+  constexpr uint32_t idesc = (1u << 4) | (HALF >> 3) << 17 | (kTileM >> 4) << 24;
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
-  const uint64_t ad0 = sdesc_sw128(smem, 1024u), bd0 = sdesc_sw128(smem + kBytesA + h * (kBytesA / 2), 1024u);
+  const uint64_t ad0 = sdesc_sw128(smem, 1024u), bd0 = sdesc_sw128(smem + kBytesA + h * (L::kBytesB / 2), 1024u);
   uint32_t s = 0, full = 0, d = 0, freed = 1;
   for (int t = blockIdx.x / 2; t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     for (int b = 0; b < a.blocks; ++b) {
@@ -134,15 +147,15 @@ __device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ct
       if (!warp_wait(&ctl.full[s], full)) return false;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t ad = ad0 + s * (kStageBytes >> 4), bd = bd0 + s * (kStageBytes >> 4);
+        const uint64_t ad = ad0 + s * (L::kStageBytes >> 4), bd = bd0 + s * (L::kStageBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_e4m3_pair(tm + d * kTileN + h * 128, ad + 2 * k, bd + 2 * k, idesc, k != 0);
+        for (int k = 0; k < 4; ++k) umma_e4m3_pair(tm + d * L::kTileN + h * HALF, ad + 2 * k, bd + 2 * k, idesc, k != 0);
         umma_commit_pair(&ctl.empty[s]);
         umma_commit_pair(&ctl.sum_full[d][h]);
       }
       __syncwarp();
-      if (++s == kStages) s = 0, full ^= 1;
-      if (++d == kBuffers) d = 0, freed ^= 1;
+      if (++s == L::kStages) s = 0, full ^= 1;
+      if (++d == L::kBuffers) d = 0, freed ^= 1;
     }
   }
   return true;
@@ -176,16 +189,16 @@ __device__ __forceinline__ void stores_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 
-// 32 rows (a lane each) of 128 columns out, through shared memory, in pieces of 128 bytes a row, two of which alternate.
-template <bool F32>
-__device__ __forceinline__ void wide_store(const WideArgs& a, const CUtensorMap* map, const uint64_t (&acc)[64], uint32_t staging,
+// 32 rows (a lane each) of HALF columns out, through shared memory, in pieces of 128 bytes a row, two of which alternate.
+template <bool F32, int HALF>
+__device__ __forceinline__ void wide_store(const WideArgs& a, const CUtensorMap* map, const uint64_t (&acc)[HALF / 2], uint32_t staging,
                                            int64_t row0, int col0) {
   constexpr int kSize = F32 ? 4 : 2, kColumns = 128 / kSize;
   const int lane = threadIdx.x & 31;
   const int rows = static_cast<int>(min(a.M - row0, static_cast<int64_t>(32)));
   if (rows <= 0) return;
 #pragma unroll
-  for (int c = 0; c < 128; c += kColumns) {
+  for (int c = 0; c < HALF; c += kColumns) {
     if (col0 + c >= a.N) break;
     const uint32_t piece = staging + (c / kColumns & 1) * kPiece;
     if (lane == 0 && c == 0) stores_read<0>();  // the last tile's
@@ -228,11 +241,12 @@ __device__ __forceinline__ void wide_store(const WideArgs& a, const CUtensorMap*
   }
 }
 
-template <bool GATED>
+template <bool GATED, int HALF>
 __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, const CUtensorMap* out_map, uint32_t staging, int rank) {
   const int warp = (threadIdx.x >> 5) - kFirstSum, quarter = warp & 3, half = warp >> 2, lane = threadIdx.x & 31;
   const uint32_t tm = ctl.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  const uint32_t released[kBuffers] = {leaders(&ctl.sum_empty[0][half]), leaders(&ctl.sum_empty[1][half])};
+  using L = Wide<HALF>;
+  const uint32_t released = leaders(&ctl.sum_empty[0][half]);
   const uint32_t scales = staging + kSumWarps * kStaging + (threadIdx.x - kFirstSum * 32) * 4;  // this thread's, kAhead slots
   const uint32_t swaps_at = scales - (threadIdx.x - kFirstSum * 32) * 4 + kAhead * kSumWarps * 128;
   staging += warp * kStaging;
@@ -240,8 +254,8 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, c
   for (int t = blockIdx.x / 2; t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     const Tile tile = tile_of(a, t);
     const int64_t row0 = static_cast<int64_t>(tile.m) * kTileM + rank * kHalf + quarter * 32, row = row0 + lane;
-    // a thread's columns: 128 of the tile's 256, or 64 of the gate's and the same of up's
-    const int n_block = GATED ? tile.n : min(tile.n * 2 + half, a.n_blocks - 1);
+    // a thread's columns: half of the tile's, or 64 of the gate's and the same of up's
+    const int n_block = GATED ? tile.n : HALF == 128 ? min(tile.n * 2 + half, a.n_blocks - 1) : tile.n;
     const float* ws = a.ws + static_cast<int64_t>(n_block) * a.blocks;
     const float* us = GATED ? a.us + static_cast<int64_t>(n_block) * a.blocks : nullptr;
     const float* xs = a.xs + min(row, a.M - 1);
@@ -253,32 +267,32 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, c
       cp_async_commit();
     };
     for (int b = 0; b < kAhead; ++b) fetch(b);
-    uint64_t acc[64];
+    uint64_t acc[HALF / 2];
 #pragma unroll
-    for (int j = 0; j < 64; ++j) acc[j] = 0;
+    for (int j = 0; j < HALF / 2; ++j) acc[j] = 0;
     for (int b = 0; b < a.blocks; ++b, ++it) {
-      const uint32_t d = it % kBuffers, cols = tm + d * kTileN + half * 128;
+      const uint32_t d = it % L::kBuffers, cols = tm + d * L::kTileN + half * HALF;
       const float w = __ldg(ws + b), u = GATED ? __ldg(us + b) : 0.f;
       cp_async_wait<kAhead - 1>();
       const float x = __uint_as_float(lds_at(scales + (b % kAhead) * (kSumWarps * 128)));
       fetch(b + kAhead);
-      if (!warp_wait(&ctl.sum_full[d][half], it / kBuffers & 1)) return false;
+      if (!warp_wait(&ctl.sum_full[d][half], it / L::kBuffers & 1)) return false;
       tc_fence_after();
-      if (GATED) {
+      if constexpr (GATED) {
         add_block<64>(cols, x * w, acc);
         add_block<64>(cols + 64, x * u, acc + 32);
       } else {
-        add_block<128>(cols, x * w, acc);
+        add_block<HALF>(cols, x * w, acc);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) cluster_arrive(released[d]);
+      if (lane == 0) cluster_arrive(released + d * sizeof(ctl.sum_empty[0]));
     }
-    if (!GATED) {
-      if (a.f32) wide_store<true>(a, out_map, acc, staging, row0, tile.n * kTileN + half * 128);
-      else wide_store<false>(a, out_map, acc, staging, row0, tile.n * kTileN + half * 128);
+    if constexpr (!GATED) {
+      if (a.f32) wide_store<true, HALF>(a, out_map, acc, staging, row0, tile.n * L::kTileN + half * HALF);
+      else wide_store<false, HALF>(a, out_map, acc, staging, row0, tile.n * L::kTileN + half * HALF);
       continue;
-    }
+    } else {
     // A thread has half of its row's block of 128: two threads swap their maxima. No rounding before the codes'.
     float h[64];
     uint32_t most = 0;
@@ -312,32 +326,41 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, c
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0 && row0 < a.M && col < a.N) store_box(out_map, col, static_cast<int>(row0), staging);  // 64-byte swizzle
-    } else if (row < a.M) {  // a copy writes 16 bytes at a time, also past the end of a row
+    } else if (row < a.M) {  // a tensor copy writes 16 bytes at a time, also past the end of a row
       uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.ld + col;
 #pragma unroll
-      for (int j = 0; j < 64; ++j)
-        if (col + j < a.N) out[j] = static_cast<uint8_t>(codes[j / 4] >> (8 * (j & 3)));
+      for (int j = 0; j < 64; j += 16) {
+        if (col + j + 16 <= a.N) {
+          *reinterpret_cast<uint4*>(out + j) = make_uint4(codes[j / 4], codes[j / 4 + 1], codes[j / 4 + 2], codes[j / 4 + 3]);
+          continue;
+        }
+#pragma unroll
+        for (int i = j; i < j + 16; ++i)
+          if (col + i < a.N) out[i] = static_cast<uint8_t>(codes[i / 4] >> (8 * (i & 3)));
+      }
     }
     if (half == 0 && row < a.M) a.out_scales[static_cast<int64_t>(tile.n) * a.M + row] = fp8_scale(most);
+    }
   }
   if (lane == 0) stores_read<0>();  // the CTA's shared memory lives until then
   return true;
 }
 
-template <bool GATED>
+template <bool GATED, int HALF>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     fp8_wide_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap w, const __grid_constant__ CUtensorMap u,
                     const __grid_constant__ CUtensorMap out, WideArgs a) {
+  using L = Wide<HALF>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ WideControl ctl;
   const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, rank = static_cast<int>(cluster_rank());
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&ctl.full[i], 1);
       mbar_init(&ctl.empty[i], 2);
     }
-    for (int i = 0; i < kBuffers; ++i) {
+    for (int i = 0; i < L::kBuffers; ++i) {
       for (int h = 0; h < 2; ++h) {
         mbar_init(&ctl.sum_full[i][h], 1);
         mbar_init(&ctl.sum_empty[i][h], kSumWarps);  // half of the warps of either CTA
@@ -361,15 +384,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   bool ok = true;
   if (warp >= kFirstSum) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
-    ok = wide_sums<GATED>(a, ctl, &out, smem + kStages * kStageBytes, rank);
+    ok = wide_sums<GATED, HALF>(a, ctl, &out, smem + L::kStages * L::kStageBytes, rank);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 0) {
-      if (threadIdx.x == 0) ok = wide_copies<GATED>(a, ctl, &x, &w, &u, smem, rank);
+      if (threadIdx.x == 0) ok = wide_copies<GATED, HALF>(a, ctl, &x, &w, &u, smem, rank);
     } else if (warp == 1 && rank == 0) {
-      ok = wide_products(a, ctl, smem, 0);
+      ok = wide_products<HALF>(a, ctl, smem, 0);
     } else if (warp == 2 && rank == 0) {
-      ok = wide_products(a, ctl, smem, 1);
+      ok = wide_products<HALF>(a, ctl, smem, 1);
     }
   }
   if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
@@ -382,13 +405,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   }
 }
 
-template <bool GATED>
+template <bool GATED, int HALF>
 int launch_wide(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& out, const WideArgs& a, cudaStream_t st) {
-  const size_t smem = 1024 + kStages * kStageBytes + kSumWarps * kStaging + kAhead * kSumWarps * 128 + 2048;
-  const int rc = allow_smem(reinterpret_cast<const void*>(fp8_wide_kernel<GATED>), smem);
+  using L = Wide<HALF>;
+  const size_t smem = 1024 + L::kStages * L::kStageBytes + kSumWarps * kStaging + kAhead * kSumWarps * 128 + 2048;
+  const int rc = allow_smem(reinterpret_cast<const void*>(fp8_wide_kernel<GATED, HALF>), smem);
   if (rc) return rc;
   const int tiles = a.tiles_m * a.tiles_n, pairs = sm_count() / 2;
-  cudaError_t e = launch_dependent(fp8_wide_kernel<GATED>, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kThreads), smem, st, x, w, u, out, a);
+  cudaError_t e =
+      launch_dependent(fp8_wide_kernel<GATED, HALF>, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kThreads), smem, st, x, w, u, out, a);
   if (e != cudaSuccess) return cuda_error(e, "fp8_wide_kernel");
   count_launch();
   return QK_OK;

@@ -268,6 +268,21 @@ def test_gated(cuda_device, m, k, inner):
     check_product(out, value, weight_values(down), 2.0 ** -8)
 
 
+# More rows: tiles of 256 x 128, with a ragged end on every side, and in several rounds; of 256 x 256 in one round and
+# in two; of few rows after all, 128 at a time.
+@pytest.mark.parametrize("m,k,n", [(65, 256, 512), (129, 130, 777), (300, 384, 130), (700, 1000, 3001), (1500, 520, 5000), (257, 2048, 9216),
+                                   (512, 2000, 9216), (520, 2040, 9100), (256, 4096, 2048), (250, 8100, 2041), (390, 500, 12200)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_matmul_of_more_rows(cuda_device, m, k, n, f32):
+    test_matmul(cuda_device, m, k, n, f32)
+
+
+@pytest.mark.parametrize("m,k,inner", [(40, 2048, 512), (33, 600, 6000), (500, 4100, 760), (513, 300, 3001), (1000, 256, 1000),
+                                       (900, 2048, 5000)])
+def test_gated_of_more_rows(cuda_device, m, k, inner):
+    test_gated(cuda_device, m, k, inner)
+
+
 # ---- together, and as the decoder uses them ----------------------------------------------------
 
 
