@@ -263,12 +263,12 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl<M
   return true;
 }
 
-// A warp per owner sends it its tokens.
+// A warp per other owner sends it its tokens.
 template <int MT, bool GATED>
 __device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl<MT>& ctl, uint32_t smem, int owned, int live, int rank) {
   using L = Narrow<MT, GATED>;
   const int owner = (threadIdx.x >> 5) - kNarrowFirstSum, tokens = min(owned, live - owner * owned);
-  if (owner >= a.splits || tokens <= 0) return true;
+  if (owner >= a.splits || owner == rank || tokens <= 0) return true;
   if (!warp_wait(&ctl.stored, 0)) return false;
   if (elect_one())
     send(in_rank(smem + a.ring + rank * owned * L::kToken, owner), smem + owner * owned * L::kToken, tokens * L::kToken,
@@ -279,7 +279,8 @@ __device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl<M
 
 // The sums of the tokens that this CTA owns, a warp per token and four weight rows per lane, and the output.
 template <int MT, bool GATED>
-__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t sums, int owned, int mine, int64_t first, int tile) {
+__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t own, uint32_t sums, int owned, int mine, int rank, int64_t first,
+                                            int tile) {
   using L = Narrow<MT, GATED>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = tile * 128 + lane * 4;
 #pragma unroll 1
@@ -290,7 +291,7 @@ __device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t sums, 
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[o][j] = 0.f;
       for (int r = 0; r < a.splits; ++r) {
-        const uint4 v = lds_v4_at(sums + (((r * owned + i) * L::kOperands + o) * 128 + lane * 4) * 4);
+        const uint4 v = lds_v4_at((r == rank ? own : sums + r * owned * L::kToken) + ((i * L::kOperands + o) * 128 + lane * 4) * 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[o][j] += __uint_as_float(word(v, j));
       }
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
     mbar_init(&ctl.stored, kNarrowSumWarps);
     mbar_init(&ctl.joined, 1);
     fence_mbar_init();
-    mbar_expect_tx(&ctl.joined, a.splits * mine * L::kToken);
+    mbar_expect_tx(&ctl.joined, (a.splits - 1) * mine * L::kToken);
     pdl_wait();
     // the first copies are on their way while the others set up
     for (int i = 0; i < min(count, a.stages); ++i) narrow_copy<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, i, b0, tile, row0);
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
   if (!warp_wait(&ctl.joined, 0)) ok = false;
   if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
   cluster_arrive_relaxed();  // what the others sent has been read from their memory
-  narrow_join<MT, GATED>(a, smem + a.ring, owned, mine, row0 + static_cast<int64_t>(rank) * owned, tile);
+  narrow_join<MT, GATED>(a, smem + rank * owned * L::kToken, smem + a.ring, owned, mine, rank, row0 + static_cast<int64_t>(rank) * owned, tile);
   __syncwarp();
   cluster_wait();
 }
