@@ -3,14 +3,14 @@
 // The weights are the M = 128 operand and MT tokens the N operand, so a tile of 128 columns of the output is 128 rows
 // of the weights. Its blocks of K are split over a cluster of CTAs, which all stream their part of the weights at
 // once; each adds its blocks' sums, times their scales, in registers (a thread per weight row and half of the
-// tokens) and sends every token's to the CTA that owns it, which adds them in rank order and writes.
+// tokens) and sends every token's to the CTA that owns it, which adds them (its own, then the others' by rank) and writes.
 // x comes as codes, by tensor copies beside the weights', or (ROWS) as BF16 that every CTA quantises for itself while
 // its weights are on their way: that saves a launch, and the values are the same.
 //
 // Measured in a graph of calls over weights larger than L2 (floor: the weights' bytes at the measured HBM rate):
-//   1 row of BF16, 2048 x 9216        5.5 us, floor 2.9 (18.9 MB: 3.4 TB/s);  8 rows 6.4, 32 rows 10.3
-//   64 rows of BF16, 4096 x 2048      10.9 us, floor 1.4 (from codes 6.6);  1 row 4.0, floor 1.3
-//   gated, 32 rows of codes, 2048 x 2 x 6144   10.5 us, floor 3.9
+//   1 row of BF16, 2048 x 9216        5.3 us, floor 2.9 (18.9 MB: 3.6 TB/s);  8 rows 6.1; 32 rows of codes 5.8, 64 7.4
+//   64 rows of BF16, 4096 x 2048      10.5 us, floor 1.4 (from codes 5.9);  1 row 4.3, floor 1.3
+//   feed-forward block, 32 rows, 2048 x 6144   17.4 us, floor 5.8, quantisation and down product included
 // What bounds it is latency: the set-up, the first copy from memory (2 us), then for each block the issue of its MMAs
 // (about 300 cycles), its sums and, at the end, the exchange and the output, most of it instructions that run once
 // and come cold from L2.
@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kNarrowStages = 8, kNarrowSumWarps = 8, kNarrowFirstSum = 2;
 constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
+constexpr int kNarrowAhead = 4;      // blocks whose scales of x are on their way
 constexpr int kMostSplits = 8;       // the portable cluster size
 // Rows of BF16, and blocks of them, that a CTA quantises itself, at most (gated: half, their rings are short). 32 rows of
 // 4096 x 2048 (128 blocks per CTA) take 7.2 us, with a launch of its own for that 7.5; 32 of 2048 x 9216 (256) 10.3 and
@@ -50,18 +51,20 @@ struct Narrow {
   static constexpr uint32_t kBytesW = kOperands * 128 * kFp8Block, kBytesX = MT * kFp8Block, kStage = kBytesW + kBytesX;
   static constexpr int kColumns = kOperands * MT;                           // TMEM columns of a block's sums
   static constexpr int kBuffers = 256 / kColumns < 2 ? 2 : 256 / kColumns > 8 ? 8 : 256 / kColumns;
+  // 256 of 512 columns at most; registers (77 and more per thread) keep a third CTA from an SM, so that none waits for
+  // tensor memory while it holds up its cluster
   static constexpr uint32_t kAlloc = kColumns * kBuffers < 32 ? 32 : kColumns * kBuffers;
   static constexpr int kEach = MT / 2;                                      // tokens per thread
   static constexpr bool kTwo = kColumns <= 64;                              // room for two CTAs per SM
-  // shared memory: the ring (and x's tiles), then [CTA of the cluster][token it owns][operand][weight row] sums
-  // (whose own sums go where the ring was)
+  // shared memory: the ring (and x's tiles), then [other CTA of the cluster][owned token][operand][weight row] sums
+  // (the CTA's own go where the ring was)
   static constexpr uint32_t kToken = kOperands * 512, kSums = MT * kToken;
   static uint32_t ring(int stages, int inline_blocks) {
     const uint32_t bytes = stages * (inline_blocks ? kBytesW : kStage) + inline_blocks * kBytesX;
     return bytes > kSums ? bytes : kSums;
   }
   static size_t smem(int stages, int inline_blocks, int splits, int live) {
-    return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits) * ((live + splits - 1) / splits) * kToken;
+    return 1024 + ring(stages, inline_blocks) + static_cast<size_t>(splits - 1) * ((live + splits - 1) / splits) * kToken;
   }
 };
 
@@ -70,8 +73,8 @@ struct NarrowControl {
   uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], stored, joined;
   uint32_t tmem;
   static constexpr int kSlot = MT > 64 ? 64 : 32;
-  alignas(16) float scales[kNarrowSumWarps * 2 * kSlot];  // of x: a warp's two slots of its tokens, or (ROWS) [block][MT]
-  static_assert(kInlineTokens <= kNarrowSumWarps * 2 * kSlot, "a scale for each");
+  alignas(16) float scales[kNarrowSumWarps * kNarrowAhead * kSlot];  // of x: a warp's slots of its tokens, or (ROWS) [block][MT]
+  static_assert(kInlineTokens <= kNarrowSumWarps * kNarrowAhead * kSlot, "a scale for each");
 };
 
 // The address of this CTA's `addr` in the cluster's CTA `rank`.
@@ -197,29 +200,33 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl<M
   for (int o = 0; o < L::kOperands; ++o)
 #pragma unroll
     for (int j = 0; j < kEach / 2; ++j) acc[o][j] = 0;
-  // codes: a warp brings its tokens' scales of a block to its own two slots, one block ahead
+  // codes: a warp brings its tokens' scales of a block to its own slots, kNarrowAhead blocks ahead (one ahead, each block
+  // waited for its scales' way from memory: 32 rows of 2048 x 9216 7.8 us instead of 5.8)
   constexpr int kSlot = NarrowControl<MT>::kSlot;
-  float* slots = ctl.scales + warp * (2 * kSlot);
-  float next[kEach > 32 ? 2 : 1];
+  float* slots = ctl.scales + warp * (kNarrowAhead * kSlot);
   auto fetch = [&](int i) {
 #pragma unroll
-    for (int c = 0; c < (kEach > 32 ? 2 : 1); ++c) {
-      const int64_t row = row0 + half * kEach + c * 32 + lane;
-      next[c] = i < count && c * 32 + lane < kEach && row < a.M ? a.xs[static_cast<int64_t>(b0 + i) * a.M + row] : 0.f;
+    for (int c = 0; c < kEach; c += 32) {
+      const int64_t row = row0 + half * kEach + c + lane;
+      if (i < count && c + lane < kEach && row < a.M)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(slots + i % kNarrowAhead * kSlot + c + lane)),
+                     "l"(a.xs + static_cast<int64_t>(b0 + i) * a.M + row)
+                     : "memory");
     }
+    cp_async_commit();
   };
-  if (!ROWS) fetch(0);
+  if (!ROWS) {
+#pragma unroll
+    for (int i = 0; i < kNarrowAhead; ++i) fetch(i);
+  }
   float w = ws[0], u = GATED ? us[0] : 0.f;
   for (int it = 0; it < count; ++it) {
     const int d = it % L::kBuffers;
     const float* scales = ctl.scales + it * MT + half * kEach;
     if (!ROWS) {
-      float* slot = slots + (it & 1) * kSlot;
-#pragma unroll
-      for (int c = 0; c < (kEach > 32 ? 2 : 1); ++c) slot[c * 32 + lane] = next[c];
+      cp_async_wait<kNarrowAhead - 1>();
       __syncwarp();
-      scales = slot;
-      fetch(it + 1);
+      scales = slots + it % kNarrowAhead * kSlot;
     }
     const float by_w = w, by_u = u;
     if (it + 1 < count) {
@@ -246,6 +253,7 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl<M
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl.sum_empty[d]);
+    if (!ROWS) fetch(it + kNarrowAhead);
   }
   // All products are done, so nothing reads or fills the ring any more: [token][operand][weight row] goes there.
   const uint32_t to = smem + half * kEach * L::kToken + (quarter * 32 + lane) * 4;
@@ -271,27 +279,34 @@ __device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl<M
   if (owner >= a.splits || owner == rank || tokens <= 0) return true;
   if (!warp_wait(&ctl.stored, 0)) return false;
   if (elect_one())
-    send(in_rank(smem + a.ring + rank * owned * L::kToken, owner), smem + owner * owned * L::kToken, tokens * L::kToken,
+    send(in_rank(smem + a.ring + (rank - (rank > owner)) * owned * L::kToken, owner), smem + owner * owned * L::kToken, tokens * L::kToken,
          in_rank(smem_addr(&ctl.joined), owner));
   __syncwarp();
   return true;
 }
 
-// The sums of the tokens that this CTA owns, a warp per token and four weight rows per lane, and the output.
+// The sums of the tokens that this CTA owns, its own first and then the others' by rank, a warp per token and four
+// weight rows per lane, and the output. One short loop over both operands: its instructions come cold (a loop for each
+// and its unrolled form cost 0.3 us).
 template <int MT, bool GATED>
-__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t own, uint32_t sums, int owned, int mine, int rank, int64_t first,
-                                            int tile) {
+__device__ __forceinline__ void narrow_join(const NarrowArgs& a, uint32_t own, uint32_t sums, int owned, int mine, int64_t first, int tile) {
   using L = Narrow<MT, GATED>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = tile * 128 + lane * 4;
 #pragma unroll 1
   for (int i = warp; i < mine; i += kNarrowThreads / 32) {
     float f[2][4];
+    const uint32_t at = i * L::kToken + lane * 16;
 #pragma unroll
     for (int o = 0; o < L::kOperands; ++o) {
+      const uint4 v = lds_v4_at(own + at + o * 512);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[o][j] = 0.f;
-      for (int r = 0; r < a.splits; ++r) {
-        const uint4 v = lds_v4_at((r == rank ? own : sums + r * owned * L::kToken) + ((i * L::kOperands + o) * 128 + lane * 4) * 4);
+      for (int j = 0; j < 4; ++j) f[o][j] = __uint_as_float(word(v, j));
+    }
+#pragma unroll 2
+    for (int s = 0; s < a.splits - 1; ++s) {
+#pragma unroll
+      for (int o = 0; o < L::kOperands; ++o) {
+        const uint4 v = lds_v4_at(sums + s * owned * L::kToken + at + o * 512);
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[o][j] += __uint_as_float(word(v, j));
       }
@@ -403,7 +418,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
   if (!warp_wait(&ctl.joined, 0)) ok = false;
   if (!ok) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
   cluster_arrive_relaxed();  // what the others sent has been read from their memory
-  narrow_join<MT, GATED>(a, smem + rank * owned * L::kToken, smem + a.ring, owned, mine, rank, row0 + static_cast<int64_t>(rank) * owned, tile);
+  narrow_join<MT, GATED>(a, smem + rank * owned * L::kToken, smem + a.ring, owned, mine, row0 + static_cast<int64_t>(rank) * owned, tile);
   __syncwarp();
   cluster_wait();
 }
@@ -453,7 +468,7 @@ template <int MT, bool GATED, bool ROWS>
 int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, NarrowArgs a, const NarrowPlan& plan, cudaStream_t st) {
   using L = Narrow<MT, GATED>;
   const int each = plan.each(a.blocks);
-  const size_t room = L::kTwo ? 109 * 1024 : 220 * 1024;
+  const size_t room = L::kTwo ? 108 * 1024 : 220 * 1024;
   const int tiles_of_x = ROWS ? each : 0, live = static_cast<int>(a.M < MT ? a.M : MT);
   a.splits = plan.splits;
   a.stages = each < kNarrowStages ? each : kNarrowStages;
