@@ -26,9 +26,9 @@ constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
 constexpr int kNarrowAhead = 4;      // blocks whose scales of x are on their way
 constexpr int kMostSplits = 8;       // the portable cluster size
 // Rows of BF16, and blocks of them, that a CTA quantises itself, at most (gated: half, their rings are short). 32 rows of
-// 4096 x 2048 (128 blocks per CTA) take 7.2 us, with a launch of its own for that 7.5; 32 of 2048 x 9216 (256) 10.3 and
-// 9.5, 64 of 4096 x 2048 (256) 10.9 and 8.6, but that launch takes the host 4 us more, which is where such calls end:
-// by wall clock 11.1 and 13.5, 11.1 and 13.3. Gated, 192 blocks (32 rows of 2048 x 6144) cost 3 us and save 1.
+// 4096 x 2048 (128 blocks per CTA) take 7.0 us, with a launch of its own for that 7.4; 32 of 2048 x 9216 (256) 9.6 and
+// 8.3, 64 of 4096 x 2048 (256) 10.5 and 8.5, but that launch takes the host 4 us more, which is where such calls end:
+// by wall clock 9.9 and 13.7, 10.8 and 13.6. Gated, 192 blocks (32 rows of 2048 x 6144) cost 3 us and save 1.
 constexpr int kInline = 256, kInlineTokens = 256;  // kInlineTokens: of their tiles in shared memory
 
 struct NarrowArgs {
@@ -424,14 +424,15 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
 }
 
 // What a call does, by its sizes alone: a cluster's CTAs share a tile's blocks of K, as many as give every SM one CTA
-// at most (one row of 2048 x 9216, 72 tiles: 1 / 2 / 3 / 4 CTAs take 7.4 / 5.9 / 6.3 / 8.4 us, of 4096 x 2048, 16
-// tiles: 4 / 6 / 8 take 4.8 / 4.7 / 4.4). A cluster lies within a group of SMs: of 4 there is room for 33 where a CTA
+// at most (one row of 2048 x 9216, 72 tiles: 1 / 2 / 3 / 4 CTAs take 8.2 / 5.3 / 5.8 / 8.2 us, of 4096 x 2048, 16
+// tiles: 4 / 6 / 8 take 4.7 / 4.6 / 4.3). A cluster lies within a group of SMs: of 4 there is room for 33 where a CTA
 // takes an SM for itself, of 8 for 15, and one cluster too many costs a second round (64 rows of 4096 x 2048 with
-// eight: 7.2 us where two fit an SM, 11.1 else). So all but the largest leave room for a second, and those have four.
+// eight: 6.2 us where two fit an SM, 10.0 else). So all but the largest leave room for a second, and those have four.
 // Tokens per tile: all of them up to 64 (gated 32). Beyond, tiles of 64 (32) or of twice as many, which read the
 // weights less often but have only one CTA per SM: the ones with the smaller cost, about the ns of a call in a graph
-// (96 rows of 4096 x 2048: 7.8 and 9.3 us, 512 of 1024 x 1000 5.7 and 7.4; but 256 of 4096 x 2048 11.9 and 10.7. Gated, 128 rows
-// of 2048 x 512 11.9 and 16.1 with the down product, of 2048 x 6144 29.6 and 30.7).
+// (before the last steps 96 rows of 4096 x 2048 took 7.8 and 9.3 us, 512 of 1024 x 1000 5.7 and 7.4; but 256 of
+// 4096 x 2048 11.9 and 10.7. Gated, 128 rows of 2048 x 512 11.9 and 16.1 with the down product). Of the products a
+// block takes about 0.42 and 0.46 us beside 3.7 and 5.8 for all the rest.
 struct NarrowPlan {
   int tokens, splits, rows, most;  // rows: that a CTA quantises itself, at most, and (most) blocks of them
   int64_t cost;
@@ -452,8 +453,9 @@ struct NarrowPlan {
     splits = static_cast<int>(room < 1 ? 1 : room > kMostSplits ? kMostSplits : room);
     if (large) splits = tiles * 4 <= sm_count() * 7 / 8 ? 4 : splits > 2 ? 2 : splits;
     if (splits > blocks) splits = blocks;
-    const int64_t work = each(blocks) * ((tiles * splits + sm_count() - 1) / sm_count());  // blocks that an SM goes through
-    cost = gated ? (large ? 6500 : 4000) + 600 * work : large ? 5800 + 560 * work : 3500 + 540 * work;
+    int64_t work = each(blocks) * ((tiles * splits + sm_count() - 1) / sm_count());  // blocks that an SM goes through
+    if (splits > 2 && tiles * splits * 10 > sm_count() * 9) work += work / 2;         // the last clusters share their SMs
+    cost = gated ? (large ? 6500 + 560 * work : 4000 + 520 * work) : large ? 5800 + 460 * work : 3700 + 420 * work;
   }
   int each(int blocks) const { return (blocks + splits - 1) / splits; }
   // Whether the CTAs can quantise rows of x themselves.
@@ -468,7 +470,8 @@ template <int MT, bool GATED, bool ROWS>
 int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, NarrowArgs a, const NarrowPlan& plan, cudaStream_t st) {
   using L = Narrow<MT, GATED>;
   const int each = plan.each(a.blocks);
-  const size_t room = L::kTwo ? 108 * 1024 : 220 * 1024;
+  // of an SM's 228 KB, 1 KB of which each CTA reserves (and some for the alignment of what is static)
+  const size_t room = (L::kTwo ? 113 : 227) * 1024 - sizeof(NarrowControl<MT>) - 256;
   const int tiles_of_x = ROWS ? each : 0, live = static_cast<int>(a.M < MT ? a.M : MT);
   a.splits = plan.splits;
   a.stages = each < kNarrowStages ? each : kNarrowStages;

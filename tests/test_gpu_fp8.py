@@ -271,7 +271,9 @@ def test_gated(cuda_device, m, k, inner):
 # More rows: tiles of 256 x 128, with a ragged end on every side, and in several rounds; of 256 x 256 in one round and
 # in two; of few rows after all, 128 at a time.
 @pytest.mark.parametrize("m,k,n", [(65, 256, 512), (129, 130, 777), (300, 384, 130), (700, 1000, 3001), (1500, 520, 5000), (257, 2048, 9216),
-                                   (512, 2000, 9216), (520, 2040, 9100), (256, 4096, 2048), (250, 8100, 2041), (390, 500, 12200)])
+                                   (512, 2000, 9216), (520, 2040, 9100), (256, 4096, 2048), (250, 8100, 2041), (390, 500, 12200),
+                                   # as much shared memory as a CTA can have
+                                   (70, 8192, 3840), (66, 8100, 3777)])
 @pytest.mark.parametrize("f32", [False, True])
 def test_matmul_of_more_rows(cuda_device, m, k, n, f32):
     test_matmul(cuda_device, m, k, n, f32)
