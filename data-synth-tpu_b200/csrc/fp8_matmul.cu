@@ -42,12 +42,13 @@ int check_rows(const void* x, int in_dtype, int64_t stride, int64_t M, int64_t K
   return QK_OK;
 }
 
-// Which form a call takes: the one with the smaller of these costs, about its ns in a graph (fitted to 65 to 4096 rows, K 256 to
-// 8192, N 128 to 12288); up to 64 rows (gated 32) the narrow one, whose CTAs may quantise them. The wide form has tiles
-// of 256 x 256, or half as wide where that fills no more rounds of the pairs of SMs. Both sides, us, narrow / half / whole:
-// 128 rows of 2048 x 9216 11.5 / 8.8 / 11.3, 256 of 4096 x 2048 10.7 / 13.0 / 16.6, 512 15.0 / 13.1 / 16.8, 1024 of
-// 8192 x 2048 40 / 23 / 30, 512 of 2048 x 9216 28 / 14.5 / 12.2, 2048 of 4096 x 2048 45 / 23.6 / 18. A gated pair with
-// its down product, narrow / wide: 256 rows of 2048 x 512 12.8 / 17.3, 128 of 2048 x 6144 29.6 / 26.4.
+// Which form a call takes: the one with the smaller of these costs, about its ns in a graph (fitted to 65 to 4096 rows, K 256
+// to 8192, N 128 to 12288); up to 64 rows (gated 32) the narrow one, whose CTAs may quantise them. The wide form has
+// tiles of 256 x 256, or half as wide where that fills no more rounds of the pairs of SMs. All sides, us, narrow (before
+// its last steps, which took about a tenth off) / half / whole: 128 rows of 2048 x 9216 11.5 / 8.8 / 11.3, 256 of
+// 4096 x 2048 10.7 / 13.0 / 16.6, 512 15.0 / 13.1 / 16.8, 1024 of 8192 x 2048 40 / 23 / 30, 512 of 2048 x 9216
+// 28 / 14.5 / 12.2, 2048 of 4096 x 2048 45 / 23.6 / 18. A gated pair with its down product, narrow / wide: 256 rows of
+// 2048 x 512 12.8 / 17.3, 128 of 2048 x 6144 29.6 / 26.4.
 struct WidePlan {
   bool half;
   int64_t cost;
@@ -75,8 +76,7 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
   CUtensorMap xm, wm, um;
   bool ok;
   const NarrowPlan plan(M, N, blocks, u != nullptr);
-  const WidePlan wide(M, N, blocks, u != nullptr);
-  if (M <= plan.rows || plan.cost <= wide.cost) {
+  if (M <= plan.rows || plan.cost <= WidePlan(M, N, blocks, u != nullptr).cost) {
     ok = encode(&xm, x, M, K, x_ld, plan.tokens) && encode(&wm, w.codes, N, K, w.ld, 128) && (!u || encode(&um, u->codes, N, K, u->ld, 128));
     if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
     NarrowArgs a{};
@@ -93,6 +93,7 @@ int product(const uint8_t* x, int64_t x_ld, const float* xs, int64_t M, int64_t 
     a.vectors = vectors;
     return u ? launch_narrow<true>(false, xm, wm, um, a, plan, st) : launch_narrow<false>(false, xm, wm, wm, a, plan, st);
   }
+  const WidePlan wide(M, N, blocks, u != nullptr);
   ok = encode(&xm, x, M, K, x_ld, kHalf) && encode(&wm, w.codes, N, K, w.ld, wide.half ? 32 : 64) &&
        (!u || encode(&um, u->codes, N, K, u->ld, 64));
   if (!ok) return set_error(QK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable or refused the codes");
@@ -131,7 +132,7 @@ size_t row_bytes(int64_t M, int64_t K) {
 // Whether a product of BF16 rows quantises them itself: by the sizes alone, so that the workspace's size is.
 bool quantises(int in_dtype, int64_t M, int64_t K, int64_t N, bool gated) {
   const int blocks = static_cast<int>((K + 127) / 128);
-  return in_dtype == QK_OUT_BF16 && K % 8 == 0 && NarrowPlan(M, N, blocks, gated).quantises(M, blocks);
+  return in_dtype == QK_OUT_BF16 && K % 8 == 0 && M <= 64 && NarrowPlan(M, N, blocks, gated).quantises(M, blocks);
 }
 size_t room_for(int in_dtype, int64_t M, int64_t K, int64_t N, bool gated) {
   return quantises(in_dtype, M, K, N, gated) ? 0 : row_bytes(M, K);
@@ -236,10 +237,11 @@ int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t
   if (!rc) rc = check_weights(M, inner, down, down_ld, down_scales, N, out);
   if (rc || M == 0) return rc;
   QK_REQUIRE((reinterpret_cast<uintptr_t>(out) & 1) == 0, "misaligned out");
-  rc = check_room(workspace, workspace_bytes, room_for(in_dtype, M, K, inner, true) + row_bytes(M, inner));
+  const size_t for_x = room_for(in_dtype, M, K, inner, true);
+  rc = check_room(workspace, workspace_bytes, for_x + row_bytes(M, inner));
   if (rc) return rc;
   cudaStream_t st = as_stream(stream);
-  uint8_t* h = static_cast<uint8_t*>(workspace) + room_for(in_dtype, M, K, inner, true);
+  uint8_t* h = static_cast<uint8_t*>(workspace) + for_x;
   const int64_t ld = (inner + 15) / 16 * 16;
   float* h_scales = reinterpret_cast<float*>(h + (static_cast<size_t>(M) * ld + 255) / 256 * 256);
   const Weights u{up, up_ld, up_scales};
