@@ -41,10 +41,11 @@ class Fp8Weights(NamedTuple):
 
 # The allocation that compiled graphs make, at half the cost of torch.empty_strided: on the current device only.
 _lean_empty = getattr(getattr(torch._C._dynamo, "guards", None), "_empty_strided_cuda", None)
+_current = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _empty(size, stride, dtype, index):
-    if _lean_empty is not None and torch._C._cuda_getDevice() == index:
+    if _lean_empty is not None and _current() == index:
         return _lean_empty(size, stride, dtype)
     return torch.empty_strided(size, stride, dtype=dtype, device=torch.device("cuda", index))
 
@@ -98,9 +99,12 @@ def _weights(weights, k, index, name):
 
 
 def _matrix(x, name):
-    """``x`` BF16 or FP32 ``[rows, width]`` with dense rows: ``(x, type code, stride, device number)``."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] < 1:
+    """``x`` BF16 or FP32 ``[rows, width]`` with dense rows: ``(x, rows, width, type code, stride, device
+    number)``."""
+    shape = x.shape if isinstance(x, torch.Tensor) else ()
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{name} must be a BF16 or FP32 matrix")
+    rows, width = shape
     code = _TYPES.get(x.dtype)
     if code is None:
         raise TypeError(f"{name} must be BF16 or FP32")
@@ -108,11 +112,10 @@ def _matrix(x, name):
     if index < 0:
         raise ValueError("expected CUDA tensors")
     if x.is_contiguous():
-        return x, code, x.shape[1], index
-    rows, width = x.shape
+        return x, rows, width, code, width, index
     if width > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < width:
-        return x.contiguous(), code, width, index
-    return x, code, max(x.stride(0), width), index
+        return x.contiguous(), rows, width, code, width, index
+    return x, rows, width, code, max(x.stride(0), width), index
 
 
 _needs = {}
@@ -137,8 +140,7 @@ def quantize_fp8(x):
     """``x`` BF16 or FP32 ``[M, K]`` (rows may be strided) -> :class:`Fp8Rows`. A block of a row with
     the largest magnitude ``m`` (at least 2^-100) has the scale ``m / 448`` and the codes
     ``e4m3(448 x / m)``. A block that holds an infinity or a NaN has no finite values."""
-    x, code, stride, index = _matrix(x, "x")
-    rows, width = x.shape
+    x, rows, width, code, stride, index = _matrix(x, "x")
     out, pitch = _empty_rows(rows, width, index)
     _lib.call_at(index, "qk_fp8_quantize", x.data_ptr(), code, stride, rows, width, out.codes.data_ptr(), pitch,
                  out.scales.data_ptr())
@@ -148,8 +150,7 @@ def quantize_fp8(x):
 def pack_fp8(weight):
     """``weight`` BF16 or FP32 ``[N, K]`` -> :class:`Fp8Weights`, by the rule of :func:`quantize_fp8`
     for blocks of 128 x 128."""
-    weight, code, stride, index = _matrix(weight, "weight")
-    rows, width = weight.shape
+    weight, rows, width, code, stride, index = _matrix(weight, "weight")
     pitch = (width + 15) // 16 * 16
     codes = torch.empty_strided((rows, width), (pitch, 1), dtype=_E4M3, device=weight.device)
     scales = torch.empty((_blocks(rows), _blocks(width)), dtype=_F32, device=weight.device)
@@ -198,8 +199,7 @@ def fp8_matmul(x, weights, *, output_dtype=None, out=None):
         _lib.call_at(index, "qk_fp8_matmul", codes.data_ptr(), pitch, scales.data_ptr(), m, k, w, w_pitch, w_scales, n,
                      out_code, out.data_ptr())
         return out
-    x, code, stride, index = _matrix(x, "x")
-    m, k = x.shape
+    x, m, k, code, stride, index = _matrix(x, "x")
     n, w, w_pitch, w_scales, _keep = _weights(weights, k, index, "weights")
     out = _output(out, m, n, dtype, index, x)
     x, stride, room, need = _room("qk_fp8_linear_workspace_bytes", index, code, m, k, n, x, stride)
@@ -231,8 +231,7 @@ def gated_ffn_fp8(x, gate, up, down, *, out=None):
     of :func:`gated_fp8` with ``down`` ``[H, I]``. ``out`` may be ``x``."""
     if isinstance(x, Fp8Rows):
         return fp8_matmul(gated_fp8(x, gate, up), down, out=out, output_dtype=torch.bfloat16)
-    x, code, stride, index = _matrix(x, "x")
-    m, k = x.shape
+    x, m, k, code, stride, index = _matrix(x, "x")
     inner, g, g_pitch, g_scales, _keep_g = _weights(gate, k, index, "gate")
     n, u, u_pitch, u_scales, _keep_u = _weights(up, k, index, "up")
     if n != inner:
@@ -255,18 +254,19 @@ def rms_norm_fp8(x, gamma, eps=1e-6, *, residual=None):
     ``(Fp8Rows of rms(s) * gamma, s)`` with ``s = bf16(x + residual)``, or ``(Fp8Rows of rms(x) * gamma,
     None)`` without a residual. The norm is not rounded before its codes. ``H``: a multiple of 8, 8192 at
     most."""
-    if x.dtype != torch.bfloat16 or gamma.dtype != torch.bfloat16 or x.dim() != 2 or gamma.shape != x.shape[1:]:
+    shape = x.shape
+    if x.dtype != torch.bfloat16 or gamma.dtype != torch.bfloat16 or len(shape) != 2 or gamma.shape != shape[1:]:
         raise TypeError("x and gamma must be BF16, [M, H] and [H]")
+    rows, width = shape
     index = x.get_device()
     if index < 0:
         raise ValueError("expected CUDA tensors")
     if gamma.get_device() != index:
         raise ValueError("gamma must be on the device of x")
-    rows, width = x.shape
     x, gamma = _dense(x), _dense(gamma)
     total = y = kept = None
     if residual is not None:
-        if residual.dtype != torch.bfloat16 or residual.shape != x.shape or residual.get_device() != index:
+        if residual.dtype != torch.bfloat16 or residual.shape != shape or residual.get_device() != index:
             raise ValueError("residual must be BF16 of x's shape on its device")
         residual = _dense(residual)
         total = _empty((rows, width), (width, 1), torch.bfloat16, index)
