@@ -10,7 +10,6 @@ With ``own`` false, ``run`` computes each operator in its plain form (elementary
 32 bits, rounded once at the end); with ``own`` true it calls ``qk_b200``.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -142,28 +141,21 @@ def prepare(case, seed):
 # ---- the framework's operators -------------------------------------------------------------
 
 
-@functools.cache
-def _package():
-    """The framework's module, imported once as a program does."""
+def _run_own(s):
     folder = str(Path(__file__).resolve().parents[1] / "data-synth-tpu_b200")
     if folder not in sys.path:
         sys.path.insert(0, folder)
-    from qk_b200 import fp8
+    from qk_b200.fp8 import Fp8Rows, Fp8Weights, fp8_matmul, gated_ffn_fp8, quantize_fp8, rms_norm_fp8
 
-    return fp8
-
-
-def _run_own(s):
-    fp8 = _package()
     if s["op"] == "quantize":
-        return list(fp8.quantize_fp8(s["x"]))
+        return list(quantize_fp8(s["x"]))
     if s["op"] == "norm":
-        rows, total = fp8.rms_norm_fp8(s["x"], s["gamma"], s["eps"], residual=s["residual"])
+        rows, total = rms_norm_fp8(s["x"], s["gamma"], s["eps"], residual=s["residual"])
         return [rows.codes, rows.scales] + ([] if total is None else [total])
     if s["op"] == "matmul":
-        x = s["x"] if "x" in s else fp8.Fp8Rows(s["codes"], s["scales"])
-        return fp8.fp8_matmul(x, fp8.Fp8Weights(*s["weights"]), output_dtype=s["out"])
-    return fp8.gated_ffn_fp8(s["x"], *(fp8.Fp8Weights(*s[name]) for name in ("gate", "up", "down")))
+        x = s["x"] if "x" in s else Fp8Rows(s["codes"], s["scales"])
+        return fp8_matmul(x, Fp8Weights(*s["weights"]), output_dtype=s["out"])
+    return gated_ffn_fp8(s["x"], Fp8Weights(*s["gate"]), Fp8Weights(*s["up"]), Fp8Weights(*s["down"]))
 
 
 # ---- the plain forms -----------------------------------------------------------------------
