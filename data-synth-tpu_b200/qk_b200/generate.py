@@ -127,10 +127,11 @@ class StaticGeneration:
             o = torch.nn.functional.scaled_dot_product_attention(qh, kh, vh, is_causal=True)
             del kh, vh
             o = o.transpose(1, 2).reshape(n, hq, hd) * torch.sigmoid(gate)
+            o = o.reshape(n, hq * hd).contiguous()  # of one sequence it may be a view with the heads outside
             if fp8:
                 fp8.out(o, L.w_o, a, s)
             else:
-                torch.matmul(o.reshape(n, hq * hd), L.w_o.t(), out=a)
+                torch.matmul(o, L.w_o.t(), out=a)
             _lib.check(lib.qk_residual_add(P(x), P(a), n * H, P(x), s))
             _lib.check(lib.qk_rms_norm(P(x), P(L.ffn_norm), n, H, cfg.eps, P(h), s))
             _lib.check(lib.qk_router_topk(P(h), P(L.router), None, n, H, cfg.experts, cfg.top_k, P(ids), P(w), None,
