@@ -19,8 +19,7 @@ second model.
 import torch
 
 from . import _lib
-from .decoder import checked_argmax
-from .fp8 import Fp8Weights, fp8_matmul
+from .decoder import Fp8Projections, checked_argmax
 from .packed import linear_bf16, linear_workspace
 from .paged import empty_pool, empty_tables, plan_step, tree_attention, write_slots
 from .sampling import process_logits
@@ -101,12 +100,11 @@ class SpeculativeGeneration:
         self.ids = torch.empty((rows, cfg.top_k + 1), dtype=torch.int32, device=dev)
         self.weights = torch.empty((rows, cfg.top_k + 1), **bf)
         self.linear_ws = {}
+        self.fp8 = Fp8Projections(cfg, rows, dev) if cfg.dense == "fp8" else None
         self.moe_ws = torch.empty(max(int(_lib.load().qk_moe_workspace_bytes(model.desc, rows)), 16), dtype=torch.uint8,
                                   device=dev)
 
     def _linear(self, x, w, out):
-        if isinstance(w, Fp8Weights):
-            return fp8_matmul(x, w, out=out)
         if x.shape[0] > 256:  # a library product beyond the decode batches of the tcgen05 pass
             return torch.matmul(x, w.t(), out=out)
         key = tuple(w.shape)
@@ -127,16 +125,26 @@ class SpeculativeGeneration:
         self.status |= plan.status
         x = self.embedding.index_select(0, tokens.reshape(-1).long().clamp(0, self.embedding.shape[0] - 1))
         st = _lib.stream_handle(m.device)
-        _lib.check(lib.qk_rms_norm(P(x), P(m.layers[0].attn_norm), rows, H, cfg.eps, P(self.h), st))
+        fp8, last = self.fp8, len(m.layers) - 1
+        if fp8:  # as in the decode step: the attention norms leave as codes
+            fp8.norm(x, None, m.layers[0].attn_norm, st)
+        else:
+            _lib.check(lib.qk_rms_norm(P(x), P(m.layers[0].attn_norm), rows, H, cfg.eps, P(self.h), st))
         for li, L in enumerate(m.layers):
             k, v = self.keys[li], self.values[li]
-            self._linear(self.h, L.w_qkv, self.qkv)
+            if fp8:
+                fp8.qkv(L.w_qkv, self.qkv, st)
+            else:
+                self._linear(self.h, L.w_qkv, self.qkv)
             _lib.check(lib.qk_qk_norm_rope(P(self.qkv), P(L.q_norm), P(L.k_norm), P(m.inv_freq), P(plan.positions), rows,
                                            hq, kv, hd, cfg.rotary_dim, cfg.eps, P(self.q), P(self.gate), P(k), P(v), st))
             write_slots(self.pools[li], k, v, plan.slots)
             o = tree_attention(self.q, self.pools[li], self.table, self.cached, plan.ancestors, page_size=self.page,
                                counts=counts, gate=self.gate)
-            self._linear(o.view(rows, hq * hd), L.w_o, self.a)
+            if fp8:
+                fp8.out(o.view(rows, hq * hd), L.w_o, self.a, st)
+            else:
+                self._linear(o.view(rows, hq * hd), L.w_o, self.a)
             _lib.check(lib.qk_residual_rms_norm(P(x), P(self.a), P(L.ffn_norm), rows, H, cfg.eps, P(x), P(self.h), st))
             _lib.check(lib.qk_router_logits(P(self.h), P(L.router), rows, H, cfg.experts, P(self.router), st))
             _lib.check(lib.qk_router_select_shared(P(self.router), None, rows, cfg.experts, cfg.top_k, P(self.h),
@@ -144,7 +152,10 @@ class SpeculativeGeneration:
             _lib.check(lib.qk_moe_forward(m.desc, P(L.experts["gate"]), P(L.experts["up"]), P(L.experts["down"]), P(self.h),
                                           P(self.ids), P(self.weights), rows, _lib.QK_OUT_BF16, P(self.y), P(self.moe_ws),
                                           self.moe_ws.numel(), st))
-            norm = m.layers[li + 1].attn_norm if li + 1 < len(m.layers) else self.final_norm
+            if fp8 and li < last:
+                fp8.norm(x, self.y, m.layers[li + 1].attn_norm, st)
+                continue
+            norm = m.layers[li + 1].attn_norm if li < last else self.final_norm
             _lib.check(lib.qk_residual_rms_norm(P(x), P(self.y), P(norm), rows, H, cfg.eps, P(x), P(self.h), st))
         return self.h, plan
 

@@ -74,3 +74,127 @@ def test_prefill_of_one_sequence_matches_steps(cuda_device, monkeypatch):
     assert np.abs(a - b).max() < 0.1 * np.abs(b).max()
     gen.close()
     ref.close()
+
+
+def same_rows(a, b):
+    import torch
+
+    return torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales, b.scales)
+
+
+@pytest.mark.parametrize("batch", [1, 3])
+def test_a_verified_token_has_the_projections_of_a_decode_step(cuda_device, batch):
+    """The first layer's projections of one token, of the same hidden rows: equal bits in a decode step, in a
+    pass of one node and from the operators themselves."""
+    import torch
+
+    from qk_b200.fp8 import fp8_matmul, rms_norm_fp8
+    from qk_b200.speculate import SpeculativeGeneration
+
+    model = model_of(cuda_device, layers=1)
+    L = model.layers[0]
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    L.attn_norm = (1 + 0.3 * torch.randn(model.cfg.hidden, device=cuda_device, generator=g)).to(torch.bfloat16)
+    gen = SpeculativeGeneration(model, batch, 64, nodes=1, page_size=16, vocab=VOCAB)
+    gen.prefill([[7 + b] for b in range(batch)])
+    tokens = torch.tensor([[7 + b] for b in range(batch)], dtype=torch.int32, device=cuda_device)
+    gen.forward(tokens, torch.ones(batch, dtype=torch.int32, device=cuda_device))
+    x = gen.embedding.index_select(0, tokens[:, 0].long())
+    want = fp8_matmul(rms_norm_fp8(x, L.attn_norm, model.cfg.eps)[0], L.w_qkv)
+    state = model.state(batch)
+    state.x.copy_(x)
+    state.step()
+    assert torch.equal(bits(state.qkv), bits(want))
+    assert torch.equal(bits(gen.qkv), bits(want))
+
+
+def test_later_layers_of_a_verify_pass_take_codes_of_the_unrounded_norm(cuda_device):
+    """In a pass of 2 x 3 nodes: the last layer's q, gate, k and v are the product of the codes that the residual
+    add and norm leave, from the layer's own input."""
+    import torch
+
+    from qk_b200 import speculate
+    from qk_b200.fp8 import Fp8Rows, fp8_matmul, quantize_fp8
+    from qk_b200.speculate import SpeculativeGeneration
+
+    model = model_of(cuda_device)
+    gen = SpeculativeGeneration(model, 2, 64, nodes=3, page_size=16, vocab=VOCAB)
+    gen.prefill([[5, 6], [7]])
+    tokens = torch.tensor([[6, 1, 2], [7, 3, 4]], dtype=torch.int32, device=cuda_device)
+    seen, attention = [], speculate.tree_attention
+
+    def spied(*args, **kwargs):
+        seen.append(attention(*args, **kwargs))
+        return seen[-1]
+
+    speculate.tree_attention = spied
+    try:
+        gen.forward(tokens, torch.tensor([3, 3], dtype=torch.int32, device=cuda_device))
+    finally:
+        speculate.tree_attention = attention
+    width = model.cfg.hidden
+    rows = Fp8Rows(gen.fp8.codes[:, :width], gen.fp8.scales)
+    L = model.layers[-1]
+    assert torch.equal(bits(gen.qkv), bits(fp8_matmul(rows, L.w_qkv)))
+    assert torch.equal(bits(gen.a), bits(fp8_matmul(seen[-1].reshape(6, -1), L.w_o)))
+    # all but a BF16 norm's codes: quantising the rounded row would give others
+    norm = rows.codes.float() * rows.scales.t().repeat_interleave(128, 1)[:, :width]
+    assert not same_rows(rows, quantize_fp8(norm.to(torch.bfloat16)))
+
+
+@pytest.mark.parametrize("nodes", [4, 7])
+def test_tree_hidden_states_match_token_by_token(cuda_device, nodes):
+    """As for BF16 projections: each node of a tree agrees with feeding its path a token at a time."""
+    import torch
+
+    from qk_b200.speculate import SpeculativeGeneration
+
+    model, rng = model_of(cuda_device), np.random.default_rng(1)
+    prompts = [rng.integers(0, VOCAB, n).tolist() for n in (4, 19, 27)]
+    tree = SpeculativeGeneration(model, 3, 64, nodes=nodes, page_size=16, vocab=VOCAB)
+    tree.prefill(prompts)
+    up = [-1, 0, 0, 1, 1, 2, 3][:nodes]
+    parents = torch.tensor([up] * 3, dtype=torch.int32, device=cuda_device)
+    tokens = torch.from_numpy(rng.integers(0, VOCAB, (3, nodes)).astype(np.int32)).to(cuda_device)
+    tokens[:, 0] = torch.tensor([p[-1] for p in prompts])
+    counts = torch.tensor([nodes, nodes - 2, 1], dtype=torch.int32, device=cuda_device)
+    got = to_f32(tree.forward(tokens, counts, parents)[0]).reshape(3, nodes, -1).copy()
+    one = torch.ones(3, dtype=torch.int32, device=cuda_device)
+    for node in range(nodes):
+        path, j = [], node
+        while j >= 0:
+            path.append(j)
+            j = up[j]
+        single = SpeculativeGeneration(model, 3, 64, nodes=1, page_size=16, vocab=VOCAB)
+        single.prefill(prompts)
+        for j in reversed(path):
+            want = to_f32(single.forward(tokens[:, j:j + 1].contiguous(), one)[0])
+            single.cached = single.cached + one
+        for b in range(3):
+            if node < int(counts[b]):
+                assert np.abs(got[b, node] - want[b]).max() <= 0.1 * np.abs(want[b]).max()
+
+
+def test_generated_tokens_are_greedy_choices(cuda_device):
+    """As for BF16 projections: each generated token, scored by passes of one token, is the best one up to the
+    difference between the two passes."""
+    import torch
+
+    from qk_b200.speculate import SpeculativeGeneration
+
+    model, rng = model_of(cuda_device), np.random.default_rng(2)
+    prompts = [rng.integers(0, VOCAB, n).tolist() for n in (3, 12, 25)]
+    spec = SpeculativeGeneration(model, 3, 60, nodes=6, page_size=16, vocab=VOCAB)
+    spec.prefill(prompts)
+    out = spec.generate(6)
+    assert all(o[:len(p)] == p and 6 <= len(o) - len(p) <= 36 for o, p in zip(out, prompts))
+    single = SpeculativeGeneration(model, 3, 60, nodes=1, page_size=16, vocab=VOCAB)
+    one = torch.ones(3, dtype=torch.int32, device=cuda_device)
+    for t in range(max(len(o) for o in out) - 1):
+        tokens = torch.tensor([[o[min(t, len(o) - 1)]] for o in out], dtype=torch.int32, device=cuda_device)
+        hidden, _ = single.forward(tokens, one)
+        single.cached = single.cached + one
+        logits = to_f32(torch.matmul(hidden, single.embedding.t()))
+        for b, o in enumerate(out):
+            if len(prompts[b]) - 1 <= t < len(o) - 1:
+                assert logits[b, o[t + 1]] >= logits[b].max() - 0.1 * np.abs(logits[b]).max()
