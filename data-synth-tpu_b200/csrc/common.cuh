@@ -280,13 +280,13 @@ __device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t pa
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr uint32_t kWaitHintNs = 1000;
 
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, uint32_t limit = kWaitLimit) {
   if (mbar_try_wait(bar, parity)) return true;
   // Not unrolled: the loop is inlined at every wait of a kernel, and unrolled copies of it
   // made the projection kernels' code several times larger than their hot loops (a kernel
   // whose warps run different roles then misses in the instruction cache).
 #pragma unroll 1
-  for (uint32_t i = 0; i < kWaitLimit; ++i)
+  for (uint32_t i = 0; i < limit; ++i)
     if (mbar_try_wait_suspend(bar, parity, kWaitHintNs)) return true;
   return false;
 }

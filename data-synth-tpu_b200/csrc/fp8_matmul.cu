@@ -170,6 +170,17 @@ int product_of_rows(const void* x, int in_dtype, int64_t x_stride, int64_t M, in
   return rc ? rc : product(room, x_ld, scales, M, K, w, u, N, f32, out, ld, out_scales, st);
 }
 
+// A wait as the products have it, for an arrival that never comes, and its report.
+__global__ void fp8_expire_kernel(int polls) {
+  __shared__ uint64_t bar;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bar, 0, static_cast<uint32_t>(polls)))) atomicExch(&g_fp8_status, QK_ERR_TIMEOUT);
+}
+
 int check_room(const void* room, size_t bytes, size_t need) {
   if (need && (!room || bytes < need)) return set_error(QK_ERR_WORKSPACE, "the FP8 product needs a workspace of %zu bytes, got %zu", need, bytes);
   QK_REQUIRE((reinterpret_cast<uintptr_t>(room) & 255) == 0, "workspace must be 256-byte aligned");
@@ -249,6 +260,15 @@ int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t
                        static_cast<uint8_t*>(workspace), st);
   if (rc) return rc;
   return product(h, ld, h_scales, M, inner, Weights{down, down_ld, down_scales}, nullptr, N, false, out, 0, nullptr, st);
+}
+
+int qk_fp8_expire(int polls, qk_stream_t stream) {
+  QK_REQUIRE(polls >= 1 && polls <= 1000000, "polls must be 1 to 1000000");
+  fp8_expire_kernel<<<1, 32, 0, as_stream(stream)>>>(polls);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_error(e, "fp8_expire_kernel");
+  count_launch();
+  return QK_OK;
 }
 
 int qk_fp8_check(qk_stream_t stream) {

@@ -104,6 +104,7 @@ SIGNATURES = {
     "qk_fp8_ffn_workspace_bytes": (_sz, [_i, _i64, _i64, _i64]),
     "qk_fp8_ffn": (_i, [_p, _i, _i64, _i64, _i64] + [_p, _i64, _p] * 2 + [_i64, _p, _i64, _p, _i64, _p, _p, _sz, _p]),
     "qk_fp8_check": (_i, [_p]),
+    "qk_fp8_expire": (_i, [_i, _p]),
     "qk_router_select_shared": (_i, [_p, _p, _i, _i, _i, _p, _p, _i, _i, _i, _p, _p, _p]),
     "qk_moe_workspace_bytes": (_sz, [ctypes.POINTER(MoeDesc), _i]),
     "qk_moe_forward": (

@@ -278,7 +278,8 @@ class DecodeState:
                                      experts_per_rank=model.per + 1, top_k=k + 1, max_tokens=batch, device=dev)
 
     def step(self):
-        """One decode step of every layer on the current stream (no allocation, capturable)."""
+        """One decode step of every layer on the current stream (no allocation, capturable). With
+        ``dense="fp8"``, :func:`~qk_b200.fp8.check_status` raises what its products reported."""
         cfg, m = self.model.cfg, self.model
         lib = _lib.load()
         st = _lib.stream_handle(m.device)

@@ -32,6 +32,7 @@ import torch
 
 from . import _lib
 from .decoder import Fp8Projections, checked_argmax
+from .fp8 import check_status
 
 
 class StaticGeneration:
@@ -158,7 +159,14 @@ class StaticGeneration:
         st.x.copy_(x.view(B, W, H)[:, W - 1])
         st.positions.fill_(W)
         self._choose(0)
+        self._check_status()
         return self.tokens
+
+    def _check_status(self):
+        """Raise what FP8 products reported, so that no token of an output that is not valid is handed back;
+        synchronises where the projections are FP8, and asks nothing while a graph is captured."""
+        if self.model.cfg.dense == "fp8" and not torch.cuda.is_current_stream_capturing():
+            check_status(self.model.device)
 
     # ---- one greedy step ------------------------------------------------------------
     def _choose(self, column):
@@ -216,6 +224,7 @@ class StaticGeneration:
         self.capture()
         for _ in range(steps):
             self._graph.replay()
+        self._check_status()
         return self.generated
 
     def close(self):

@@ -20,6 +20,7 @@ import torch
 
 from . import _lib
 from .decoder import Fp8Projections, checked_argmax
+from .fp8 import check_status
 from .packed import linear_bf16, linear_workspace
 from .paged import empty_pool, empty_tables, plan_step, tree_attention, write_slots
 from .sampling import process_logits
@@ -225,6 +226,8 @@ class SpeculativeGeneration:
         if bool(self.status.any()):
             raise RuntimeError(f"the pool of pages ran out or a draft was invalid: {self.status.tolist()}")
         tree_attention.check_status(self.model.device)
+        if self.fp8:
+            check_status(self.model.device)
         return [row[:n] for row, n in zip(self.history.tolist(), lengths)]
 
 

@@ -194,6 +194,9 @@ int qk_fp8_ffn(const void* x, int in_dtype, int64_t x_stride, int64_t M, int64_t
 /* QK_ERR_TIMEOUT if a bounded wait of an earlier FP8 product on the current device gave up (its
  * output is then not valid), else QK_OK; clears the report. Synchronises `stream`. */
 int qk_fp8_check(qk_stream_t stream);
+/* A wait that nothing ends, given up after `polls` polls (1 to 1000000, a microsecond each at most)
+ * and reported as a product's is: so that a caller can test what it does with QK_ERR_TIMEOUT. */
+int qk_fp8_expire(int polls, qk_stream_t stream);
 
 /* ---- router ------------------------------------------------------------------
  * Replaces the router of qwen38_tpu/math.py:277-281 (routes_and_shared):

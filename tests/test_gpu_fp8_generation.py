@@ -198,3 +198,72 @@ def test_generated_tokens_are_greedy_choices(cuda_device):
         for b, o in enumerate(out):
             if len(prompts[b]) - 1 <= t < len(o) - 1:
                 assert logits[b, o[t + 1]] >= logits[b].max() - 0.1 * np.abs(logits[b]).max()
+
+
+def expire(device):
+    """A bounded wait of 200 microseconds at most that nothing ends, reported as a product's is."""
+    from qk_b200 import _lib
+
+    _lib.call("qk_fp8_expire", 200, _lib.stream_handle(device))
+
+
+def test_a_wait_that_gave_up_is_reported_once(cuda_device):
+    import torch
+
+    from qk_b200.fp8 import check_status
+
+    check_status(cuda_device)
+    expire(cuda_device)
+    with pytest.raises(RuntimeError):
+        check_status(cuda_device)
+    check_status(cuda_device)  # the report is cleared
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        expire(cuda_device)
+    check_status(cuda_device)
+    graph.replay()
+    with pytest.raises(RuntimeError):
+        check_status()
+    check_status()
+
+
+def test_generation_hands_back_no_tokens_of_a_product_that_gave_up(cuda_device):
+    from qk_b200.generate import StaticGeneration
+    from qk_b200.speculate import SpeculativeGeneration
+
+    model = model_of(cuda_device, layers=1)
+    spec = SpeculativeGeneration(model, 1, 64, nodes=2, page_size=16, vocab=VOCAB)
+    spec.prefill([[5, 6]])
+    expire(cuda_device)
+    with pytest.raises(RuntimeError):
+        spec.generate(1)
+    assert len(spec.generate(1)[0]) >= 4  # asked once
+    gen = StaticGeneration(model, 1, 8, 4, vocab=VOCAB, seed=1)
+    expire(cuda_device)
+    with pytest.raises(RuntimeError):
+        gen.prefill()
+    gen.prefill()
+    expire(cuda_device)
+    with pytest.raises(RuntimeError):
+        gen.decode(1)
+    gen.decode(1)
+    gen.close()
+
+
+def test_bf16_generation_does_not_ask(cuda_device):
+    """What FP8 products reported is not a BF16 model's."""
+    from qk_b200.fp8 import check_status
+    from qk_b200.generate import StaticGeneration
+    from qk_b200.speculate import SpeculativeGeneration
+
+    model = model_of(cuda_device, layers=1, dense="bf16")
+    expire(cuda_device)
+    spec = SpeculativeGeneration(model, 1, 64, nodes=2, page_size=16, vocab=VOCAB)
+    spec.prefill([[5, 6]])
+    spec.generate(1)
+    gen = StaticGeneration(model, 1, 8, 4, vocab=VOCAB, seed=1)
+    gen.prefill()
+    gen.decode(1)
+    gen.close()
+    with pytest.raises(RuntimeError):
+        check_status(cuda_device)
