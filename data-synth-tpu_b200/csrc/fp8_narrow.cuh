@@ -71,6 +71,7 @@ struct Narrow {
 template <int MT>
 struct NarrowControl {
   uint64_t full[kNarrowStages], empty[kNarrowStages], sum_full[8], sum_empty[8], stored, joined;
+  int64_t began;  // clock
   uint32_t tmem;
   static constexpr int kSlot = MT > 64 ? 64 : 32;
   alignas(16) float scales[kNarrowSumWarps * kNarrowAhead * kSlot];  // of x: a warp's slots of its tokens, or (ROWS) [block][MT]
@@ -129,9 +130,10 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
   const uint64_t wd0 = sdesc_sw128(smem, 1024u), xd0 = sdesc_sw128(smem + (ROWS ? a.stages * kStage : L::kBytesW), 1024u);
   int s = 0, d = 0;
   uint32_t full = 0, freed = 1;
+  bool ok = true;
   for (int it = 0; it < count; ++it) {
-    if (it >= L::kBuffers && !warp_wait(&ctl.sum_empty[d], freed)) return false;
-    if (!warp_wait(&ctl.full[s], full)) return false;
+    ok = (it < L::kBuffers || warp_wait(&ctl.sum_empty[d], freed)) && warp_wait(&ctl.full[s], full);
+    if (!ok) break;
     tc_fence_after();
     if (elect_one()) {
       const uint64_t wd = wd0 + s * (kStage >> 4), xd = xd0 + (ROWS ? it * (L::kBytesX >> 4) : s * (kStage >> 4));
@@ -147,7 +149,9 @@ __device__ __forceinline__ bool narrow_products(const NarrowArgs& a, NarrowContr
     if (++s == a.stages) s = 0, full ^= 1;
     if (++d == L::kBuffers) d = 0, freed ^= 1;
   }
-  return true;
+  // The last products are complete before the tensor memory is given back, also where a wait gave up. Where none were
+  // issued, this asks for the phase before the first.
+  return warp_wait(&ctl.sum_full[d ? d - 1 : L::kBuffers - 1], (d ? freed : freed ^ 1) ^ 1) && ok;
 }
 
 // The CTA's blocks of x, quantised into the operand tiles and ctl.scales [block][MT]. Rows past M hold whatever the
@@ -271,7 +275,9 @@ __device__ __forceinline__ bool narrow_sums(const NarrowArgs& a, NarrowControl<M
   return true;
 }
 
-// A warp per other owner sends it its tokens.
+// A warp per other owner sends it its tokens. Who receives them waits for them, and a CTA leaves behind all the others'
+// waits, so this one's memory lives while it is read. But a wait that gave up ends without them, 2^22 polls (more than
+// 2^26 cycles) behind the start: sent that late, they get the time that they need before this CTA lets the others go.
 template <int MT, bool GATED>
 __device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl<MT>& ctl, uint32_t smem, int owned, int live, int rank) {
   using L = Narrow<MT, GATED>;
@@ -281,6 +287,10 @@ __device__ __forceinline__ bool narrow_send(const NarrowArgs& a, NarrowControl<M
   if (elect_one())
     send(in_rank(smem + a.ring + (rank - (rank > owner)) * owned * L::kToken, owner), smem + owner * owned * L::kToken, tokens * L::kToken,
          in_rank(smem_addr(&ctl.joined), owner));
+  if (const int64_t sent = clock64(); sent - ctl.began > (1 << 25)) {
+    while (clock64() - sent < (1 << 18)) {
+    }
+  }
   __syncwarp();
   return true;
 }
@@ -382,6 +392,7 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
     pdl_wait();
     // the first copies are on their way while the others set up
     for (int i = 0; i < min(count, a.stages); ++i) narrow_copy<MT, GATED, ROWS>(a, ctl, &x, &w, &u, smem, i, b0, tile, row0);
+    ctl.began = clock64();
   }
   if (warp == 1) tmem_alloc(&ctl.tmem, L::kAlloc);
   pdl_wait();

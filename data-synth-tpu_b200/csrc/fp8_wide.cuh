@@ -141,10 +141,11 @@ __device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ct
   const uint32_t tm = __shfl_sync(0xffffffffu, ctl.tmem, 0);
   const uint64_t ad0 = sdesc_sw128(smem, 1024u), bd0 = sdesc_sw128(smem + kBytesA + h * (L::kBytesB / 2), 1024u);
   uint32_t s = 0, full = 0, d = 0, freed = 1;
-  for (int t = blockIdx.x / 2; t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
+  bool ok = true;
+  for (int t = blockIdx.x / 2; ok && t < a.tiles_m * a.tiles_n; t += gridDim.x / 2) {
     for (int b = 0; b < a.blocks; ++b) {
-      if (!warp_wait(&ctl.sum_empty[d][h], freed)) return false;
-      if (!warp_wait(&ctl.full[s], full)) return false;
+      ok = warp_wait(&ctl.sum_empty[d][h], freed) && warp_wait(&ctl.full[s], full);
+      if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t ad = ad0 + s * (L::kStageBytes >> 4), bd = bd0 + s * (L::kStageBytes >> 4);
@@ -158,7 +159,10 @@ __device__ __forceinline__ bool wide_products(const WideArgs& a, WideControl& ct
       if (++d == L::kBuffers) d = 0, freed ^= 1;
     }
   }
-  return true;
+  // The last products are complete before the tensor memory is given back, also where a wait gave up (beside the warps
+  // that add them, so it costs nothing). Where none were issued, this asks for the phase before the first.
+  const uint32_t last = d ? d - 1 : L::kBuffers - 1;
+  return warp_wait(&ctl.sum_full[last][h], (d ? freed : freed ^ 1) ^ 1) && ok;
 }
 
 // One block's sums, 64 columns at a time, times `by`, added to `acc`.
@@ -342,7 +346,6 @@ __device__ __forceinline__ bool wide_sums(const WideArgs& a, WideControl& ctl, c
     if (half == 0 && row < a.M) a.out_scales[static_cast<int64_t>(tile.n) * a.M + row] = fp8_scale(most);
     }
   }
-  if (lane == 0) stores_read<0>();  // the CTA's shared memory lives until then
   return true;
 }
 
@@ -385,6 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   if (warp >= kFirstSum) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
     ok = wide_sums<GATED, HALF>(a, ctl, &out, smem + L::kStages * L::kStageBytes, rank);
+    if ((threadIdx.x & 31) == 0) stores_read<0>();  // on every way out: the CTA's shared memory lives until then
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 0) {
