@@ -357,6 +357,7 @@ int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma,
   if (rows == 0) return QK_OK;
   QK_REQUIRE(x && gamma && codes && scales && (!y || x_out), "null pointer");
   QK_REQUIRE(aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(x_out) && aligned16(codes), "pointers must be 16-byte aligned");
+  QK_REQUIRE((reinterpret_cast<uintptr_t>(scales) & 3) == 0, "misaligned scales");
   NormArgs a{x, y, gamma, rows, ld, width, eps, x_out, codes, scales};
   const dim3 warps(static_cast<unsigned>((rows + 7) / 8));
   cudaStream_t st = as_stream(stream);

@@ -157,7 +157,7 @@ int qk_fp8_quantize_blocks(const void* w, int in_dtype, int64_t w_stride, int64_
 /* qk_residual_rms_norm (y NULL: qk_rms_norm) with its output quantised: x_out = bf16(x + y), then
  * with p = x_out * gamma and r = rsqrt(mean(x_out^2) + eps), codes e4m3(448 p / m) and scales
  * r m / 448, m = max(max |p| of the block, 2^-100). The normed row is not rounded to BF16.
- * Width a multiple of 8, 8192 at most; all arrays 16-byte aligned; x_out may be x. */
+ * Width a multiple of 8, 8192 at most; all arrays 16-byte aligned (scales: 4); x_out may be x. */
 int qk_fp8_rms_norm(const uint16_t* x, const uint16_t* y, const uint16_t* gamma, int64_t rows,
                     int width, float eps, uint16_t* x_out, uint8_t* codes, int64_t ld, float* scales,
                     qk_stream_t stream);
