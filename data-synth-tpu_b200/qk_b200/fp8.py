@@ -163,7 +163,7 @@ def fp8_weights(codes, scales, device=None):
     """A checkpoint's codes ``[N, K]`` (float8_e4m3fn, or uint8 of the same bits) and scales
     ``[ceil(N / 128), ceil(K / 128)]`` (what the codes are multiplied by) on ``device``, laid out once
     so that calls need not copy them."""
-    device = torch.device(device or (codes.device if codes.is_cuda else "cuda"))
+    device = torch.device(device if device is not None else codes.device if codes.is_cuda else "cuda")
     if codes.dtype == torch.uint8:
         codes = codes.view(_E4M3)
     codes, _, scales = _quantised(codes.to(device), scales, False, "the weights")
