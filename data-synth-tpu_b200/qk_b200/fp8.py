@@ -170,13 +170,14 @@ def fp8_weights(codes, scales, device=None):
     return Fp8Weights(codes, scales)
 
 
-def _output(out, m, n, dtype, index, x=None):
+def _output(out, m, n, dtype, index, *inputs):
+    """``out``, or a new output; it must not share memory with ``inputs``, matrices of dense rows."""
     if out is None:
         return _empty((m, n), (n, 1), dtype, index)
     if out.dtype != dtype or out.shape != (m, n) or out.get_device() != index or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {dtype} {[m, n]} on the device of x")
-    if x is not None and m:
-        first, size = x.data_ptr(), ((m - 1) * x.stride(0) + x.shape[1]) * x.element_size()
+    for x in inputs if m else ():
+        first, size = x.data_ptr(), ((x.shape[0] - 1) * x.stride(0) + x.shape[1]) * x.element_size()
         if first < out.data_ptr() + out.nbytes and out.data_ptr() < first + size:
             raise ValueError("out must not share memory with x, which is read while out is written")
     return out
@@ -185,7 +186,7 @@ def _output(out, m, n, dtype, index, x=None):
 def fp8_matmul(x, weights, *, output_dtype=None, out=None):
     """``x @ weights.T`` as ``[M, N]`` BF16 (default) or FP32 (``output_dtype``). ``x`` is BF16 or FP32
     ``[M, K]``, quantised in the call, or :class:`Fp8Rows`. Products of codes are exact, sums FP32. ``out``
-    must not share memory with ``x``."""
+    must not share memory with ``x`` (codes or scales)."""
     dtype = output_dtype or (torch.bfloat16 if out is None else out.dtype)
     out_code = _TYPES.get(dtype)
     if out_code is None:
@@ -195,7 +196,7 @@ def fp8_matmul(x, weights, *, output_dtype=None, out=None):
         m, k = codes.shape
         index = codes.get_device()
         n, w, w_pitch, w_scales, _keep = _weights(weights, k, index, "weights")
-        out = _output(out, m, n, dtype, index, codes)
+        out = _output(out, m, n, dtype, index, codes, scales)
         _lib.call_at(index, "qk_fp8_matmul", codes.data_ptr(), pitch, scales.data_ptr(), m, k, w, w_pitch, w_scales, n,
                      out_code, out.data_ptr())
         return out

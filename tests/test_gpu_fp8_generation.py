@@ -267,3 +267,25 @@ def test_bf16_generation_does_not_ask(cuda_device):
     gen.close()
     with pytest.raises(RuntimeError):
         check_status(cuda_device)
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_a_product_over_its_scales_is_refused(cuda_device, m):
+    """The scales of x are read while the output is written, as its codes are."""
+    import torch
+
+    from qk_b200.fp8 import Fp8Rows, fp8_matmul, pack_fp8, quantize_fp8
+
+    g = torch.Generator(device=cuda_device).manual_seed(m)
+    w = pack_fp8(torch.randn((16, 512), device=cuda_device, generator=g).to(torch.bfloat16))
+    rows = quantize_fp8(torch.randn((m, 512), device=cuda_device, generator=g).to(torch.bfloat16))
+    store = torch.zeros(m * 64, device=cuda_device)
+    scales = store[m * 24:m * 28].view(4, m)
+    scales.copy_(rows.scales)
+    rows = Fp8Rows(rows.codes, scales)
+    want = fp8_matmul(rows, w, output_dtype=torch.float32)
+    for at in (m * 24, m * 28 - 1, m * 9):  # all of them, the last, the first m
+        with pytest.raises(ValueError):
+            fp8_matmul(rows, w, out=store[at:at + m * 16].view(m, 16))
+    for at in (m * 28, m * 8):  # behind them, and up to them
+        assert torch.equal(fp8_matmul(rows, w, out=store[at:at + m * 16].view(m, 16)), want)
