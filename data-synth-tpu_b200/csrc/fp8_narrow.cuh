@@ -25,6 +25,9 @@ constexpr int kNarrowStages = 8, kNarrowSumWarps = 8, kNarrowFirstSum = 2;
 constexpr int kNarrowThreads = (kNarrowFirstSum + kNarrowSumWarps) * 32;
 constexpr int kNarrowAhead = 4;      // blocks whose scales of x are on their way
 constexpr int kMostSplits = 8;       // the portable cluster size
+// Three CTAs with as much shared memory do not fit the 228 KB of an SM. Registers do not see to that: with 16 tokens a
+// thread has 56, so that three fit, and they need not stay as they are from one compiler to the next.
+constexpr size_t kLeastSmem = 77 * 1024;
 // Rows of BF16, and blocks of them, that a CTA quantises itself, at most (gated: half, their rings are short). 32 rows of
 // 4096 x 2048 (128 blocks per CTA) take 7.0 us, with a launch of its own for that 7.4; 32 of 2048 x 9216 (256) 9.6 and
 // 8.3, 64 of 4096 x 2048 (256) 10.5 and 8.5, but that launch takes the host 4 us more, which is where such calls end:
@@ -51,8 +54,8 @@ struct Narrow {
   static constexpr uint32_t kBytesW = kOperands * 128 * kFp8Block, kBytesX = MT * kFp8Block, kStage = kBytesW + kBytesX;
   static constexpr int kColumns = kOperands * MT;                           // TMEM columns of a block's sums
   static constexpr int kBuffers = 256 / kColumns < 2 ? 2 : 256 / kColumns > 8 ? 8 : 256 / kColumns;
-  // 256 of 512 columns at most; registers (77 and more per thread) keep a third CTA from an SM, so that none waits for
-  // tensor memory while it holds up its cluster
+  // 256 of 512 columns at most, and two CTAs per SM at most, of whatever calls (kLeastSmem): none waits for tensor memory
+  // while it holds up its cluster, whose other CTAs hold some that another cluster's may wait for
   static constexpr uint32_t kAlloc = kColumns * kBuffers < 32 ? 32 : kColumns * kBuffers;
   static constexpr int kEach = MT / 2;                                      // tokens per thread
   static constexpr bool kTwo = kColumns <= 64;                              // room for two CTAs per SM
@@ -488,9 +491,10 @@ int launch_narrow(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap&
   a.stages = each < kNarrowStages ? each : kNarrowStages;
   while (a.stages > 1 && L::smem(a.stages, tiles_of_x, a.splits, live) > room) --a.stages;
   a.ring = L::ring(a.stages, tiles_of_x);
-  const size_t smem = L::smem(a.stages, tiles_of_x, a.splits, live);
+  size_t smem = L::smem(a.stages, tiles_of_x, a.splits, live);
+  if (smem < kLeastSmem) smem = kLeastSmem;
   const void* kernel = reinterpret_cast<const void*>(fp8_narrow_kernel<MT, GATED, ROWS>);
-  const int rc = allow_smem(kernel, smem > 64 * 1024 ? smem : 64 * 1024);  // with the static part, 48 KB are soon passed
+  const int rc = allow_smem(kernel, smem);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(plan.splits * ((a.N + 127) / 128)), static_cast<unsigned>((a.M + MT - 1) / MT));
