@@ -126,8 +126,9 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
 
 // numerics.py:13-14 accurate FP32 exp (AccuracyMode.HIGHEST): CUDA's expf, whose documented
 // maximum error is 2 ulp, inside the reference's 5e-7 relative budget
-// (numerics_validation.py:40). Every exponential of the kernels goes through it; qk_numerics
-// evaluates it for the FP64 check.
+// (numerics_validation.py:40). The exponentials of the reference's operators go through it
+// (router, sigmoid, SwiGLU, decode attention); qk_numerics evaluates it for the FP64 check.
+// The tree attention and the FP8 gated block, which have no counterpart there, have their own.
 __device__ __forceinline__ float exp_ref(float x) { return expf(x); }
 
 // numerics.py:42-45 sigmoid: divide(x >= 0 ? 1 : e, 1 + e), e = exp(-|x|), IEEE divide.

@@ -6,7 +6,8 @@
 // All are bound by HBM: one pass, a block of a row in 16 lanes of 8 values each, whose maximum is one reduction.
 // Measured: 32768 x 4096 BF16 66 us (407 MB, 6.2 TB/s, 94 % of the measured copy), 8192 x 4096 FP32 28 us (6.0 TB/s),
 // the norm with a residual over 16384 x 2048 40 us (236 MB, 5.8 TB/s); 64 rows of 4096 1.4 us, the norm of 8 rows 1.6.
-// FP32 of odd widths (8111 x 1111: 10.2 us, 4.5 TB/s) pays for single loads.
+// FP32 of odd widths (8111 x 1111: 10.8 us, 4.2 TB/s) pays for single loads, a choice of this code. Weights, which are
+// packed once: 8192 x 8192 BF16 48 us (201 MB, 4.2 TB/s), FP32 50 (6.7), 9216 x 2048 BF16 16.
 #include "fp8.cuh"
 
 namespace qk {

@@ -44,11 +44,13 @@ int check_rows(const void* x, int in_dtype, int64_t stride, int64_t M, int64_t K
 
 // Which form a call takes: the one with the smaller of these costs, about its ns in a graph (fitted to 65 to 4096 rows, K 256
 // to 8192, N 128 to 12288); up to 64 rows (gated 32) the narrow one, whose CTAs may quantise them. The wide form has
-// tiles of 256 x 256, or half as wide where that fills no more rounds of the pairs of SMs. All sides, us, narrow (before
-// its last steps, which took about a tenth off) / half / whole: 128 rows of 2048 x 9216 11.5 / 8.8 / 11.3, 256 of
-// 4096 x 2048 10.7 / 13.0 / 16.6, 512 15.0 / 13.1 / 16.8, 1024 of 8192 x 2048 40 / 23 / 30, 512 of 2048 x 9216
-// 28 / 14.5 / 12.2, 2048 of 4096 x 2048 45 / 23.6 / 18. A gated pair with its down product, narrow / wide: 256 rows of
-// 2048 x 512 12.8 / 17.3, 128 of 2048 x 6144 29.6 / 26.4.
+// tiles of 256 x 256, or half as wide where that fills no more rounds of the pairs of SMs. All sides, us, narrow /
+// half / whole: 128 rows of 2048 x 9216 9.3 / 8.8 / 11.2, 256 of 4096 x 2048 9.2 / 13.0 / 16.5, 512 12.8 / 13.1 / 16.6,
+// 1024 of 8192 x 2048 34 / 23 / 29, 512 of 2048 x 9216 25 / 14.3 / 12.0, 2048 of 4096 x 2048 38 / 23.5 / 18.0. A gated
+// pair with its down product in the same form, narrow / wide: 256 rows of 2048 x 512 11.9 / 18.6, 512 of 2048 x 1536
+// 23.7 / 23.1; 128 of 2048 x 6144 28.2 / 37.6, and 26.2 with the down product narrow, which is what is taken.
+// Of 110 sizes of 65 to 2048 rows the form taken is 0.1 % slower than the best in the median, 15 % at most
+// (384 rows of 256 x 512), and more than 10 % in 8.
 struct WidePlan {
   bool half;
   int64_t cost;

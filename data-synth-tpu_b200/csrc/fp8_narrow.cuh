@@ -8,9 +8,9 @@
 // its weights are on their way: that saves a launch, and the values are the same.
 //
 // Measured in a graph of calls over weights larger than L2 (floor: the weights' bytes at the measured HBM rate):
-//   1 row of BF16, 2048 x 9216        5.3 us, floor 2.9 (18.9 MB: 3.6 TB/s);  8 rows 6.1; 32 rows of codes 5.8, 64 7.4
-//   64 rows of BF16, 4096 x 2048      10.5 us, floor 1.4 (from codes 5.9);  1 row 4.3, floor 1.3
-//   feed-forward block, 32 rows, 2048 x 6144   17.4 us, floor 5.8, quantisation and down product included
+//   1 row of BF16, 2048 x 9216        5.4 us, floor 2.9 (18.9 MB: 3.5 TB/s);  8 rows 6.1; 32 rows of codes 5.9, 64 7.3
+//   64 rows of BF16, 4096 x 2048      10.5 us, floor 1.4 (from codes 6.1);  1 row of codes 4.0, floor 1.3
+//   feed-forward block, 32 rows, 2048 x 6144   17.2 to 18 us, floor 5.8, quantisation and down product included
 // What bounds it is latency: the set-up, the first copy from memory (2 us), then for each block the issue of its MMAs
 // (about 300 cycles), its sums and, at the end, the exchange and the output, most of it instructions that run once
 // and come cold from L2.
@@ -29,9 +29,10 @@ constexpr int kMostSplits = 8;       // the portable cluster size
 // thread has 56, so that three fit, and they need not stay as they are from one compiler to the next.
 constexpr size_t kLeastSmem = 77 * 1024;
 // Rows of BF16, and blocks of them, that a CTA quantises itself, at most (gated: half, their rings are short). 32 rows of
-// 4096 x 2048 (128 blocks per CTA) take 7.0 us, with a launch of its own for that 7.4; 32 of 2048 x 9216 (256) 9.6 and
-// 8.3, 64 of 4096 x 2048 (256) 10.5 and 8.5, but that launch takes the host 4 us more, which is where such calls end:
-// by wall clock 9.9 and 13.7, 10.8 and 13.6. Gated, 192 blocks (32 rows of 2048 x 6144) cost 3 us and save 1.
+// 4096 x 2048 (128 blocks per CTA) take 7.0 us, with a launch of its own for that 7.3; 32 of 2048 x 9216 (256) 9.7 and
+// 8.5, 64 of 4096 x 2048 (256) 10.5 and 8.5, but that launch takes the host 4 us more, which is where such calls end:
+// by wall clock 9.9 and 13.7, 10.8 and 13.6. So beyond 128 it is the host's time that decides, and in a captured graph a
+// launch of its own is the faster way. Gated, 192 blocks (32 rows of 2048 x 6144) cost 3 us and save 1.
 constexpr int kInline = 256, kInlineTokens = 256;  // kInlineTokens: of their tiles in shared memory
 
 struct NarrowArgs {
@@ -438,15 +439,16 @@ __global__ void __launch_bounds__(kNarrowThreads, Narrow<MT, GATED>::kTwo ? 2 : 
 }
 
 // What a call does, by its sizes alone: a cluster's CTAs share a tile's blocks of K, as many as give every SM one CTA
-// at most (one row of 2048 x 9216, 72 tiles: 1 / 2 / 3 / 4 CTAs take 8.2 / 5.3 / 5.8 / 8.2 us, of 4096 x 2048, 16
-// tiles: 4 / 6 / 8 take 4.7 / 4.6 / 4.3). A cluster lies within a group of SMs: of 4 there is room for 33 where a CTA
+// at most (one row of 2048 x 9216, 72 tiles: 1 / 2 / 3 / 4 CTAs take 7.4 / 5.1 / 5.9 / 7.8 us, of 4096 x 2048, 16
+// tiles: 4 / 6 / 8 take 4.3 / 4.2 / 4.0). That is not always the best number: where it shortens no CTA's part, or the
+// clusters fill the card, fewer are faster (192 rows of 1024 x 1000 with 6 5.3 us, with 4 or 5 4.1; 64 of 2000 x 3000
+// with 6 6.2, with 5 5.2; in 7 of 99 sizes by more than a tenth). A cluster lies within a group of SMs: of 4 there is room for 33 where a CTA
 // takes an SM for itself, of 8 for 15, and one cluster too many costs a second round (64 rows of 4096 x 2048 with
 // eight: 6.2 us where two fit an SM, 10.0 else). So all but the largest leave room for a second, and those have four.
 // Tokens per tile: all of them up to 64 (gated 32). Beyond, tiles of 64 (32) or of twice as many, which read the
 // weights less often but have only one CTA per SM: the ones with the smaller cost, about the ns of a call in a graph
-// (before the last steps 96 rows of 4096 x 2048 took 7.8 and 9.3 us, 512 of 1024 x 1000 5.7 and 7.4; but 256 of
-// 4096 x 2048 11.9 and 10.7. Gated, 128 rows of 2048 x 512 11.9 and 16.1 with the down product). Of the products a
-// block takes about 0.42 and 0.46 us beside 3.7 and 5.8 for all the rest.
+// (96 rows of 4096 x 2048 take 6.6 and 8.2 us, 512 of 1024 x 1000 4.8 and 6.4; but 512 of 4096 x 2048 14.4 and 12.8.
+// Gated, 128 rows of 2048 x 512 11.4 and 14.4 with the down product). Of the products a block takes about 0.42 and 0.46 us beside 3.7 and 5.8 for all the rest.
 struct NarrowPlan {
   int tokens, splits, rows, most;  // rows: that a CTA quantises itself, at most, and (most) blocks of them
   int64_t cost;

@@ -78,7 +78,9 @@ __device__ __forceinline__ void cluster_sync() {
   cluster_wait();
 }
 
-// silu(g) u
+// silu(g) u. The exponential is within 2 + 1.2 |g| units of the last place, the quotient within 2, so that silu is within
+// 2^-19 up to |g| = 8. 5e-6 to 8e-6 of the quantised values take the other code of two next to a border; sums of FP32 in
+// the plain form move 5e-5 of them, and an IEEE quotient and expf here left as many as this.
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

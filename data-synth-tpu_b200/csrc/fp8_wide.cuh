@@ -13,13 +13,16 @@
 // 0.25, but 0.7 more at the end, where they join their sums; summing a block while the next is read 0.30.
 //
 // Measured (B200, 1.9 GHz, in bursts / in a loop of seconds under the power cap):
-//   x 16384 x 2048 of codes, 9216 columns, BF16 out   285 / 330 us, 2170 / 1870 TFLOP/s
-//   4096 x 8192, 8192 columns                         235 / 273 us, 2340 / 2010 TFLOP/s
-//   gated, 8192 x 2048, 6144 columns of each          225 / 235 us, 1830 / 1750 TFLOP/s
-// What bounds it: without the additions to the sums the first takes 258 us, without them and the output 210, without the
-// exchange of buffers too 188 (3300 TFLOP/s): the sums' instructions, a buffer's round trip and shared memory (x's tile
-// is read once for either half), in this order, and in long loops the power. One buffer of 256 columns for both halves
-// saves that second read, but takes 317 us; sixteen warps for the sums take 360, five or six stages nothing less.
+//   x 16384 x 2048 of codes, 9216 columns, BF16 out   285 / 330 us, 2170 / 1870 TFLOP/s; FP32 out 334 in bursts
+//   4096 x 8192, 8192 columns                         235 / 273 us, 2340 / 2010 TFLOP/s; FP32 out 240
+//   gated, 8192 x 2048, 6144 columns of each          208 to 225 / 235 us, 1980 to 1830 / 1750 TFLOP/s
+// What bounds it: the first takes 287 us; without the sums' loads from tensor memory and additions 237, without the output
+// 255, without both 202 (2048 columns of K; of 8192 236, 196, 229 and 186), and the products alone would take 187 at
+// twice the rate of BF16. So the sums come first, then the output, which runs beside the next tile's copies but not
+// beside its sums, then the exchange of buffers and shared memory (x's tile is read once for either half); and the rounds:
+// 2304 tiles on 74 pairs are 31.1 rounds in 32. In long loops it is the power. One buffer of 256 columns for both halves
+// saves that second read, but took 317 us where this form took 303; sixteen warps for the sums took 360, five or six
+// stages nothing less.
 #pragma once
 
 #include "fp8_product.cuh"

@@ -39,7 +39,8 @@ class Fp8Weights(NamedTuple):
     scales: torch.Tensor  # FP32 [ceil(N / 128), ceil(K / 128)]
 
 
-# The allocation that compiled graphs make, at half the cost of torch.empty_strided: on the current device only.
+# The allocation that compiled graphs make, at half the cost of torch.empty_strided: on the current device only. A private
+# function of torch, taken where it is there; dispatch modes do not see what it allocates.
 _lean_empty = getattr(getattr(torch._C._dynamo, "guards", None), "_empty_strided_cuda", None)
 _current = getattr(torch._C, "_cuda_getDevice", None)
 

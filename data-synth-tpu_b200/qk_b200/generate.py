@@ -7,8 +7,8 @@ share of the expert-parallel model):
 
 * **Prefill** (``engine.py:449-500`` ``forward_chunk``): the whole prompt of every sequence
   is one chunk of ``batch * prompt`` tokens. Per layer: RMSNorm, the q | gate, k, v
-  projection (cuBLAS; with ``dense="fp8"`` qk_fp8_rms_norm and qk_fp8_matmul), per-head q/k RMSNorm and rotary at each token's position
-  (``qk_qk_norm_rope``), the chunk's keys and values quantised into the Q8 cache
+  projection (cuBLAS; with ``dense="fp8"`` qk_fp8_rms_norm and qk_fp8_matmul), per-head q/k
+  RMSNorm and rotary at each token's position (``qk_qk_norm_rope``), the chunk's keys and values quantised into the Q8 cache
   (``qk_kv_q8_append_chunk``), causal attention of the chunk over the dequantised cache
   (``qk_kv_q8_read`` feeding PyTorch's fused attention; the cache's own keys and values, as
   ``attention_cache.py:152-170`` reads them), the sigmoid output gate, the output
